@@ -13,7 +13,7 @@ import numpy as np
 
 from ._build import LIB_PATH
 
-ABI_VERSION = 26
+ABI_VERSION = 27
 
 # dtype codes
 F32, BF16, F16, U8, I8 = 0, 1, 2, 3, 4
@@ -151,6 +151,12 @@ GRAD_PREP_DTYPE = np.dtype([("g", np.uint64), ("out", np.uint64), ("n", np.int64
                             ("dtype", np.uint32), ("reserved", np.uint32)])
 assert GRAD_PREP_DTYPE.itemsize == 40
 GRAD_PREP_CHUNK = 2048
+# apexw_clip_tensor: one gradient of a clip by the global norm
+CLIP_TENSOR_DTYPE = np.dtype([("g", np.uint64), ("out", np.uint64), ("n", np.int64), ("first_unit", np.int64),
+                              ("g_dtype", np.uint32), ("out_dtype", np.uint32)])
+assert CLIP_TENSOR_DTYPE.itemsize == 40
+CLIP_PARTIALS = 2048
+EXPERT_NK, EXPERT_KN = 0, 1
 # apexw_fv_tensor: one factored-v tensor of a group
 FV_TENSOR_DTYPE = np.dtype([("tensor", np.uint32), ("rows", np.int32), ("cols", np.int32), ("flags", np.uint32),
                             ("ws", np.int64), ("band0", np.int32), ("cb0", np.int32)])
@@ -211,6 +217,18 @@ SIGNATURES = {
     "apexw_amp_prepare": (ctypes.c_int, [_vp, _vp, _vp, _i32, _vp, _i32, _vp, _vp]),
     "apexw_state_decode": (ctypes.c_int, [ctypes.POINTER(StateLayout), _vp, _vp, _vp]),
     "apexw_state_encode": (ctypes.c_int, [ctypes.POINTER(StateLayout), _vp, _vp, _vp]),
+    "apexw_layer_norm_forward": (ctypes.c_int, [_vp, _i64, _i64, _i64, _i32, _vp, _vp, _i32, _f32, _vp, _vp, _vp, _vp]),
+    "apexw_layer_norm_workspace": (ctypes.c_int64, [_i64, _i64]),
+    "apexw_layer_norm_backward": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _vp,
+                                                 _vp, _vp, _vp, _vp]),
+    "apexw_expert_rows": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i64, _i32, _vp, _i32, _i64, _i64, _i64, _i32, _vp,
+                                         _i64, _vp]),
+    "apexw_expert_weight_grad": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i32, _i64, _i64, _i64, _i32, _vp, _i32,
+                                                _vp]),
+    "apexw_clip_layout": (ctypes.c_int64, [_vp, _i32]),
+    "apexw_grad_norm": (ctypes.c_int, [_vp, _i32, _i64, _i32, _vp, _vp, _vp]),
+    "apexw_grad_scale": (ctypes.c_int, [_vp, _i32, _i64, _vp, _f32, _vp]),
+    "apexw_clip_grads": (ctypes.c_int, [_vp, _i32, _i64, _i32, _f32, _vp, _vp, _vp]),
 }
 
 GEMM_TILE = 256

@@ -1,0 +1,289 @@
+// Global norm of a list of gradients, and their clipped copies (gfx950).
+//
+//   norm = (sum |g|^p)^(1/p) over every element of every tensor, p = 1, 2 or infinity
+//   c = min(max_norm / (norm + 1e-6), 1), out = round(c g)
+//
+// Bound by memory: the norm reads every gradient, the scaling reads them again and writes the copies.
+// Two launches.  The first leaves one partial sum per workgroup; every workgroup of the second adds the
+// partials up in the same order, so all use one coefficient bit for bit, and nothing is atomic or cleared
+// beforehand.
+#include "common.h"
+
+namespace {
+
+constexpr int kUnit = APEXW_CLIP_UNIT;   // elements of a work unit: 32 per thread
+
+struct __attribute__((packed, aligned(2))) Bytes16 { u32x4 v; };
+
+// 8 elements from element e of a tensor, those below cnt (the rest 0): no alignment beyond the element's
+template <int DT> APEXW_DEV void load_some(const void* base, int64_t e, int64_t cnt, float (&x)[8]) {
+  if (cnt >= 8) {
+    if constexpr (DT == APEXW_F32) {
+      const auto p = APEXW_GLOBAL(const Bytes16, (const float*)base + e);
+      const u32x4 a = p[0].v, b = p[1].v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[j] = __uint_as_float(a[j]);
+        x[4 + j] = __uint_as_float(b[j]);
+      }
+    } else {
+      const u32x4 a = APEXW_GLOBAL(const Bytes16, (const uint16_t*)base + e)->v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (DT == APEXW_BF16) {
+          x[2 * j] = __uint_as_float(a[j] << 16);
+          x[2 * j + 1] = __uint_as_float(a[j] & 0xFFFF0000u);
+        } else {
+          x[2 * j] = f16_bits_to_f32(a[j] & 0xFFFFu);
+          x[2 * j + 1] = f16_bits_to_f32(a[j] >> 16);
+        }
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = j < cnt ? load1<DT>(base, e + j) : 0.0f;
+}
+
+template <int DT> APEXW_DEV void store_some(void* base, int64_t e, int64_t cnt, const float (&x)[8]) {
+  uint32_t w[8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (DT == APEXW_BF16) w[j] = pack_bf16x2(x[2 * j], x[2 * j + 1]);
+    else if constexpr (DT == APEXW_F16) w[j] = f32_to_f16_bits(x[2 * j]) | (f32_to_f16_bits(x[2 * j + 1]) << 16);
+  }
+  if (cnt >= 8) {
+    if constexpr (DT == APEXW_F32) {
+      auto p = APEXW_GLOBAL(Bytes16, (float*)base + e);
+      p[0].v = u32x4{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
+      p[1].v = u32x4{__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7])};
+    } else {
+      APEXW_GLOBAL(Bytes16, (uint16_t*)base + e)->v = u32x4{w[0], w[1], w[2], w[3]};
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < cnt) {
+      if constexpr (DT == APEXW_F32) APEXW_GLOBAL(float, base)[e + j] = x[j];
+      else APEXW_GLOBAL(uint16_t, base)[e + j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+    }
+}
+
+// the tensor of the table that holds unit u: the last one whose first unit is <= u (a tensor without
+// elements has no units and the first unit of the next)
+APEXW_DEV int find_tensor(const apexw_clip_tensor* __restrict__ tab, int n, int64_t u) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (tab[mid].first_unit <= u) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// the magnitudes of one thread's 32 elements of a unit joined into acc: sums of |x|^order (1, 2; a sum of
+// squares that leaves the fp32 range is formed again in 64 bits), or (order 0) the largest magnitude's bits,
+// which order NaN above infinity above every number
+template <int GD> APEXW_DEV void unit_norm(const apexw_clip_tensor& t, int64_t e0, int order, double& acc, uint32_t& top) {
+  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < kUnit / 2048; ++i) {
+    const int64_t e = e0 + 2048 * i + 8 * threadIdx.x;
+    float x[8];
+    load_some<GD>(t.g, e, t.n - e, x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (order == 2) s[j & 3] = fmaf(x[j], x[j], s[j & 3]);
+      else if (order == 1) s[j & 3] += fabsf(x[j]);
+      else {
+        const uint32_t b = __float_as_uint(x[j]) & 0x7FFFFFFFu;
+        top = b > top ? b : top;
+      }
+    }
+  }
+  if (order == 0) return;
+  const float sum = (s[0] + s[1]) + (s[2] + s[3]);
+  if (__builtin_isinf(sum)) {
+    double d = 0.0;
+    for (int i = 0; i < kUnit / 2048; ++i) {
+      const int64_t e = e0 + 2048 * i + 8 * threadIdx.x;
+      float x[8];
+      load_some<GD>(t.g, e, t.n - e, x);
+      for (int j = 0; j < 8; ++j) d += order == 2 ? (double)x[j] * x[j] : fabs((double)x[j]);
+    }
+    acc += d;
+  } else {
+    acc += (double)sum;
+  }
+}
+
+APEXW_DEV double wave_sum_d(double x) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
+  return x;
+}
+APEXW_DEV uint32_t wave_max_u(uint32_t x) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    const uint32_t y = __shfl_xor(x, off, 64);
+    x = y > x ? y : x;
+  }
+  return x;
+}
+
+// sum (or, order 0, the largest magnitude) over the workgroup's threads, on all of them
+APEXW_DEV double join(double acc, uint32_t top, int order, double* red) {
+  const double v = order == 0 ? (double)__uint_as_float(wave_max_u(top)) : wave_sum_d(acc);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  double s = red[0];
+  for (int i = 1; i < 4; ++i) s = order != 0 ? s + red[i] : red[i] > s || red[i] != red[i] ? red[i] : s;
+  __syncthreads();
+  return s;
+}
+
+__global__ __launch_bounds__(256) void grad_norm_kernel(const apexw_clip_tensor* __restrict__ tab, int32_t n_tensors,
+                                                        int64_t n_units, int32_t order, double* __restrict__ partial) {
+  __shared__ double red[4];
+  const int64_t u0 = n_units * blockIdx.x / gridDim.x, u1 = n_units * (blockIdx.x + 1) / gridDim.x;
+  double acc = 0.0;
+  uint32_t top = 0u;
+  if (u0 < u1) {
+    int k = find_tensor(tab, n_tensors, u0);
+    apexw_clip_tensor t = tab[k];
+    for (int64_t u = u0; u < u1; ++u) {
+      while (u >= t.first_unit + (t.n + kUnit - 1) / kUnit) t = tab[++k];
+      const int64_t e0 = (u - t.first_unit) * kUnit;
+      if (t.g_dtype == APEXW_F32) unit_norm<APEXW_F32>(t, e0, order, acc, top);
+      else if (t.g_dtype == APEXW_BF16) unit_norm<APEXW_BF16>(t, e0, order, acc, top);
+      else unit_norm<APEXW_F16>(t, e0, order, acc, top);
+    }
+  }
+  const double s = join(acc, top, order, red);
+  if (threadIdx.x == 0) partial[blockIdx.x] = s;
+}
+
+// the norm from the first launch's partials, in one order for every workgroup
+APEXW_DEV float total_norm(const double* __restrict__ partial, int32_t n_partial, int32_t order, double* red) {
+  double acc = 0.0;
+  float top = 0.0f;
+  for (int i = threadIdx.x; i < n_partial; i += 256) {
+    if (order != 0) acc += partial[i];
+    else {
+      const float v = (float)partial[i];
+      top = __float_as_uint(v) > __float_as_uint(top) ? v : top;
+    }
+  }
+  const double s = join(acc, __float_as_uint(top), order, red);
+  return (float)(order == 2 ? sqrt(s) : s);
+}
+
+__global__ __launch_bounds__(256) void total_norm_kernel(const double* __restrict__ partial, int32_t n_partial,
+                                                         int32_t order, float* __restrict__ norm) {
+  __shared__ double red[4];
+  const float v = total_norm(partial, n_partial, order, red);
+  if (threadIdx.x == 0) *norm = v;
+}
+
+template <int GD, int OD> APEXW_DEV void unit_scale(const apexw_clip_tensor& t, int64_t e0, float c) {
+#pragma unroll
+  for (int i = 0; i < kUnit / 2048; ++i) {
+    const int64_t e = e0 + 2048 * i + 8 * threadIdx.x;
+    if (e >= t.n) break;
+    float x[8];
+    load_some<GD>(t.g, e, t.n - e, x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] *= c;
+    store_some<OD>(t.out, e, t.n - e, x);
+  }
+}
+
+template <int GD> APEXW_DEV void unit_scale_to(const apexw_clip_tensor& t, int64_t e0, float c) {
+  if (t.out_dtype == APEXW_F32) unit_scale<GD, APEXW_F32>(t, e0, c);
+  else if (t.out_dtype == APEXW_BF16) unit_scale<GD, APEXW_BF16>(t, e0, c);
+  else unit_scale<GD, APEXW_F16>(t, e0, c);
+}
+
+// given: a norm that the caller formed (over more than these tensors); else the partials' norm, written to *norm.
+// A tensor clipped in place is left alone where the coefficient is one.
+__global__ __launch_bounds__(256) void grad_scale_kernel(const apexw_clip_tensor* __restrict__ tab, int32_t n_tensors,
+                                                         int64_t n_units, int32_t order,
+                                                         const double* __restrict__ partial, int32_t n_partial,
+                                                         const float* __restrict__ given, float max_norm,
+                                                         float* __restrict__ norm) {
+  __shared__ double red[4];
+  const float total = given ? *given : total_norm(partial, n_partial, order, red);
+  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = total;
+  const float q = max_norm / (total + 1e-6f), c = q > 1.0f ? 1.0f : q;   // NaN stays NaN
+  // the last units first: what the norm's pass read last is still in the cache
+  const int64_t b = gridDim.x - 1 - blockIdx.x;
+  const int64_t u0 = n_units * b / gridDim.x, u1 = n_units * (b + 1) / gridDim.x;
+  if (u0 >= u1) return;
+  int k = find_tensor(tab, n_tensors, u1 - 1);
+  apexw_clip_tensor t = tab[k];
+  for (int64_t u = u1 - 1; u >= u0; --u) {
+    while (u < t.first_unit) t = tab[--k];
+    if (c == 1.0f && t.out == t.g) continue;
+    const int64_t e0 = (u - t.first_unit) * kUnit;
+    if (t.g_dtype == APEXW_F32) unit_scale_to<APEXW_F32>(t, e0, c);
+    else if (t.g_dtype == APEXW_BF16) unit_scale_to<APEXW_BF16>(t, e0, c);
+    else unit_scale_to<APEXW_F16>(t, e0, c);
+  }
+}
+
+int norm_grid(int64_t n_units) { return (int)(n_units < APEXW_CLIP_PARTIALS ? (n_units > 0 ? n_units : 1) : APEXW_CLIP_PARTIALS); }
+
+bool table_ok(const apexw_clip_tensor* tensors, int32_t n_tensors, int64_t n_units) {
+  return n_tensors >= 0 && n_units >= 0 && (n_units == 0 || (tensors && n_tensors > 0 && !((uintptr_t)tensors & 7u)));
+}
+bool order_ok(int32_t order) { return order >= 0 && order <= 2; }
+bool max_ok(float m) { return m >= 0.0f; }
+
+}  // namespace
+
+extern "C" int64_t apexw_clip_layout(apexw_clip_tensor* t, int32_t n_tensors) {
+  if (n_tensors < 0 || (n_tensors > 0 && !t)) return -APEXW_ERR_ARG;
+  int64_t units = 0;
+  for (int32_t i = 0; i < n_tensors; ++i) {
+    if (t[i].n < 0 || (t[i].n > 0 && !t[i].g)) return -APEXW_ERR_ARG;
+    if (t[i].g_dtype > APEXW_F16 || t[i].out_dtype > APEXW_F16) return -APEXW_ERR_DTYPE;
+    if (((uintptr_t)t[i].g & (t[i].g_dtype == APEXW_F32 ? 3u : 1u)) ||
+        ((uintptr_t)t[i].out & (t[i].out_dtype == APEXW_F32 ? 3u : 1u)))
+      return -APEXW_ERR_ALIGN;
+    t[i].first_unit = units;
+    units += (t[i].n + kUnit - 1) / kUnit;
+  }
+  return units;
+}
+
+extern "C" int apexw_grad_norm(const apexw_clip_tensor* tensors, int32_t n_tensors, int64_t n_units, int32_t order,
+                               double* workspace, float* norm, void* stream) {
+  if (!table_ok(tensors, n_tensors, n_units) || !order_ok(order) || !workspace || !norm) return APEXW_ERR_ARG;
+  const int grid = norm_grid(n_units);
+  hipLaunchKernelGGL(grad_norm_kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, tensors, n_tensors, n_units,
+                     order, workspace);
+  hipLaunchKernelGGL(total_norm_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, workspace, grid, order, norm);
+  return hipGetLastError() == hipSuccess ? APEXW_OK : APEXW_ERR_LAUNCH;
+}
+
+extern "C" int apexw_grad_scale(const apexw_clip_tensor* tensors, int32_t n_tensors, int64_t n_units,
+                                const float* norm, float max_norm, void* stream) {
+  if (!table_ok(tensors, n_tensors, n_units) || !norm || !max_ok(max_norm)) return APEXW_ERR_ARG;
+  if (n_units == 0) return APEXW_OK;
+  hipLaunchKernelGGL(grad_scale_kernel, dim3(norm_grid(n_units)), dim3(256), 0, (hipStream_t)stream, tensors,
+                     n_tensors, n_units, 2, (const double*)nullptr, 0, norm, max_norm, (float*)nullptr);
+  return hipGetLastError() == hipSuccess ? APEXW_OK : APEXW_ERR_LAUNCH;
+}
+
+extern "C" int apexw_clip_grads(const apexw_clip_tensor* tensors, int32_t n_tensors, int64_t n_units, int32_t order,
+                                float max_norm, double* workspace, float* norm, void* stream) {
+  if (!table_ok(tensors, n_tensors, n_units) || !order_ok(order) || !max_ok(max_norm) || !workspace || !norm)
+    return APEXW_ERR_ARG;
+  const int grid = norm_grid(n_units);
+  hipLaunchKernelGGL(grad_norm_kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, tensors, n_tensors, n_units,
+                     order, workspace);
+  hipLaunchKernelGGL(grad_scale_kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, tensors, n_tensors, n_units,
+                     order, workspace, grid, (const float*)nullptr, max_norm, norm);
+  return hipGetLastError() == hipSuccess ? APEXW_OK : APEXW_ERR_LAUNCH;
+}

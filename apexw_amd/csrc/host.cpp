@@ -120,7 +120,78 @@ PyObject* scan(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return PyLong_FromLong(moved ? kGradsMoved : kSame);
 }
 
+// apexw_clip_tensor of include/apexw_hip.h
+struct ClipTensor {
+  const void* g;
+  void* out;
+  int64_t n, first_unit;
+  uint32_t g_dtype, out_dtype;
+};
+
+bool dtype_code(const at::Tensor& t, uint32_t* code) {
+  switch (t.scalar_type()) {
+    case at::kFloat: *code = 0; return true;
+    case at::kBFloat16: *code = 1; return true;
+    case at::kHalf: *code = 2; return true;
+    default: return false;
+  }
+}
+
+// clip_table(grads, out, table_addr, name): the entries of a clip's table (first_unit left 0).
+// Raises for tensors that the clip does not take: another device, type or layout.
+PyObject* clip_table(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 4) {
+    PyErr_SetString(PyExc_TypeError, "clip_table(grads, out, table_addr, name)");
+    return nullptr;
+  }
+  uintptr_t ta;
+  if (!unpack_list(args[0], "grads") || !unpack_list(args[1], "out") || !as_addr(args[2], &ta)) return nullptr;
+  const char* name = PyUnicode_AsUTF8(args[3]);
+  if (!name) return nullptr;
+  auto* table = reinterpret_cast<ClipTensor*>(ta);
+  const Py_ssize_t n = PyList_GET_SIZE(args[0]);
+  if (PyList_GET_SIZE(args[1]) != n) {
+    PyErr_SetString(PyExc_ValueError, "clip_table: lists of different lengths");
+    return nullptr;
+  }
+  if (n == 0) Py_RETURN_NONE;
+  const bool in_place = args[0] == args[1];
+  const at::Device device = THPVariable_Unpack(PyList_GET_ITEM(args[0], 0)).device();
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    const at::Tensor& g = THPVariable_Unpack(PyList_GET_ITEM(args[0], i));
+    const at::Tensor& o = in_place ? g : THPVariable_Unpack(PyList_GET_ITEM(args[1], i));
+    ClipTensor& t = table[i];
+    if (g.layout() != at::kStrided || o.layout() != at::kStrided) {
+      PyErr_Format(PyExc_ValueError, "%s: tensor %zd is sparse", name, i);
+      return nullptr;
+    }
+    if (g.device() != device || o.device() != device) {
+      PyErr_Format(PyExc_ValueError, "%s: tensor %zd is on another device than the first one", name, i);
+      return nullptr;
+    }
+    if (!dtype_code(g, &t.g_dtype) || !dtype_code(o, &t.out_dtype)) {
+      PyErr_Format(PyExc_TypeError, "%s: tensor %zd is not float32, bfloat16 or float16", name, i);
+      return nullptr;
+    }
+    if (!g.is_contiguous() && !g.is_non_overlapping_and_dense()) {
+      PyErr_Format(PyExc_ValueError, "%s: tensor %zd is not dense", name, i);
+      return nullptr;
+    }
+    if (!in_place && (g.sizes() != o.sizes() || (g.strides() != o.strides() && !(g.is_contiguous() && o.is_contiguous())))) {
+      PyErr_Format(PyExc_ValueError, "%s: the copy of tensor %zd has another shape or layout", name, i);
+      return nullptr;
+    }
+    t.g = g.data_ptr();
+    t.out = o.data_ptr();
+    t.n = g.numel();
+    t.first_unit = 0;
+  }
+  Py_RETURN_NONE;
+}
+
 PyMethodDef kMethods[] = {
+    {"clip_table", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(clip_table)), METH_FASTCALL,
+     "Fill the table of a clip by the global norm from lists of tensors."},
     {"snapshot", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(snapshot)), METH_FASTCALL,
      "Record data pointers and dtypes of a list of tensors."},
     {"scan", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(scan)), METH_FASTCALL,

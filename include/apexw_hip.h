@@ -44,7 +44,7 @@
 extern "C" {
 #endif
 
-#define APEXW_ABI_VERSION 26
+#define APEXW_ABI_VERSION 27
 
 /* status codes */
 enum apexw_status {
@@ -827,6 +827,82 @@ int apexw_state_decode(const apexw_state_layout* s, float* m_out, float* v_out, 
  * :277-357, :381-448), round to nearest.
  */
 int apexw_state_encode(const apexw_state_layout* s, const float* m_in, const float* v_in, void* stream);
+
+/* ------------------------------------------------------------------------- */
+/* Around the step: layer norm, expert products, the clip as an operator       */
+/* ------------------------------------------------------------------------- */
+
+/*
+ * Layer norm of `rows` rows of `width` elements (dtype F32 / BF16 / F16; rows x_stride elements apart,
+ * any alignment beyond the element's):
+ *   mean = mean(x), rstd = 1 / sqrt(mean((x - mean)^2) + eps), y = (x - mean) rstd weight + bias
+ * in fp32, y rounded once.  weight / bias (w_dtype: dtype, or F32 with 16-bit rows) may be NULL (1, 0).
+ * y is contiguous; mean and rstd (one fp32 per row) are what the backward pass takes.
+ */
+int apexw_layer_norm_forward(const void* x, int64_t rows, int64_t width, int64_t x_stride, int32_t dtype,
+                             const void* weight, const void* bias, int32_t w_dtype, float eps, void* y,
+                             float* mean, float* rstd, void* stream);
+
+/*
+ * Its backward pass: with xh = (x - mean) rstd and g = dy weight,
+ *   dx = rstd (g - mean(g) - xh mean(g xh)),  dw = sum over rows of dy xh,  db = sum over rows of dy
+ * dx (dtype, contiguous), dw and db (w_dtype) may be NULL.  workspace: apexw_layer_norm_workspace floats
+ * (needed for dw or db).  The sums over rows are taken in a fixed order: equal calls give equal bits.
+ */
+int64_t apexw_layer_norm_workspace(int64_t rows, int64_t width);   /* < 0: minus an apexw_status */
+int apexw_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const float* mean,
+                              const float* rstd, const void* weight, int64_t rows, int64_t width, int32_t dtype,
+                              int32_t w_dtype, void* dx, void* dw, void* db, float* workspace, void* stream);
+
+/*
+ * Products grouped by expert.  The rows of a buffer are sorted by expert; ends[e] (device memory) is one
+ * past expert e's last row, expert 0's first row is row 0.  Ends below an earlier one or past `rows` count
+ * as clamped to them.  Operands are BF16 or F16, sums fp32, outputs rounded once.
+ *
+ * apexw_expert_rows: out[i] (n elements) = W_e a[i] (k elements) for the rows i of expert e; rows behind the
+ *   last end are set to 0.  Weights: APEXW_EXPERT_NK: W_e[j][l] at w + e w_expert_stride + j w_row_stride + l,
+ *   APEXW_EXPERT_KN: at .. + l w_row_stride + j (the rows' gradient of NK weights, and the other way round).
+ * apexw_expert_weight_grad: dw[e] ([n x k], contiguous, dtype or F32) = sum over e's rows of dy[i] x[i]^T, 0
+ *   for an expert without rows; rows behind the last end are not read.
+ * Strides are in elements.  APEXW_ERR_SIZE: more tiles than a launch holds.
+ */
+#define APEXW_EXPERT_NK 0
+#define APEXW_EXPERT_KN 1
+int apexw_expert_rows(const void* a, int64_t lda, const void* w, int64_t w_row_stride, int64_t w_expert_stride,
+                      int32_t w_order, const int32_t* ends, int32_t experts, int64_t rows, int64_t k, int64_t n,
+                      int32_t dtype, void* out, int64_t ldo, void* stream);
+int apexw_expert_weight_grad(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, const int32_t* ends,
+                             int32_t experts, int64_t rows, int64_t n, int64_t k, int32_t dtype, void* dw,
+                             int32_t dw_dtype, void* stream);
+
+/*
+ * The clip of a list of gradients by their global norm, with torch.nn.utils.clip_grad_norm_'s arithmetic:
+ *   norm = (sum |g|^p)^(1/p),  c = min(max_norm / (norm + 1e-6), 1),  out = round(c g)
+ * for p = 1, 2 (order 1, 2) or infinity (order 0); a NaN makes norm and outputs NaN.  (The optimizer's own
+ * clip, apexw_grad_clip_coef, leaves a coefficient for the step and sanitizes; this one writes the grads.)
+ * Each entry of the table reads n elements at g and writes them at out (another buffer, also of another
+ * dtype, or g itself, which is left alone where c is 1), element by element in memory order.
+ * apexw_clip_layout checks a HOST table, fills in first_unit and returns the number of work units (or minus
+ * an apexw_status); the calls take its device copy.  workspace: APEXW_CLIP_PARTIALS doubles, in any state.
+ * apexw_grad_norm and apexw_grad_scale are the two halves, for a norm over more than one process's grads.
+ */
+#define APEXW_CLIP_UNIT 8192
+#define APEXW_CLIP_PARTIALS 2048
+typedef struct apexw_clip_tensor {
+  const void* g;
+  void* out;
+  int64_t n;
+  int64_t first_unit;
+  uint32_t g_dtype;
+  uint32_t out_dtype;
+} apexw_clip_tensor;   /* 40 bytes */
+int64_t apexw_clip_layout(apexw_clip_tensor* tensors, int32_t n_tensors);
+int apexw_grad_norm(const apexw_clip_tensor* tensors, int32_t n_tensors, int64_t n_units, int32_t order,
+                    double* workspace, float* norm, void* stream);
+int apexw_grad_scale(const apexw_clip_tensor* tensors, int32_t n_tensors, int64_t n_units, const float* norm,
+                     float max_norm, void* stream);
+int apexw_clip_grads(const apexw_clip_tensor* tensors, int32_t n_tensors, int64_t n_units, int32_t order,
+                     float max_norm, double* workspace, float* norm, void* stream);
 
 #ifdef __cplusplus
 }
