@@ -110,6 +110,8 @@ bool hp_ok(const apexw_hparams* hp) {
 
 }  // namespace
 
+int apexw_cu_count() { return cu_count(); }
+
 int apexw_resident_grid(const void* kernel, int64_t n_units) {
   const int64_t want = (n_units + 3) / 4;
   // 16 workgroups per resident slot: workgroups queue behind the resident ones,

@@ -5,18 +5,20 @@
 //   weight grad:   dW_e = sum over e's rows of dy_i x_i^T
 // 16-bit operands, products on the matrix cores, fp32 accumulation, one rounding at the end.
 //
-// The number of rows of an expert is known on the device alone.  A launch has as many workgroups as tiles
-// could exist (an expert adds at most one partly filled tile); each finds its tile from the ends, those
-// without one return.  Ends that decrease or pass the buffer count as clamped, so no access leaves it.
+// The number of rows of an expert is known on the device alone: each workgroup finds its tiles from the ends.
+// Ends that decrease or pass the buffer count as clamped, so no access leaves it.
 #include <type_traits>
 
 #include "common.h"
+
+int apexw_cu_count();
 
 namespace {
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(4))) short v4i16;
 
 constexpr int kTile = 128, kBK = 32;
@@ -32,87 +34,157 @@ struct ExpertArgs {
   int32_t experts, n, k;      // out [rows x n] over k, or [experts x n x k]
 };
 
-struct Group {
-  int expert;                 // the number of experts: rows that belong to none; -1: no tile
-  int64_t first, last, tile;  // its rows, and which of its tiles
-};
-
-APEXW_DEV int64_t wave_prefix_max(int64_t x) {
+APEXW_DEV int wave_prefix_max(int x) {
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
-    const int64_t y = __shfl_up(x, off, 64);
+    const int y = __shfl_up(x, off, 64);
     if (lane_id() >= off && y > x) x = y;
   }
   return x;
 }
-APEXW_DEV int64_t wave_prefix_sum(int64_t x) {
+APEXW_DEV int wave_prefix_sum(int x) {
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
-    const int64_t y = __shfl_up(x, off, 64);
+    const int y = __shfl_up(x, off, 64);
     if (lane_id() >= off) x += y;
   }
   return x;
 }
+APEXW_DEV int lane_of(int x, int l) { return __builtin_amdgcn_readlane(x, l); }
 
-// One wave's look at 64 groups from e0 on: lane l gets the rows [begin, end) of group e0 + l and the row tiles
-// of `size` rows up to and with it; row, tiles: the end of the groups before e0, and their tiles.
-APEXW_DEV void look(const ExpertArgs& g, int e0, int size, int64_t& row, int64_t& tiles, int64_t& begin, int64_t& end,
-                    int64_t& mine, int64_t& upto) {
-  const int e = e0 + lane_id();
-  end = e < g.experts ? (int64_t)g.ends[e] : g.rows;
-  end = end > g.rows ? g.rows : end < row ? row : end;
-  end = wave_prefix_max(end);
+// The rows [begin, end) of 64 experts from e0 on, a lane each (behind the last one: no rows); row: the end of
+// the ones before, then of these
+APEXW_DEV void look(const ExpertArgs& g, int e0, int& row, int& begin, int& end) {
+  const int e = e0 + lane_id(), most = (int)g.rows;
+  end = e < g.experts ? g.ends[e] : row;
+  end = wave_prefix_max(end > most ? most : end < row ? row : end);
   begin = __shfl_up(end, 1, 64);
   if (lane_id() == 0) begin = row;
-  mine = e <= g.experts ? (end - begin + size - 1) / size : 0;
-  upto = tiles + wave_prefix_sum(mine);
-  row = __shfl(end, 63, 64);
-  tiles = __shfl(upto, 63, 64);
+  row = lane_of(end, 63);
 }
 
-// The workgroup's group (an expert, or the rows behind the last end) and tile of it, of `cols` tiles to a row
-// of tiles.  Workgroups go to the 8 XCDs in turn: each XCD gets a contiguous part of the tiles, so that
-// those that share rows and weights share its L2.
-APEXW_DEV Group find_group(const ExpertArgs& g, int size, int cols) {
-  int64_t row = 0, tiles = 0, begin, end, mine, upto;
-  look(g, 0, size, row, tiles, begin, end, mine, upto);
-  for (int e0 = 64; e0 <= g.experts; e0 += 64) look(g, e0, size, row, tiles, begin, end, mine, upto);
-  const int64_t all = tiles * cols, part = (all + 7) / 8, in = blockIdx.x / 8, t = (blockIdx.x % 8) * part + in;
-  if (in >= part || t >= all) return {-1, 0, 0, 0};
-  if (g.experts >= 64) row = tiles = 0;
-  for (int e0 = 0; e0 <= g.experts; e0 += 64) {
-    if (g.experts >= 64) look(g, e0, size, row, tiles, begin, end, mine, upto);
-    const uint64_t hit = __ballot(t < upto * cols);
-    if (hit) {
-      const int l = __builtin_ctzll(hit);
-      return {e0 + l, __shfl(begin, l, 64), __shfl(end, l, 64), t - __shfl(upto - mine, l, 64) * cols};
-    }
-  }
-  return {-1, 0, 0, 0};
-}
+struct Job {
+  int expert;          // -1: none
+  int first, last;     // its rows
+  int row, col;        // the tile's first row among its rows; its place across, in tiles
+};
 
-// Tile (row, column) of index t among rows x cols tiles: bands of 8 tile rows, column by column
-APEXW_DEV void place(int64_t t, int64_t rows, int cols, int64_t& r, int64_t& c) {
-  const int64_t band = t / (8 * cols), in = t - band * 8 * cols;
-  const int64_t high = rows - band * 8 < 8 ? rows - band * 8 : 8;
+// Tile (row, column) of index t among rows x cols tiles: bands of 8 tile rows, column by column, so that the
+// tiles that run at a time share both operands' lines in L2
+APEXW_DEV void place(int t, int rows, int cols, int& r, int& c) {
+  const int band = t / (8 * cols), in = t - band * 8 * cols;
+  const int high = rows - band * 8 < 8 ? rows - band * 8 : 8;
   c = in / high;
   r = band * 8 + in - c * high;
 }
 
-// the rows of expert e
-APEXW_DEV void expert_rows(const ExpertArgs& g, int e, int64_t& first, int64_t& last) {
-  first = last = 0;
-  for (int e0 = 0; e0 <= e; e0 += 64) {
-    const int i = e0 + lane_id();
-    int64_t x = i <= e ? (int64_t)g.ends[i] : 0, y = i < e ? x : 0;
-    x = x > g.rows ? g.rows : x < 0 ? 0 : x;
-    y = y > g.rows ? g.rows : y < 0 ? 0 : y;
-    x = __shfl(wave_prefix_max(x), 63, 64);
-    y = __shfl(wave_prefix_max(y), 63, 64);
-    first = y > first ? y : first;
-    last = x > last ? x : last;
+// The tiles of a rows product, expert by expert.  Workgroups go to the 8 XCDs in turn: each XCD gets a
+// contiguous part of the tiles, of which its workgroups take every (number of them)th.
+template <bool kSplit> struct RowJobs {
+  const ExpertArgs& g;
+  int size, cols;              // rows of a tile, tiles across
+  int begin, end, upto;        // per lane, of the first 64 experts: rows, and tiles up to and with it
+  int all, rows;               // tiles, and rows that belong to experts
+
+  __device__ __forceinline__ RowJobs(const ExpertArgs& a, int bm, int bn)
+      : g(a), size(bm), cols((a.n + bn - 1) / bn), all(0), rows(0) {
+    for (int e0 = 0; e0 < g.experts; e0 += 64) step(e0);
   }
-}
+  __device__ __forceinline__ void step(int e0) {
+    look(g, e0, rows, begin, end);
+    upto = all + wave_prefix_sum((end - begin + size - 1) / size * cols);
+    all = lane_of(upto, 63);
+  }
+  __device__ __forceinline__ int find_at(int t, int e0, Job& j) const {
+    const uint64_t hit = __ballot(t < upto);
+    if (!hit) return 0;
+    const int l = __builtin_ctzll(hit);
+    j.expert = e0 + l, j.first = lane_of(begin, l), j.last = lane_of(end, l);
+    const int high = (j.last - j.first + size - 1) / size;
+    place(t - (lane_of(upto, l) - high * cols), high, cols, j.row, j.col);
+    j.row *= size;
+    return 1;
+  }
+  // the i-th tile of this workgroup.  Round i's tiles go to the XCD's workgroups in turn from another one on
+  // each time, since a tile of few rows takes less time and stands at the same place of every column; where
+  // the last round has tiles for less than half or a quarter of them, it takes halves or quarters of tiles.
+  __device__ __forceinline__ Job get(int i) {
+    Job j{-1, 0, 0, 0, 0};
+    const int part = (all + 7) / 8, from = (int)(blockIdx.x % 8) * part, groups = (int)(gridDim.x / 8);
+    const int mine = all - from < part ? all - from : part;
+    int in = i * groups + (int)((blockIdx.x / 8 + 5u * i) % groups), sub = 0, cut = 1;
+    const int rest = mine - i * groups;
+    if (kSplit && rest > 0 && 2 * rest <= groups) {
+      cut = 4 * rest <= groups ? 4 : 2;
+      sub = (in - i * groups) % cut, in = i * groups + (in - i * groups) / cut;
+    }
+    if (in >= mine) return j;
+    const int t = from + in;
+    if (g.experts <= 64) {
+      find_at(t, 0, j);
+    } else {
+      const int keep_all = all, keep_rows = rows;
+      all = rows = 0;
+      for (int e0 = 0; e0 < g.experts; e0 += 64) {
+        step(e0);
+        if (find_at(t, e0, j)) break;
+      }
+      all = keep_all, rows = keep_rows;
+    }
+    if (cut > 1) {
+      const int end = j.first + j.row + (sub + 1) * (size / cut);
+      j.row += sub * (size / cut);
+      j.last = j.last < end ? j.last : end;
+      if (j.first + j.row >= j.last) j.last = j.first;   // no rows in this part: nothing to do
+    }
+    return j;
+  }
+};
+
+// The tiles of a weight gradient.  Experts differ in rows, and so their tiles in work: each XCD takes a part of
+// every expert's tiles, and up to 64 experts come in the order of their rows, the most first, so that the
+// last tiles are short.
+struct WeightJobs {
+  const ExpertArgs& g;
+  int size, high, cols, part;
+  int begin, end, rank;        // per lane, of the first 64 experts
+  int next_rank;               // experts that have rows
+
+  __device__ __forceinline__ WeightJobs(const ExpertArgs& a, int bm, int bn)
+      : g(a), size(bm), high((a.n + bm - 1) / bm), cols((a.k + bn - 1) / bn) {
+    part = (high * cols + 7) / 8;
+    int row = 0;
+    look(g, 0, row, begin, end);
+    rank = 0;
+    for (int l = 0; l < 64; ++l) {
+      const int n = lane_of(end - begin, l);
+      rank += n > end - begin || (n == end - begin && l < lane_id());
+    }
+    next_rank = __builtin_popcountll(__ballot(end > begin));
+  }
+  __device__ __forceinline__ Job get(int i) const {
+    Job j{-1, 0, 0, 0, 0};
+    // forth and back, so that the first workgroups do not get the most rows in every round
+    const int groups = (int)(gridDim.x / 8), w = (int)(blockIdx.x / 8), in = i * groups + (i & 1 ? groups - 1 - w : w);
+    const int t = (int)(blockIdx.x % 8) * part + in % part;
+    int e = in / part;
+    if (g.experts <= 64) {
+      if (e >= next_rank) return j;
+      e = __builtin_ctzll(__ballot(rank == e));
+      j.first = lane_of(begin, e), j.last = lane_of(end, e);
+    } else {
+      if (e >= g.experts) return j;
+      int row = 0, b, n;
+      for (int e0 = 0; e0 <= e; e0 += 64) look(g, e0, row, b, n);
+      j.first = lane_of(b, e & 63), j.last = lane_of(n, e & 63);
+    }
+    j.expert = e;
+    if (t >= high * cols) j.last = j.first;   // no tile here: nothing to do
+    else place(t, high, cols, j.row, j.col);
+    j.row *= size;
+    return j;
+  }
+};
 
 struct __attribute__((packed, aligned(2))) Chunk { u32x4 v; };
 
@@ -178,10 +250,42 @@ template <int DT> APEXW_DEV f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
+template <int DT> APEXW_DEV f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (DT == APEXW_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
 template <int OD> APEXW_DEV void store_elem(void* base, int64_t i, float x) {
   if constexpr (OD == APEXW_F32) APEXW_GLOBAL(float, base)[i] = x;
   else if constexpr (OD == APEXW_BF16) APEXW_GLOBAL(uint16_t, base)[i] = (uint16_t)f32_to_bf16_bits(x);
   else APEXW_GLOBAL(uint16_t, base)[i] = (uint16_t)f32_to_f16_bits(x);
+}
+
+// zeros in the rows from `row` on, which belong to no expert
+template <bool kVec> APEXW_DEV void zero_rows(const ExpertArgs& g, int row) {
+  constexpr int V = kVec ? 8 : 1;
+  const int64_t per = g.n / V, n = (g.rows - row) * per, step = (int64_t)gridDim.x * blockDim.x;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += step) {
+    uint16_t* p = (uint16_t*)g.out + (row + i / per) * g.ldo + i % per * V;
+    if constexpr (kVec) *APEXW_GLOBAL(u32x4, p) = u32x4{0u, 0u, 0u, 0u};
+    else *APEXW_GLOBAL(uint16_t, p) = 0;
+  }
+}
+
+// zeros in the gradients of the experts without rows
+template <int OD> APEXW_DEV void zero_weights(const ExpertArgs& g) {
+  const int64_t per = (int64_t)g.n * g.k, step = (int64_t)gridDim.x * blockDim.x;
+  int row = 0, begin, end;
+  for (int e0 = 0; e0 < g.experts; e0 += 64) {
+    look(g, e0, row, begin, end);
+    uint64_t none = __ballot(begin == end && e0 + lane_id() < g.experts);
+    for (; none; none &= none - 1) {
+      const int64_t at = (e0 + __builtin_ctzll(none)) * per;
+      for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < per; i += step) store_elem<OD>(g.out, at + i, 0.0f);
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -195,6 +299,7 @@ template <int OD> APEXW_DEV void store_elem(void* base, int64_t i, float x) {
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 APEXW_DEV void lds_copy16(uint32_t lds_base, uint32_t voff, u32x4 buffer) {
+  lds_base = uniform(lds_base);
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :
                : "s"(lds_base), "v"(voff), "s"(buffer)
@@ -215,286 +320,316 @@ APEXW_DEV void barrier() {
 constexpr int kDepth = 64;              // k of a stage: a row's 128 bytes, one cache line
 constexpr uint32_t kNowhere = 0xFFFFFFF0u;   // a buffer offset past every end
 
-// One operand of a tile: `kSize` of its rows (or, kKN, columns) over the k of a stage.
+APEXW_DEV uint64_t uniform64(uint64_t x) { return (uint64_t)uniform((uint32_t)(x >> 32)) << 32 | uniform((uint32_t)x); }
+
+// The memory of one operand of a tile: its origin (row or column 0, k 0), the bytes from there to its end, its
+// stages and the k of the last one
+struct Span {
+  const uint16_t* base;
+  int64_t left;
+  int stages, tail;
+  __device__ __forceinline__ void fix() {   // into scalar registers
+    base = (const uint16_t*)uniform64((uint64_t)base), left = (int64_t)uniform64((uint64_t)left);
+    stages = uniform(stages), tail = uniform(tail);
+  }
+  // rows: rows (columns) from the origin on; depth: k; ld: elements from row to row (k row to k row)
+  template <bool kKN> __device__ __forceinline__ void set(const uint16_t* p, int64_t ld, int64_t rows, int depth, int size) {
+    base = p;
+    left = kKN ? ((depth - 1) * ld + rows) * 2 : (((rows < size ? rows : size) - 1) * ld + depth) * 2;
+    stages = (depth + kDepth - 1) / kDepth;
+    tail = (depth - 1) % kDepth + 1;
+  }
+};
+
+// How one operand of a tile gets into LDS and out: kSize of its rows (or, kKN, columns) over the k of a stage.
 //   k-contiguous: LDS [kSize rows][64 k]; the 8 chunks of row r are swapped by XOR with (r / 2) % 8, so that the
 //     fragment reads of 16 consecutive rows touch every bank once
-//   kKN: LDS [64 k][kSize columns]; the chunks of k row r are swapped by XOR with 4 (r % 4), so that the
-//     transposing reads of 4 consecutive k rows do
+//   kKN: LDS [64 k][kSize columns]; the chunks of k row r are swapped by XOR with 4 (r % 4) + 2 (r / 8 % 2), so
+//     that the transposing reads of rows r .. r + 3 and r + 8 .. r + 11 do
 template <bool kKN, int kSize, int kWaves> struct Operand {
   static constexpr int kElems = kSize * kDepth;            // of a stage
-  static constexpr int kCopies = kSize / 8 / kWaves;       // 1 KB each
-  const uint16_t* base;
-  int64_t step, left;     // bytes from stage to stage, and from the base to the operand's end
+  static constexpr int kCopies = kSize / 8 / kWaves;       // of a wave and stage, 1 KB each
+  int64_t step;           // bytes from stage to stage
   uint32_t voff[kCopies]; // per lane
   uint32_t lds0;          // of this wave's first copy in stage 0
-  int tail;               // k-contiguous: k of the last stage that this lane's chunks must stay below
 
-  // base: row (column) 0, k 0; ld: elements from row to row (k row to k row); rows: rows (columns) that
-  // exist; depth: k that exist; width: elements of a memory row from the base on (kKN: columns that exist)
-  __device__ __forceinline__ void init(const uint16_t* p, int64_t ld, int64_t rows, int64_t depth, const uint16_t* lds) {
+  __device__ __forceinline__ void init(int64_t ld, const uint16_t* lds) {
     const int lane = lane_id(), wave = threadIdx.x >> 6;
-    base = p;
     step = (kKN ? (int64_t)kDepth * ld : kDepth) * 2;
-    left = kKN ? ((depth - 1) * ld + rows) * 2 : (((rows < kSize ? rows : kSize) - 1) * ld + depth) * 2;
-    tail = (int)((depth - 1) % kDepth) + 1;
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) {
       const int q = wave * kCopies + i;
       if constexpr (kKN) {
         constexpr int kChunks = kSize / 8;
-        const int k = q * (64 / kChunks) + lane / kChunks, chunk = (lane % kChunks) ^ (4 * (k & 3));
+        const int k = q * (64 / kChunks) + lane / kChunks, chunk = (lane % kChunks) ^ swap(k);
         voff[i] = (uint32_t)(k * ld + chunk * 8) * 2u;
       } else {
-        const int row = q * 8 + (lane >> 3);
-        voff[i] = (uint32_t)(row * ld + chunk_of(i) * 8) * 2u;
+        voff[i] = (uint32_t)((q * 8 + (lane >> 3)) * ld + chunk_of(i) * 8) * 2u;
       }
     }
-    lds0 = __builtin_amdgcn_readfirstlane(
-        (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)(lds + wave * kCopies * 512));
+    lds0 = uniform((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)(lds + wave * kCopies * 512));
   }
   __device__ __forceinline__ int chunk_of(int i) const {   // k-contiguous: the chunk that this lane's copy i brings
     const int lane = lane_id(), q = (threadIdx.x >> 6) * kCopies + i;
     return (lane & 7) ^ ((4 * (q & 1) + (lane >> 4)) & 7);
   }
-  __device__ __forceinline__ u32x4 buffer(int h) const {
-    const uint64_t at = (uint64_t)base + (uint64_t)(h * step);
-    int64_t n = left - h * step;
+  __device__ __forceinline__ u32x4 buffer(const Span& m, int h) const {
+    const uint64_t at = (uint64_t)m.base + (uint64_t)(h * step);
+    int64_t n = m.left - h * step;
     n = n < 0 ? 0 : n > 0xFFFFFF00ll ? 0xFFFFFF00ll : n;
     return u32x4{uniform((uint32_t)at), uniform((uint32_t)(at >> 32)), uniform((uint32_t)n), 0x00020000u};
   }
-  // copy i of a stage into the buffer at LDS byte `to`; last: the stage where k may end
-  __device__ __forceinline__ void copy(u32x4 b, int i, uint32_t to, bool last) const {
+  // copy i of a stage into the buffer at LDS byte `to`; tail: the k that exist in this stage
+  __device__ __forceinline__ void copy(u32x4 b, int i, uint32_t to, int tail) const {
     uint32_t v = voff[i];
-    if constexpr (!kKN) v = last && chunk_of(i) * 8 >= tail ? kNowhere : v;
+    if constexpr (!kKN) v = chunk_of(i) * 8 >= tail ? kNowhere : v;
     lds_copy16(lds0 + to + i * 1024, v, b);
   }
-  // the fragment of 32 rows (columns) from `row` at k step s
+  static __device__ __forceinline__ int swap(int k) { return 4 * (k & 3) + 2 * (k >> 3 & 1); }
+  // the fragment of 16 rows (columns) from `row` at step s of 32 k: lane l has row l % 16, k = 8 (l / 16) .. + 7.
+  // From [k][column] by two transposing reads: in each 16 lanes, lane 4 r + c gets element c of the 8-byte rows
+  // that lanes r, r + 4, r + 8, r + 12 address.
   static __device__ __forceinline__ u32x4 frag(const uint16_t* lds, int row, int s) {
     const int lane = lane_id();
     if constexpr (kKN) {
-      const int g = lane >> 4, r = lane & 3, jr = (lane >> 2) & 3;
-      const int n = row + 16 * (g & 1) + 4 * r, k = 16 * s + 8 * (g >> 1) + jr;
-      const int e = k * kSize + (((n >> 3) ^ (4 * jr)) << 3) + (n & 7);
+      const int r = lane & 3, k = 32 * s + 8 * (lane >> 4) + (lane >> 2 & 3), n = row + 4 * r;
+      const int e = k * kSize + (((n >> 3) ^ swap(k)) << 3) + (n & 7);
       const v4i16 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4i16*)&lds[e]);
       const v4i16 hi =
           __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4i16*)&lds[e + 4 * kSize]);
       const u32x2 wl = __builtin_bit_cast(u32x2, lo), wh = __builtin_bit_cast(u32x2, hi);
       return u32x4{wl[0], wl[1], wh[0], wh[1]};
     } else {
-      const int r = row + (lane & 31), c = (2 * s + (lane >> 5)) ^ ((lane >> 1) & 7);   // row: a multiple of 32
+      const int r = row + (lane & 15), c = (4 * s + (lane >> 4)) ^ ((lane >> 1) & 7);   // row: a multiple of 16
       return *(const u32x4*)&lds[r * kDepth + c * 8];
     }
   }
 };
 
-// A tile's shape: BM x BN by waves of WM x WN, kStages stages of 64 k in LDS
-template <int BM_, int BN_, int WM_, int WN_, int kStages_> struct Shape {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, kStages = kStages_;
+// A tile's shape: BM x BN by waves of WM x WN; LDS holds kStages stages of 64 k and 16 rows of 128 bytes of each
+// wave's output
+template <int BM_, int BN_, int WM_, int WN_, int kStages_, int kPerCU_> struct Shape {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, kStages = kStages_, kPerCU = kPerCU_;
   static constexpr int kWaves = (BM / WM) * (BN / WN), kThreads = kWaves * 64;
-  static constexpr int kStageElems = (BM + BN) * kDepth, kLds = kStages * kStageElems;
+  static constexpr int kStageElems = (BM + BN) * kDepth, kOut = 16 * 64, kLds = kStages * kStageElems + kWaves * kOut;
+  static_assert(kLds * 2 * kPerCU <= 160 * 1024, "LDS of a CU");
 };
-typedef Shape<256, 256, 128, 64, 2> Large;
-typedef Shape<128, 256, 128, 64, 3> Wide;
+typedef Shape<256, 256, 128, 64, 2, 1> Large;
+typedef Shape<128, 256, 64, 64, 3, 1> Wide;
+typedef Shape<32, 128, 32, 32, 3, 2> Small;
 
-// One tile of A B^T: `rows` x `cols` of it exist, over `depth` > 0.  In a stage's four k steps each MFMA is
-// followed by at most one fragment read of the next step and one copy, fenced in place: issued in bursts they
-// stall the wave's in-order issue.  The barrier stands before the last step, whose fragments are in registers
-// by then: behind it the stage's buffer is free for the copies of kStages stages on, and the next stage,
-// landed, gives its first fragments.
-template <class S, bool kAKN, bool kBKN, int DT, int OD>
-APEXW_DEV void fast_tile(const uint16_t* a, int64_t lda, const uint16_t* b, int64_t ldb, int64_t rows, int64_t cols,
-                         int64_t depth, void* out, int64_t out0, int64_t ldo, uint16_t* lds) {
-  constexpr int FA = S::WM / 32, FB = S::WN / 32, kFrags = FA + FB, kMM = FA * FB;
+// The tiles of a workgroup, each A B^T over its k, as one stream of stages: the copies of a tile's first
+// stages are under way while the tile before is multiplied and written out.
+//
+// A stage is two steps of 32 k by 16 x 16 x 32 MFMAs (at the power limit, which bounds large products of real
+// numbers, they reach 2160 TFLOP/s from registers where 32 x 32 x 16 ones reach 1950).  After an MFMA come at
+// most one fragment read of the next step and one copy, fenced in place: issued in bursts they stall the
+// wave's in-order issue.  The barrier stands between the steps, when the second one's fragments are in
+// registers: behind it the stage's buffer is free for the copies of the stage kStages on, and the next stage,
+// landed, gives its first fragments.  A's fragments are read into the registers of the ones just used.
+template <class S, bool kAKN, bool kBKN, int DT, int OD, bool kHalves, class Jobs, class Place>
+APEXW_DEV void stream(const ExpertArgs& g, Jobs& jobs, Place&& locate, uint16_t* lds) {
   typedef Operand<kAKN, S::BM, S::kWaves> OpA;
   typedef Operand<kBKN, S::BN, S::kWaves> OpB;
   constexpr int kCopies = OpA::kCopies + OpB::kCopies;
   constexpr uint32_t kStageBytes = S::kStageElems * 2;
-  // 16-bit results leave through LDS by rows: their blocks are computed transposed (four consecutive columns
-  // to a lane); fp32 ones leave as they are (32 lanes, 32 columns)
-  constexpr bool kSwap = OD != APEXW_F32;
-  const int lane = lane_id(), wave = threadIdx.x >> 6;
-  const int wm = wave / (S::BN / S::WN) * S::WM, wn = wave % (S::BN / S::WN) * S::WN;
+  const int wave = uniform(threadIdx.x >> 6), across = wave % (S::BN / S::WN), down = wave / (S::BN / S::WN);
+  uint16_t* mine = lds + S::kStages * S::kStageElems + wave * S::kOut;
   OpA A;
   OpB B;
-  A.init(a, lda, rows, depth, lds);
-  B.init(b, ldb, cols, depth, lds + OpA::kElems);
-  const int n = (int)((depth + kDepth - 1) / kDepth);
+  A.init(g.lda, lds);
+  B.init(g.ldb, lds + OpA::kElems);
 
-  f32x16 acc[FA][FB];
-#pragma unroll
-  for (int i = 0; i < FA; ++i)
-#pragma unroll
-    for (int j = 0; j < FB; ++j) acc[i][j] = f32x16{};
-  u32x4 fa[2][FA], fb[2][FB];
-  auto frag = [&](const uint16_t* st, int s, int i) {
-    if (i < FA) fa[s & 1][i] = OpA::frag(st, wm + 32 * i, s);
-    else fb[s & 1][i - FA] = OpB::frag(st + OpA::kElems, wn + 32 * (i - FA), s);
-  };
-  auto step = [&](int s, auto&& side) {
-#pragma unroll
-    for (int j = 0; j < kMM; ++j) {
-      const int x = j / FB, y = j % FB;
-      if constexpr (kSwap) acc[x][y] = mfma<DT>(fb[s & 1][y], fa[s & 1][x], acc[x][y]);
-      else acc[x][y] = mfma<DT>(fa[s & 1][x], fb[s & 1][y], acc[x][y]);
-      __builtin_amdgcn_sched_barrier(0);
-      side(j);
-      __builtin_amdgcn_sched_barrier(0);
+  // the tile being copied, its next stage, and how many tiles were before it
+  Span ia, ib;
+  int copying = 0, at = 0, rows, cols;
+  int64_t out0;
+  // job i that has work, from i on: its place and its operands; false: no more
+  auto take = [&](int& i, Span& a, Span& b, int& r, int& c, int64_t& o) {
+    for (;; ++i) {
+      const Job j = jobs.get(i);
+      if (j.expert < 0) return false;
+      if (j.first == j.last) continue;
+      locate(j, a, b, r, c, o);
+      r = uniform(r), c = uniform(c);
+      a.fix(), b.fix();
+      return true;
     }
   };
+  bool more = take(copying, ia, ib, rows, cols, out0);
+  if (!more) return;
+  int here = copying, n = ia.stages, buf = 0;   // the tile being multiplied, its stages, the stage's buffer
 
-  const int first = n < S::kStages ? n : S::kStages;
-  for (int h = 0; h < first; ++h) {
-    const u32x4 ba = A.buffer(h), bb = B.buffer(h);
+  auto advance = [&]() {     // past the stage whose copies were issued
+    at = uniform(at + 1);
+    if (at < ia.stages) return;
+    at = 0, ++copying;
+    int r, c;
+    int64_t o;
+    more = take(copying, ia, ib, r, c, o);
+  };
+  int ready = 0;             // stages in flight at the start
+  for (; ready < S::kStages && more; ++ready) {
+    const u32x4 ba = A.buffer(ia, at), bb = B.buffer(ib, at);
+    const int tail = at == ia.stages - 1 ? ia.tail : kDepth;
 #pragma unroll
-    for (int i = 0; i < OpA::kCopies; ++i) A.copy(ba, i, h * kStageBytes, h == n - 1);
+    for (int i = 0; i < OpA::kCopies; ++i) A.copy(ba, i, ready * kStageBytes, tail);
 #pragma unroll
-    for (int i = 0; i < OpB::kCopies; ++i) B.copy(bb, i, h * kStageBytes, h == n - 1);
+    for (int i = 0; i < OpB::kCopies; ++i) B.copy(bb, i, ready * kStageBytes, tail);
+    advance();
   }
-  if (first == S::kStages) wait_copies<kCopies*(S::kStages - 1)>();
+
+  bool full = ready == S::kStages;   // the copies of the stage kStages - 1 on are under way
+  if (full) wait_copies<kCopies*(S::kStages - 1)>();
   else wait_copies<0>();
   barrier();
-#pragma unroll
-  for (int i = 0; i < kFrags; ++i) frag(lds, 0, i);
 
-  // kRefill: stage h + kStages exists; kNext: stage h + 1 does
-  auto stage = [&](int h, int buf, auto refill_c, auto next_c) {
-    constexpr bool kRefill = decltype(refill_c)::value, kNext = decltype(next_c)::value;
-    const uint16_t* st = lds + buf * S::kStageElems;
-    const int next = buf + 1 == S::kStages ? 0 : buf + 1;
+  constexpr int kStores = S::WM / 16 * (S::WN * (OD == APEXW_F32 ? 4 : 2) / 64);   // of a wave and whole tile
+  bool fresh = false;                // such a tile was written since the last stage
+  // a tile of up to kHigh rows: its waves take kWM rows each
+  auto tile = [&](auto high_c) {
+    constexpr int kHigh = decltype(high_c)::value, kWM = kHigh / (S::BM / S::WM);
+    constexpr int FA = kWM / 16, FB = S::WN / 16, kMM = FA * FB;
+    const int wm = down * kWM, wn = across * S::WN;
+    f32x4 acc[FA][FB];
 #pragma unroll
-    for (int s = 0; s < 3; ++s)
-      step(s, [&](int j) {
-        if (j < kFrags) frag(st, s + 1, j);
+    for (int i = 0; i < FA; ++i)
+#pragma unroll
+      for (int j = 0; j < FB; ++j) acc[i][j] = f32x4{};
+    u32x4 fa[FA], fb[2][FB];
+    auto frag_a = [&](const uint16_t* st, int s, int i) { fa[i] = OpA::frag(st, wm + 16 * i, s); };
+    auto frag_b = [&](const uint16_t* st, int s, int i) { fb[s][i] = OpB::frag(st + OpA::kElems, wn + 16 * i, s); };
+#pragma unroll
+    for (int i = 0; i < FA; ++i) frag_a(lds + buf * S::kStageElems, 0, i);
+#pragma unroll
+    for (int i = 0; i < FB; ++i) frag_b(lds + buf * S::kStageElems, 0, i);
+    // step s; blocks are computed transposed: a lane has four consecutive columns of a row.  Step s1 of the stage
+    // at st1 is next; side: what else is issued
+    auto step = [&](int s, const uint16_t* st1, int s1, auto&& side) {
+#pragma unroll
+      for (int j = 0; j < kMM; ++j) {
+        const int x = j / FB, y = j % FB;
+        acc[x][y] = mfma16<DT>(fb[s][y], fa[x], acc[x][y]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (j < FB) frag_b(st1, s1, j);
+        if (y == FB - 1) frag_a(st1, s1, x);
+        side(j);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    for (int h = 0; h < n; ++h) {
+      const uint16_t* st = lds + buf * S::kStageElems;
+      const int after = uniform(buf + 1 == S::kStages ? 0 : buf + 1);
+      step(0, st, 1, [](int) {});
+      // the next stage has landed; those after it may be on their way, and behind them the stores of the tile
+      // before (memory operations are counted off in their order)
+      if (fresh) {
+        if (full) wait_copies<kCopies*(S::kStages - 2) + kStores>();
+        else wait_copies<kStores>();
+        fresh = false;
+      } else {
+        if (full) wait_copies<kCopies*(S::kStages - 2)>();
+        else wait_copies<0>();
+      }
+      barrier();
+      const bool refill = more;
+      const u32x4 ba = A.buffer(ia, at), bb = B.buffer(ib, at);   // (of no use without a stage to copy)
+      const int tail = at == ia.stages - 1 ? ia.tail : kDepth;
+      // (the last stage's reads of the next fragments are of no use)
+      step(1, lds + after * S::kStageElems, 0, [&](int j) {
+        if (refill) {
+#pragma unroll
+          for (int i = 0; i < kCopies; ++i)
+            if ((kMM >= 2 * kCopies ? 2 * i + 1 : i * kMM / kCopies) == j) {
+              if (i < OpA::kCopies) A.copy(ba, i, buf * kStageBytes, tail);
+              else B.copy(bb, i - OpA::kCopies, buf * kStageBytes, tail);
+            }
+        }
       });
-    // stage h + 1 has landed; those after it may be on their way
-    if constexpr (kRefill) wait_copies<kCopies*(S::kStages - 2)>();
-    else wait_copies<0>();
-    barrier();
-    u32x4 ba{}, bb{};
-    bool last = false;
-    if constexpr (kRefill) {
-      ba = A.buffer(h + S::kStages);
-      bb = B.buffer(h + S::kStages);
-      last = h + S::kStages == n - 1;
+      if (refill) advance();
+      full = refill;
+      buf = after;
     }
-    step(3, [&](int j) {
-      if constexpr (kNext) {
-        if (j < kFrags) frag(lds + next * S::kStageElems, 0, j);
-      }
-      if constexpr (kRefill) {
+    // Write the tile out: lane l has row l % 16, columns 4 (l / 16) .. + 3 of a block.  Each wave puts 16 rows of
+    // 128 bytes into LDS of its own, chunks swapped by XOR with the row, and writes them out in whole lines.
+    // (Addresses are formed here, not kept in registers over the stages.)
+    int lane = lane_id();
+    asm volatile("" : "+v"(lane));
+    constexpr int kBlocks = OD == APEXW_F32 ? 2 : FB < 4 ? FB : 4, kPer = OD == APEXW_F32 ? 4 : 8;
+    constexpr int kChunks = kBlocks * 16 / kPer, kRows = 64 / kChunks;   // of a staged row; rows of a store
+    const int r0 = lane & 15, c0 = lane >> 4;
 #pragma unroll
-        for (int i = j * kCopies / kMM; i < (j + 1) * kCopies / kMM; ++i) {
-          if (i < OpA::kCopies) A.copy(ba, i, buf * kStageBytes, last);
-          else B.copy(bb, i - OpA::kCopies, buf * kStageBytes, last);
+    for (int i = 0; i < FA; ++i)
+#pragma unroll
+      for (int j0 = 0; j0 < FB; j0 += kBlocks) {
+#pragma unroll
+        for (int j = 0; j < kBlocks; ++j) {
+          const f32x4 v = acc[i][j0 + j];
+          if constexpr (OD == APEXW_F32) {
+            *(u32x4*)&mine[(r0 * kChunks + ((4 * j + c0) ^ (r0 & (kChunks - 1)))) * 8] =
+                u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+          } else {
+            u32x2 w;
+            if constexpr (OD == APEXW_BF16) w = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+            else
+              w = u32x2{f32_to_f16_bits(v[0]) | (f32_to_f16_bits(v[1]) << 16),
+                        f32_to_f16_bits(v[2]) | (f32_to_f16_bits(v[3]) << 16)};
+            *(u32x2*)&mine[(r0 * kChunks + ((2 * j + (c0 >> 1)) ^ (r0 & (kChunks - 1)))) * 8 + 4 * (c0 & 1)] = w;
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < 16 / kRows; ++t) {
+          const int r = kRows * t + lane / kChunks, c = lane % kChunks;
+          const u32x4 w = *(const u32x4*)&mine[(r * kChunks + (c ^ (r & (kChunks - 1)))) * 8];
+          const int row = wm + 16 * i + r, col = wn + 16 * j0 + kPer * c;
+          if (row < rows && col < cols) {
+            if constexpr (OD == APEXW_F32) *APEXW_GLOBAL(u32x4, (float*)g.out + out0 + row * g.ldo + col) = w;
+            else *APEXW_GLOBAL(u32x4, (uint16_t*)g.out + out0 + row * g.ldo + col) = w;
+          }
         }
       }
-    });
+    fresh = kHigh == S::BM && rows >= S::BM && cols >= S::BN;
   };
-  typedef std::integral_constant<bool, true> yes;
-  typedef std::integral_constant<bool, false> no;
-  int h = 0, buf = 0;
-  for (; h + S::kStages < n; ++h) {
-    stage(h, buf, yes(), yes());
-    buf = buf + 1 == S::kStages ? 0 : buf + 1;
-  }
-  for (; h + 1 < n; ++h) {
-    stage(h, buf, no(), yes());
-    buf = buf + 1 == S::kStages ? 0 : buf + 1;
-  }
-  stage(h, buf, no(), no());
 
-  if constexpr (kSwap) {
-    // lane l has row l % 32, columns 8 (q / 4) + 4 (l / 32) + q % 4 of a block.  Each wave puts its block into
-    // LDS of its own (the operands there are dead behind the last barrier) in rows of WN, chunks swapped by
-    // XOR with the row, and writes it out in whole lines.
-    static_assert(S::WN == 64, "rows of 8 chunks");
-    uint16_t* mine = lds + wave * S::WM * S::WN;
-#pragma unroll
-    for (int i = 0; i < FA; ++i)
-#pragma unroll
-      for (int j = 0; j < FB; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int r = 32 * i + (lane & 31), c = 4 * j + q;
-          const f32x16& v = acc[i][j];
-          u32x2 w;
-          if constexpr (OD == APEXW_BF16)
-            w = u32x2{pack_bf16x2(v[4 * q], v[4 * q + 1]), pack_bf16x2(v[4 * q + 2], v[4 * q + 3])};
-          else
-            w = u32x2{f32_to_f16_bits(v[4 * q]) | (f32_to_f16_bits(v[4 * q + 1]) << 16),
-                      f32_to_f16_bits(v[4 * q + 2]) | (f32_to_f16_bits(v[4 * q + 3]) << 16)};
-          *(u32x2*)&mine[r * 64 + ((c ^ (r & 7)) << 3) + 4 * (lane >> 5)] = w;
-        }
-#pragma unroll 4
-    for (int i = 0; i < S::WM / 8; ++i) {
-      const int r = 8 * i + (lane >> 3), c = lane & 7;
-      const u32x4 w = *(const u32x4*)&mine[r * 64 + ((c ^ (r & 7)) << 3)];
-      if (wm + r < rows && wn + 8 * c < cols)
-        *APEXW_GLOBAL(u32x4, (uint16_t*)out + out0 + (wm + r) * ldo + wn + 8 * c) = w;
+  for (;;) {
+    if constexpr (kHalves) {
+      if (rows <= S::BM / 4 && S::WM >= 64) tile(std::integral_constant<int, (S::WM >= 64 ? S::BM / 4 : S::BM)>());
+      else if (rows <= S::BM / 2) tile(std::integral_constant<int, S::BM / 2>());
+      else tile(std::integral_constant<int, S::BM>());
+    } else {
+      tile(std::integral_constant<int, S::BM>());
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < FA; ++i)
-#pragma unroll
-      for (int j = 0; j < FB; ++j)
-#pragma unroll
-        for (int q = 0; q < 16; ++q) {
-          const int r = wm + 32 * i + 8 * (q >> 2) + 4 * (lane >> 5) + (q & 3), c = wn + 32 * j + (lane & 31);
-          if (r < rows && c < cols) APEXW_GLOBAL(float, out)[out0 + r * ldo + c] = acc[i][j][q];
-        }
-  }
-}
-
-// Zeros for rows that belong to no expert
-template <class S> APEXW_DEV void zero_tile(void* out, int64_t out0, int64_t ldo, int64_t rows, int64_t cols) {
-  for (int c = threadIdx.x; c < S::BM * S::BN / 8; c += S::kThreads) {
-    const int r = c / (S::BN / 8), e = c % (S::BN / 8) * 8;
-    if (r < rows && e < cols) *APEXW_GLOBAL(u32x4, (uint16_t*)out + out0 + r * ldo + e) = u32x4{0u, 0u, 0u, 0u};
+    Span a, b;
+    ++here;
+    if (!take(here, a, b, rows, cols, out0)) return;
+    n = a.stages;
   }
 }
 
 template <class S, bool kBKN, int DT>
-__global__ __launch_bounds__(S::kThreads, S::kWaves / 4) void expert_rows_fast_kernel(ExpertArgs g) {
+__global__ __launch_bounds__(S::kThreads, 2) void expert_rows_stream_kernel(ExpertArgs g) {
   __shared__ __attribute__((aligned(16))) uint16_t lds[S::kLds];
-  const int cols = (g.n + S::BN - 1) / S::BN;
-  const Group at = find_group(g, S::BM, cols);
-  if (at.expert < 0) return;
-  int64_t row, col;
-  place(at.tile, (at.last - at.first + S::BM - 1) / S::BM, cols, row, col);
-  row = at.first + row * S::BM, col *= S::BN;
-  if (at.expert == g.experts) {
-    zero_tile<S>(g.out, row * g.ldo + col, g.ldo, at.last - row, g.n - col);
-    return;
-  }
-  const uint16_t* w = g.b + at.expert * g.sb + (kBKN ? col : col * g.ldb);
-  fast_tile<S, false, kBKN, DT, DT>(g.a + row * g.lda, g.lda, w, g.ldb, at.last - row, g.n - col, g.k, g.out,
-                                    row * g.ldo + col, g.ldo, lds);
+  RowJobs<true> jobs(g, S::BM, S::BN);
+  zero_rows<true>(g, jobs.rows);
+  stream<S, false, kBKN, DT, DT, true>(g, jobs, [&](const Job& j, Span& a, Span& b, int& rows, int& cols, int64_t& out0) {
+    const int64_t row = j.first + j.row, col = j.col * S::BN;
+    rows = j.last - (int)row, cols = g.n - (int)col, out0 = row * g.ldo + col;
+    a.set<false>(g.a + row * g.lda, g.lda, rows, g.k, S::BM);
+    b.set<kBKN>(g.b + j.expert * g.sb + (kBKN ? col : col * g.ldb), g.ldb, cols, g.k, S::BN);
+  }, lds);
 }
 
 template <class S, int DT, int OD>
-__global__ __launch_bounds__(S::kThreads, S::kWaves / 4) void expert_weight_fast_kernel(ExpertArgs g) {
+__global__ __launch_bounds__(S::kThreads, 2) void expert_weight_stream_kernel(ExpertArgs g) {
   __shared__ __attribute__((aligned(16))) uint16_t lds[S::kLds];
-  const int tn = (g.n + S::BM - 1) / S::BM, tk = (g.k + S::BN - 1) / S::BN, per = tn * tk;
-  // each XCD takes a contiguous part of every expert's tiles: experts differ in rows, and so in work
-  const int part = (per + 7) / 8, i = blockIdx.x / 8, e = i / part, t = (blockIdx.x % 8) * part + i % part;
-  if (t >= per) return;
-  int64_t row, col, first, last;
-  place(t, tn, tk, row, col);
-  row *= S::BM, col *= S::BN;
-  expert_rows(g, e, first, last);
-  const int64_t at = ((int64_t)e * g.n + row) * g.k + col;
-  if (first == last) {
-    for (int c = threadIdx.x; c < S::BM * S::BN / 4; c += S::kThreads) {
-      const int r = c / (S::BN / 4), x = c % (S::BN / 4) * 4;
-      if (row + r < g.n && col + x < g.k) {
-        if constexpr (OD == APEXW_F32) *APEXW_GLOBAL(u32x4, (float*)g.out + at + (int64_t)r * g.k + x) = u32x4{0u, 0u, 0u, 0u};
-        else *APEXW_GLOBAL(u32x2, (uint16_t*)g.out + at + (int64_t)r * g.k + x) = u32x2{0u, 0u};
-      }
-    }
-    return;
-  }
-  fast_tile<S, true, true, DT, OD>(g.a + first * g.lda + row, g.lda, g.b + first * g.ldb + col, g.ldb, g.n - row,
-                                   g.k - col, last - first, g.out, at, g.k, lds);
+  zero_weights<OD>(g);
+  WeightJobs jobs(g, S::BM, S::BN);
+  stream<S, true, true, DT, OD, false>(g, jobs, [&](const Job& j, Span& a, Span& b, int& rows, int& cols, int64_t& out0) {
+    const int64_t row = j.row, col = j.col * S::BN, first = j.first;
+    rows = g.n - (int)row, cols = g.k - (int)col, out0 = (j.expert * (int64_t)g.n + row) * g.k + col;
+    a.set<true>(g.a + first * g.lda + row, g.lda, rows, j.last - j.first, S::BM);
+    b.set<true>(g.b + first * g.ldb + col, g.ldb, cols, j.last - j.first, S::BN);
+  }, lds);
 }
 
 // ---------------------------------------------------------------------------
@@ -555,27 +690,24 @@ APEXW_DEV void tile(const uint16_t* a, int64_t lda, const uint16_t* b, int64_t l
 
 template <bool kBKN, int DT>
 __global__ __launch_bounds__(256) void expert_rows_kernel(ExpertArgs g) {
-  const int cols = (g.n + kTile - 1) / kTile;
-  const Group at = find_group(g, kTile, cols);
-  if (at.expert < 0) return;
-  int64_t row, col;
-  place(at.tile, (at.last - at.first + kTile - 1) / kTile, cols, row, col);
-  row = at.first + row * kTile, col *= kTile;
-  const bool none = at.expert == g.experts;
-  const uint16_t* w = g.b + (none ? 0 : at.expert * g.sb) + (kBKN ? col : col * g.ldb);
-  tile<false, kBKN, DT, DT>(g.a + row * g.lda, g.lda, w, g.ldb, at.last - row, g.n - col, none ? 0 : g.k, g.out,
-                            row * g.ldo + col, g.ldo);
+  RowJobs<false> jobs(g, kTile, kTile);
+  zero_rows<false>(g, jobs.rows);
+  const Job j = jobs.get(0);
+  if (j.expert < 0) return;
+  const int64_t row = j.first + j.row, col = (int64_t)j.col * kTile;
+  const uint16_t* w = g.b + j.expert * g.sb + (kBKN ? col : col * g.ldb);
+  tile<false, kBKN, DT, DT>(g.a + row * g.lda, g.lda, w, g.ldb, j.last - row, g.n - col, g.k, g.out, row * g.ldo + col,
+                            g.ldo);
 }
 
 template <int DT, int OD>
 __global__ __launch_bounds__(256) void expert_weight_kernel(ExpertArgs g) {
-  const int tn = (g.n + kTile - 1) / kTile, tk = (g.k + kTile - 1) / kTile;
-  const int e = blockIdx.x / (tn * tk), t = blockIdx.x % (tn * tk);
-  const int64_t row = (int64_t)(t / tk) * kTile, col = (int64_t)(t % tk) * kTile;
-  int64_t first, last;
-  expert_rows(g, e, first, last);
-  tile<true, true, DT, OD>(g.a + first * g.lda + row, g.lda, g.b + first * g.ldb + col, g.ldb, g.n - row, g.k - col,
-                           last - first, g.out, ((int64_t)e * g.n + row) * g.k + col, g.k);
+  zero_weights<OD>(g);
+  const Job j = WeightJobs(g, kTile, kTile).get(0);
+  if (j.expert < 0 || j.first == j.last) return;
+  const int64_t row = j.row, col = (int64_t)j.col * kTile;
+  tile<true, true, DT, OD>(g.a + j.first * g.lda + row, g.lda, g.b + j.first * g.ldb + col, g.ldb, g.n - row, g.k - col,
+                           j.last - j.first, g.out, ((int64_t)j.expert * g.n + row) * g.k + col, g.k);
 }
 
 // rows of whole 16-byte chunks at 16-byte addresses, within the 32-bit offsets of a stage's copies
@@ -583,23 +715,30 @@ bool chunks_ok(const void* p, int64_t ld, int64_t width, int64_t step = 0) {
   return ((uintptr_t)p & 15u) == 0 && ld % 8 == 0 && width % 8 == 0 && step % 8 == 0 && ld <= (1 << 22);
 }
 
+// workgroups of a stream: as many as the chip holds at a time, and no more than there are tiles
+template <class S> unsigned stream_grid(int64_t tiles) {
+  const int64_t most = (int64_t)apexw_cu_count() * S::kPerCU;
+  return (unsigned)(((tiles < most ? tiles : most) + 7) / 8 * 8);
+}
+
 template <class S, int DT>
-void launch_rows(const ExpertArgs& g, bool kn, int64_t tiles, hipStream_t s) {
-  const dim3 grid((unsigned)((tiles + 7) / 8 * 8)), block(S::kThreads);
-  if (kn) hipLaunchKernelGGL((expert_rows_fast_kernel<S, true, DT>), grid, block, 0, s, g);
-  else hipLaunchKernelGGL((expert_rows_fast_kernel<S, false, DT>), grid, block, 0, s, g);
+void launch_rows(const ExpertArgs& g, bool kn, hipStream_t s) {
+  const int64_t most = (g.rows / S::BM + (g.rows < g.experts ? g.rows : g.experts)) * ((g.n + S::BN - 1) / S::BN);
+  const dim3 grid(stream_grid<S>(most)), block(S::kThreads);
+  if (kn) hipLaunchKernelGGL((expert_rows_stream_kernel<S, true, DT>), grid, block, 0, s, g);
+  else hipLaunchKernelGGL((expert_rows_stream_kernel<S, false, DT>), grid, block, 0, s, g);
 }
 
 template <class S, int DT>
 void launch_weight(const ExpertArgs& g, int32_t out_dtype, hipStream_t s) {
-  const int64_t per = (int64_t)((g.n + S::BM - 1) / S::BM) * ((g.k + S::BN - 1) / S::BN);
-  const dim3 grid((unsigned)((per + 7) / 8 * 8 * g.experts)), block(S::kThreads);
-  if (out_dtype == APEXW_F32) hipLaunchKernelGGL((expert_weight_fast_kernel<S, DT, APEXW_F32>), grid, block, 0, s, g);
-  else hipLaunchKernelGGL((expert_weight_fast_kernel<S, DT, DT>), grid, block, 0, s, g);
+  const int64_t most = (int64_t)((g.n + S::BM - 1) / S::BM) * ((g.k + S::BN - 1) / S::BN) * g.experts;
+  const dim3 grid(stream_grid<S>(most)), block(S::kThreads);
+  if (out_dtype == APEXW_F32) hipLaunchKernelGGL((expert_weight_stream_kernel<S, DT, APEXW_F32>), grid, block, 0, s, g);
+  else hipLaunchKernelGGL((expert_weight_stream_kernel<S, DT, DT>), grid, block, 0, s, g);
 }
 
 bool sizes_ok(int64_t rows, int32_t experts, int64_t n, int64_t k) {
-  return rows >= 0 && rows <= INT32_MAX && experts > 0 && n > 0 && k > 0 && n <= INT32_MAX - 256 && k <= INT32_MAX - 256;
+  return rows >= 0 && rows <= INT32_MAX - 256 && experts > 0 && n > 0 && k > 0 && n <= INT32_MAX - 256 && k <= INT32_MAX - 256;
 }
 
 }  // namespace
@@ -613,25 +752,23 @@ extern "C" int apexw_expert_rows(const void* a, int64_t lda, const void* w, int6
   if (dtype != APEXW_BF16 && dtype != APEXW_F16) return APEXW_ERR_DTYPE;
   if (((uintptr_t)a | (uintptr_t)w | (uintptr_t)out) & 1u || (uintptr_t)ends & 3u) return APEXW_ERR_ALIGN;
   if (rows == 0) return APEXW_OK;
-  const int64_t tiles = (rows / kTile + (rows < experts + 1 ? rows : experts + 1)) * ((n + kTile - 1) / kTile);
-  if (tiles > INT32_MAX) return APEXW_ERR_SIZE;
+  const int64_t tiles = (rows / kTile + (rows < experts ? rows : experts)) * ((n + kTile - 1) / kTile);
+  if ((rows / Small::BM + (rows < experts ? rows : experts)) * ((n + Small::BN - 1) / Small::BN) > INT32_MAX) return APEXW_ERR_SIZE;
   ExpertArgs g{(const uint16_t*)a, (const uint16_t*)w, ends, out, lda, w_row_stride, w_expert_stride, ldo, rows,
                experts, (int32_t)n, (int32_t)k};
   const dim3 grid((unsigned)((tiles + 7) / 8 * 8)), block(256);
   hipStream_t s = (hipStream_t)stream;
   const bool kn = w_order == APEXW_EXPERT_KN;
   if (chunks_ok(a, lda, k) && chunks_ok(w, w_row_stride, kn ? n : k, w_expert_stride) && chunks_ok(out, ldo, n)) {
-    auto most = [&](int bm, int bn) {
-      return (rows / bm + (rows < experts + 1 ? rows : experts + 1)) * ((n + bn - 1) / bn);
-    };
-    const bool large = rows >= (int64_t)experts * 512;
-    const int64_t count = large ? most(Large::BM, Large::BN) : most(Wide::BM, Wide::BN);
+    const int shape = rows >= (int64_t)experts * 512 ? 2 : rows >= (int64_t)experts * 48 ? 1 : 0;
     if (dtype == APEXW_BF16) {
-      if (large) launch_rows<Large, APEXW_BF16>(g, kn, count, s);
-      else launch_rows<Wide, APEXW_BF16>(g, kn, count, s);
+      if (shape == 2) launch_rows<Large, APEXW_BF16>(g, kn, s);
+      else if (shape == 1) launch_rows<Wide, APEXW_BF16>(g, kn, s);
+      else launch_rows<Small, APEXW_BF16>(g, kn, s);
     } else {
-      if (large) launch_rows<Large, APEXW_F16>(g, kn, count, s);
-      else launch_rows<Wide, APEXW_F16>(g, kn, count, s);
+      if (shape == 2) launch_rows<Large, APEXW_F16>(g, kn, s);
+      else if (shape == 1) launch_rows<Wide, APEXW_F16>(g, kn, s);
+      else launch_rows<Small, APEXW_F16>(g, kn, s);
     }
     return hipGetLastError() == hipSuccess ? APEXW_OK : APEXW_ERR_LAUNCH;
   }
@@ -653,7 +790,7 @@ extern "C" int apexw_expert_weight_grad(const void* dy, int64_t ld_dy, const voi
   if ((dtype != APEXW_BF16 && dtype != APEXW_F16) || (dw_dtype != dtype && dw_dtype != APEXW_F32)) return APEXW_ERR_DTYPE;
   if (((uintptr_t)dy | (uintptr_t)x) & 1u || (uintptr_t)ends & 3u || (uintptr_t)dw & (dw_dtype == APEXW_F32 ? 3u : 1u))
     return APEXW_ERR_ALIGN;
-  const int64_t tiles = (int64_t)experts * ((n + kTile - 1) / kTile) * ((k + kTile - 1) / kTile);
+  const int64_t tiles = (((n + kTile - 1) / kTile) * ((k + kTile - 1) / kTile) + 7) / 8 * 8 * experts;
   if (tiles > INT32_MAX) return APEXW_ERR_SIZE;
   ExpertArgs g{(const uint16_t*)dy, (const uint16_t*)x, ends, dw, ld_dy, ld_x, 0, k, rows, experts, (int32_t)n,
                (int32_t)k};
