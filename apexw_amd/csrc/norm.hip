@@ -88,9 +88,15 @@ template <int DT> APEXW_DEV void store_elem(void* base, int64_t i, float x) {
   else APEXW_GLOBAL(uint16_t, base)[i] = (uint16_t)f32_to_f16_bits(x);
 }
 
+// Sum over T <= 64 lanes that stand together
+template <int T> APEXW_DEV float lanes_sum(float x) {
+#pragma unroll
+  for (int off = T < 64 ? T / 2 : 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
+  return x;
+}
 // Sum over the T threads of a row; red: T / 64 floats that nobody else uses until the next barrier
 template <int T> APEXW_DEV float row_sum(float x, float* red) {
-  x = wave_sum(x);
+  x = lanes_sum<T>(x);
   if constexpr (T > 64) {
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
     __syncthreads();
@@ -112,11 +118,11 @@ struct LnArgs {
 
 APEXW_DEV int clamp_cnt(int left, int most) { return left < 0 ? 0 : left < most ? left : most; }
 
-// One row per T threads (T = 64: a wave each), rows r, r + grid's rows, ...; the weights stay in registers.
+// One row per T threads (T = 64: a wave each; narrow rows share one), rows r, r + grid's rows, ...; the weights stay in registers.
 template <int XD, int WD, int T, int NC>
 __global__ __launch_bounds__(T < kWG ? kWG : T) void ln_forward_kernel(LnArgs a) {
   constexpr int V = kVec<XD>, kRows = T < kWG ? kWG / T : 1;
-  __shared__ float red[2][T / 64];
+  __shared__ float red[2][T > 64 ? T / 64 : 1];
   const int t = T < kWG ? threadIdx.x % T : threadIdx.x;
   int64_t row = (int64_t)blockIdx.x * kRows + (T < kWG ? threadIdx.x / T : 0);
   const int64_t step = (int64_t)gridDim.x * kRows;
@@ -137,11 +143,13 @@ __global__ __launch_bounds__(T < kWG ? kWG : T) void ln_forward_kernel(LnArgs a)
     float q = 0.0f;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
+      // what is missing was read as 0 and deviates by 0: from the mean taken as 0 where a whole chunk is
       const int cnt = clamp_cnt(a.width - (t + T * i) * V, V);
+      const float mu = cnt > 0 ? mean : 0.0f;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float d = j < cnt ? chunk_get<XD>(raw[i], j) - mean : 0.0f;
-        q = fmaf(d, d, q);
+        const float d = chunk_get<XD>(raw[i], j) - mu;
+        if (cnt == V || cnt == 0 || j < cnt) q = fmaf(d, d, q);
       }
     }
     const float rstd = 1.0f / sqrtf(fmaf(row_sum<T>(q, red[1]), a.inv_width, a.eps));
@@ -216,7 +224,7 @@ __global__ __launch_bounds__(1024) void ln_forward_long_kernel(LnArgs a) {
 template <int XD, int WD, int T, int NC>
 __global__ __launch_bounds__(T < kWG ? kWG : T) void ln_backward_kernel(LnArgs a) {
   constexpr int V = kVec<XD>, kThreads = T < kWG ? kWG : T, kRows = kThreads / T;
-  __shared__ float red[2][2][T / 64];
+  __shared__ float red[2][2][T > 64 ? T / 64 : 1];
   __shared__ float join[kRows > 1 ? (kRows - 1) * T * V : 1];
   const int t = threadIdx.x % T, group = threadIdx.x / T;
   float dw[NC][V], db[NC][V];
@@ -228,32 +236,34 @@ __global__ __launch_bounds__(T < kWG ? kWG : T) void ln_backward_kernel(LnArgs a
   for (int64_t row = (int64_t)blockIdx.x * kRows + group; row < a.rows; row += (int64_t)gridDim.x * kRows) {
     const char* xs = (const char*)a.x + row * a.x_stride * (int64_t)Elem<XD>::bytes;
     const char* ds = (const char*)a.dy + row * a.dy_stride * (int64_t)Elem<XD>::bytes;
-    const float mean = a.mean[row], rstd = a.rstd[row];
-    float xh[NC][V], g[NC][V], s1 = 0.0f, s2 = 0.0f;
+    const float mu = a.mean[row], rs = a.rstd[row];
+    u32x4 x[NC], dy[NC];
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int e = (t + T * i) * V, cnt = clamp_cnt(a.width - e, V);
-      const u32x4 xr = load_chunk<XD>(xs, e, cnt), dr = load_chunk<XD>(ds, e, cnt);
-      float w[V];
+      x[i] = load_chunk<XD>(xs, e, cnt);
+      dy[i] = load_chunk<XD>(ds, e, cnt);
+    }
+    float w[NC][V], s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
-      for (int j = 0; j < V; ++j) w[j] = 1.0f;
-      if (a.w) load_param<WD>(a.w, e, cnt, w);
+    for (int i = 0; i < NC; ++i) {
+      const int e = (t + T * i) * V, cnt = clamp_cnt(a.width - e, V);
+#pragma unroll
+      for (int j = 0; j < V; ++j) w[i][j] = 1.0f;
+      if (a.w) load_param<WD>(a.w, e, cnt, w[i]);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        xh[i][j] = (chunk_get<XD>(xr, j) - mean) * rstd;
-        const float d = chunk_get<XD>(dr, j);
-        if (j < cnt) {
-          dw[i][j] = fmaf(d, xh[i][j], dw[i][j]);
-          db[i][j] += d;
-        }
-        g[i][j] = j < cnt ? d * w[j] : 0.0f;
-        s1 += g[i][j];
-        if (j < cnt) s2 = fmaf(g[i][j], xh[i][j], s2);
+        // behind the row's end dy is 0, and so is every product
+        const float xh = (chunk_get<XD>(x[i], j) - mu) * rs, d = chunk_get<XD>(dy[i], j), g = d * w[i][j];
+        dw[i][j] = fmaf(d, xh, dw[i][j]);
+        db[i][j] += d;
+        s1 += g;
+        s2 = fmaf(g, xh, s2);
       }
     }
     if (!a.y) continue;
-    s1 = wave_sum(s1);
-    s2 = wave_sum(s2);
+    s1 = lanes_sum<T>(s1);
+    s2 = lanes_sum<T>(s2);
     if constexpr (T > 64) {
       if ((threadIdx.x & 63) == 0) {
         red[parity][0][t >> 6] = s1;
@@ -277,7 +287,10 @@ __global__ __launch_bounds__(T < kWG ? kWG : T) void ln_backward_kernel(LnArgs a
       if (cnt == 0) continue;
       float y[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) y[j] = rstd * (g[i][j] - fmaf(xh[i][j], s2, s1));
+      for (int j = 0; j < V; ++j) {
+        const float xh = (chunk_get<XD>(x[i], j) - mu) * rs;
+        y[j] = rs * (chunk_get<XD>(dy[i], j) * w[i][j] - fmaf(xh, s2, s1));
+      }
       store_chunk<XD>(dst, e, cnt, chunk_of<XD>(y));
     }
   }
@@ -365,9 +378,16 @@ __global__ __launch_bounds__(1024) void ln_reduce_kernel(const float* __restrict
   if (!out) return;
   const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
   const int64_t e = (int64_t)blockIdx.x * 32 + c;
-  float s = 0.0f;
-  if (e < width)
-    for (int i = g; i < n; i += 32) s += partial[((int64_t)i * 2 + blockIdx.y) * width + e];
+  float q[8] = {};   // eight loads in flight
+  if (e < width) {
+    const float* p = partial + (int64_t)blockIdx.y * width + e;
+    int i = g;
+    for (; i + 224 < n; i += 256)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) q[j] += p[(int64_t)(i + 32 * j) * 2 * width];
+    for (; i < n; i += 32) q[0] += p[(int64_t)i * 2 * width];
+  }
+  float s = ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
   red[g][c] = s;
   __syncthreads();
   if (g != 0 || e >= width) return;
@@ -377,7 +397,11 @@ __global__ __launch_bounds__(1024) void ln_reduce_kernel(const float* __restrict
   store_elem<WD>(out, e, s);
 }
 
-constexpr int kMaxGroups = 1024;   // workgroups of a backward pass, each with its partial sums
+// Workgroups of a backward pass, at most: each leaves 8 bytes of partial sums a column.  Measured with 256, 512
+// and 1024 of them: 16384 x 768 bf16 (rows of a wave) 42 / 28 / 20 us, 8192 x 4096 fp32 (256 threads) 122 / 93 /
+// 111 us, 4096 x 8192 bf16 (512 threads) 68 / 68 / 92 us, 2048 x 16384 bf16 (1024 threads) 68 / 93 / 146 us.
+constexpr int kMaxGroups = 1024;
+template <int T> constexpr int kGroups = T <= 64 ? kMaxGroups : T == 256 ? 512 : 256;
 
 template <int XD, int WD, int T, int NC>
 void forward_as(const LnArgs& a, hipStream_t stream) {
@@ -390,7 +414,9 @@ void forward_as(const LnArgs& a, hipStream_t stream) {
 template <int XD, int WD>
 void forward(const LnArgs& a, hipStream_t stream) {
   const int chunks = (int)(((int64_t)a.width + kVec<XD> - 1) / kVec<XD>);
-  if (chunks <= 64) forward_as<XD, WD, 64, 1>(a, stream);
+  if (chunks <= 16) forward_as<XD, WD, 16, 1>(a, stream);
+  else if (chunks <= 32) forward_as<XD, WD, 32, 1>(a, stream);
+  else if (chunks <= 64) forward_as<XD, WD, 64, 1>(a, stream);
   else if (chunks <= 128) forward_as<XD, WD, 64, 2>(a, stream);
   else if (chunks <= 256) forward_as<XD, WD, 64, 4>(a, stream);
   else if (chunks <= 512) forward_as<XD, WD, 256, 2>(a, stream);
@@ -406,7 +432,7 @@ template <int XD, int WD, int T, int NC>
 int backward_as(const LnArgs& a, hipStream_t stream) {
   constexpr int kThreads = T < kWG ? kWG : T, kRows = kThreads / T;
   const int64_t want = (a.rows + kRows - 1) / kRows;
-  const int grid = (int)(want < kMaxGroups ? want : kMaxGroups);
+  const int grid = (int)(want < kGroups<T> ? want : kGroups<T>);
   hipLaunchKernelGGL((ln_backward_kernel<XD, WD, T, NC>), dim3(grid), dim3(kThreads), 0, stream, a);
   return grid;
 }
@@ -414,12 +440,14 @@ int backward_as(const LnArgs& a, hipStream_t stream) {
 template <int XD, int WD>
 int backward(const LnArgs& a, hipStream_t stream) {
   const int chunks = (int)(((int64_t)a.width + kVec<XD> - 1) / kVec<XD>);
-  if (chunks <= 64) return backward_as<XD, WD, 64, 1>(a, stream);
-  if (chunks <= 128) return backward_as<XD, WD, 64, 2>(a, stream);
-  if (chunks <= 256) return backward_as<XD, WD, 256, 1>(a, stream);
-  if (chunks <= 512) return backward_as<XD, WD, 256, 2>(a, stream);
-  if (chunks <= 1024) return backward_as<XD, WD, 1024, 1>(a, stream);
-  if (chunks <= 2048) return backward_as<XD, WD, 1024, 2>(a, stream);
+  constexpr int C = 8 / kVec<XD>;   // chunks of 8 elements: up to 16 elements a thread
+  if (chunks <= 16 * C) return backward_as<XD, WD, 16, C>(a, stream);
+  if (chunks <= 32 * C) return backward_as<XD, WD, 32, C>(a, stream);
+  if (chunks <= 64 * C) return backward_as<XD, WD, 64, C>(a, stream);
+  if (chunks <= 128 * C) return backward_as<XD, WD, 64, 2 * C>(a, stream);
+  if (chunks <= 512 * C) return backward_as<XD, WD, 256, 2 * C>(a, stream);
+  if (chunks <= 1024 * C) return backward_as<XD, WD, 512, 2 * C>(a, stream);
+  if (chunks <= 2048 * C) return backward_as<XD, WD, 1024, 2 * C>(a, stream);
   if (a.y)
     hipLaunchKernelGGL((ln_backward_long_kernel<XD, WD>), dim3((unsigned)(a.rows < 65536 ? a.rows : 65536)), dim3(1024),
                        0, stream, a);
