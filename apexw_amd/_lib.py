@@ -229,6 +229,7 @@ SIGNATURES = {
     "apexw_grad_norm": (ctypes.c_int, [_vp, _i32, _i64, _i32, _vp, _vp, _vp]),
     "apexw_grad_scale": (ctypes.c_int, [_vp, _i32, _i64, _vp, _f32, _vp]),
     "apexw_clip_grads": (ctypes.c_int, [_vp, _i32, _i64, _i32, _f32, _vp, _vp, _vp]),
+    "apexw_clip_grads_small": (ctypes.c_int, [_vp, _i32, _i64, _i32, _f32, _vp, _vp, _vp]),
 }
 
 GEMM_TILE = 256

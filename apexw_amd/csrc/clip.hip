@@ -70,13 +70,21 @@ template <int DT> APEXW_DEV void store_some(void* base, int64_t e, int64_t cnt, 
     }
 }
 
+// A list's table in device memory, or, a short list's, in the launch's own arguments: nothing to upload
+struct Long {
+  const apexw_clip_tensor* t;
+};
+struct Short {
+  apexw_clip_tensor t[APEXW_CLIP_SMALL];
+};
+
 // the tensor of the table that holds unit u: the last one whose first unit is <= u (a tensor without
 // elements has no units and the first unit of the next)
-APEXW_DEV int find_tensor(const apexw_clip_tensor* __restrict__ tab, int n, int64_t u) {
+template <class Table> APEXW_DEV int find_tensor(const Table& tab, int n, int64_t u) {
   int lo = 0, hi = n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (tab[mid].first_unit <= u) lo = mid;
+    if (tab.t[mid].first_unit <= u) lo = mid;
     else hi = mid - 1;
   }
   return lo;
@@ -143,7 +151,8 @@ APEXW_DEV double join(double acc, uint32_t top, int order, double* red) {
   return s;
 }
 
-__global__ __launch_bounds__(256) void grad_norm_kernel(const apexw_clip_tensor* __restrict__ tab, int32_t n_tensors,
+template <class Table>
+__global__ __launch_bounds__(256) void grad_norm_kernel(Table tab, int32_t n_tensors,
                                                         int64_t n_units, int32_t order, double* __restrict__ partial) {
   __shared__ double red[4];
   const int64_t u0 = n_units * blockIdx.x / gridDim.x, u1 = n_units * (blockIdx.x + 1) / gridDim.x;
@@ -151,9 +160,9 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(const apexw_clip_tensor*
   uint32_t top = 0u;
   if (u0 < u1) {
     int k = find_tensor(tab, n_tensors, u0);
-    apexw_clip_tensor t = tab[k];
+    apexw_clip_tensor t = tab.t[k];
     for (int64_t u = u0; u < u1; ++u) {
-      while (u >= t.first_unit + (t.n + kUnit - 1) / kUnit) t = tab[++k];
+      while (u >= t.first_unit + (t.n + kUnit - 1) / kUnit) t = tab.t[++k];
       const int64_t e0 = (u - t.first_unit) * kUnit;
       if (t.g_dtype == APEXW_F32) unit_norm<APEXW_F32>(t, e0, order, acc, top);
       else if (t.g_dtype == APEXW_BF16) unit_norm<APEXW_BF16>(t, e0, order, acc, top);
@@ -207,7 +216,8 @@ template <int GD> APEXW_DEV void unit_scale_to(const apexw_clip_tensor& t, int64
 
 // given: a norm that the caller formed (over more than these tensors); else the partials' norm, written to *norm.
 // A tensor clipped in place is left alone where the coefficient is one.
-__global__ __launch_bounds__(256) void grad_scale_kernel(const apexw_clip_tensor* __restrict__ tab, int32_t n_tensors,
+template <class Table>
+__global__ __launch_bounds__(256) void grad_scale_kernel(Table tab, int32_t n_tensors,
                                                          int64_t n_units, int32_t order,
                                                          const double* __restrict__ partial, int32_t n_partial,
                                                          const float* __restrict__ given, float max_norm,
@@ -221,9 +231,9 @@ __global__ __launch_bounds__(256) void grad_scale_kernel(const apexw_clip_tensor
   const int64_t u0 = n_units * b / gridDim.x, u1 = n_units * (b + 1) / gridDim.x;
   if (u0 >= u1) return;
   int k = find_tensor(tab, n_tensors, u1 - 1);
-  apexw_clip_tensor t = tab[k];
+  apexw_clip_tensor t = tab.t[k];
   for (int64_t u = u1 - 1; u >= u0; --u) {
-    while (u < t.first_unit) t = tab[--k];
+    while (u < t.first_unit) t = tab.t[--k];
     if (c == 1.0f && t.out == t.g) continue;
     const int64_t e0 = (u - t.first_unit) * kUnit;
     if (t.g_dtype == APEXW_F32) unit_scale_to<APEXW_F32>(t, e0, c);
@@ -257,12 +267,26 @@ extern "C" int64_t apexw_clip_layout(apexw_clip_tensor* t, int32_t n_tensors) {
   return units;
 }
 
+namespace {
+
+template <class Table>
+int clip(const Table& tab, int32_t n_tensors, int64_t n_units, int32_t order, float max_norm, double* workspace,
+         float* norm, hipStream_t stream) {
+  const int grid = norm_grid(n_units);
+  hipLaunchKernelGGL(grad_norm_kernel<Table>, dim3(grid), dim3(256), 0, stream, tab, n_tensors, n_units, order, workspace);
+  hipLaunchKernelGGL(grad_scale_kernel<Table>, dim3(grid), dim3(256), 0, stream, tab, n_tensors, n_units, order,
+                     workspace, grid, (const float*)nullptr, max_norm, norm);
+  return hipGetLastError() == hipSuccess ? APEXW_OK : APEXW_ERR_LAUNCH;
+}
+
+}  // namespace
+
 extern "C" int apexw_grad_norm(const apexw_clip_tensor* tensors, int32_t n_tensors, int64_t n_units, int32_t order,
                                double* workspace, float* norm, void* stream) {
   if (!table_ok(tensors, n_tensors, n_units) || !order_ok(order) || !workspace || !norm) return APEXW_ERR_ARG;
   const int grid = norm_grid(n_units);
-  hipLaunchKernelGGL(grad_norm_kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, tensors, n_tensors, n_units,
-                     order, workspace);
+  hipLaunchKernelGGL(grad_norm_kernel<Long>, dim3(grid), dim3(256), 0, (hipStream_t)stream, Long{tensors}, n_tensors,
+                     n_units, order, workspace);
   hipLaunchKernelGGL(total_norm_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, workspace, grid, order, norm);
   return hipGetLastError() == hipSuccess ? APEXW_OK : APEXW_ERR_LAUNCH;
 }
@@ -271,8 +295,8 @@ extern "C" int apexw_grad_scale(const apexw_clip_tensor* tensors, int32_t n_tens
                                 const float* norm, float max_norm, void* stream) {
   if (!table_ok(tensors, n_tensors, n_units) || !norm || !max_ok(max_norm)) return APEXW_ERR_ARG;
   if (n_units == 0) return APEXW_OK;
-  hipLaunchKernelGGL(grad_scale_kernel, dim3(norm_grid(n_units)), dim3(256), 0, (hipStream_t)stream, tensors,
-                     n_tensors, n_units, 2, (const double*)nullptr, 0, norm, max_norm, (float*)nullptr);
+  hipLaunchKernelGGL(grad_scale_kernel<Long>, dim3(norm_grid(n_units)), dim3(256), 0, (hipStream_t)stream,
+                     Long{tensors}, n_tensors, n_units, 2, (const double*)nullptr, 0, norm, max_norm, (float*)nullptr);
   return hipGetLastError() == hipSuccess ? APEXW_OK : APEXW_ERR_LAUNCH;
 }
 
@@ -280,10 +304,15 @@ extern "C" int apexw_clip_grads(const apexw_clip_tensor* tensors, int32_t n_tens
                                 float max_norm, double* workspace, float* norm, void* stream) {
   if (!table_ok(tensors, n_tensors, n_units) || !order_ok(order) || !max_ok(max_norm) || !workspace || !norm)
     return APEXW_ERR_ARG;
-  const int grid = norm_grid(n_units);
-  hipLaunchKernelGGL(grad_norm_kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, tensors, n_tensors, n_units,
-                     order, workspace);
-  hipLaunchKernelGGL(grad_scale_kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, tensors, n_tensors, n_units,
-                     order, workspace, grid, (const float*)nullptr, max_norm, norm);
-  return hipGetLastError() == hipSuccess ? APEXW_OK : APEXW_ERR_LAUNCH;
+  return clip(Long{tensors}, n_tensors, n_units, order, max_norm, workspace, norm, (hipStream_t)stream);
+}
+
+extern "C" int apexw_clip_grads_small(const apexw_clip_tensor* tensors, int32_t n_tensors, int64_t n_units, int32_t order,
+                                      float max_norm, double* workspace, float* norm, void* stream) {
+  if (!table_ok(tensors, n_tensors, n_units) || !order_ok(order) || !max_ok(max_norm) || !workspace || !norm)
+    return APEXW_ERR_ARG;
+  if (n_tensors > APEXW_CLIP_SMALL) return APEXW_ERR_SIZE;
+  Short tab{};
+  for (int32_t i = 0; i < n_tensors; ++i) tab.t[i] = tensors[i];
+  return clip(tab, n_tensors, n_units, order, max_norm, workspace, norm, (hipStream_t)stream);
 }

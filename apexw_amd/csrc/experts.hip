@@ -738,7 +738,7 @@ void launch_weight(const ExpertArgs& g, int32_t out_dtype, hipStream_t s) {
 }
 
 bool sizes_ok(int64_t rows, int32_t experts, int64_t n, int64_t k) {
-  return rows >= 0 && rows <= INT32_MAX - 256 && experts > 0 && n > 0 && k > 0 && n <= INT32_MAX - 256 && k <= INT32_MAX - 256;
+  return rows >= 0 && rows <= INT32_MAX && experts > 0 && n > 0 && k > 0 && n <= INT32_MAX - 256 && k <= INT32_MAX - 256;
 }
 
 }  // namespace
@@ -753,7 +753,9 @@ extern "C" int apexw_expert_rows(const void* a, int64_t lda, const void* w, int6
   if (((uintptr_t)a | (uintptr_t)w | (uintptr_t)out) & 1u || (uintptr_t)ends & 3u) return APEXW_ERR_ALIGN;
   if (rows == 0) return APEXW_OK;
   const int64_t tiles = (rows / kTile + (rows < experts ? rows : experts)) * ((n + kTile - 1) / kTile);
-  if ((rows / Small::BM + (rows < experts ? rows : experts)) * ((n + Small::BN - 1) / Small::BN) > INT32_MAX) return APEXW_ERR_SIZE;
+  // 32-bit tile counts and rows, with room to round them up
+  if (rows > INT32_MAX - 256 || (rows / Small::BM + (rows < experts ? rows : experts)) * ((n + Small::BN - 1) / Small::BN) > INT32_MAX)
+    return APEXW_ERR_SIZE;
   ExpertArgs g{(const uint16_t*)a, (const uint16_t*)w, ends, out, lda, w_row_stride, w_expert_stride, ldo, rows,
                experts, (int32_t)n, (int32_t)k};
   const dim3 grid((unsigned)((tiles + 7) / 8 * 8)), block(256);
@@ -791,7 +793,7 @@ extern "C" int apexw_expert_weight_grad(const void* dy, int64_t ld_dy, const voi
   if (((uintptr_t)dy | (uintptr_t)x) & 1u || (uintptr_t)ends & 3u || (uintptr_t)dw & (dw_dtype == APEXW_F32 ? 3u : 1u))
     return APEXW_ERR_ALIGN;
   const int64_t tiles = (((n + kTile - 1) / kTile) * ((k + kTile - 1) / kTile) + 7) / 8 * 8 * experts;
-  if (tiles > INT32_MAX) return APEXW_ERR_SIZE;
+  if (tiles > INT32_MAX || rows > INT32_MAX - 256) return APEXW_ERR_SIZE;
   ExpertArgs g{(const uint16_t*)dy, (const uint16_t*)x, ends, dw, ld_dy, ld_x, 0, k, rows, experts, (int32_t)n,
                (int32_t)k};
   const dim3 grid((unsigned)tiles), block(256);

@@ -9,13 +9,17 @@
 // attribute read per tensor; this scan reads the tensors directly (about 10 ns
 // each), which matters for groups of tens of thousands of tensors.
 //
-// Plain CPython module (no pybind11): every function takes Python lists of
-// torch tensors and the addresses of caller-owned numpy buffers.
+// Plain CPython module (no pybind11): the step's functions take Python lists of
+// torch tensors and the addresses of caller-owned numpy buffers, the operators'
+// ones (below) tensors.
 
 #include <Python.h>
 
 #include <cstdint>
+#include <cstring>
 
+#include <ATen/ATen.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 namespace {
@@ -120,13 +124,50 @@ PyObject* scan(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return PyLong_FromLong(moved ? kGradsMoved : kSame);
 }
 
-// apexw_clip_tensor of include/apexw_hip.h
-struct ClipTensor {
+// ---------------------------------------------------------------------------
+// The operators around the step (apexw_amd/ops.py): the usual call checked, its outputs allocated and the
+// library called in one go, which takes a third of the time that the same takes from Python.  Each function
+// returns None for what it does not take (another layout, device or type); the Python form then copies,
+// converts or raises.  A nonzero apexw_status comes back as an int.
+// ---------------------------------------------------------------------------
+struct ClipTensor {   // apexw_clip_tensor of include/apexw_hip.h
   const void* g;
   void* out;
   int64_t n, first_unit;
   uint32_t g_dtype, out_dtype;
 };
+constexpr int kClipSmall = 48;        // APEXW_CLIP_SMALL
+constexpr int kClipPartials = 2048;   // APEXW_CLIP_PARTIALS
+
+struct Library {
+  int (*norm_forward)(const void*, int64_t, int64_t, int64_t, int32_t, const void*, const void*, int32_t, float, void*,
+                      float*, float*, void*);
+  int (*norm_backward)(const void*, int64_t, const void*, int64_t, const float*, const float*, const void*, int64_t,
+                       int64_t, int32_t, int32_t, void*, void*, void*, float*, void*);
+  int64_t (*norm_workspace)(int64_t, int64_t);
+  int (*expert_rows)(const void*, int64_t, const void*, int64_t, int64_t, int32_t, const int32_t*, int32_t, int64_t,
+                     int64_t, int64_t, int32_t, void*, int64_t, void*);
+  int (*expert_weight_grad)(const void*, int64_t, const void*, int64_t, const int32_t*, int32_t, int64_t, int64_t,
+                            int64_t, int32_t, void*, int32_t, void*);
+  int64_t (*clip_layout)(ClipTensor*, int32_t);
+  int (*clip_grads)(const ClipTensor*, int32_t, int64_t, int32_t, float, double*, float*, void*);
+  int (*clip_grads_small)(const ClipTensor*, int32_t, int64_t, int32_t, float, double*, float*, void*);
+} lib;
+constexpr int kEntries = sizeof(Library) / sizeof(void*);
+
+// bind(addresses): the entry points, in the order of Library
+PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != kEntries) {
+    PyErr_Format(PyExc_TypeError, "bind takes %d addresses", kEntries);
+    return nullptr;
+  }
+  uintptr_t at[kEntries];
+  for (int i = 0; i < kEntries; ++i)
+    if (!as_addr(args[i], &at[i])) return nullptr;
+  static_assert(sizeof(at) == sizeof(lib), "function pointers");
+  std::memcpy(&lib, at, sizeof(lib));
+  Py_RETURN_NONE;
+}
 
 bool dtype_code(const at::Tensor& t, uint32_t* code) {
   switch (t.scalar_type()) {
@@ -137,9 +178,237 @@ bool dtype_code(const at::Tensor& t, uint32_t* code) {
   }
 }
 
-// clip_table(grads, out, table_addr, name): the entries of a clip's table (first_unit left 0).
-// Raises for tensors that the clip does not take: another device, type or layout.
+// where a call runs: the current stream and device
+struct Where {
+  void* stream;
+  long device;
+  bool set(PyObject* s, PyObject* d) {
+    uintptr_t p;
+    if (!lib.norm_forward || !as_addr(s, &p)) return false;
+    stream = reinterpret_cast<void*>(p);
+    device = PyLong_AsLong(d);
+    return !PyErr_Occurred();
+  }
+  bool has(const at::Tensor& t) const {
+    return t.is_cuda() && t.layout() == at::kStrided && t.get_device() == device;
+  }
+};
+
+PyObject* none_or_error() {
+  if (PyErr_Occurred()) return nullptr;
+  Py_RETURN_NONE;
+}
+
+PyObject* pack(const at::Tensor* const* t, int n) {
+  PyObject* out = PyTuple_New(n);
+  if (!out) return nullptr;
+  for (int i = 0; i < n; ++i) {
+    PyObject* v;
+    if (t[i]->defined()) {
+      v = THPVariable_Wrap(*t[i]);
+    } else {
+      v = Py_None;
+      Py_INCREF(v);
+    }
+    if (!v) {
+      Py_DECREF(out);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(out, i, v);
+  }
+  return out;
+}
+
+bool optional_tensor(PyObject* o, at::Tensor* t) {
+  if (o == Py_None) return true;
+  if (!THPVariable_Check(o)) return false;
+  *t = THPVariable_Unpack(o);
+  return true;
+}
+
+// a weight or bias of `width` elements for rows of `code`; sets their common type
+bool norm_param(const at::Tensor& t, const Where& w, int64_t width, uint32_t code, uint32_t* w_code) {
+  if (!t.defined()) return true;
+  uint32_t c;
+  if (!w.has(t) || !dtype_code(t, &c) || t.dim() != 1 || t.size(0) != width || !t.is_contiguous()) return false;
+  if ((c != code && c != 0) || (*w_code != ~0u && *w_code != c)) return false;
+  *w_code = c;
+  return true;
+}
+
+const void* address(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// layer_norm_forward(x, weight, bias, eps, stream, device) -> (y, mean, rstd)
+PyObject* layer_norm_forward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Where where;
+  at::Tensor w, b;
+  if (nargs != 6 || !THPVariable_Check(args[0]) || !optional_tensor(args[1], &w) || !optional_tensor(args[2], &b) ||
+      !where.set(args[4], args[5]))
+    return none_or_error();
+  const at::Tensor& x = THPVariable_Unpack(args[0]);
+  const double eps = PyFloat_AsDouble(args[3]);
+  if (PyErr_Occurred()) return nullptr;
+  uint32_t code, w_code = ~0u;
+  if (!where.has(x) || !dtype_code(x, &code) || x.dim() < 1 || x.numel() == 0 || !x.is_contiguous() || !(eps >= 0)) return none_or_error();
+  const int64_t width = x.size(-1), rows = x.numel() / width;
+  if (!norm_param(w, where, width, code, &w_code) || !norm_param(b, where, width, code, &w_code)) return none_or_error();
+  if (w_code == ~0u) w_code = code;
+  const at::Tensor y = at::empty(x.sizes(), x.options());
+  const auto per_row = x.sizes().slice(0, x.dim() - 1);
+  const at::Tensor mean = at::empty(per_row, x.options().dtype(at::kFloat)), rstd = at::empty(per_row, mean.options());
+  const int status = lib.norm_forward(x.data_ptr(), rows, width, width, code, address(w), address(b), w_code,
+                                      static_cast<float>(eps), y.data_ptr(), static_cast<float*>(mean.data_ptr()),
+                                      static_cast<float*>(rstd.data_ptr()), where.stream);
+  if (status) return PyLong_FromLong(status);
+  const at::Tensor* out[] = {&y, &mean, &rstd};
+  return pack(out, 3);
+  END_HANDLE_TH_ERRORS
+}
+
+// layer_norm_backward(dy, x, mean, rstd, weight, bias, need_x, need_w, need_b, stream, device) -> (dx, dw, db)
+PyObject* layer_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Where where;
+  at::Tensor w, b;
+  if (nargs != 11) return none_or_error();
+  for (int i = 0; i < 4; ++i)
+    if (!THPVariable_Check(args[i])) return none_or_error();
+  if (!optional_tensor(args[4], &w) || !optional_tensor(args[5], &b) || !where.set(args[9], args[10]))
+    return none_or_error();
+  const at::Tensor &dy = THPVariable_Unpack(args[0]), &x = THPVariable_Unpack(args[1]),
+                   &mean = THPVariable_Unpack(args[2]), &rstd = THPVariable_Unpack(args[3]);
+  uint32_t code, w_code = ~0u;
+  if (!where.has(x) || !dtype_code(x, &code) || x.dim() < 1 || x.numel() == 0 || !x.is_contiguous()) return none_or_error();
+  const int64_t width = x.size(-1), rows = x.numel() / width;
+  if (!where.has(dy) || dy.scalar_type() != x.scalar_type() || dy.sizes() != x.sizes() || !dy.is_contiguous())
+    return none_or_error();
+  for (const at::Tensor* t : {&mean, &rstd})
+    if (!where.has(*t) || t->scalar_type() != at::kFloat || t->numel() != rows || !t->is_contiguous())
+      return none_or_error();
+  if (!norm_param(w, where, width, code, &w_code) || !norm_param(b, where, width, code, &w_code)) return none_or_error();
+  if (w_code == ~0u) w_code = code;
+  at::Tensor dx, dw, db, ws;
+  if (args[6] == Py_True) dx = at::empty(x.sizes(), x.options());
+  if (args[7] == Py_True && w.defined()) dw = at::empty({width}, w.options());
+  if (args[8] == Py_True && b.defined()) db = at::empty({width}, b.options());
+  if (dw.defined() || db.defined()) {
+    const int64_t floats = lib.norm_workspace(rows, width);
+    if (floats < 0) return PyLong_FromLong(static_cast<long>(-floats));
+    ws = at::empty({floats}, mean.options());
+  }
+  if (dx.defined() || ws.defined()) {
+    const int status = lib.norm_backward(
+        dy.data_ptr(), width, x.data_ptr(), width, static_cast<const float*>(mean.data_ptr()),
+        static_cast<const float*>(rstd.data_ptr()), address(w), rows, width, code, w_code, const_cast<void*>(address(dx)),
+        const_cast<void*>(address(dw)), const_cast<void*>(address(db)),
+        static_cast<float*>(const_cast<void*>(address(ws))), where.stream);
+    if (status) return PyLong_FromLong(status);
+  }
+  const at::Tensor* out[] = {&dx, &dw, &db};
+  return pack(out, 3);
+  END_HANDLE_TH_ERRORS
+}
+
+// rows of 16-bit elements, whole in their last dimension
+bool expert_operand(const at::Tensor& t, const Where& w, uint32_t* code) {
+  return w.has(t) && dtype_code(t, code) && *code != 0 && t.dim() == 2 && t.size(1) > 0 && t.stride(1) == 1;
+}
+bool expert_ends(const at::Tensor& t, const Where& w) {
+  return w.has(t) && t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) > 0 && t.is_contiguous();
+}
+
+// expert_rows(a, weight, ends, transposed, stream, device) -> weight[e] a[i], or weight[e]^T a[i]
+PyObject* expert_rows(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Where where;
+  if (nargs != 6 || !THPVariable_Check(args[0]) || !THPVariable_Check(args[1]) || !THPVariable_Check(args[2]) ||
+      !where.set(args[4], args[5]))
+    return none_or_error();
+  const at::Tensor &a = THPVariable_Unpack(args[0]), &w = THPVariable_Unpack(args[1]), &ends = THPVariable_Unpack(args[2]);
+  const bool transposed = args[3] == Py_True;
+  uint32_t code;
+  if (!expert_operand(a, where, &code) || !expert_ends(ends, where) || !where.has(w) ||
+      w.scalar_type() != a.scalar_type() || w.dim() != 3 || w.numel() == 0 || w.stride(2) != 1 ||
+      w.size(0) != ends.size(0) || w.size(transposed ? 1 : 2) != a.size(1) || a.size(0) == 0)
+    return none_or_error();
+  const int64_t n = w.size(transposed ? 2 : 1);
+  const at::Tensor out = at::empty({a.size(0), n}, a.options());
+  const int status = lib.expert_rows(a.data_ptr(), a.stride(0), w.data_ptr(), w.stride(1), w.stride(0), transposed,
+                                     static_cast<const int32_t*>(ends.data_ptr()), static_cast<int32_t>(ends.size(0)),
+                                     a.size(0), a.size(1), n, code, out.data_ptr(), n, where.stream);
+  return status ? PyLong_FromLong(status) : THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// expert_weight_grad(dy, x, ends, fp32, stream, device) -> dW
+PyObject* expert_weight_grad(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Where where;
+  if (nargs != 6 || !THPVariable_Check(args[0]) || !THPVariable_Check(args[1]) || !THPVariable_Check(args[2]) ||
+      !where.set(args[4], args[5]))
+    return none_or_error();
+  const at::Tensor &dy = THPVariable_Unpack(args[0]), &x = THPVariable_Unpack(args[1]), &ends = THPVariable_Unpack(args[2]);
+  const bool fp32 = args[3] == Py_True;
+  uint32_t code, x_code;
+  if (!expert_operand(dy, where, &code) || !expert_operand(x, where, &x_code) || code != x_code ||
+      !expert_ends(ends, where) || dy.size(0) != x.size(0) || dy.size(0) == 0)
+    return none_or_error();
+  const at::Tensor dw = at::empty({ends.size(0), dy.size(1), x.size(1)}, fp32 ? dy.options().dtype(at::kFloat) : dy.options());
+  const int status = lib.expert_weight_grad(dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0),
+                                            static_cast<const int32_t*>(ends.data_ptr()),
+                                            static_cast<int32_t>(ends.size(0)), dy.size(0), dy.size(1), x.size(1), code,
+                                            dw.data_ptr(), fp32 ? 0 : code, where.stream);
+  return status ? PyLong_FromLong(status) : THPVariable_Wrap(dw);
+  END_HANDLE_TH_ERRORS
+}
+
+// The entries of a clip's table (first_unit left 0).  Raises for tensors that the clip does not take:
+// another device, type or layout.
+bool fill_clip(PyObject* grads, PyObject* outs, ClipTensor* table, const char* name) {
+  const Py_ssize_t n = PyList_GET_SIZE(grads);
+  if (PyList_GET_SIZE(outs) != n) {
+    PyErr_SetString(PyExc_ValueError, "clip: lists of different lengths");
+    return false;
+  }
+  const bool in_place = grads == outs;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    const at::Tensor& g = THPVariable_Unpack(PyList_GET_ITEM(grads, i));
+    const at::Tensor& o = in_place ? g : THPVariable_Unpack(PyList_GET_ITEM(outs, i));
+    ClipTensor& t = table[i];
+    if (g.layout() != at::kStrided || o.layout() != at::kStrided) {
+      PyErr_Format(PyExc_ValueError, "%s: tensor %zd is sparse", name, i);
+      return false;
+    }
+    const at::Device device = THPVariable_Unpack(PyList_GET_ITEM(grads, 0)).device();
+    if (g.device() != device || o.device() != device) {
+      PyErr_Format(PyExc_ValueError, "%s: tensor %zd is on another device than the first one", name, i);
+      return false;
+    }
+    if (!dtype_code(g, &t.g_dtype) || !dtype_code(o, &t.out_dtype)) {
+      PyErr_Format(PyExc_TypeError, "%s: tensor %zd is not float32, bfloat16 or float16", name, i);
+      return false;
+    }
+    const bool whole = g.is_contiguous();
+    if (!whole && !g.is_non_overlapping_and_dense()) {
+      PyErr_Format(PyExc_ValueError, "%s: tensor %zd is not dense", name, i);
+      return false;
+    }
+    if (!in_place && (g.sizes() != o.sizes() || (whole ? !o.is_contiguous() : g.strides() != o.strides()))) {
+      PyErr_Format(PyExc_ValueError, "%s: the copy of tensor %zd has another shape or layout", name, i);
+      return false;
+    }
+    t.g = g.data_ptr();
+    t.out = o.data_ptr();
+    t.n = g.numel();
+    t.first_unit = 0;
+  }
+  return true;
+}
+
+// clip_table(grads, out, table_addr, name): fill_clip into the table at table_addr
 PyObject* clip_table(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
   if (nargs != 4) {
     PyErr_SetString(PyExc_TypeError, "clip_table(grads, out, table_addr, name)");
     return nullptr;
@@ -147,50 +416,55 @@ PyObject* clip_table(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   uintptr_t ta;
   if (!unpack_list(args[0], "grads") || !unpack_list(args[1], "out") || !as_addr(args[2], &ta)) return nullptr;
   const char* name = PyUnicode_AsUTF8(args[3]);
-  if (!name) return nullptr;
-  auto* table = reinterpret_cast<ClipTensor*>(ta);
-  const Py_ssize_t n = PyList_GET_SIZE(args[0]);
-  if (PyList_GET_SIZE(args[1]) != n) {
-    PyErr_SetString(PyExc_ValueError, "clip_table: lists of different lengths");
-    return nullptr;
-  }
-  if (n == 0) Py_RETURN_NONE;
-  const bool in_place = args[0] == args[1];
-  const at::Device device = THPVariable_Unpack(PyList_GET_ITEM(args[0], 0)).device();
-  for (Py_ssize_t i = 0; i < n; ++i) {
-    const at::Tensor& g = THPVariable_Unpack(PyList_GET_ITEM(args[0], i));
-    const at::Tensor& o = in_place ? g : THPVariable_Unpack(PyList_GET_ITEM(args[1], i));
-    ClipTensor& t = table[i];
-    if (g.layout() != at::kStrided || o.layout() != at::kStrided) {
-      PyErr_Format(PyExc_ValueError, "%s: tensor %zd is sparse", name, i);
-      return nullptr;
-    }
-    if (g.device() != device || o.device() != device) {
-      PyErr_Format(PyExc_ValueError, "%s: tensor %zd is on another device than the first one", name, i);
-      return nullptr;
-    }
-    if (!dtype_code(g, &t.g_dtype) || !dtype_code(o, &t.out_dtype)) {
-      PyErr_Format(PyExc_TypeError, "%s: tensor %zd is not float32, bfloat16 or float16", name, i);
-      return nullptr;
-    }
-    if (!g.is_contiguous() && !g.is_non_overlapping_and_dense()) {
-      PyErr_Format(PyExc_ValueError, "%s: tensor %zd is not dense", name, i);
-      return nullptr;
-    }
-    if (!in_place && (g.sizes() != o.sizes() || (g.strides() != o.strides() && !(g.is_contiguous() && o.is_contiguous())))) {
-      PyErr_Format(PyExc_ValueError, "%s: the copy of tensor %zd has another shape or layout", name, i);
-      return nullptr;
-    }
-    t.g = g.data_ptr();
-    t.out = o.data_ptr();
-    t.n = g.numel();
-    t.first_unit = 0;
-  }
+  if (!name || !fill_clip(args[0], args[1], reinterpret_cast<ClipTensor*>(ta), name)) return nullptr;
   Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
 }
 
+// clip_grads(grads, out, max_norm, order, stream, device) -> the norm
+PyObject* clip_grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Where where;
+  if (nargs != 6 || !where.set(args[4], args[5])) return none_or_error();
+  if (!unpack_list(args[0], "grads") || !unpack_list(args[1], "out")) return nullptr;
+  const Py_ssize_t n = PyList_GET_SIZE(args[0]);
+  if (n == 0 || n > INT32_MAX) return none_or_error();
+  const at::Tensor& first = THPVariable_Unpack(PyList_GET_ITEM(args[0], 0));
+  const double max_norm = PyFloat_AsDouble(args[2]);
+  const long order = PyLong_AsLong(args[3]);
+  if (PyErr_Occurred()) return nullptr;
+  if (!where.has(first)) return none_or_error();
+  ClipTensor small[kClipSmall];
+  at::Tensor host, table;
+  ClipTensor* t = small;
+  if (n > kClipSmall) {
+    host = at::empty({static_cast<int64_t>(n * sizeof(ClipTensor))}, at::TensorOptions().dtype(at::kByte).pinned_memory(true));
+    t = static_cast<ClipTensor*>(host.data_ptr());
+  }
+  if (!fill_clip(args[0], args[1], t, "clip_grads")) return nullptr;
+  const int64_t units = lib.clip_layout(t, static_cast<int32_t>(n));
+  if (units < 0) return PyLong_FromLong(static_cast<long>(-units));
+  const auto options = at::TensorOptions().device(first.device());
+  const at::Tensor ws = at::empty({kClipPartials}, options.dtype(at::kDouble)), norm = at::empty({}, options.dtype(at::kFloat));
+  if (n > kClipSmall) table = host.to(first.device(), /*non_blocking=*/true);
+  auto* call = n > kClipSmall ? lib.clip_grads : lib.clip_grads_small;
+  const int status = call(n > kClipSmall ? static_cast<const ClipTensor*>(table.data_ptr()) : small, static_cast<int32_t>(n),
+                          units, static_cast<int32_t>(order), static_cast<float>(max_norm),
+                          static_cast<double*>(ws.data_ptr()), static_cast<float*>(norm.data_ptr()), where.stream);
+  return status ? PyLong_FromLong(status) : THPVariable_Wrap(norm);
+  END_HANDLE_TH_ERRORS
+}
+
+template <class F> PyCFunction fast(F* f) { return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)); }
+
 PyMethodDef kMethods[] = {
-    {"clip_table", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(clip_table)), METH_FASTCALL,
+    {"bind", fast(bind), METH_FASTCALL, "The addresses of the library's entry points."},
+    {"layer_norm_forward", fast(layer_norm_forward), METH_FASTCALL, "The usual call, or None."},
+    {"layer_norm_backward", fast(layer_norm_backward), METH_FASTCALL, "The usual call, or None."},
+    {"expert_rows", fast(expert_rows), METH_FASTCALL, "The usual call, or None."},
+    {"expert_weight_grad", fast(expert_weight_grad), METH_FASTCALL, "The usual call, or None."},
+    {"clip_grads", fast(clip_grads), METH_FASTCALL, "The usual call, or None."},
+    {"clip_table", fast(clip_table), METH_FASTCALL,
      "Fill the table of a clip by the global norm from lists of tensors."},
     {"snapshot", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(snapshot)), METH_FASTCALL,
      "Record data pointers and dtypes of a list of tensors."},

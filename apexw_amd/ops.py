@@ -9,13 +9,39 @@ They take CUDA (ROCm) tensors, run on the current stream of the tensors' device 
 there; nothing is read back on the host.  What they do not support raises before anything is launched.
 """
 
+import ctypes
+
 import torch
 
 from . import _lib
+from ._plan import _host
 
 _CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 _ORDER = {1.0: 1, 2.0: 2, float("inf"): 0}
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else None
+_NATIVE = None
+_ENTRIES = ("apexw_layer_norm_forward", "apexw_layer_norm_backward", "apexw_layer_norm_workspace", "apexw_expert_rows",
+            "apexw_expert_weight_grad", "apexw_clip_layout", "apexw_clip_grads", "apexw_clip_grads_small")
+
+
+def _native(t):
+    """The host module with the library's entry points, for a call on the GPU tensor t (else None)."""
+    global _NATIVE
+    if _NATIVE is None:
+        if not (isinstance(t, torch.Tensor) and t.is_cuda):
+            return None
+        lib, mod = _lib.load(), _host()
+        mod.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _ENTRIES))
+        _NATIVE = mod
+    return _NATIVE if isinstance(t, torch.Tensor) and t.is_cuda else None
+
+
+def _done(out, what):
+    """A native call's result; raises for a status."""
+    if type(out) is int:
+        _lib.check(out, what)
+    return out
 
 
 def _on_device(t, name, device=None):
@@ -89,6 +115,12 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5):
     ``y = (x - mean) * rstd * weight + bias`` has x's shape and type, contiguous; ``mean`` and
     ``rstd = 1 / sqrt(var + eps)`` (float32, x's shape without its last dimension) are what
     ``layer_norm_backward`` takes.  weight and bias are of x's type, or float32 with 16-bit rows."""
+    native = _native(x)
+    if native is not None:
+        dev = _current()
+        out = native.layer_norm_forward(x, weight, bias, eps, _raw_stream(dev), dev)
+        if out is not None:
+            return _done(out, "apexw_layer_norm_forward")
     width, w_dtype = _check_norm(x, weight, bias)
     if not eps >= 0:
         raise ValueError(f"layer_norm: expected eps >= 0, got {eps}")
@@ -112,6 +144,12 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, bias=None, need=(True, T
 
     dw and db are None without a weight or a bias; ``need`` leaves out gradients nobody wants (None).  The
     sums over rows are taken in a fixed order, so equal calls give equal bits."""
+    native = _native(x)
+    if native is not None:
+        dev = _current()
+        out = native.layer_norm_backward(dy, x, mean, rstd, weight, bias, *need, _raw_stream(dev), dev)
+        if out is not None:
+            return _done(out, "apexw_layer_norm_backward")
     width, w_dtype = _check_norm(x, weight, bias)
     if dy.shape != x.shape or dy.dtype != x.dtype:
         raise ValueError(f"layer_norm: expected dy of shape {tuple(x.shape)} and {x.dtype}, got {tuple(dy.shape)} "
@@ -218,6 +256,12 @@ def expert_matmul_forward(x, weight, ends):
     x: (rows, inner), sorted by expert; weight: (experts, outer, inner), contiguous in either of its last two
     dimensions; ends: int32, ends[e] one past expert e's last row (int64 is converted).  bfloat16 or float16,
     summed in fp32."""
+    native = _native(x)
+    if native is not None:
+        dev = _current()
+        out = native.expert_rows(x, weight, ends, False, _raw_stream(dev), dev)
+        if out is not None:
+            return _done(out, "apexw_expert_rows")
     x = _check_rows(x, "x")
     _check_weight(weight, x)
     if weight.shape[2] != x.shape[1]:
@@ -227,6 +271,12 @@ def expert_matmul_forward(x, weight, ends):
 
 def expert_matmul_rows_grad(dy, weight, ends):
     """dx[i] = weight[e]^T @ dy[i]: the gradient of expert_matmul's rows; zeros behind the last end."""
+    native = _native(dy)
+    if native is not None:
+        dev = _current()
+        out = native.expert_rows(dy, weight, ends, True, _raw_stream(dev), dev)
+        if out is not None:
+            return _done(out, "apexw_expert_rows")
     dy = _check_rows(dy, "dy")
     _check_weight(weight, dy)
     if weight.shape[1] != dy.shape[1]:
@@ -237,6 +287,12 @@ def expert_matmul_rows_grad(dy, weight, ends):
 def expert_matmul_weight_grad(dy, x, ends, dtype=None):
     """dW[e] = sum over expert e's rows of dy[i] x[i]^T, (experts, outer, inner): the gradient of
     expert_matmul's weights, zero for an expert without rows; dtype: dy's (the default) or float32."""
+    native = _native(dy)
+    if native is not None and dtype in (None, dy.dtype, torch.float32):
+        dev = _current()
+        out = native.expert_weight_grad(dy, x, ends, dtype is torch.float32, _raw_stream(dev), dev)
+        if out is not None:
+            return _done(out, "apexw_expert_weight_grad")
     dy, x = _check_rows(dy, "dy"), _check_rows(x, "x")
     if x.dtype != dy.dtype or x.device != dy.device or x.shape[0] != dy.shape[0]:
         raise ValueError(f"expert_matmul: dy {tuple(dy.shape)} of {dy.dtype} on {dy.device} and x {tuple(x.shape)} of "
@@ -275,28 +331,28 @@ def expert_matmul(x, weight, ends):
 
 
 # ---------------------------------------------------------------------------- clip by the global norm
-def _clip_table(grads, out, name):
-    """The launch table of a list of gradients and of where their copies go: (device table or None, entries,
-    units, device)."""
-    from . import _host
-    grads = list(grads)
-    to = grads if out is None else list(out)
+def _clip_lists(grads, out, name):
+    """The lists of a clip, the same one twice in place, and their device (None: nothing to clip)."""
+    grads = grads if type(grads) is list else list(grads)
+    to = grads if out is None else out if type(out) is list else list(out)
     if len(to) != len(grads):
         raise ValueError(f"{name}: {len(grads)} gradients and {len(to)} tensors for their copies")
-    device = None
-    for t in grads[:1]:
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name}: expected a list of tensors")
-        _on_device(t, name)
-        device = t.device
-    if device is None:
-        return None, 0, 0, None
+    if not grads:
+        return grads, to, None
+    if not isinstance(grads[0], torch.Tensor):
+        raise TypeError(f"{name}: expected a list of tensors")
+    _on_device(grads[0], name)
+    return grads, to, grads[0].device
+
+
+def _clip_table(grads, to, device, name):
+    """The launch table on the device (made the current one): (table, entries, units)."""
     host = torch.empty(len(grads) * _lib.CLIP_TENSOR_DTYPE.itemsize, dtype=torch.uint8, pin_memory=True)
-    _host.clip_table(grads, to, host.data_ptr(), name)
+    _host().clip_table(grads, to, host.data_ptr(), name)
     units = _lib.load().apexw_clip_layout(host.data_ptr(), len(grads))
     if units < 0:
         _lib.check(-units, "apexw_clip_layout")
-    return host.to(device, non_blocking=True), len(grads), units, device
+    return host.to(device, non_blocking=True), len(grads), units
 
 
 def _order(norm_type, name):
@@ -309,10 +365,11 @@ def _order(norm_type, name):
 def grad_norm(grads, norm_type=2.0):
     """The norm of all elements of a list of gradients, as a float32 scalar on their device (p = 1, 2, inf)."""
     order = _order(norm_type, "grad_norm")
-    table, n, units, device = _clip_table(grads, None, "grad_norm")
-    if table is None:
+    grads, to, device = _clip_lists(grads, None, "grad_norm")
+    if device is None:
         return torch.tensor(0.0)
     with _Launch(device) as stream:
+        table, n, units = _clip_table(grads, to, device, "grad_norm")
         ws = torch.empty(_lib.CLIP_PARTIALS, dtype=torch.float64, device=device)
         norm = torch.empty((), dtype=torch.float32, device=device)
         _lib.check(_lib.load().apexw_grad_norm(table.data_ptr(), n, units, order, ws.data_ptr(), norm.data_ptr(), stream),
@@ -325,13 +382,14 @@ def scale_grads(grads, max_norm, total_norm, out=None):
     device), for instance over the gradients of all processes."""
     if not max_norm >= 0:
         raise ValueError(f"scale_grads: expected max_norm >= 0, got {max_norm}")
-    table, n, units, device = _clip_table(grads, out, "scale_grads")
-    if table is None:
+    grads, to, device = _clip_lists(grads, out, "scale_grads")
+    if device is None:
         return
     if total_norm.dtype != torch.float32 or total_norm.numel() != 1:
         raise ValueError("scale_grads: expected total_norm as one float32")
     _on_device(total_norm, "scale_grads: total_norm", device)
     with _Launch(device) as stream:
+        table, n, units = _clip_table(grads, to, device, "scale_grads")
         _lib.check(_lib.load().apexw_grad_scale(table.data_ptr(), n, units, total_norm.data_ptr(), max_norm, stream),
                    "apexw_grad_scale")
 
@@ -347,10 +405,15 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None):
     order = _order(norm_type, "clip_grads")
     if not max_norm >= 0:
         raise ValueError(f"clip_grads: expected max_norm >= 0, got {max_norm}")
-    table, n, units, device = _clip_table(grads, out, "clip_grads")
-    if table is None:
+    grads, to, device = _clip_lists(grads, out, "clip_grads")
+    if device is None:
         return torch.tensor(0.0)
+    dev = _current()
+    norm = _native(grads[0]).clip_grads(grads, to, max_norm, order, _raw_stream(dev), dev)
+    if norm is not None:
+        return _done(norm, "apexw_clip_grads")
     with _Launch(device) as stream:
+        table, n, units = _clip_table(grads, to, device, "clip_grads")
         ws = torch.empty(_lib.CLIP_PARTIALS, dtype=torch.float64, device=device)
         norm = torch.empty((), dtype=torch.float32, device=device)
         _lib.check(_lib.load().apexw_clip_grads(table.data_ptr(), n, units, order, max_norm, ws.data_ptr(),

@@ -888,6 +888,7 @@ int apexw_expert_weight_grad(const void* dy, int64_t ld_dy, const void* x, int64
  */
 #define APEXW_CLIP_UNIT 8192
 #define APEXW_CLIP_PARTIALS 2048
+#define APEXW_CLIP_SMALL 48
 typedef struct apexw_clip_tensor {
   const void* g;
   void* out;
@@ -903,6 +904,9 @@ int apexw_grad_scale(const apexw_clip_tensor* tensors, int32_t n_tensors, int64_
                      float max_norm, void* stream);
 int apexw_clip_grads(const apexw_clip_tensor* tensors, int32_t n_tensors, int64_t n_units, int32_t order,
                      float max_norm, double* workspace, float* norm, void* stream);
+/* the same from the HOST table of up to APEXW_CLIP_SMALL tensors, passed in the launches' arguments */
+int apexw_clip_grads_small(const apexw_clip_tensor* tensors, int32_t n_tensors, int64_t n_units, int32_t order,
+                           float max_norm, double* workspace, float* norm, void* stream);
 
 #ifdef __cplusplus
 }
