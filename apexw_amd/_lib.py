@@ -222,9 +222,11 @@ SIGNATURES = {
     "apexw_layer_norm_backward": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _vp,
                                                  _vp, _vp, _vp, _vp]),
     "apexw_expert_rows": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i64, _i32, _vp, _i32, _i64, _i64, _i64, _i32, _vp,
-                                         _i64, _vp]),
+                                         _i64, _vp, _vp]),
+    "apexw_expert_rows_workspace": (ctypes.c_int64, [_vp, _i64, _vp, _i64, _i64, _i32, _i32, _i64, _i64, _i64]),
     "apexw_expert_weight_grad": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i32, _i64, _i64, _i64, _i32, _vp, _i32,
-                                                _vp]),
+                                                _vp, _vp]),
+    "apexw_expert_weight_grad_workspace": (ctypes.c_int64, [_vp, _i64, _vp, _i64, _i32, _i64, _i64, _i64]),
     "apexw_clip_layout": (ctypes.c_int64, [_vp, _i32]),
     "apexw_grad_norm": (ctypes.c_int, [_vp, _i32, _i64, _i32, _vp, _vp, _vp]),
     "apexw_grad_scale": (ctypes.c_int, [_vp, _i32, _i64, _vp, _f32, _vp]),

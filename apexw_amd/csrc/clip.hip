@@ -93,7 +93,7 @@ template <class Table> APEXW_DEV int find_tensor(const Table& tab, int n, int64_
 // the magnitudes of one thread's 32 elements of a unit joined into acc: sums of |x|^order (1, 2; a sum of
 // squares that leaves the fp32 range is formed again in 64 bits), or (order 0) the largest magnitude's bits,
 // which order NaN above infinity above every number
-template <int GD> APEXW_DEV void unit_norm(const apexw_clip_tensor& t, int64_t e0, int order, double& acc, uint32_t& top) {
+template <int GD, int order> APEXW_DEV void unit_norm(const apexw_clip_tensor& t, int64_t e0, double& acc, uint32_t& top) {
   float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int i = 0; i < kUnit / 2048; ++i) {
@@ -102,8 +102,8 @@ template <int GD> APEXW_DEV void unit_norm(const apexw_clip_tensor& t, int64_t e
     load_some<GD>(t.g, e, t.n - e, x);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      if (order == 2) s[j & 3] = fmaf(x[j], x[j], s[j & 3]);
-      else if (order == 1) s[j & 3] += fabsf(x[j]);
+      if constexpr (order == 2) s[j & 3] = fmaf(x[j], x[j], s[j & 3]);
+      else if constexpr (order == 1) s[j & 3] += fabsf(x[j]);
       else {
         const uint32_t b = __float_as_uint(x[j]) & 0x7FFFFFFFu;
         top = b > top ? b : top;
@@ -151,9 +151,9 @@ APEXW_DEV double join(double acc, uint32_t top, int order, double* red) {
   return s;
 }
 
-template <class Table>
-__global__ __launch_bounds__(256) void grad_norm_kernel(Table tab, int32_t n_tensors,
-                                                        int64_t n_units, int32_t order, double* __restrict__ partial) {
+template <class Table, int order>
+__global__ __launch_bounds__(256) void grad_norm_kernel(Table tab, int32_t n_tensors, int64_t n_units,
+                                                        double* __restrict__ partial) {
   __shared__ double red[4];
   const int64_t u0 = n_units * blockIdx.x / gridDim.x, u1 = n_units * (blockIdx.x + 1) / gridDim.x;
   double acc = 0.0;
@@ -164,9 +164,9 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(Table tab, int32_t n_ten
     for (int64_t u = u0; u < u1; ++u) {
       while (u >= t.first_unit + (t.n + kUnit - 1) / kUnit) t = tab.t[++k];
       const int64_t e0 = (u - t.first_unit) * kUnit;
-      if (t.g_dtype == APEXW_F32) unit_norm<APEXW_F32>(t, e0, order, acc, top);
-      else if (t.g_dtype == APEXW_BF16) unit_norm<APEXW_BF16>(t, e0, order, acc, top);
-      else unit_norm<APEXW_F16>(t, e0, order, acc, top);
+      if (t.g_dtype == APEXW_F32) unit_norm<APEXW_F32, order>(t, e0, acc, top);
+      else if (t.g_dtype == APEXW_BF16) unit_norm<APEXW_BF16, order>(t, e0, acc, top);
+      else unit_norm<APEXW_F16, order>(t, e0, acc, top);
     }
   }
   const double s = join(acc, top, order, red);
@@ -270,10 +270,21 @@ extern "C" int64_t apexw_clip_layout(apexw_clip_tensor* t, int32_t n_tensors) {
 namespace {
 
 template <class Table>
+void norm_partials(const Table& tab, int32_t n_tensors, int64_t n_units, int32_t order, double* workspace, int grid,
+                   hipStream_t stream) {
+  if (order == 2)
+    hipLaunchKernelGGL((grad_norm_kernel<Table, 2>), dim3(grid), dim3(256), 0, stream, tab, n_tensors, n_units, workspace);
+  else if (order == 1)
+    hipLaunchKernelGGL((grad_norm_kernel<Table, 1>), dim3(grid), dim3(256), 0, stream, tab, n_tensors, n_units, workspace);
+  else
+    hipLaunchKernelGGL((grad_norm_kernel<Table, 0>), dim3(grid), dim3(256), 0, stream, tab, n_tensors, n_units, workspace);
+}
+
+template <class Table>
 int clip(const Table& tab, int32_t n_tensors, int64_t n_units, int32_t order, float max_norm, double* workspace,
          float* norm, hipStream_t stream) {
   const int grid = norm_grid(n_units);
-  hipLaunchKernelGGL(grad_norm_kernel<Table>, dim3(grid), dim3(256), 0, stream, tab, n_tensors, n_units, order, workspace);
+  norm_partials(tab, n_tensors, n_units, order, workspace, grid, stream);
   hipLaunchKernelGGL(grad_scale_kernel<Table>, dim3(grid), dim3(256), 0, stream, tab, n_tensors, n_units, order,
                      workspace, grid, (const float*)nullptr, max_norm, norm);
   return hipGetLastError() == hipSuccess ? APEXW_OK : APEXW_ERR_LAUNCH;
@@ -285,8 +296,7 @@ extern "C" int apexw_grad_norm(const apexw_clip_tensor* tensors, int32_t n_tenso
                                double* workspace, float* norm, void* stream) {
   if (!table_ok(tensors, n_tensors, n_units) || !order_ok(order) || !workspace || !norm) return APEXW_ERR_ARG;
   const int grid = norm_grid(n_units);
-  hipLaunchKernelGGL(grad_norm_kernel<Long>, dim3(grid), dim3(256), 0, (hipStream_t)stream, Long{tensors}, n_tensors,
-                     n_units, order, workspace);
+  norm_partials(Long{tensors}, n_tensors, n_units, order, workspace, grid, (hipStream_t)stream);
   hipLaunchKernelGGL(total_norm_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, workspace, grid, order, norm);
   return hipGetLastError() == hipSuccess ? APEXW_OK : APEXW_ERR_LAUNCH;
 }

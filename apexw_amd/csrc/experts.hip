@@ -7,6 +7,7 @@
 //
 // The number of rows of an expert is known on the device alone: each workgroup finds its tiles from the ends.
 // Ends that decrease or pass the buffer count as clamped, so no access leaves it.
+#include <cmath>
 #include <type_traits>
 
 #include "common.h"
@@ -32,6 +33,7 @@ struct ExpertArgs {
   int64_t lda, ldb, sb, ldo;  // row strides; expert stride of the weights
   int64_t rows;
   int32_t experts, n, k;      // out [rows x n] over k, or [experts x n x k]
+  int32_t wide;               // k, or the k that rows copied for their alignment were filled up to with zeros
 };
 
 APEXW_DEV int wave_prefix_max(int x) {
@@ -187,6 +189,7 @@ struct WeightJobs {
 };
 
 struct __attribute__((packed, aligned(2))) Chunk { u32x4 v; };
+struct __attribute__((packed, aligned(4))) Chunk32 { u32x4 v; };
 
 // 8 elements from p, those below cnt (the rest 0), at any element address
 APEXW_DEV u32x4 load_chunk(const uint16_t* p, int cnt) {
@@ -264,12 +267,13 @@ template <int OD> APEXW_DEV void store_elem(void* base, int64_t i, float x) {
 }
 
 // zeros in the rows from `row` on, which belong to no expert
-template <bool kVec> APEXW_DEV void zero_rows(const ExpertArgs& g, int row) {
-  constexpr int V = kVec ? 8 : 1;
+APEXW_DEV void zero_rows(const ExpertArgs& g, int row) {
+  const bool vec = g.n % 8 == 0;
+  const int V = vec ? 8 : 1;
   const int64_t per = g.n / V, n = (g.rows - row) * per, step = (int64_t)gridDim.x * blockDim.x;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += step) {
     uint16_t* p = (uint16_t*)g.out + (row + i / per) * g.ldo + i % per * V;
-    if constexpr (kVec) *APEXW_GLOBAL(u32x4, p) = u32x4{0u, 0u, 0u, 0u};
+    if (vec) APEXW_GLOBAL(Chunk, p)->v = u32x4{0u, 0u, 0u, 0u};
     else *APEXW_GLOBAL(uint16_t, p) = 0;
   }
 }
@@ -416,6 +420,7 @@ template <int BM_, int BN_, int WM_, int WN_, int kStages_, int kPerCU_> struct 
 };
 typedef Shape<256, 256, 128, 64, 2, 1> Large;
 typedef Shape<128, 256, 64, 64, 3, 1> Wide;
+typedef Shape<64, 128, 32, 64, 3, 2> Mid;
 typedef Shape<32, 128, 32, 32, 3, 2> Small;
 
 // The tiles of a workgroup, each A B^T over its k, as one stream of stages: the copies of a tile's first
@@ -582,9 +587,18 @@ APEXW_DEV void stream(const ExpertArgs& g, Jobs& jobs, Place&& locate, uint16_t*
           const int r = kRows * t + lane / kChunks, c = lane % kChunks;
           const u32x4 w = *(const u32x4*)&mine[(r * kChunks + (c ^ (r & (kChunks - 1)))) * 8];
           const int row = wm + 16 * i + r, col = wn + 16 * j0 + kPer * c;
-          if (row < rows && col < cols) {
-            if constexpr (OD == APEXW_F32) *APEXW_GLOBAL(u32x4, (float*)g.out + out0 + row * g.ldo + col) = w;
-            else *APEXW_GLOBAL(u32x4, (uint16_t*)g.out + out0 + row * g.ldo + col) = w;
+          if (row >= rows || col >= cols) continue;
+          const int64_t o = out0 + row * g.ldo + col;
+          if (col + kPer <= cols) {   // at any element address: rows of odd width start anywhere
+            if constexpr (OD == APEXW_F32) APEXW_GLOBAL(Chunk32, (float*)g.out + o)->v = w;
+            else APEXW_GLOBAL(Chunk, (uint16_t*)g.out + o)->v = w;
+          } else {
+#pragma unroll
+            for (int x = 0; x < kPer; ++x)
+              if (col + x < cols) {
+                if constexpr (OD == APEXW_F32) APEXW_GLOBAL(uint32_t, g.out)[o + x] = w[x];
+                else APEXW_GLOBAL(uint16_t, g.out)[o + x] = (uint16_t)(w[x >> 1] >> (16 * (x & 1)));
+              }
           }
         }
       }
@@ -610,12 +624,14 @@ template <class S, bool kBKN, int DT>
 __global__ __launch_bounds__(S::kThreads, 2) void expert_rows_stream_kernel(ExpertArgs g) {
   __shared__ __attribute__((aligned(16))) uint16_t lds[S::kLds];
   RowJobs<true> jobs(g, S::BM, S::BN);
-  zero_rows<true>(g, jobs.rows);
+  zero_rows(g, jobs.rows);
   stream<S, false, kBKN, DT, DT, true>(g, jobs, [&](const Job& j, Span& a, Span& b, int& rows, int& cols, int64_t& out0) {
     const int64_t row = j.first + j.row, col = j.col * S::BN;
     rows = j.last - (int)row, cols = g.n - (int)col, out0 = row * g.ldo + col;
-    a.set<false>(g.a + row * g.lda, g.lda, rows, g.k, S::BM);
-    b.set<kBKN>(g.b + j.expert * g.sb + (kBKN ? col : col * g.ldb), g.ldb, cols, g.k, S::BN);
+    a.set<false>(g.a + row * g.lda, g.lda, rows, g.wide, S::BM);
+    // whole chunks of columns: rows of another width have been copied to such
+    b.set<kBKN>(g.b + j.expert * g.sb + (kBKN ? col : col * g.ldb), g.ldb, kBKN ? (cols + 7) / 8 * 8 : cols,
+                kBKN ? g.k : g.wide, S::BN);
   }, lds);
 }
 
@@ -627,9 +643,33 @@ __global__ __launch_bounds__(S::kThreads, 2) void expert_weight_stream_kernel(Ex
   stream<S, true, true, DT, OD, false>(g, jobs, [&](const Job& j, Span& a, Span& b, int& rows, int& cols, int64_t& out0) {
     const int64_t row = j.row, col = j.col * S::BN, first = j.first;
     rows = g.n - (int)row, cols = g.k - (int)col, out0 = (j.expert * (int64_t)g.n + row) * g.k + col;
-    a.set<true>(g.a + first * g.lda + row, g.lda, rows, j.last - j.first, S::BM);
-    b.set<true>(g.b + first * g.ldb + col, g.ldb, cols, j.last - j.first, S::BN);
+    a.set<true>(g.a + first * g.lda + row, g.lda, (rows + 7) / 8 * 8, j.last - j.first, S::BM);
+    b.set<true>(g.b + first * g.ldb + col, g.ldb, (cols + 7) / 8 * 8, j.last - j.first, S::BN);
   }, lds);
+}
+
+// Rows of `width` elements, ld apart, groups of `high` of them `step` apart, copied to rows of whole chunks with
+// zeros behind their end: what the asynchronous copies need of an operand of another width or address.
+struct Pad {
+  const uint16_t* src;
+  int64_t ld, step, high, rows;
+  int32_t width;
+  u32x4* dst;
+};
+
+// I: the index type; 32-bit quotients where all chunks are counted in 32 bits
+template <class I> APEXW_DEV void pad_rows(const Pad& p) {
+  const I per = (I)((p.width + 7) / 8), high = (I)p.high, n = (I)p.rows * per, stride = (I)gridDim.x * 256;
+  for (I i = (I)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
+    const I row = i / per, c = i - row * per, group = row / high;
+    p.dst[i] = load_chunk(p.src + (int64_t)group * p.step + (int64_t)(row - group * high) * p.ld + (int64_t)c * 8,
+                          clamp8(p.width - (int64_t)c * 8));
+  }
+}
+__global__ __launch_bounds__(256) void pad_kernel(Pad a, Pad b) {
+  const Pad& p = blockIdx.y ? b : a;
+  if (p.rows * ((p.width + 7) / 8) < (1ll << 31)) pad_rows<uint32_t>(p);
+  else pad_rows<uint64_t>(p);
 }
 
 // ---------------------------------------------------------------------------
@@ -691,7 +731,7 @@ APEXW_DEV void tile(const uint16_t* a, int64_t lda, const uint16_t* b, int64_t l
 template <bool kBKN, int DT>
 __global__ __launch_bounds__(256) void expert_rows_kernel(ExpertArgs g) {
   RowJobs<false> jobs(g, kTile, kTile);
-  zero_rows<false>(g, jobs.rows);
+  zero_rows(g, jobs.rows);
   const Job j = jobs.get(0);
   if (j.expert < 0) return;
   const int64_t row = j.first + j.row, col = (int64_t)j.col * kTile;
@@ -729,6 +769,35 @@ void launch_rows(const ExpertArgs& g, bool kn, hipStream_t s) {
   else hipLaunchKernelGGL((expert_rows_stream_kernel<S, false, DT>), grid, block, 0, s, g);
 }
 
+// The shape of a rows product's tiles: the one whose stages take the least time over the rounds that its tiles
+// need.  A stage takes, with every workgroup of the chip at work and with few: 256 x 256 1.75 and 0.95 us,
+// 128 x 256 1.0 and 0.65, 64 x 128 0.72 and 0.45, 32 x 128 0.55 and 0.42 (from products of 64 to 4096 rows with
+// 4096 x 4096 weights).  An expert's last tile is taken as half full.  Measured by shape, the smallest first:
+// 4096 rows of one expert 287, 188, 133, 121 us; 1024 rows 76, 51, 59, 94; 64 rows 32, 34, 46, 64; 8192 rows in
+// 8 experts of 2048 x 2048 180, 121, 94, 95; 512 rows in 16 experts of 4096 x 2048 63, 80, 70, 102.
+template <class S> float rows_cost(const ExpertArgs& g, float most, float least) {
+  const float used = (float)(g.rows < g.experts ? g.rows : g.experts);
+  const float high = g.experts == 1 ? (float)((g.rows + S::BM - 1) / S::BM) : (float)g.rows / S::BM + 0.5f * used;
+  const float rounds = high * (float)((g.n + S::BN - 1) / S::BN) / (float)(apexw_cu_count() * S::kPerCU);
+  return rounds <= 1.0f ? least + (most - least) * rounds : most * ceilf(4.0f * rounds) * 0.25f;
+}
+
+int rows_shape(const ExpertArgs& g) {
+  const float cost[4] = {rows_cost<Small>(g, 0.55f, 0.42f), rows_cost<Mid>(g, 0.72f, 0.45f),
+                         rows_cost<Wide>(g, 1.0f, 0.65f), rows_cost<Large>(g, 1.75f, 0.95f)};
+  int best = 0;
+  for (int i = 1; i < 4; ++i)
+    if (cost[i] < cost[best]) best = i;
+  return best;
+}
+
+template <int DT> void launch_rows_as(const ExpertArgs& g, bool kn, int shape, hipStream_t s) {
+  if (shape == 3) launch_rows<Large, DT>(g, kn, s);
+  else if (shape == 2) launch_rows<Wide, DT>(g, kn, s);
+  else if (shape == 1) launch_rows<Mid, DT>(g, kn, s);
+  else launch_rows<Small, DT>(g, kn, s);
+}
+
 template <class S, int DT>
 void launch_weight(const ExpertArgs& g, int32_t out_dtype, hipStream_t s) {
   const int64_t most = (int64_t)((g.n + S::BM - 1) / S::BM) * ((g.k + S::BN - 1) / S::BN) * g.experts;
@@ -737,15 +806,51 @@ void launch_weight(const ExpertArgs& g, int32_t out_dtype, hipStream_t s) {
   else hipLaunchKernelGGL((expert_weight_stream_kernel<S, DT, DT>), grid, block, 0, s, g);
 }
 
+// An operand to be copied to `at` as rows of whole chunks: advances `at`, replaces address and strides
+Pad pad(const uint16_t*& p, int64_t& ld, int64_t& step, int64_t high, int64_t rows, int32_t width, uint16_t*& at) {
+  const int64_t wide = (width + 7) / 8 * 8;
+  const Pad job{p, ld, step, high, rows, width, (u32x4*)at};
+  p = at, ld = wide, step = high * wide;
+  at += rows * wide;
+  return job;
+}
+void launch_pad(const Pad& a, const Pad& b, hipStream_t s) {
+  const int64_t most = (a.rows * a.width > b.rows * b.width ? a.rows * a.width : b.rows * b.width) / 2048 + 1;
+  hipLaunchKernelGGL(pad_kernel, dim3((unsigned)(most < 8192 ? most : 8192), b.rows ? 2 : 1), dim3(256), 0, s, a, b);
+}
+
+// Operands of other widths are copied where the products take longer on the general kernel than the copies:
+// from about 32 rows an expert on (the weights, copied whole, are most of them).  4096 rows of 500 elements
+// in 8 experts of 386: 21.9 us on the general kernel.
+bool worth_padding(int64_t rows, int32_t experts) { return rows >= 32 * (int64_t)experts; }
+int64_t padded(int64_t rows, int64_t width) { return rows * ((width + 7) / 8 * 8) * 2; }
+
 bool sizes_ok(int64_t rows, int32_t experts, int64_t n, int64_t k) {
   return rows >= 0 && rows <= INT32_MAX && experts > 0 && n > 0 && k > 0 && n <= INT32_MAX - 256 && k <= INT32_MAX - 256;
 }
 
 }  // namespace
 
+extern "C" int64_t apexw_expert_rows_workspace(const void* a, int64_t lda, const void* w, int64_t w_row_stride,
+                                               int64_t w_expert_stride, int32_t w_order, int32_t experts, int64_t rows,
+                                               int64_t k, int64_t n) {
+  if (!sizes_ok(rows, experts, n, k)) return -APEXW_ERR_ARG;
+  const bool kn = w_order == APEXW_EXPERT_KN;
+  const bool fast_a = chunks_ok(a, lda, k), fast_w = chunks_ok(w, w_row_stride, kn ? n : k, w_expert_stride);
+  if ((fast_a && fast_w) || !worth_padding(rows, experts)) return 0;
+  return (fast_a ? 0 : padded(rows, k)) + (fast_w ? 0 : padded(experts * (kn ? k : n), kn ? n : k));
+}
+
+extern "C" int64_t apexw_expert_weight_grad_workspace(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x,
+                                                      int32_t experts, int64_t rows, int64_t n, int64_t k) {
+  if (!sizes_ok(rows, experts, n, k)) return -APEXW_ERR_ARG;
+  if (!worth_padding(rows, experts)) return 0;
+  return (chunks_ok(dy, ld_dy, n) ? 0 : padded(rows, n)) + (chunks_ok(x, ld_x, k) ? 0 : padded(rows, k));
+}
+
 extern "C" int apexw_expert_rows(const void* a, int64_t lda, const void* w, int64_t w_row_stride, int64_t w_expert_stride,
                                  int32_t w_order, const int32_t* ends, int32_t experts, int64_t rows, int64_t k,
-                                 int64_t n, int32_t dtype, void* out, int64_t ldo, void* stream) {
+                                 int64_t n, int32_t dtype, void* out, int64_t ldo, void* workspace, void* stream) {
   if (!a || !w || !ends || !out || !sizes_ok(rows, experts, n, k)) return APEXW_ERR_ARG;
   if (lda < 0 || w_row_stride < 0 || w_expert_stride < 0 || ldo < n) return APEXW_ERR_ARG;
   if (w_order != APEXW_EXPERT_NK && w_order != APEXW_EXPERT_KN) return APEXW_ERR_ARG;
@@ -757,21 +862,27 @@ extern "C" int apexw_expert_rows(const void* a, int64_t lda, const void* w, int6
   if (rows > INT32_MAX - 256 || (rows / Small::BM + (rows < experts ? rows : experts)) * ((n + Small::BN - 1) / Small::BN) > INT32_MAX)
     return APEXW_ERR_SIZE;
   ExpertArgs g{(const uint16_t*)a, (const uint16_t*)w, ends, out, lda, w_row_stride, w_expert_stride, ldo, rows,
-               experts, (int32_t)n, (int32_t)k};
+               experts, (int32_t)n, (int32_t)k, (int32_t)k};
   const dim3 grid((unsigned)((tiles + 7) / 8 * 8)), block(256);
   hipStream_t s = (hipStream_t)stream;
   const bool kn = w_order == APEXW_EXPERT_KN;
-  if (chunks_ok(a, lda, k) && chunks_ok(w, w_row_stride, kn ? n : k, w_expert_stride) && chunks_ok(out, ldo, n)) {
-    const int shape = rows >= (int64_t)experts * 512 ? 2 : rows >= (int64_t)experts * 48 ? 1 : 0;
-    if (dtype == APEXW_BF16) {
-      if (shape == 2) launch_rows<Large, APEXW_BF16>(g, kn, s);
-      else if (shape == 1) launch_rows<Wide, APEXW_BF16>(g, kn, s);
-      else launch_rows<Small, APEXW_BF16>(g, kn, s);
-    } else {
-      if (shape == 2) launch_rows<Large, APEXW_F16>(g, kn, s);
-      else if (shape == 1) launch_rows<Wide, APEXW_F16>(g, kn, s);
-      else launch_rows<Small, APEXW_F16>(g, kn, s);
-    }
+  bool fast_a = chunks_ok(a, lda, k), fast_w = chunks_ok(w, w_row_stride, kn ? n : k, w_expert_stride);
+  if (workspace && (!fast_a || !fast_w) && worth_padding(rows, experts)) {
+    if ((uintptr_t)workspace & 15u) return APEXW_ERR_ALIGN;
+    uint16_t* at = (uint16_t*)workspace;
+    int64_t none = 0;
+    Pad jobs[2] = {};
+    int count = 0;
+    if (!fast_a) jobs[count++] = pad(g.a, g.lda, none, rows, rows, (int32_t)k, at);
+    if (!fast_w) jobs[count++] = pad(g.b, g.ldb, g.sb, kn ? k : n, experts * (kn ? k : n), (int32_t)(kn ? n : k), at);
+    launch_pad(jobs[0], jobs[1], s);
+    g.wide = (int32_t)((k + 7) / 8 * 8);
+    fast_a = fast_w = true;
+  }
+  if (fast_a && fast_w) {
+    const int shape = rows_shape(g);
+    if (dtype == APEXW_BF16) launch_rows_as<APEXW_BF16>(g, kn, shape, s);
+    else launch_rows_as<APEXW_F16>(g, kn, shape, s);
     return hipGetLastError() == hipSuccess ? APEXW_OK : APEXW_ERR_LAUNCH;
   }
   if (dtype == APEXW_BF16) {
@@ -786,7 +897,7 @@ extern "C" int apexw_expert_rows(const void* a, int64_t lda, const void* w, int6
 
 extern "C" int apexw_expert_weight_grad(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, const int32_t* ends,
                                         int32_t experts, int64_t rows, int64_t n, int64_t k, int32_t dtype, void* dw,
-                                        int32_t dw_dtype, void* stream) {
+                                        int32_t dw_dtype, void* workspace, void* stream) {
   if (!ends || !dw || !sizes_ok(rows, experts, n, k) || (rows > 0 && (!dy || !x))) return APEXW_ERR_ARG;
   if (ld_dy < 0 || ld_x < 0) return APEXW_ERR_ARG;
   if ((dtype != APEXW_BF16 && dtype != APEXW_F16) || (dw_dtype != dtype && dw_dtype != APEXW_F32)) return APEXW_ERR_DTYPE;
@@ -795,10 +906,22 @@ extern "C" int apexw_expert_weight_grad(const void* dy, int64_t ld_dy, const voi
   const int64_t tiles = (((n + kTile - 1) / kTile) * ((k + kTile - 1) / kTile) + 7) / 8 * 8 * experts;
   if (tiles > INT32_MAX || rows > INT32_MAX - 256) return APEXW_ERR_SIZE;
   ExpertArgs g{(const uint16_t*)dy, (const uint16_t*)x, ends, dw, ld_dy, ld_x, 0, k, rows, experts, (int32_t)n,
-               (int32_t)k};
+               (int32_t)k, 0};
   const dim3 grid((unsigned)tiles), block(256);
   hipStream_t s = (hipStream_t)stream;
-  if (chunks_ok(dy, ld_dy, n) && chunks_ok(x, ld_x, k) && chunks_ok(dw, k, k)) {
+  const bool fast_y = chunks_ok(dy, ld_dy, n), fast_x = chunks_ok(x, ld_x, k);
+  const bool copies = workspace && (!fast_y || !fast_x) && worth_padding(rows, experts);
+  if (copies) {
+    if ((uintptr_t)workspace & 15u) return APEXW_ERR_ALIGN;
+    uint16_t* at = (uint16_t*)workspace;
+    int64_t none = 0;
+    Pad jobs[2] = {};
+    int count = 0;
+    if (!fast_y) jobs[count++] = pad(g.a, g.lda, none, rows, rows, (int32_t)n, at);
+    if (!fast_x) jobs[count++] = pad(g.b, g.ldb, none, rows, rows, (int32_t)k, at);
+    launch_pad(jobs[0], jobs[1], s);
+  }
+  if (copies || (fast_y && fast_x)) {
     if (dtype == APEXW_BF16) launch_weight<Large, APEXW_BF16>(g, dw_dtype, s);
     else launch_weight<Large, APEXW_F16>(g, dw_dtype, s);
     return hipGetLastError() == hipSuccess ? APEXW_OK : APEXW_ERR_LAUNCH;

@@ -146,9 +146,12 @@ struct Library {
                        int64_t, int32_t, int32_t, void*, void*, void*, float*, void*);
   int64_t (*norm_workspace)(int64_t, int64_t);
   int (*expert_rows)(const void*, int64_t, const void*, int64_t, int64_t, int32_t, const int32_t*, int32_t, int64_t,
-                     int64_t, int64_t, int32_t, void*, int64_t, void*);
+                     int64_t, int64_t, int32_t, void*, int64_t, void*, void*);
+  int64_t (*expert_rows_workspace)(const void*, int64_t, const void*, int64_t, int64_t, int32_t, int32_t, int64_t,
+                                   int64_t, int64_t);
   int (*expert_weight_grad)(const void*, int64_t, const void*, int64_t, const int32_t*, int32_t, int64_t, int64_t,
-                            int64_t, int32_t, void*, int32_t, void*);
+                            int64_t, int32_t, void*, int32_t, void*, void*);
+  int64_t (*expert_weight_grad_workspace)(const void*, int64_t, const void*, int64_t, int32_t, int64_t, int64_t, int64_t);
   int64_t (*clip_layout)(ClipTensor*, int32_t);
   int (*clip_grads)(const ClipTensor*, int32_t, int64_t, int32_t, float, double*, float*, void*);
   int (*clip_grads_small)(const ClipTensor*, int32_t, int64_t, int32_t, float, double*, float*, void*);
@@ -333,10 +336,16 @@ PyObject* expert_rows(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       w.size(0) != ends.size(0) || w.size(transposed ? 1 : 2) != a.size(1) || a.size(0) == 0)
     return none_or_error();
   const int64_t n = w.size(transposed ? 2 : 1);
+  const auto experts = static_cast<int32_t>(ends.size(0));
+  const int64_t bytes = lib.expert_rows_workspace(a.data_ptr(), a.stride(0), w.data_ptr(), w.stride(1), w.stride(0),
+                                                  transposed, experts, a.size(0), a.size(1), n);
+  if (bytes < 0) return PyLong_FromLong(static_cast<long>(-bytes));
   const at::Tensor out = at::empty({a.size(0), n}, a.options());
+  at::Tensor ws;
+  if (bytes > 0) ws = at::empty({bytes}, a.options().dtype(at::kByte));
   const int status = lib.expert_rows(a.data_ptr(), a.stride(0), w.data_ptr(), w.stride(1), w.stride(0), transposed,
-                                     static_cast<const int32_t*>(ends.data_ptr()), static_cast<int32_t>(ends.size(0)),
-                                     a.size(0), a.size(1), n, code, out.data_ptr(), n, where.stream);
+                                     static_cast<const int32_t*>(ends.data_ptr()), experts, a.size(0), a.size(1), n, code,
+                                     out.data_ptr(), n, const_cast<void*>(address(ws)), where.stream);
   return status ? PyLong_FromLong(status) : THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS
 }
@@ -354,11 +363,17 @@ PyObject* expert_weight_grad(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   if (!expert_operand(dy, where, &code) || !expert_operand(x, where, &x_code) || code != x_code ||
       !expert_ends(ends, where) || dy.size(0) != x.size(0) || dy.size(0) == 0)
     return none_or_error();
+  const auto experts = static_cast<int32_t>(ends.size(0));
+  const int64_t bytes = lib.expert_weight_grad_workspace(dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), experts,
+                                                         dy.size(0), dy.size(1), x.size(1));
+  if (bytes < 0) return PyLong_FromLong(static_cast<long>(-bytes));
+  at::Tensor ws;
+  if (bytes > 0) ws = at::empty({bytes}, dy.options().dtype(at::kByte));
   const at::Tensor dw = at::empty({ends.size(0), dy.size(1), x.size(1)}, fp32 ? dy.options().dtype(at::kFloat) : dy.options());
   const int status = lib.expert_weight_grad(dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0),
-                                            static_cast<const int32_t*>(ends.data_ptr()),
-                                            static_cast<int32_t>(ends.size(0)), dy.size(0), dy.size(1), x.size(1), code,
-                                            dw.data_ptr(), fp32 ? 0 : code, where.stream);
+                                            static_cast<const int32_t*>(ends.data_ptr()), experts, dy.size(0),
+                                            dy.size(1), x.size(1), code, dw.data_ptr(), fp32 ? 0 : code,
+                                            const_cast<void*>(address(ws)), where.stream);
   return status ? PyLong_FromLong(status) : THPVariable_Wrap(dw);
   END_HANDLE_TH_ERRORS
 }

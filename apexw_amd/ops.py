@@ -22,7 +22,8 @@ _raw_stream = torch._C._cuda_getCurrentRawStream
 _current = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else None
 _NATIVE = None
 _ENTRIES = ("apexw_layer_norm_forward", "apexw_layer_norm_backward", "apexw_layer_norm_workspace", "apexw_expert_rows",
-            "apexw_expert_weight_grad", "apexw_clip_layout", "apexw_clip_grads", "apexw_clip_grads_small")
+            "apexw_expert_rows_workspace", "apexw_expert_weight_grad", "apexw_expert_weight_grad_workspace",
+            "apexw_clip_layout", "apexw_clip_grads", "apexw_clip_grads_small")
 
 
 def _native(t):
@@ -229,6 +230,12 @@ def _check_weight(weight, like):
     _on_device(weight, "expert_matmul: weight", like.device)
 
 
+def _workspace(size, device):
+    if size < 0:
+        _lib.check(-size, "expert_matmul")
+    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
+
+
 def _row_products(a, weight, ends, outer_first):
     """out[i] = W_e a[i] with W_e = weight[e] (outer_first) or its transpose."""
     w = weight if outer_first else weight.transpose(1, 2)      # [experts, n, k]
@@ -243,10 +250,11 @@ def _row_products(a, weight, ends, outer_first):
     with _Launch(a.device) as stream:
         out = torch.empty((a.shape[0], w.shape[1]), dtype=a.dtype, device=a.device)
         if a.shape[0]:
-            _lib.check(lib.apexw_expert_rows(a.data_ptr(), a.stride(0), w.data_ptr(), ldw, w.stride(0), order,
-                                             ends.data_ptr(), ends.shape[0], a.shape[0], a.shape[1], w.shape[1],
-                                             _CODE[a.dtype], out.data_ptr(), out.shape[1], stream),
-                       "apexw_expert_rows")
+            operands = (a.data_ptr(), a.stride(0), w.data_ptr(), ldw, w.stride(0), order)
+            sizes = (ends.shape[0], a.shape[0], a.shape[1], w.shape[1])
+            ws = _workspace(lib.apexw_expert_rows_workspace(*operands, *sizes), a.device)
+            _lib.check(lib.apexw_expert_rows(*operands, ends.data_ptr(), *sizes, _CODE[a.dtype], out.data_ptr(),
+                                             out.shape[1], _ptr(ws), stream), "apexw_expert_rows")
     return out
 
 
@@ -304,9 +312,11 @@ def expert_matmul_weight_grad(dy, x, ends, dtype=None):
     lib = _lib.load()
     with _Launch(dy.device) as stream:
         dw = torch.empty((ends.shape[0], dy.shape[1], x.shape[1]), dtype=dtype, device=dy.device)
-        _lib.check(lib.apexw_expert_weight_grad(_ptr(dy), dy.stride(0), _ptr(x), x.stride(0), ends.data_ptr(),
-                                                ends.shape[0], dy.shape[0], dy.shape[1], x.shape[1], _CODE[dy.dtype],
-                                                dw.data_ptr(), _CODE[dtype], stream), "apexw_expert_weight_grad")
+        operands = (_ptr(dy), dy.stride(0), _ptr(x), x.stride(0))
+        sizes = (ends.shape[0], dy.shape[0], dy.shape[1], x.shape[1])
+        ws = _workspace(lib.apexw_expert_weight_grad_workspace(*operands, *sizes), dy.device)
+        _lib.check(lib.apexw_expert_weight_grad(*operands, ends.data_ptr(), *sizes, _CODE[dy.dtype], dw.data_ptr(),
+                                                _CODE[dtype], _ptr(ws), stream), "apexw_expert_weight_grad")
     return dw
 
 

@@ -864,16 +864,24 @@ int apexw_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, 
  *   APEXW_EXPERT_KN: at .. + l w_row_stride + j (the rows' gradient of NK weights, and the other way round).
  * apexw_expert_weight_grad: dw[e] ([n x k], contiguous, dtype or F32) = sum over e's rows of dy[i] x[i]^T, 0
  *   for an expert without rows; rows behind the last end are not read.
- * Strides are in elements.  APEXW_ERR_SIZE: more tiles than a launch holds.
+ * Strides are in elements, of any alignment.  APEXW_ERR_SIZE: more tiles than a launch holds.
+ * workspace (16-byte aligned, in any state): as many bytes as the _workspace call answers, 0 for most
+ * operands; widths that are no multiple of 8, or rows at other addresses than multiples of 16 bytes, are
+ * copied there first where that pays, and slower without (NULL).
  */
 #define APEXW_EXPERT_NK 0
 #define APEXW_EXPERT_KN 1
 int apexw_expert_rows(const void* a, int64_t lda, const void* w, int64_t w_row_stride, int64_t w_expert_stride,
                       int32_t w_order, const int32_t* ends, int32_t experts, int64_t rows, int64_t k, int64_t n,
-                      int32_t dtype, void* out, int64_t ldo, void* stream);
+                      int32_t dtype, void* out, int64_t ldo, void* workspace, void* stream);
+int64_t apexw_expert_rows_workspace(const void* a, int64_t lda, const void* w, int64_t w_row_stride,
+                                    int64_t w_expert_stride, int32_t w_order, int32_t experts, int64_t rows, int64_t k,
+                                    int64_t n);
 int apexw_expert_weight_grad(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, const int32_t* ends,
                              int32_t experts, int64_t rows, int64_t n, int64_t k, int32_t dtype, void* dw,
-                             int32_t dw_dtype, void* stream);
+                             int32_t dw_dtype, void* workspace, void* stream);
+int64_t apexw_expert_weight_grad_workspace(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, int32_t experts,
+                                           int64_t rows, int64_t n, int64_t k);
 
 /*
  * The clip of a list of gradients by their global norm, with torch.nn.utils.clip_grad_norm_'s arithmetic:

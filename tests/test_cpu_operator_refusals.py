@@ -72,20 +72,20 @@ def test_entry_points_refuse_without_launching():
     assert lib.apexw_layer_norm_workspace(5, 8) >= 80
 
     rows, grad = lib.apexw_expert_rows, lib.apexw_expert_weight_grad
-    assert rows(None, 8, ok, 8, 64, 0, ok, 2, 4, 8, 8, BF16, ok, 8, None) == 1
-    assert rows(ok, 8, ok, 8, 64, 2, ok, 2, 4, 8, 8, BF16, ok, 8, None) == 1
-    assert rows(ok, 8, ok, 8, 64, 0, ok, 0, 4, 8, 8, BF16, ok, 8, None) == 1
-    assert rows(ok, 8, ok, 8, 64, 0, ok, 2, 4, 0, 8, BF16, ok, 8, None) == 1
-    assert rows(ok, 8, ok, 8, 64, 0, ok, 2, 4, 8, 8, BF16, ok, 7, None) == 1
-    assert rows(ok, 8, ok, 8, 64, 0, ok, 2, 4, 8, 8, F32, ok, 8, None) == 2
-    assert rows(ok + 1, 8, ok, 8, 64, 0, ok, 2, 4, 8, 8, BF16, ok, 8, None) == 4
-    assert rows(ok, 8, ok, 8, 64, 0, ok + 2, 2, 4, 8, 8, BF16, ok, 8, None) == 4
-    assert rows(ok, 8, ok, 8, 64, 0, ok, 2, 2 ** 31 - 1, 8, 2 ** 31 - 300, BF16, ok, 2 ** 31, None) == 5
-    assert grad(ok, 8, ok, 8, ok, 2, 4, 8, 8, BF16, ok, F16, None) == 2
-    assert grad(ok, 8, ok, 8, ok, 2, 4, 8, 8, F32, ok, F32, None) == 2
-    assert grad(ok, 8, ok, 8, ok, 2, 4, 8, 8, BF16, ok + 2, F32, None) == 4
-    assert grad(None, 8, ok, 8, ok, 2, 4, 8, 8, BF16, ok, F32, None) == 1
-    assert grad(ok, 8, ok, 8, ok, 2 ** 20, 4, 2 ** 20, 2 ** 20, BF16, ok, F32, None) == 5
+    assert rows(None, 8, ok, 8, 64, 0, ok, 2, 4, 8, 8, BF16, ok, 8, None, None) == 1
+    assert rows(ok, 8, ok, 8, 64, 2, ok, 2, 4, 8, 8, BF16, ok, 8, None, None) == 1
+    assert rows(ok, 8, ok, 8, 64, 0, ok, 0, 4, 8, 8, BF16, ok, 8, None, None) == 1
+    assert rows(ok, 8, ok, 8, 64, 0, ok, 2, 4, 0, 8, BF16, ok, 8, None, None) == 1
+    assert rows(ok, 8, ok, 8, 64, 0, ok, 2, 4, 8, 8, BF16, ok, 7, None, None) == 1
+    assert rows(ok, 8, ok, 8, 64, 0, ok, 2, 4, 8, 8, F32, ok, 8, None, None) == 2
+    assert rows(ok + 1, 8, ok, 8, 64, 0, ok, 2, 4, 8, 8, BF16, ok, 8, None, None) == 4
+    assert rows(ok, 8, ok, 8, 64, 0, ok + 2, 2, 4, 8, 8, BF16, ok, 8, None, None) == 4
+    assert rows(ok, 8, ok, 8, 64, 0, ok, 2, 2 ** 31 - 1, 8, 2 ** 31 - 300, BF16, ok, 2 ** 31, None, None) == 5
+    assert grad(ok, 8, ok, 8, ok, 2, 4, 8, 8, BF16, ok, F16, None, None) == 2
+    assert grad(ok, 8, ok, 8, ok, 2, 4, 8, 8, F32, ok, F32, None, None) == 2
+    assert grad(ok, 8, ok, 8, ok, 2, 4, 8, 8, BF16, ok + 2, F32, None, None) == 4
+    assert grad(None, 8, ok, 8, ok, 2, 4, 8, 8, BF16, ok, F32, None, None) == 1
+    assert grad(ok, 8, ok, 8, ok, 2 ** 20, 4, 2 ** 20, 2 ** 20, BF16, ok, F32, None, None) == 5
 
     norm, scale, clip = lib.apexw_grad_norm, lib.apexw_grad_scale, lib.apexw_clip_grads
     assert norm(ok, 1, 1, 3, ok, ok, None) == 1 and norm(ok, 1, 1, 2, None, ok, None) == 1
