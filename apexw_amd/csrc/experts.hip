@@ -34,6 +34,10 @@ struct ExpertArgs {
   int64_t rows;
   int32_t experts, n, k;      // out [rows x n] over k, or [experts x n x k]
   int32_t wide;               // k, or the k that rows copied for their alignment were filled up to with zeros
+  // a product whose tiles are few is cut along what it sums over: `splits` parts (of `part` k in a rows product,
+  // of an expert's rows in a weight grad) leave fp32 sums split_stride elements apart, which join_* add up
+  int32_t splits, part;
+  int64_t split_stride;
 };
 
 APEXW_DEV int wave_prefix_max(int x) {
@@ -69,6 +73,7 @@ struct Job {
   int expert;          // -1: none
   int first, last;     // its rows
   int row, col;        // the tile's first row among its rows; its place across, in tiles
+  int split;           // which part of what is summed over
 };
 
 // Tile (row, column) of index t among rows x cols tiles: bands of 8 tile rows, column by column, so that the
@@ -82,7 +87,7 @@ APEXW_DEV void place(int t, int rows, int cols, int& r, int& c) {
 
 // The tiles of a rows product, expert by expert.  Workgroups go to the 8 XCDs in turn: each XCD gets a
 // contiguous part of the tiles, of which its workgroups take every (number of them)th.
-template <bool kSplit> struct RowJobs {
+template <bool kCut> struct RowJobs {
   const ExpertArgs& g;
   int size, cols;              // rows of a tile, tiles across
   int begin, end, upto;        // per lane, of the first 64 experts: rows, and tiles up to and with it
@@ -111,17 +116,18 @@ template <bool kSplit> struct RowJobs {
   // each time, since a tile of few rows takes less time and stands at the same place of every column; where
   // the last round has tiles for less than half or a quarter of them, it takes halves or quarters of tiles.
   __device__ __forceinline__ Job get(int i) {
-    Job j{-1, 0, 0, 0, 0};
-    const int part = (all + 7) / 8, from = (int)(blockIdx.x % 8) * part, groups = (int)(gridDim.x / 8);
-    const int mine = all - from < part ? all - from : part;
+    Job j{-1, 0, 0, 0, 0, 0};
+    const int units = all * g.splits, part = (units + 7) / 8, from = (int)(blockIdx.x % 8) * part;
+    const int groups = (int)(gridDim.x / 8), mine = units - from < part ? units - from : part;
     int in = i * groups + (int)((blockIdx.x / 8 + 5u * i) % groups), sub = 0, cut = 1;
     const int rest = mine - i * groups;
-    if (kSplit && rest > 0 && 2 * rest <= groups) {
+    if (kCut && g.splits == 1 && rest > 0 && 2 * rest <= groups) {
       cut = 4 * rest <= groups ? 4 : 2;
       sub = (in - i * groups) % cut, in = i * groups + (in - i * groups) / cut;
     }
     if (in >= mine) return j;
-    const int t = from + in;
+    const int t = (from + in) / g.splits;
+    j.split = (from + in) % g.splits;
     if (g.experts <= 64) {
       find_at(t, 0, j);
     } else {
@@ -143,6 +149,9 @@ template <bool kSplit> struct RowJobs {
   }
 };
 
+// the rows of a part of an expert's: whole stages
+APEXW_DEV int split_rows(int rows, int splits) { return ((rows + splits - 1) / splits + 63) / 64 * 64; }
+
 // The tiles of a weight gradient.  Experts differ in rows, and so their tiles in work: each XCD takes a part of
 // every expert's tiles, and up to 64 experts come in the order of their rows, the most first, so that the
 // last tiles are short.
@@ -154,7 +163,7 @@ struct WeightJobs {
 
   __device__ __forceinline__ WeightJobs(const ExpertArgs& a, int bm, int bn)
       : g(a), size(bm), high((a.n + bm - 1) / bm), cols((a.k + bn - 1) / bn) {
-    part = (high * cols + 7) / 8;
+    part = (high * cols * g.splits + 7) / 8;
     int row = 0;
     look(g, 0, row, begin, end);
     rank = 0;
@@ -165,7 +174,7 @@ struct WeightJobs {
     next_rank = __builtin_popcountll(__ballot(end > begin));
   }
   __device__ __forceinline__ Job get(int i) const {
-    Job j{-1, 0, 0, 0, 0};
+    Job j{-1, 0, 0, 0, 0, 0};
     // forth and back, so that the first workgroups do not get the most rows in every round
     const int groups = (int)(gridDim.x / 8), w = (int)(blockIdx.x / 8), in = i * groups + (i & 1 ? groups - 1 - w : w);
     const int t = (int)(blockIdx.x % 8) * part + in % part;
@@ -181,9 +190,18 @@ struct WeightJobs {
       j.first = lane_of(b, e & 63), j.last = lane_of(n, e & 63);
     }
     j.expert = e;
-    if (t >= high * cols) j.last = j.first;   // no tile here: nothing to do
-    else place(t, high, cols, j.row, j.col);
+    if (t >= high * cols * g.splits) {
+      j.last = j.first;   // no tile here: nothing to do
+      return j;
+    }
+    place(t / g.splits, high, cols, j.row, j.col);
     j.row *= size;
+    if (g.splits > 1) {
+      j.split = t % g.splits;
+      const int len = split_rows(j.last - j.first, g.splits), from = j.split * len, n = j.last - j.first - from;
+      j.first += from < j.last - j.first ? from : j.last - j.first;
+      j.last = j.first + (n <= 0 ? 0 : n < len ? n : len);
+    }
     return j;
   }
 };
@@ -278,17 +296,33 @@ APEXW_DEV void zero_rows(const ExpertArgs& g, int row) {
   }
 }
 
-// zeros in the gradients of the experts without rows
+// Zeros in the gradients of the experts without rows, in pieces of 16 K elements: piece p of them all goes to
+// workgroup p modulo the grid
 template <int OD> APEXW_DEV void zero_weights(const ExpertArgs& g) {
-  const int64_t per = (int64_t)g.n * g.k, step = (int64_t)gridDim.x * blockDim.x;
+  constexpr int kPiece = 16384, V = OD == APEXW_F32 ? 4 : 8;
+  const int64_t per = (int64_t)g.n * g.k, pieces = (per + kPiece - 1) / kPiece;
+  int64_t before = 0, p = blockIdx.x;
   int row = 0, begin, end;
   for (int e0 = 0; e0 < g.experts; e0 += 64) {
     look(g, e0, row, begin, end);
-    uint64_t none = __ballot(begin == end && e0 + lane_id() < g.experts);
-    for (; none; none &= none - 1) {
-      const int64_t at = (e0 + __builtin_ctzll(none)) * per;
-      for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < per; i += step) store_elem<OD>(g.out, at + i, 0.0f);
+    const uint64_t none = __ballot(begin == end && e0 + lane_id() < g.experts);
+    const int64_t upto = before + __builtin_popcountll(none) * pieces;
+    for (; p < upto; p += gridDim.x) {
+      uint64_t left = none;
+      for (int64_t skip = (p - before) / pieces; skip > 0; --skip) left &= left - 1;
+      const int64_t at = (e0 + __builtin_ctzll(left)) * per, i0 = (p - before) % pieces * kPiece;
+      const int n = (int)(per - i0 < kPiece ? per - i0 : kPiece);
+      for (int i = threadIdx.x * V; i < n; i += blockDim.x * V) {
+        const int64_t o = at + i0 + i;
+        if (i + V <= n) {
+          if constexpr (OD == APEXW_F32) APEXW_GLOBAL(Chunk32, (float*)g.out + o)->v = u32x4{0u, 0u, 0u, 0u};
+          else APEXW_GLOBAL(Chunk, (uint16_t*)g.out + o)->v = u32x4{0u, 0u, 0u, 0u};
+        } else {
+          for (int j = i; j < n; ++j) store_elem<OD>(g.out, at + i0 + j, 0.0f);
+        }
+      }
     }
+    before = upto;
   }
 }
 
@@ -620,32 +654,72 @@ APEXW_DEV void stream(const ExpertArgs& g, Jobs& jobs, Place&& locate, uint16_t*
   }
 }
 
-template <class S, bool kBKN, int DT>
+template <class S, bool kBKN, int DT, int OD>
 __global__ __launch_bounds__(S::kThreads, 2) void expert_rows_stream_kernel(ExpertArgs g) {
   __shared__ __attribute__((aligned(16))) uint16_t lds[S::kLds];
   RowJobs<true> jobs(g, S::BM, S::BN);
-  zero_rows(g, jobs.rows);
-  stream<S, false, kBKN, DT, DT, true>(g, jobs, [&](const Job& j, Span& a, Span& b, int& rows, int& cols, int64_t& out0) {
+  if (OD != APEXW_F32) zero_rows(g, jobs.rows);
+  stream<S, false, kBKN, DT, OD, true>(g, jobs, [&](const Job& j, Span& a, Span& b, int& rows, int& cols, int64_t& out0) {
     const int64_t row = j.first + j.row, col = j.col * S::BN;
-    rows = j.last - (int)row, cols = g.n - (int)col, out0 = row * g.ldo + col;
-    a.set<false>(g.a + row * g.lda, g.lda, rows, g.wide, S::BM);
+    const int k0 = j.split * g.part, wide = g.wide - k0 < g.part ? g.wide - k0 : g.part;
+    const int deep = g.k - k0 < g.part ? g.k - k0 : g.part;
+    rows = j.last - (int)row, cols = g.n - (int)col, out0 = j.split * g.split_stride + row * g.ldo + col;
+    a.set<false>(g.a + row * g.lda + k0, g.lda, rows, wide, S::BM);
     // whole chunks of columns: rows of another width have been copied to such
-    b.set<kBKN>(g.b + j.expert * g.sb + (kBKN ? col : col * g.ldb), g.ldb, kBKN ? (cols + 7) / 8 * 8 : cols,
-                kBKN ? g.k : g.wide, S::BN);
+    b.set<kBKN>(g.b + j.expert * g.sb + (kBKN ? k0 * g.ldb + col : col * g.ldb + k0), g.ldb,
+                kBKN ? (cols + 7) / 8 * 8 : cols, kBKN ? deep : wide, S::BN);
   }, lds);
 }
 
 template <class S, int DT, int OD>
 __global__ __launch_bounds__(S::kThreads, 2) void expert_weight_stream_kernel(ExpertArgs g) {
   __shared__ __attribute__((aligned(16))) uint16_t lds[S::kLds];
-  zero_weights<OD>(g);
+  if (g.splits == 1) zero_weights<OD>(g);
   WeightJobs jobs(g, S::BM, S::BN);
   stream<S, true, true, DT, OD, false>(g, jobs, [&](const Job& j, Span& a, Span& b, int& rows, int& cols, int64_t& out0) {
     const int64_t row = j.row, col = j.col * S::BN, first = j.first;
-    rows = g.n - (int)row, cols = g.k - (int)col, out0 = (j.expert * (int64_t)g.n + row) * g.k + col;
+    rows = g.n - (int)row, cols = g.k - (int)col;
+    out0 = j.split * g.split_stride + (j.expert * (int64_t)g.n + row) * g.k + col;
     a.set<true>(g.a + first * g.lda + row, g.lda, (rows + 7) / 8 * 8, j.last - j.first, S::BM);
     b.set<true>(g.b + first * g.ldb + col, g.ldb, (cols + 7) / 8 * 8, j.last - j.first, S::BN);
   }, lds);
+}
+
+// The sum of n partial sums, in their order
+APEXW_DEV float join(const float* p, int64_t stride, int n) {
+  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  int i = 0;
+  for (; i + 4 <= n; i += 4)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[j] += p[(i + j) * stride];
+  for (; i < n; ++i) s[0] += p[i * stride];
+  return (s[0] + s[1]) + (s[2] + s[3]);
+}
+
+// The parts of a rows product added up (partial: [splits][rows][n]); zeros behind the last end
+template <int OD> __global__ __launch_bounds__(256) void join_rows_kernel(ExpertArgs g, const float* __restrict__ partial) {
+  int row = 0, begin, end;
+  for (int e0 = 0; e0 < g.experts; e0 += 64) look(g, e0, row, begin, end);
+  const int64_t n = g.rows * g.n, some = (int64_t)row * g.n;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const float x = i < some ? join(partial + i, g.split_stride, g.splits) : 0.0f;
+    if (g.ldo == g.n) store_elem<OD>(g.out, i, x);
+    else store_elem<OD>(g.out, i / g.n * g.ldo + i % g.n, x);
+  }
+}
+
+// The parts of a weight grad (partial: [splits][experts][n][k]), blockIdx.y an expert: those that have rows
+template <int OD>
+__global__ __launch_bounds__(256) void join_weight_kernel(ExpertArgs g, const float* __restrict__ partial) {
+  const int64_t per = (int64_t)g.n * g.k;
+  for (int e = blockIdx.y; e < g.experts; e += gridDim.y) {
+    int row = 0, begin, end;
+    for (int e0 = 0; e0 <= e; e0 += 64) look(g, e0, row, begin, end);
+    const int rows = lane_of(end, e & 63) - lane_of(begin, e & 63);
+    const int parts = rows ? (rows + split_rows(rows, g.splits) - 1) / split_rows(rows, g.splits) : 0;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < per; i += (int64_t)gridDim.x * 256)
+      store_elem<OD>(g.out, e * per + i, join(partial + e * per + i, g.split_stride, parts));
+  }
 }
 
 // Rows of `width` elements, ld apart, groups of `high` of them `step` apart, copied to rows of whole chunks with
@@ -761,49 +835,97 @@ template <class S> unsigned stream_grid(int64_t tiles) {
   return (unsigned)(((tiles < most ? tiles : most) + 7) / 8 * 8);
 }
 
-template <class S, int DT>
-void launch_rows(const ExpertArgs& g, bool kn, hipStream_t s) {
-  const int64_t most = (g.rows / S::BM + (g.rows < g.experts ? g.rows : g.experts)) * ((g.n + S::BN - 1) / S::BN);
-  const dim3 grid(stream_grid<S>(most)), block(S::kThreads);
-  if (kn) hipLaunchKernelGGL((expert_rows_stream_kernel<S, true, DT>), grid, block, 0, s, g);
-  else hipLaunchKernelGGL((expert_rows_stream_kernel<S, false, DT>), grid, block, 0, s, g);
+template <class S> int64_t rows_tiles(const ExpertArgs& g) {
+  return (g.rows / S::BM + (g.rows < g.experts ? g.rows : g.experts)) * ((g.n + S::BN - 1) / S::BN);
+}
+template <class S> int64_t weight_tiles(const ExpertArgs& g) {
+  return (int64_t)((g.n + S::BM - 1) / S::BM) * ((g.k + S::BN - 1) / S::BN) * g.experts;
 }
 
-// The shape of a rows product's tiles: the one whose stages take the least time over the rounds that its tiles
-// need.  A stage takes, with every workgroup of the chip at work and with few: 256 x 256 1.75 and 0.95 us,
-// 128 x 256 1.0 and 0.65, 64 x 128 0.72 and 0.45, 32 x 128 0.55 and 0.42 (from products of 64 to 4096 rows with
-// 4096 x 4096 weights).  An expert's last tile is taken as half full.  Measured by shape, the smallest first:
-// 4096 rows of one expert 287, 188, 133, 121 us; 1024 rows 76, 51, 59, 94; 64 rows 32, 34, 46, 64; 8192 rows in
-// 8 experts of 2048 x 2048 180, 121, 94, 95; 512 rows in 16 experts of 4096 x 2048 63, 80, 70, 102.
-template <class S> float rows_cost(const ExpertArgs& g, float most, float least) {
-  const float used = (float)(g.rows < g.experts ? g.rows : g.experts);
-  const float high = g.experts == 1 ? (float)((g.rows + S::BM - 1) / S::BM) : (float)g.rows / S::BM + 0.5f * used;
-  const float rounds = high * (float)((g.n + S::BN - 1) / S::BN) / (float)(apexw_cu_count() * S::kPerCU);
-  return rounds <= 1.0f ? least + (most - least) * rounds : most * ceilf(4.0f * rounds) * 0.25f;
+template <class S, int DT, int OD> void launch_rows(const ExpertArgs& g, bool kn, hipStream_t s) {
+  const dim3 grid(stream_grid<S>(rows_tiles<S>(g) * g.splits)), block(S::kThreads);
+  if (kn) hipLaunchKernelGGL((expert_rows_stream_kernel<S, true, DT, OD>), grid, block, 0, s, g);
+  else hipLaunchKernelGGL((expert_rows_stream_kernel<S, false, DT, OD>), grid, block, 0, s, g);
+}
+template <class S, int DT, int OD> void launch_weight(const ExpertArgs& g, hipStream_t s) {
+  const dim3 grid(stream_grid<S>(weight_tiles<S>(g) * g.splits)), block(S::kThreads);
+  hipLaunchKernelGGL((expert_weight_stream_kernel<S, DT, OD>), grid, block, 0, s, g);
 }
 
-int rows_shape(const ExpertArgs& g) {
-  const float cost[4] = {rows_cost<Small>(g, 0.55f, 0.42f), rows_cost<Mid>(g, 0.72f, 0.45f),
-                         rows_cost<Wide>(g, 1.0f, 0.65f), rows_cost<Large>(g, 1.75f, 0.95f)};
-  int best = 0;
-  for (int i = 1; i < 4; ++i)
-    if (cost[i] < cost[best]) best = i;
+// How a product is cut: the shape of its tiles (0: 32 x 128, 1: 64 x 128, 2: 128 x 256, 3: 256 x 256) and the
+// parts of what it sums over, chosen for the least time by what a stage takes with every workgroup of the chip
+// at work and with few: 256 x 256 1.75 and 0.95 us, 128 x 256 1.0 and 0.65, 64 x 128 0.72 and 0.45, 32 x 128
+// 0.55 and 0.42 (from products of 64 to 4096 rows with 4096 x 4096 weights).  An expert's last tile is taken as
+// half full.  Measured by shape, the smallest first: 4096 rows of one expert 287, 188, 133, 121 us; 1024 rows
+// 76, 51, 59, 94; 64 rows 32, 34, 46, 64; 8192 rows in 8 experts of 2048 x 2048 180, 121, 94, 95; 512 rows in 16
+// experts of 4096 x 2048 63, 80, 70, 102.  Parts cost a launch that joins them and 8 bytes an element each.
+struct Cut {
+  int shape, splits;
+  float cost;
+};
+template <class S> void try_cut(Cut& best, int shape, float tiles, float stages, float elems, float most, float least,
+                                bool may_split) {
+  const float slots = (float)(apexw_cu_count() * S::kPerCU);
+  for (int n = 1; n == 1 || (may_split && n <= 64 && (float)(4 * n) <= stages && tiles * (float)n <= 1.5f * slots); n *= 2) {
+    const float rounds = tiles * (float)n / slots;
+    const float stage = rounds <= 1.0f ? least + (most - least) * rounds : most * ceilf(4.0f * rounds) * 0.25f;
+    const float cost = ceilf(stages / (float)n) * stage + (n > 1 ? 5.0f + (float)n * elems * 8.0f / 3e6f : 0.0f);
+    if (best.splits == 0 || cost < best.cost) best = {shape, n, cost};
+  }
+}
+
+Cut cut_rows(const ExpertArgs& g, bool may_split) {
+  Cut best{0, 0, 0.0f};
+  const float used = (float)(g.rows < g.experts ? g.rows : g.experts), stages = (float)((g.wide + 63) / 64);
+  const float elems = (float)g.rows * (float)g.n;
+  auto tiles = [&](int bm, int bn) {
+    const float high = g.experts == 1 ? (float)((g.rows + bm - 1) / bm) : (float)g.rows / (float)bm + 0.5f * used;
+    return high * (float)((g.n + bn - 1) / bn);
+  };
+  try_cut<Small>(best, 0, tiles(32, 128), stages, elems, 0.55f, 0.42f, may_split);
+  try_cut<Mid>(best, 1, tiles(64, 128), stages, elems, 0.72f, 0.45f, may_split);
+  try_cut<Wide>(best, 2, tiles(128, 256), stages, elems, 1.0f, 0.65f, false);
+  try_cut<Large>(best, 3, tiles(256, 256), stages, elems, 1.75f, 0.95f, false);
+  return best;
+}
+
+Cut cut_weight(const ExpertArgs& g, bool may_split) {
+  Cut best{0, 0, 0.0f};
+  const float stages = ceilf((float)g.rows / (float)g.experts / 64.0f) + 1.0f;
+  const float elems = (float)g.experts * (float)g.n * (float)g.k;
+  try_cut<Wide>(best, 2, (float)weight_tiles<Wide>(g), stages, elems, 1.0f, 0.65f, may_split);
+  try_cut<Large>(best, 3, (float)weight_tiles<Large>(g), stages, elems, 1.75f, 0.95f, may_split);
   return best;
 }
 
 template <int DT> void launch_rows_as(const ExpertArgs& g, bool kn, int shape, hipStream_t s) {
-  if (shape == 3) launch_rows<Large, DT>(g, kn, s);
-  else if (shape == 2) launch_rows<Wide, DT>(g, kn, s);
-  else if (shape == 1) launch_rows<Mid, DT>(g, kn, s);
-  else launch_rows<Small, DT>(g, kn, s);
+  if (g.splits > 1) {
+    if (shape == 1) launch_rows<Mid, DT, APEXW_F32>(g, kn, s);
+    else launch_rows<Small, DT, APEXW_F32>(g, kn, s);
+  } else if (shape == 3) {
+    launch_rows<Large, DT, DT>(g, kn, s);
+  } else if (shape == 2) {
+    launch_rows<Wide, DT, DT>(g, kn, s);
+  } else if (shape == 1) {
+    launch_rows<Mid, DT, DT>(g, kn, s);
+  } else {
+    launch_rows<Small, DT, DT>(g, kn, s);
+  }
+}
+template <int DT, int OD> void launch_weight_to(const ExpertArgs& g, int shape, hipStream_t s) {
+  if (shape == 3) launch_weight<Large, DT, OD>(g, s);
+  else launch_weight<Wide, DT, OD>(g, s);
+}
+template <int DT> void launch_weight_as(const ExpertArgs& g, int shape, bool fp32, hipStream_t s) {
+  if (fp32 || g.splits > 1) launch_weight_to<DT, APEXW_F32>(g, shape, s);
+  else launch_weight_to<DT, DT>(g, shape, s);
 }
 
-template <class S, int DT>
-void launch_weight(const ExpertArgs& g, int32_t out_dtype, hipStream_t s) {
-  const int64_t most = (int64_t)((g.n + S::BM - 1) / S::BM) * ((g.k + S::BN - 1) / S::BN) * g.experts;
-  const dim3 grid(stream_grid<S>(most)), block(S::kThreads);
-  if (out_dtype == APEXW_F32) hipLaunchKernelGGL((expert_weight_stream_kernel<S, DT, APEXW_F32>), grid, block, 0, s, g);
-  else hipLaunchKernelGGL((expert_weight_stream_kernel<S, DT, DT>), grid, block, 0, s, g);
+// f(the type code as a constant) for an output's type
+template <class F> void by_type(int32_t dtype, F&& f) {
+  if (dtype == APEXW_F32) f(std::integral_constant<int, APEXW_F32>());
+  else if (dtype == APEXW_BF16) f(std::integral_constant<int, APEXW_BF16>());
+  else f(std::integral_constant<int, APEXW_F16>());
 }
 
 // An operand to be copied to `at` as rows of whole chunks: advances `at`, replaces address and strides
@@ -821,9 +943,50 @@ void launch_pad(const Pad& a, const Pad& b, hipStream_t s) {
 
 // Operands of other widths are copied where the products take longer on the general kernel than the copies:
 // from about 32 rows an expert on (the weights, copied whole, are most of them).  4096 rows of 500 elements
-// in 8 experts of 386: 21.9 us on the general kernel.
+// in 8 experts of 386: 21.9 us on the general kernel, 20.0 with the copies.
 bool worth_padding(int64_t rows, int32_t experts) { return rows >= 32 * (int64_t)experts; }
 int64_t padded(int64_t rows, int64_t width) { return rows * ((width + 7) / 8 * 8) * 2; }
+
+// What a call does, and the workspace that it needs: the copies first, the parts' sums behind them
+struct Plan {
+  bool fast, pad_a, pad_b;
+  Cut cut;
+  int64_t pads, bytes;
+};
+Plan plan_rows(ExpertArgs& g, bool kn, bool may) {
+  Plan p{};
+  const bool fast_a = chunks_ok(g.a, g.lda, g.k), fast_w = chunks_ok(g.b, g.ldb, kn ? g.n : g.k, g.sb);
+  p.fast = (fast_a && fast_w) || (may && worth_padding(g.rows, g.experts));
+  if (!p.fast) return p;
+  p.pad_a = !fast_a, p.pad_b = !fast_w;
+  if (p.pad_a || p.pad_b) g.wide = (g.k + 7) / 8 * 8;
+  p.pads = (p.pad_a ? padded(g.rows, g.k) : 0) + (p.pad_b ? padded(g.experts * (int64_t)(kn ? g.k : g.n), kn ? g.n : g.k) : 0);
+  p.cut = cut_rows(g, may);
+  p.bytes = p.pads + (p.cut.splits > 1 ? p.cut.splits * g.rows * g.n * 4 : 0);
+  return p;
+}
+Plan plan_weight(ExpertArgs& g, bool may) {
+  Plan p{};
+  const bool fast_y = chunks_ok(g.a, g.lda, g.n), fast_x = chunks_ok(g.b, g.ldb, g.k);
+  p.fast = (fast_y && fast_x) || (may && worth_padding(g.rows, g.experts));
+  if (!p.fast) return p;
+  p.pad_a = !fast_y, p.pad_b = !fast_x;
+  p.pads = (p.pad_a ? padded(g.rows, g.n) : 0) + (p.pad_b ? padded(g.rows, g.k) : 0);
+  p.cut = cut_weight(g, may);
+  p.bytes = p.pads + (p.cut.splits > 1 ? p.cut.splits * g.split_stride * 4 : 0);
+  return p;
+}
+
+ExpertArgs rows_args(const void* a, int64_t lda, const void* w, int64_t ldw, int64_t sw, const int32_t* ends, void* out,
+                     int64_t ldo, int32_t experts, int64_t rows, int64_t k, int64_t n) {
+  return {(const uint16_t*)a, (const uint16_t*)w, ends, out, lda, ldw, sw, ldo, rows, experts, (int32_t)n, (int32_t)k,
+          (int32_t)k, 1, INT32_MAX, rows * n};
+}
+ExpertArgs weight_args(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, const int32_t* ends, void* dw,
+                       int32_t experts, int64_t rows, int64_t n, int64_t k) {
+  return {(const uint16_t*)dy, (const uint16_t*)x, ends, dw, ld_dy, ld_x, 0, k, rows, experts, (int32_t)n, (int32_t)k,
+          0, 1, 0, (int64_t)experts * n * k};
+}
 
 bool sizes_ok(int64_t rows, int32_t experts, int64_t n, int64_t k) {
   return rows >= 0 && rows <= INT32_MAX && experts > 0 && n > 0 && k > 0 && n <= INT32_MAX - 256 && k <= INT32_MAX - 256;
@@ -835,17 +998,15 @@ extern "C" int64_t apexw_expert_rows_workspace(const void* a, int64_t lda, const
                                                int64_t w_expert_stride, int32_t w_order, int32_t experts, int64_t rows,
                                                int64_t k, int64_t n) {
   if (!sizes_ok(rows, experts, n, k)) return -APEXW_ERR_ARG;
-  const bool kn = w_order == APEXW_EXPERT_KN;
-  const bool fast_a = chunks_ok(a, lda, k), fast_w = chunks_ok(w, w_row_stride, kn ? n : k, w_expert_stride);
-  if ((fast_a && fast_w) || !worth_padding(rows, experts)) return 0;
-  return (fast_a ? 0 : padded(rows, k)) + (fast_w ? 0 : padded(experts * (kn ? k : n), kn ? n : k));
+  ExpertArgs g = rows_args(a, lda, w, w_row_stride, w_expert_stride, nullptr, nullptr, n, experts, rows, k, n);
+  return plan_rows(g, w_order == APEXW_EXPERT_KN, true).bytes;
 }
 
 extern "C" int64_t apexw_expert_weight_grad_workspace(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x,
                                                       int32_t experts, int64_t rows, int64_t n, int64_t k) {
   if (!sizes_ok(rows, experts, n, k)) return -APEXW_ERR_ARG;
-  if (!worth_padding(rows, experts)) return 0;
-  return (chunks_ok(dy, ld_dy, n) ? 0 : padded(rows, n)) + (chunks_ok(x, ld_x, k) ? 0 : padded(rows, k));
+  ExpertArgs g = weight_args(dy, ld_dy, x, ld_x, nullptr, nullptr, experts, rows, n, k);
+  return plan_weight(g, true).bytes;
 }
 
 extern "C" int apexw_expert_rows(const void* a, int64_t lda, const void* w, int64_t w_row_stride, int64_t w_expert_stride,
@@ -855,36 +1016,42 @@ extern "C" int apexw_expert_rows(const void* a, int64_t lda, const void* w, int6
   if (lda < 0 || w_row_stride < 0 || w_expert_stride < 0 || ldo < n) return APEXW_ERR_ARG;
   if (w_order != APEXW_EXPERT_NK && w_order != APEXW_EXPERT_KN) return APEXW_ERR_ARG;
   if (dtype != APEXW_BF16 && dtype != APEXW_F16) return APEXW_ERR_DTYPE;
-  if (((uintptr_t)a | (uintptr_t)w | (uintptr_t)out) & 1u || (uintptr_t)ends & 3u) return APEXW_ERR_ALIGN;
+  if (((uintptr_t)a | (uintptr_t)w | (uintptr_t)out) & 1u || (uintptr_t)ends & 3u || (uintptr_t)workspace & 15u)
+    return APEXW_ERR_ALIGN;
   if (rows == 0) return APEXW_OK;
-  const int64_t tiles = (rows / kTile + (rows < experts ? rows : experts)) * ((n + kTile - 1) / kTile);
+  ExpertArgs g = rows_args(a, lda, w, w_row_stride, w_expert_stride, ends, out, ldo, experts, rows, k, n);
   // 32-bit tile counts and rows, with room to round them up
-  if (rows > INT32_MAX - 256 || (rows / Small::BM + (rows < experts ? rows : experts)) * ((n + Small::BN - 1) / Small::BN) > INT32_MAX)
-    return APEXW_ERR_SIZE;
-  ExpertArgs g{(const uint16_t*)a, (const uint16_t*)w, ends, out, lda, w_row_stride, w_expert_stride, ldo, rows,
-               experts, (int32_t)n, (int32_t)k, (int32_t)k};
-  const dim3 grid((unsigned)((tiles + 7) / 8 * 8)), block(256);
+  if (rows > INT32_MAX - 256 || rows_tiles<Small>(g) > INT32_MAX) return APEXW_ERR_SIZE;
   hipStream_t s = (hipStream_t)stream;
   const bool kn = w_order == APEXW_EXPERT_KN;
-  bool fast_a = chunks_ok(a, lda, k), fast_w = chunks_ok(w, w_row_stride, kn ? n : k, w_expert_stride);
-  if (workspace && (!fast_a || !fast_w) && worth_padding(rows, experts)) {
-    if ((uintptr_t)workspace & 15u) return APEXW_ERR_ALIGN;
+  const Plan p = plan_rows(g, kn, workspace != nullptr);
+  if (p.fast) {
     uint16_t* at = (uint16_t*)workspace;
     int64_t none = 0;
     Pad jobs[2] = {};
     int count = 0;
-    if (!fast_a) jobs[count++] = pad(g.a, g.lda, none, rows, rows, (int32_t)k, at);
-    if (!fast_w) jobs[count++] = pad(g.b, g.ldb, g.sb, kn ? k : n, experts * (kn ? k : n), (int32_t)(kn ? n : k), at);
-    launch_pad(jobs[0], jobs[1], s);
-    g.wide = (int32_t)((k + 7) / 8 * 8);
-    fast_a = fast_w = true;
-  }
-  if (fast_a && fast_w) {
-    const int shape = rows_shape(g);
-    if (dtype == APEXW_BF16) launch_rows_as<APEXW_BF16>(g, kn, shape, s);
-    else launch_rows_as<APEXW_F16>(g, kn, shape, s);
+    if (p.pad_a) jobs[count++] = pad(g.a, g.lda, none, rows, rows, (int32_t)k, at);
+    if (p.pad_b) jobs[count++] = pad(g.b, g.ldb, g.sb, kn ? k : n, experts * (kn ? k : n), (int32_t)(kn ? n : k), at);
+    if (count) launch_pad(jobs[0], jobs[1], s);
+    if (p.cut.splits > 1) {
+      g.part = (int32_t)((g.wide + 64 * p.cut.splits - 1) / (64 * p.cut.splits) * 64);
+      g.splits = (g.wide + g.part - 1) / g.part;
+    }
+    ExpertArgs h = g;
+    if (g.splits > 1) h.out = (char*)workspace + p.pads, h.ldo = n;
+    if (dtype == APEXW_BF16) launch_rows_as<APEXW_BF16>(h, kn, p.cut.shape, s);
+    else launch_rows_as<APEXW_F16>(h, kn, p.cut.shape, s);
+    if (g.splits > 1) {
+      const int64_t grid = (rows * n + 255) / 256;
+      by_type(dtype, [&](auto d) {
+        hipLaunchKernelGGL(join_rows_kernel<decltype(d)::value>, dim3((unsigned)(grid < 4096 ? grid : 4096)), dim3(256), 0,
+                           s, g, (const float*)h.out);
+      });
+    }
     return hipGetLastError() == hipSuccess ? APEXW_OK : APEXW_ERR_LAUNCH;
   }
+  const int64_t tiles = (rows / kTile + (rows < experts ? rows : experts)) * ((n + kTile - 1) / kTile);
+  const dim3 grid((unsigned)((tiles + 7) / 8 * 8)), block(256);
   if (dtype == APEXW_BF16) {
     if (kn) hipLaunchKernelGGL((expert_rows_kernel<true, APEXW_BF16>), grid, block, 0, s, g);
     else hipLaunchKernelGGL((expert_rows_kernel<false, APEXW_BF16>), grid, block, 0, s, g);
@@ -901,31 +1068,38 @@ extern "C" int apexw_expert_weight_grad(const void* dy, int64_t ld_dy, const voi
   if (!ends || !dw || !sizes_ok(rows, experts, n, k) || (rows > 0 && (!dy || !x))) return APEXW_ERR_ARG;
   if (ld_dy < 0 || ld_x < 0) return APEXW_ERR_ARG;
   if ((dtype != APEXW_BF16 && dtype != APEXW_F16) || (dw_dtype != dtype && dw_dtype != APEXW_F32)) return APEXW_ERR_DTYPE;
-  if (((uintptr_t)dy | (uintptr_t)x) & 1u || (uintptr_t)ends & 3u || (uintptr_t)dw & (dw_dtype == APEXW_F32 ? 3u : 1u))
+  if (((uintptr_t)dy | (uintptr_t)x) & 1u || (uintptr_t)ends & 3u || (uintptr_t)dw & (dw_dtype == APEXW_F32 ? 3u : 1u) ||
+      (uintptr_t)workspace & 15u)
     return APEXW_ERR_ALIGN;
   const int64_t tiles = (((n + kTile - 1) / kTile) * ((k + kTile - 1) / kTile) + 7) / 8 * 8 * experts;
   if (tiles > INT32_MAX || rows > INT32_MAX - 256) return APEXW_ERR_SIZE;
-  ExpertArgs g{(const uint16_t*)dy, (const uint16_t*)x, ends, dw, ld_dy, ld_x, 0, k, rows, experts, (int32_t)n,
-               (int32_t)k, 0};
-  const dim3 grid((unsigned)tiles), block(256);
   hipStream_t s = (hipStream_t)stream;
-  const bool fast_y = chunks_ok(dy, ld_dy, n), fast_x = chunks_ok(x, ld_x, k);
-  const bool copies = workspace && (!fast_y || !fast_x) && worth_padding(rows, experts);
-  if (copies) {
-    if ((uintptr_t)workspace & 15u) return APEXW_ERR_ALIGN;
+  ExpertArgs g = weight_args(dy, ld_dy, x, ld_x, ends, dw, experts, rows, n, k);
+  const Plan p = plan_weight(g, workspace != nullptr);
+  if (p.fast) {
     uint16_t* at = (uint16_t*)workspace;
     int64_t none = 0;
     Pad jobs[2] = {};
     int count = 0;
-    if (!fast_y) jobs[count++] = pad(g.a, g.lda, none, rows, rows, (int32_t)n, at);
-    if (!fast_x) jobs[count++] = pad(g.b, g.ldb, none, rows, rows, (int32_t)k, at);
-    launch_pad(jobs[0], jobs[1], s);
-  }
-  if (copies || (fast_y && fast_x)) {
-    if (dtype == APEXW_BF16) launch_weight<Large, APEXW_BF16>(g, dw_dtype, s);
-    else launch_weight<Large, APEXW_F16>(g, dw_dtype, s);
+    if (p.pad_a) jobs[count++] = pad(g.a, g.lda, none, rows, rows, (int32_t)n, at);
+    if (p.pad_b) jobs[count++] = pad(g.b, g.ldb, none, rows, rows, (int32_t)k, at);
+    if (count) launch_pad(jobs[0], jobs[1], s);
+    g.splits = p.cut.splits;
+    ExpertArgs h = g;
+    if (g.splits > 1) h.out = (char*)workspace + p.pads;
+    if (dtype == APEXW_BF16) launch_weight_as<APEXW_BF16>(h, p.cut.shape, dw_dtype == APEXW_F32, s);
+    else launch_weight_as<APEXW_F16>(h, p.cut.shape, dw_dtype == APEXW_F32, s);
+    if (g.splits > 1) {
+      const int64_t grid = (n * k + 255) / 256;
+      by_type(dw_dtype, [&](auto d) {
+        hipLaunchKernelGGL(join_weight_kernel<decltype(d)::value>,
+                           dim3((unsigned)(grid < 1024 ? grid : 1024), (unsigned)(experts < 1024 ? experts : 1024)),
+                           dim3(256), 0, s, g, (const float*)h.out);
+      });
+    }
     return hipGetLastError() == hipSuccess ? APEXW_OK : APEXW_ERR_LAUNCH;
   }
+  const dim3 grid((unsigned)tiles), block(256);
   if (dtype == APEXW_BF16) {
     if (dw_dtype == APEXW_F32) hipLaunchKernelGGL((expert_weight_kernel<APEXW_BF16, APEXW_F32>), grid, block, 0, s, g);
     else hipLaunchKernelGGL((expert_weight_kernel<APEXW_BF16, APEXW_BF16>), grid, block, 0, s, g);
