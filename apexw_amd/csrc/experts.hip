@@ -222,9 +222,20 @@ APEXW_DEV u32x4 load_chunk(const uint16_t* p, int cnt) {
 APEXW_DEV int clamp8(int64_t left) { return left <= 0 ? 0 : left < 8 ? (int)left : 8; }
 
 // A stage of one operand in registers: 128 rows x 32 k, kKN: given as k rows of 128 columns.
-// base: row 0, k 0 (row stride ld); rows / depth: how many of them there are.
+// base: row 0, k 0 (row stride ld); rows / depth: how many of them there are.  A whole stage loads without a
+// branch, the last row again in place of rows that do not exist: what they give is not stored.
 template <bool kKN>
 APEXW_DEV void fetch(const uint16_t* base, int64_t ld, int64_t rows, int64_t depth, int64_t k0, u32x4 (&r)[2]) {
+  if (k0 + kBK <= depth && (!kKN || rows >= kTile)) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int c = threadIdx.x + 256 * i;
+      const int64_t row = (c >> 2) < rows ? c >> 2 : rows - 1;
+      const uint16_t* p = kKN ? base + (k0 + (c >> 4)) * ld + (c & 15) * 8 : base + row * ld + k0 + (c & 3) * 8;
+      r[i] = APEXW_GLOBAL(const Chunk, p)->v;
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int c = threadIdx.x + 256 * i;
