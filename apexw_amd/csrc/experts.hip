@@ -38,7 +38,12 @@ struct ExpertArgs {
   // of an expert's rows in a weight grad) leave fp32 sums split_stride elements apart, which join_* add up
   int32_t splits, part;
   int64_t split_stride;
+  int32_t which;              // kAll, or the two launches that kMost and kRest make of a rows product's tiles
 };
+
+// Tiles of 256 rows take nearly the same time however few rows they hold (a stage waits for its copies), so a
+// launch of them leaves last tiles of up to 128 rows to a second launch, of 128-row tiles.
+constexpr int kAll = 0, kMost = 1, kRest = 2;
 
 APEXW_DEV int wave_prefix_max(int x) {
 #pragma unroll
@@ -97,9 +102,15 @@ template <bool kCut> struct RowJobs {
       : g(a), size(bm), cols((a.n + bn - 1) / bn), all(0), rows(0) {
     for (int e0 = 0; e0 < g.experts; e0 += 64) step(e0);
   }
+  // tile rows of n rows of an expert
+  __device__ __forceinline__ int high(int n) const {
+    if (g.which == kMost) return n / 256 + (n % 256 > 128);
+    if (g.which == kRest) return n % 256 > 0 && n % 256 <= 128;
+    return (n + size - 1) / size;
+  }
   __device__ __forceinline__ void step(int e0) {
     look(g, e0, rows, begin, end);
-    upto = all + wave_prefix_sum((end - begin + size - 1) / size * cols);
+    upto = all + wave_prefix_sum(high(end - begin) * cols);
     all = lane_of(upto, 63);
   }
   __device__ __forceinline__ int find_at(int t, int e0, Job& j) const {
@@ -107,9 +118,9 @@ template <bool kCut> struct RowJobs {
     if (!hit) return 0;
     const int l = __builtin_ctzll(hit);
     j.expert = e0 + l, j.first = lane_of(begin, l), j.last = lane_of(end, l);
-    const int high = (j.last - j.first + size - 1) / size;
-    place(t - (lane_of(upto, l) - high * cols), high, cols, j.row, j.col);
-    j.row *= size;
+    const int down = high(j.last - j.first);
+    place(t - (lane_of(upto, l) - down * cols), down, cols, j.row, j.col);
+    j.row = g.which == kRest ? (j.last - j.first) / 256 * 256 : j.row * size;
     return 1;
   }
   // the i-th tile of this workgroup.  Round i's tiles go to the XCD's workgroups in turn from another one on
@@ -669,7 +680,7 @@ template <class S, bool kBKN, int DT, int OD>
 __global__ __launch_bounds__(S::kThreads, 2) void expert_rows_stream_kernel(ExpertArgs g) {
   __shared__ __attribute__((aligned(16))) uint16_t lds[S::kLds];
   RowJobs<true> jobs(g, S::BM, S::BN);
-  if (OD != APEXW_F32) zero_rows(g, jobs.rows);
+  if (OD != APEXW_F32 && g.which != kRest) zero_rows(g, jobs.rows);
   stream<S, false, kBKN, DT, OD, true>(g, jobs, [&](const Job& j, Span& a, Span& b, int& rows, int& cols, int64_t& out0) {
     const int64_t row = j.first + j.row, col = j.col * S::BN;
     const int k0 = j.split * g.part, wide = g.wide - k0 < g.part ? g.wide - k0 : g.part;
@@ -914,7 +925,11 @@ template <int DT> void launch_rows_as(const ExpertArgs& g, bool kn, int shape, h
     if (shape == 1) launch_rows<Mid, DT, APEXW_F32>(g, kn, s);
     else launch_rows<Small, DT, APEXW_F32>(g, kn, s);
   } else if (shape == 3) {
-    launch_rows<Large, DT, DT>(g, kn, s);
+    ExpertArgs h = g;
+    h.which = kMost;
+    launch_rows<Large, DT, DT>(h, kn, s);
+    h.which = kRest;
+    launch_rows<Wide, DT, DT>(h, kn, s);
   } else if (shape == 2) {
     launch_rows<Wide, DT, DT>(g, kn, s);
   } else if (shape == 1) {
@@ -991,12 +1006,12 @@ Plan plan_weight(ExpertArgs& g, bool may) {
 ExpertArgs rows_args(const void* a, int64_t lda, const void* w, int64_t ldw, int64_t sw, const int32_t* ends, void* out,
                      int64_t ldo, int32_t experts, int64_t rows, int64_t k, int64_t n) {
   return {(const uint16_t*)a, (const uint16_t*)w, ends, out, lda, ldw, sw, ldo, rows, experts, (int32_t)n, (int32_t)k,
-          (int32_t)k, 1, INT32_MAX, rows * n};
+          (int32_t)k, 1, INT32_MAX, rows * n, kAll};
 }
 ExpertArgs weight_args(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, const int32_t* ends, void* dw,
                        int32_t experts, int64_t rows, int64_t n, int64_t k) {
   return {(const uint16_t*)dy, (const uint16_t*)x, ends, dw, ld_dy, ld_x, 0, k, rows, experts, (int32_t)n, (int32_t)k,
-          0, 1, 0, (int64_t)experts * n * k};
+          0, 1, 0, (int64_t)experts * n * k, kAll};
 }
 
 bool sizes_ok(int64_t rows, int32_t experts, int64_t n, int64_t k) {
