@@ -7,6 +7,16 @@
 //
 // The number of rows of an expert is known on the device alone: each workgroup finds its tiles from the ends.
 // Ends that decrease or pass the buffer count as clamped, so no access leaves it.
+//
+// Measured (bf16, random normal operands; a library's product of one matrix of the first size takes 1360 us):
+//   output, 8 experts of 14336 x 4096, 16384 rows           1770 us   1090 TFLOP/s
+//   the same, one expert                                     1500 us   1280 TFLOP/s
+//   rows' gradient, 32 uneven experts of 2048 x 4096, 8192   204 us    670 TFLOP/s, 3.1 TB/s
+//   weights' gradient in fp32, 16 of 4096 x 2048, 16384      336 us    820 TFLOP/s, 2.2 TB/s
+//   48 rows over 64 experts of 1024 x 2048                   22.4 us   4.7 TB/s of weights
+// Dense products of 8192^3 run at 1280 (rows along k), 1250 and 1270 TFLOP/s: the chip's power bounds them, at
+// 1.8 GHz and two thirds of the matrix cores' cycles.  Without its MFMAs a stage of a 256 x 256 tile still
+// takes 85% of its time, waiting for its 64 KB from L2, which is why tiles of few rows gain little.
 #include <cmath>
 #include <type_traits>
 
@@ -880,7 +890,10 @@ template <class S, int DT, int OD> void launch_weight(const ExpertArgs& g, hipSt
 // 0.55 and 0.42 (from products of 64 to 4096 rows with 4096 x 4096 weights).  An expert's last tile is taken as
 // half full.  Measured by shape, the smallest first: 4096 rows of one expert 287, 188, 133, 121 us; 1024 rows
 // 76, 51, 59, 94; 64 rows 32, 34, 46, 64; 8192 rows in 8 experts of 2048 x 2048 180, 121, 94, 95; 512 rows in 16
-// experts of 4096 x 2048 63, 80, 70, 102.  Parts cost a launch that joins them and 8 bytes an element each.
+// experts of 4096 x 2048 63, 80, 70, 102.  Parts cost a launch that joins them and 8 bytes an element each, and
+// have to gain a fifth (decode steps are soon bound by the weights' bytes): 64 rows of one expert 16 us in
+// eight parts, 32 whole; 128 rows over 16 experts of 4096 x 2048 54 in two, 62; 48 rows over 64 experts of
+// 2048 x 1024 23.0 in two, 22.4 whole.
 struct Cut {
   int shape, splits;
   float cost;
@@ -891,7 +904,7 @@ template <class S> void try_cut(Cut& best, int shape, float tiles, float stages,
   for (int n = 1; n == 1 || (may_split && n <= 64 && (float)(4 * n) <= stages && tiles * (float)n <= 1.5f * slots); n *= 2) {
     const float rounds = tiles * (float)n / slots;
     const float stage = rounds <= 1.0f ? least + (most - least) * rounds : most * ceilf(4.0f * rounds) * 0.25f;
-    const float cost = ceilf(stages / (float)n) * stage + (n > 1 ? 5.0f + (float)n * elems * 8.0f / 3e6f : 0.0f);
+    const float cost = n == 1 ? stages * stage : 1.25f * (ceilf(stages / (float)n) * stage + 5.0f + (float)n * elems * 8.0f / 3e6f);
     if (best.splits == 0 || cost < best.cost) best = {shape, n, cost};
   }
 }

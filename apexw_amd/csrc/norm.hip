@@ -6,6 +6,10 @@
 // Both passes are bound by memory: the forward reads x and writes y, the backward reads x and dy and
 // writes dx.  A row is held in registers from its only read on, so its mean is taken before its squared
 // deviations are summed (rows whose mean is far from zero lose nothing), all in fp32.
+// Measured: forward 16384 x 4096 bf16 54 us, 4.95 TB/s (a copy of 4 GiB reaches 4.75); backward 16384 x 768 bf16
+// with fp32 weights 18.8 us, 4.0 TB/s, and 3.9 for the columns; 4097 x 1021 fp32 13.9 and 4.6; 8192 x 4096 fp32
+// 88 us, 4.6 TB/s; one decode step's 8 x 768 3.7 us, most of it the launch.  Loading the next row before one is
+// worked on cost more in registers than it hid (20.4 to 23.8 us).
 // A chunk is 16 bytes of x; T threads share a row, NC chunks each.  Chunks may lie at any element
 // address: a row of odd width starts anywhere, and global accesses need no alignment.
 #include <type_traits>
