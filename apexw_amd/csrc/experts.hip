@@ -243,10 +243,27 @@ APEXW_DEV u32x4 load_chunk(const uint16_t* p, int cnt) {
 APEXW_DEV int clamp8(int64_t left) { return left <= 0 ? 0 : left < 8 ? (int)left : 8; }
 
 // A stage of one operand in registers: 128 rows x 32 k, kKN: given as k rows of 128 columns.
-// base: row 0, k 0 (row stride ld); rows / depth: how many of them there are.  A whole stage loads without a
-// branch, the last row again in place of rows that do not exist: what they give is not stored.
+// base: row 0, k 0 (row stride ld); rows / depth: how many of them there are; before: how many columns of a
+// kKN operand's rows stand ahead of base.  A whole stage loads without a branch, the last row again in place of
+// rows that do not exist: what they give is not stored.  Of a tile that ends inside a chunk, the row's last 8
+// elements are loaded in the chunk's place and shifted: 1 row of 7578 elements with an expert of 7578 x 387
+// 286 us with the tail's elements one by one.
 template <bool kKN>
-APEXW_DEV void fetch(const uint16_t* base, int64_t ld, int64_t rows, int64_t depth, int64_t k0, u32x4 (&r)[2]) {
+APEXW_DEV void fetch(const uint16_t* base, int64_t ld, int64_t rows, int64_t depth, int64_t k0, u32x4 (&r)[2],
+                     int64_t before = 0) {
+  if (kKN && k0 + kBK <= depth && rows < kTile && before + rows >= 8) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int c = threadIdx.x + 256 * i, col = (c & 15) * 8, at = col + 8 <= (int)rows ? col : (int)rows - 8;
+      const u32x4 v = APEXW_GLOBAL(const Chunk, base + (k0 + (c >> 4)) * ld + at)->v;
+      const int bits = col - at < 8 ? 16 * (col - at) : 0;   // 0: behind the last column, whatever it holds
+      const uint64_t lo = (uint64_t)v[1] << 32 | v[0], hi = (uint64_t)v[3] << 32 | v[2];
+      const uint64_t up = bits == 0 ? 0 : bits < 64 ? hi << (64 - bits) : hi >> (bits - 64);
+      const uint64_t l = bits < 64 ? lo >> bits | up : up, h = bits < 64 ? hi >> bits : 0;
+      r[i] = u32x4{(uint32_t)l, (uint32_t)(l >> 32), (uint32_t)h, (uint32_t)(h >> 32)};
+    }
+    return;
+  }
   if (k0 + kBK <= depth && (!kKN || rows >= kTile)) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -786,7 +803,7 @@ __global__ __launch_bounds__(256) void pad_kernel(Pad a, Pad b) {
 // 32 k in registers while the one before is multiplied.
 template <bool kAKN, bool kBKN, int DT, int OD>
 APEXW_DEV void tile(const uint16_t* a, int64_t lda, const uint16_t* b, int64_t ldb, int64_t rows, int64_t cols,
-                    int64_t depth, void* out, int64_t out0, int64_t ldo) {
+                    int64_t depth, void* out, int64_t out0, int64_t ldo, int64_t a_before, int64_t b_before) {
   __shared__ __attribute__((aligned(16))) uint16_t lds[2][2][kStage];
   const int lane = lane_id(), wave = threadIdx.x >> 6, wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
   f32x16 acc[2][2];
@@ -796,8 +813,8 @@ APEXW_DEV void tile(const uint16_t* a, int64_t lda, const uint16_t* b, int64_t l
     for (int j = 0; j < 2; ++j) acc[i][j] = f32x16{};
   u32x4 ra[2], rb[2];
   if (depth > 0) {
-    fetch<kAKN>(a, lda, rows, depth, 0, ra);
-    fetch<kBKN>(b, ldb, cols, depth, 0, rb);
+    fetch<kAKN>(a, lda, rows, depth, 0, ra, a_before);
+    fetch<kBKN>(b, ldb, cols, depth, 0, rb, b_before);
   }
   int p = 0;
   for (int64_t k0 = 0; k0 < depth; k0 += kBK, p ^= 1) {
@@ -805,8 +822,8 @@ APEXW_DEV void tile(const uint16_t* a, int64_t lda, const uint16_t* b, int64_t l
     put<kBKN>(lds[p][1], rb);
     __syncthreads();
     if (k0 + kBK < depth) {
-      fetch<kAKN>(a, lda, rows, depth, k0 + kBK, ra);
-      fetch<kBKN>(b, ldb, cols, depth, k0 + kBK, rb);
+      fetch<kAKN>(a, lda, rows, depth, k0 + kBK, ra, a_before);
+      fetch<kBKN>(b, ldb, cols, depth, k0 + kBK, rb, b_before);
     }
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -834,16 +851,17 @@ APEXW_DEV void tile(const uint16_t* a, int64_t lda, const uint16_t* b, int64_t l
       }
 }
 
-template <bool kBKN, int DT>
+template <bool kBKN, int DT, int OD>
 __global__ __launch_bounds__(256) void expert_rows_kernel(ExpertArgs g) {
   RowJobs<false> jobs(g, kTile, kTile);
-  zero_rows(g, jobs.rows);
+  if (OD != APEXW_F32) zero_rows(g, jobs.rows);
   const Job j = jobs.get(0);
   if (j.expert < 0) return;
-  const int64_t row = j.first + j.row, col = (int64_t)j.col * kTile;
-  const uint16_t* w = g.b + j.expert * g.sb + (kBKN ? col : col * g.ldb);
-  tile<false, kBKN, DT, DT>(g.a + row * g.lda, g.lda, w, g.ldb, j.last - row, g.n - col, g.k, g.out, row * g.ldo + col,
-                            g.ldo);
+  const int64_t row = j.first + j.row, col = (int64_t)j.col * kTile, k0 = (int64_t)j.split * g.part;
+  const uint16_t* w = g.b + j.expert * g.sb + (kBKN ? k0 * g.ldb + col : col * g.ldb + k0);
+  tile<false, kBKN, DT, OD>(g.a + row * g.lda + k0, g.lda, w, g.ldb, j.last - row, g.n - col,
+                            g.k - k0 < g.part ? g.k - k0 : g.part, g.out, j.split * g.split_stride + row * g.ldo + col,
+                            g.ldo, 0, col);
 }
 
 template <int DT, int OD>
@@ -853,7 +871,7 @@ __global__ __launch_bounds__(256) void expert_weight_kernel(ExpertArgs g) {
   if (j.expert < 0 || j.first == j.last) return;
   const int64_t row = j.row, col = (int64_t)j.col * kTile;
   tile<true, true, DT, OD>(g.a + j.first * g.lda + row, g.lda, g.b + j.first * g.ldb + col, g.ldb, g.n - row, g.k - col,
-                           j.last - j.first, g.out, ((int64_t)j.expert * g.n + row) * g.k + col, g.k);
+                           j.last - j.first, g.out, ((int64_t)j.expert * g.n + row) * g.k + col, g.k, row, col);
 }
 
 // rows of whole 16-byte chunks at 16-byte addresses, within the 32-bit offsets of a stage's copies
@@ -924,6 +942,16 @@ Cut cut_rows(const ExpertArgs& g, bool may_split) {
   return best;
 }
 
+// The general kernel's 128 x 128 tiles, stages of 32 k
+struct Any { static constexpr int kPerCU = 2; };
+Cut cut_any(const ExpertArgs& g, bool may_split) {
+  Cut best{0, 0, 0.0f};
+  const float used = (float)(g.rows < g.experts ? g.rows : g.experts);
+  const float tiles = ((float)g.rows / kTile + (g.experts == 1 ? 0.5f : used)) * (float)((g.n + kTile - 1) / kTile);
+  try_cut<Any>(best, 0, tiles, (float)((g.k + kBK - 1) / kBK), (float)g.rows * (float)g.n, 1.4f, 0.7f, may_split);
+  return best;
+}
+
 Cut cut_weight(const ExpertArgs& g, bool may_split) {
   Cut best{0, 0, 0.0f};
   const float stages = ceilf((float)g.rows / (float)g.experts / 64.0f) + 1.0f;
@@ -967,6 +995,31 @@ template <class F> void by_type(int32_t dtype, F&& f) {
   else f(std::integral_constant<int, APEXW_F16>());
 }
 
+// a product over k cut into `splits` parts of whole stages, or fewer
+void cut_up(ExpertArgs& g, int splits, int stage) {
+  if (splits <= 1) return;
+  const int32_t stages = (g.wide + stage - 1) / stage;
+  g.part = (stages + splits - 1) / splits * stage;
+  g.splits = (g.wide + g.part - 1) / g.part;
+}
+void launch_join(const ExpertArgs& g, int32_t dtype, const float* partial, hipStream_t s) {
+  const int64_t grid = (g.rows * g.n + 255) / 256;
+  by_type(dtype, [&](auto d) {
+    hipLaunchKernelGGL(join_rows_kernel<decltype(d)::value>, dim3((unsigned)(grid < 4096 ? grid : 4096)), dim3(256), 0, s,
+                       g, partial);
+  });
+}
+template <int DT, int OD> void launch_any_to(const ExpertArgs& g, bool kn, hipStream_t s) {
+  const int64_t tiles = (g.rows / kTile + (g.rows < g.experts ? g.rows : g.experts)) * ((g.n + kTile - 1) / kTile) * g.splits;
+  const dim3 grid((unsigned)((tiles + 7) / 8 * 8)), block(256);
+  if (kn) hipLaunchKernelGGL((expert_rows_kernel<true, DT, OD>), grid, block, 0, s, g);
+  else hipLaunchKernelGGL((expert_rows_kernel<false, DT, OD>), grid, block, 0, s, g);
+}
+template <int DT> void launch_any(const ExpertArgs& g, bool kn, hipStream_t s) {
+  if (g.splits > 1) launch_any_to<DT, APEXW_F32>(g, kn, s);
+  else launch_any_to<DT, DT>(g, kn, s);
+}
+
 // An operand to be copied to `at` as rows of whole chunks: advances `at`, replaces address and strides
 Pad pad(const uint16_t*& p, int64_t& ld, int64_t& step, int64_t high, int64_t rows, int32_t width, uint16_t*& at) {
   const int64_t wide = (width + 7) / 8 * 8;
@@ -996,7 +1049,11 @@ Plan plan_rows(ExpertArgs& g, bool kn, bool may) {
   Plan p{};
   const bool fast_a = chunks_ok(g.a, g.lda, g.k), fast_w = chunks_ok(g.b, g.ldb, kn ? g.n : g.k, g.sb);
   p.fast = (fast_a && fast_w) || (may && worth_padding(g.rows, g.experts));
-  if (!p.fast) return p;
+  if (!p.fast) {
+    p.cut = cut_any(g, may);
+    p.bytes = p.cut.splits > 1 ? p.cut.splits * g.rows * g.n * 4 : 0;
+    return p;
+  }
   p.pad_a = !fast_a, p.pad_b = !fast_w;
   if (p.pad_a || p.pad_b) g.wide = (g.k + 7) / 8 * 8;
   p.pads = (p.pad_a ? padded(g.rows, g.k) : 0) + (p.pad_b ? padded(g.experts * (int64_t)(kn ? g.k : g.n), kn ? g.n : g.k) : 0);
@@ -1072,32 +1129,20 @@ extern "C" int apexw_expert_rows(const void* a, int64_t lda, const void* w, int6
     if (p.pad_a) jobs[count++] = pad(g.a, g.lda, none, rows, rows, (int32_t)k, at);
     if (p.pad_b) jobs[count++] = pad(g.b, g.ldb, g.sb, kn ? k : n, experts * (kn ? k : n), (int32_t)(kn ? n : k), at);
     if (count) launch_pad(jobs[0], jobs[1], s);
-    if (p.cut.splits > 1) {
-      g.part = (int32_t)((g.wide + 64 * p.cut.splits - 1) / (64 * p.cut.splits) * 64);
-      g.splits = (g.wide + g.part - 1) / g.part;
-    }
+    cut_up(g, p.cut.splits, 64);
     ExpertArgs h = g;
     if (g.splits > 1) h.out = (char*)workspace + p.pads, h.ldo = n;
     if (dtype == APEXW_BF16) launch_rows_as<APEXW_BF16>(h, kn, p.cut.shape, s);
     else launch_rows_as<APEXW_F16>(h, kn, p.cut.shape, s);
-    if (g.splits > 1) {
-      const int64_t grid = (rows * n + 255) / 256;
-      by_type(dtype, [&](auto d) {
-        hipLaunchKernelGGL(join_rows_kernel<decltype(d)::value>, dim3((unsigned)(grid < 4096 ? grid : 4096)), dim3(256), 0,
-                           s, g, (const float*)h.out);
-      });
-    }
+    if (g.splits > 1) launch_join(g, dtype, (const float*)h.out, s);
     return hipGetLastError() == hipSuccess ? APEXW_OK : APEXW_ERR_LAUNCH;
   }
-  const int64_t tiles = (rows / kTile + (rows < experts ? rows : experts)) * ((n + kTile - 1) / kTile);
-  const dim3 grid((unsigned)((tiles + 7) / 8 * 8)), block(256);
-  if (dtype == APEXW_BF16) {
-    if (kn) hipLaunchKernelGGL((expert_rows_kernel<true, APEXW_BF16>), grid, block, 0, s, g);
-    else hipLaunchKernelGGL((expert_rows_kernel<false, APEXW_BF16>), grid, block, 0, s, g);
-  } else {
-    if (kn) hipLaunchKernelGGL((expert_rows_kernel<true, APEXW_F16>), grid, block, 0, s, g);
-    else hipLaunchKernelGGL((expert_rows_kernel<false, APEXW_F16>), grid, block, 0, s, g);
-  }
+  cut_up(g, p.cut.splits, kBK);
+  ExpertArgs h = g;
+  if (g.splits > 1) h.out = workspace, h.ldo = n;
+  if (dtype == APEXW_BF16) launch_any<APEXW_BF16>(h, kn, s);
+  else launch_any<APEXW_F16>(h, kn, s);
+  if (g.splits > 1) launch_join(g, dtype, (const float*)h.out, s);
   return hipGetLastError() == hipSuccess ? APEXW_OK : APEXW_ERR_LAUNCH;
 }
 

@@ -93,6 +93,14 @@ def test_rows_per_expert(rows):
         check(sizes, *make(sizes, 328, 256, torch.bfloat16, spare=rows % 3))
 
 
+@pytest.mark.parametrize("inner,outer", [(2311, 387), (387, 2311), (4097, 131), (5, 1030), (1531, 134), (135, 777)])
+def test_few_rows_of_odd_widths(inner, outer):
+    """Decode steps that no whole chunks serve: long sums in parts, and columns that end inside a chunk."""
+    for sizes, spare in (([1], 0), ([0, 0, 2, 0, 1, 0], 2), ([3] * 9, 1), ([40], 3)):
+        for dtype in (torch.bfloat16, torch.float16):
+            check(sizes, *make(sizes, inner, outer, dtype, spare=spare))
+
+
 def test_large():
     sizes = [900, 0, 1500, 33, 2048, 600]
     check(sizes, *make(sizes, 1536, 2048, torch.bfloat16, spare=70))
