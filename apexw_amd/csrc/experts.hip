@@ -1033,10 +1033,24 @@ void launch_pad(const Pad& a, const Pad& b, hipStream_t s) {
   hipLaunchKernelGGL(pad_kernel, dim3((unsigned)(most < 8192 ? most : 8192), b.rows ? 2 : 1), dim3(256), 0, s, a, b);
 }
 
-// Operands of other widths are copied where the products take longer on the general kernel than the copies:
-// from about 32 rows an expert on (the weights, copied whole, are most of them).  4096 rows of 500 elements
-// in 8 experts of 386: 21.9 us on the general kernel, 20.0 with the copies.
-bool worth_padding(int64_t rows, int32_t experts) { return rows >= 32 * (int64_t)experts; }
+// Operands of other widths are copied where the products gain more by it than the copies take: rows that run
+// along k at once in both need many rows an expert (the weights, copied whole, are most of the copies) and long
+// sums, weights [k][n], whose rows the general kernel turns around in LDS, fewer.  8 experts, us copied and on
+// the general kernel by rows an expert:
+//   y = x W^T, 4003 x 2001 weights      64: 80, 70    256: 115, 110   512: 147, 171   2048: 386, 533
+//   the same, 1003 x 501                64: 19, 17    256: 23, 20     512: 28, 22     2048: 53, 51
+//   dx = dy W, 4003 x 2001              64: 90, 75    128: 99, 126    512: 190, 241   2048: 428, 602
+//   the same, 1003 x 501                64: 24, 17    128: 24, 23     512: 29, 51     2048: 56, 61
+bool rows_worth_copying(const ExpertArgs& g, bool kn) {
+  if (kn) return g.rows >= 96 * (int64_t)g.experts;
+  return g.rows >= (g.k >= 1024 ? 384 : 3000) * (int64_t)g.experts;
+}
+// A weight gradient's operands are small next to its output where rows are few: 8 experts of 4003 x 2001,
+// 4 rows each 40, 51; 256 70, 99; of 1003 x 501 4 rows 13.7, 9.9; 256 24.4, 25.4; 16 of 777 x 1531, 12 rows
+// 26.7, 22.5.
+bool weight_worth_copying(const ExpertArgs& g) {
+  return g.rows >= 256 * (int64_t)g.experts || (int64_t)g.experts * g.n >= (1 << 25) / g.k;
+}
 int64_t padded(int64_t rows, int64_t width) { return rows * ((width + 7) / 8 * 8) * 2; }
 
 // What a call does, and the workspace that it needs: the copies first, the parts' sums behind them
@@ -1048,7 +1062,7 @@ struct Plan {
 Plan plan_rows(ExpertArgs& g, bool kn, bool may) {
   Plan p{};
   const bool fast_a = chunks_ok(g.a, g.lda, g.k), fast_w = chunks_ok(g.b, g.ldb, kn ? g.n : g.k, g.sb);
-  p.fast = (fast_a && fast_w) || (may && worth_padding(g.rows, g.experts));
+  p.fast = (fast_a && fast_w) || (may && rows_worth_copying(g, kn));
   if (!p.fast) {
     p.cut = cut_any(g, may);
     p.bytes = p.cut.splits > 1 ? p.cut.splits * g.rows * g.n * 4 : 0;
@@ -1064,7 +1078,7 @@ Plan plan_rows(ExpertArgs& g, bool kn, bool may) {
 Plan plan_weight(ExpertArgs& g, bool may) {
   Plan p{};
   const bool fast_y = chunks_ok(g.a, g.lda, g.n), fast_x = chunks_ok(g.b, g.ldb, g.k);
-  p.fast = (fast_y && fast_x) || (may && worth_padding(g.rows, g.experts));
+  p.fast = (fast_y && fast_x) || (may && weight_worth_copying(g));
   if (!p.fast) return p;
   p.pad_a = !fast_y, p.pad_b = !fast_x;
   p.pads = (p.pad_a ? padded(g.rows, g.n) : 0) + (p.pad_b ? padded(g.rows, g.k) : 0);
