@@ -864,10 +864,10 @@ int apexw_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, 
  *   APEXW_EXPERT_KN: at .. + l w_row_stride + j (the rows' gradient of NK weights, and the other way round).
  * apexw_expert_weight_grad: dw[e] ([n x k], contiguous, dtype or F32) = sum over e's rows of dy[i] x[i]^T, 0
  *   for an expert without rows; rows behind the last end are not read.
- * Strides are in elements, of any alignment.  APEXW_ERR_SIZE: more tiles than a launch holds.
+ * Strides are in elements, of any alignment; rows may overlap.  APEXW_ERR_SIZE: more tiles than a launch holds.
  * workspace (16-byte aligned, in any state): as many bytes as the _workspace call answers, 0 for most
- * operands; widths that are no multiple of 8, or rows at other addresses than multiples of 16 bytes, are
- * copied there first where that pays, and slower without (NULL).
+ * operands; widths that are no multiple of 8, rows at other addresses than multiples of 16 bytes, and overlapping
+ * rows of a weight grad or of KN weights are copied there first where that pays, and slower without (NULL).
  */
 #define APEXW_EXPERT_NK 0
 #define APEXW_EXPERT_KN 1

@@ -1,0 +1,27 @@
+"""Which operands of an expert product are copied to rows of whole chunks first, as the workspace's size says."""
+
+from apexw_amd import _lib
+
+OK = 4096        # an aligned address: nothing is launched here
+NK, KN = _lib.EXPERT_NK, _lib.EXPERT_KN
+
+
+def rows_bytes(lda, ldw, order, rows, k, n, experts=1):
+    sw = (n if order == NK else k) * ldw
+    return _lib.load().apexw_expert_rows_workspace(OK, lda, OK, ldw, sw, order, experts, rows, k, n)
+
+
+def weight_bytes(ld_dy, ld_x, rows, n, k, experts=1):
+    return _lib.load().apexw_expert_weight_grad_workspace(OK, ld_dy, OK, ld_x, experts, rows, n, k)
+
+
+def test_overlapping_k_rows_are_copied():
+    """Rows of k closer than their width: both operands of a weight grad and [k][n] weights, nothing else."""
+    n, k, rows = 4096, 2048, 8192
+    assert weight_bytes(n, k, rows, n, k) == 0
+    assert weight_bytes(0, k, rows, n, k) == 2 * rows * n
+    assert weight_bytes(n, 8, rows, n, k) == 2 * rows * k
+    assert weight_bytes(n - 8, k - 8, rows, n, k) == 2 * rows * (n + k)
+    assert rows_bytes(k, n, KN, rows, k, n) == 0
+    assert rows_bytes(k, n - 8, KN, rows, k, n) == 2 * k * n
+    assert rows_bytes(0, k, NK, rows, k, n) == 0 and rows_bytes(k, 0, NK, rows, k, n) == 0
