@@ -13,7 +13,7 @@ import numpy as np
 
 from ._build import LIB_PATH
 
-ABI_VERSION = 27
+ABI_VERSION = 28
 
 # dtype codes
 F32, BF16, F16, U8, I8 = 0, 1, 2, 3, 4
@@ -156,6 +156,7 @@ CLIP_TENSOR_DTYPE = np.dtype([("g", np.uint64), ("out", np.uint64), ("n", np.int
                               ("g_dtype", np.uint32), ("out_dtype", np.uint32)])
 assert CLIP_TENSOR_DTYPE.itemsize == 40
 CLIP_PARTIALS = 2048
+CLIP_SMALL = 48
 EXPERT_NK, EXPERT_KN = 0, 1
 # apexw_fv_tensor: one factored-v tensor of a group
 FV_TENSOR_DTYPE = np.dtype([("tensor", np.uint32), ("rows", np.int32), ("cols", np.int32), ("flags", np.uint32),
@@ -228,6 +229,7 @@ SIGNATURES = {
                                                 _vp, _vp]),
     "apexw_expert_weight_grad_workspace": (ctypes.c_int64, [_vp, _i64, _vp, _i64, _i32, _i64, _i64, _i64]),
     "apexw_clip_layout": (ctypes.c_int64, [_vp, _i32]),
+    "apexw_clip_upload": (ctypes.c_int, [_vp, _i32, _vp, _vp]),
     "apexw_grad_norm": (ctypes.c_int, [_vp, _i32, _i64, _i32, _vp, _vp, _vp]),
     "apexw_grad_scale": (ctypes.c_int, [_vp, _i32, _i64, _vp, _f32, _vp]),
     "apexw_clip_grads": (ctypes.c_int, [_vp, _i32, _i64, _i32, _f32, _vp, _vp, _vp]),

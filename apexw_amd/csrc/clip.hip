@@ -246,6 +246,11 @@ __global__ __launch_bounds__(256) void grad_scale_kernel(Table tab, int32_t n_te
   }
 }
 
+// entries from the launch's arguments into a table on the device
+__global__ __launch_bounds__(64) void clip_upload_kernel(Short tab, int32_t n, apexw_clip_tensor* __restrict__ to) {
+  if ((int)threadIdx.x < n) to[threadIdx.x] = tab.t[threadIdx.x];
+}
+
 int norm_grid(int64_t n_units) { return (int)(n_units < APEXW_CLIP_PARTIALS ? (n_units > 0 ? n_units : 1) : APEXW_CLIP_PARTIALS); }
 
 bool table_ok(const apexw_clip_tensor* tensors, int32_t n_tensors, int64_t n_units) {
@@ -269,6 +274,20 @@ extern "C" int64_t apexw_clip_layout(apexw_clip_tensor* t, int32_t n_tensors) {
     units += (t[i].n + kUnit - 1) / kUnit;
   }
   return units;
+}
+
+extern "C" int apexw_clip_upload(const apexw_clip_tensor* host, int32_t n_tensors, apexw_clip_tensor* device, void* stream) {
+  if (n_tensors < 0 || (n_tensors > 0 && (!host || !device))) return APEXW_ERR_ARG;
+  if ((uintptr_t)device & 7u) return APEXW_ERR_ALIGN;
+  if (n_tensors == 0) return APEXW_OK;
+  static_assert(APEXW_CLIP_SMALL <= 64, "a thread an entry");
+  for (int32_t i = 0; i < n_tensors; i += APEXW_CLIP_SMALL) {
+    const int32_t n = n_tensors - i < APEXW_CLIP_SMALL ? n_tensors - i : APEXW_CLIP_SMALL;
+    Short tab{};
+    for (int32_t j = 0; j < n; ++j) tab.t[j] = host[i + j];
+    hipLaunchKernelGGL(clip_upload_kernel, dim3(1), dim3(64), 0, (hipStream_t)stream, tab, n, device + i);
+  }
+  return hipGetLastError() == hipSuccess ? APEXW_OK : APEXW_ERR_LAUNCH;
 }
 
 namespace {

@@ -355,14 +355,22 @@ def _clip_lists(grads, out, name):
     return grads, to, grads[0].device
 
 
-def _clip_table(grads, to, device, name):
-    """The launch table on the device (made the current one): (table, entries, units)."""
-    host = torch.empty(len(grads) * _lib.CLIP_TENSOR_DTYPE.itemsize, dtype=torch.uint8, pin_memory=True)
+def _clip_table(grads, to, device, stream, name):
+    """The launch table on the device (made the current one): (table, entries, units).
+
+    A captured call puts the entries into the graph: it may not allocate pinned memory, nor copy from a block
+    that is given back when the call returns."""
+    lib, capturing = _lib.load(), torch.cuda.is_current_stream_capturing()
+    host = torch.empty(len(grads) * _lib.CLIP_TENSOR_DTYPE.itemsize, dtype=torch.uint8, pin_memory=not capturing)
     _host().clip_table(grads, to, host.data_ptr(), name)
-    units = _lib.load().apexw_clip_layout(host.data_ptr(), len(grads))
+    units = lib.apexw_clip_layout(host.data_ptr(), len(grads))
     if units < 0:
         _lib.check(-units, "apexw_clip_layout")
-    return host.to(device, non_blocking=True), len(grads), units
+    if not capturing:
+        return host.to(device, non_blocking=True), len(grads), units
+    table = torch.empty_like(host, device=device)
+    _lib.check(lib.apexw_clip_upload(host.data_ptr(), len(grads), table.data_ptr(), stream), "apexw_clip_upload")
+    return table, len(grads), units
 
 
 def _order(norm_type, name):
@@ -379,7 +387,7 @@ def grad_norm(grads, norm_type=2.0):
     if device is None:
         return torch.tensor(0.0)
     with _Launch(device) as stream:
-        table, n, units = _clip_table(grads, to, device, "grad_norm")
+        table, n, units = _clip_table(grads, to, device, stream, "grad_norm")
         ws = torch.empty(_lib.CLIP_PARTIALS, dtype=torch.float64, device=device)
         norm = torch.empty((), dtype=torch.float32, device=device)
         _lib.check(_lib.load().apexw_grad_norm(table.data_ptr(), n, units, order, ws.data_ptr(), norm.data_ptr(), stream),
@@ -399,7 +407,7 @@ def scale_grads(grads, max_norm, total_norm, out=None):
         raise ValueError("scale_grads: expected total_norm as one float32")
     _on_device(total_norm, "scale_grads: total_norm", device)
     with _Launch(device) as stream:
-        table, n, units = _clip_table(grads, to, device, "scale_grads")
+        table, n, units = _clip_table(grads, to, device, stream, "scale_grads")
         _lib.check(_lib.load().apexw_grad_scale(table.data_ptr(), n, units, total_norm.data_ptr(), max_norm, stream),
                    "apexw_grad_scale")
 
@@ -418,12 +426,14 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None):
     grads, to, device = _clip_lists(grads, out, "clip_grads")
     if device is None:
         return torch.tensor(0.0)
-    dev = _current()
-    norm = _native(grads[0]).clip_grads(grads, to, max_norm, order, _raw_stream(dev), dev)
-    if norm is not None:
-        return _done(norm, "apexw_clip_grads")
+    native = _native(grads[0])
+    if len(grads) <= _lib.CLIP_SMALL or not torch.cuda.is_current_stream_capturing():
+        dev = _current()
+        norm = native.clip_grads(grads, to, max_norm, order, _raw_stream(dev), dev)
+        if norm is not None:
+            return _done(norm, "apexw_clip_grads")
     with _Launch(device) as stream:
-        table, n, units = _clip_table(grads, to, device, "clip_grads")
+        table, n, units = _clip_table(grads, to, device, stream, "clip_grads")
         ws = torch.empty(_lib.CLIP_PARTIALS, dtype=torch.float64, device=device)
         norm = torch.empty((), dtype=torch.float32, device=device)
         _lib.check(_lib.load().apexw_clip_grads(table.data_ptr(), n, units, order, max_norm, ws.data_ptr(),

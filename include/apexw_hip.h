@@ -44,7 +44,7 @@
 extern "C" {
 #endif
 
-#define APEXW_ABI_VERSION 27
+#define APEXW_ABI_VERSION 28
 
 /* status codes */
 enum apexw_status {
@@ -891,7 +891,9 @@ int64_t apexw_expert_weight_grad_workspace(const void* dy, int64_t ld_dy, const 
  * Each entry of the table reads n elements at g and writes them at out (another buffer, also of another
  * dtype, or g itself, which is left alone where c is 1), element by element in memory order.
  * apexw_clip_layout checks a HOST table, fills in first_unit and returns the number of work units (or minus
- * an apexw_status); the calls take its device copy.  workspace: APEXW_CLIP_PARTIALS doubles, in any state.
+ * an apexw_status); the calls take its device copy.  apexw_clip_upload makes that copy by launches that carry the
+ * entries in their arguments: a captured graph holds them, where a recorded copy from host memory would read what
+ * stands there at each replay.  workspace: APEXW_CLIP_PARTIALS doubles, in any state.
  * apexw_grad_norm and apexw_grad_scale are the two halves, for a norm over more than one process's grads.
  */
 #define APEXW_CLIP_UNIT 8192
@@ -906,6 +908,7 @@ typedef struct apexw_clip_tensor {
   uint32_t out_dtype;
 } apexw_clip_tensor;   /* 40 bytes */
 int64_t apexw_clip_layout(apexw_clip_tensor* tensors, int32_t n_tensors);
+int apexw_clip_upload(const apexw_clip_tensor* host, int32_t n_tensors, apexw_clip_tensor* device, void* stream);
 int apexw_grad_norm(const apexw_clip_tensor* tensors, int32_t n_tensors, int64_t n_units, int32_t order,
                     double* workspace, float* norm, void* stream);
 int apexw_grad_scale(const apexw_clip_tensor* tensors, int32_t n_tensors, int64_t n_units, const float* norm,
