@@ -883,10 +883,15 @@ __global__ __launch_bounds__(256) void expert_weight_kernel(ExpertArgs g) {
                            j.last - j.first, g.out, ((int64_t)j.expert * g.n + row) * g.k + col, g.k, row, col);
 }
 
-// rows of whole 16-byte chunks at 16-byte addresses, within the 32-bit offsets of a stage's copies
+// the most elements from row to row: a stage's copies reach 256 rows by 32-bit byte offsets
+constexpr int64_t kMostLd = 1 << 22;
+
+// rows of whole 16-byte chunks at 16-byte addresses, within the offsets of a stage's copies
 bool chunks_ok(const void* p, int64_t ld, int64_t width, int64_t step = 0) {
-  return ((uintptr_t)p & 15u) == 0 && ld % 8 == 0 && width % 8 == 0 && step % 8 == 0 && ld <= (1 << 22);
+  return ((uintptr_t)p & 15u) == 0 && ld % 8 == 0 && width % 8 == 0 && step % 8 == 0 && ld <= kMostLd;
 }
+// rows of `width` elements may be copied to whole chunks: the copy's rows, `width` rounded up apart, keep to that
+bool copy_ok(int64_t width) { return width <= kMostLd; }
 // The same of an operand given as k rows.  Overlapping ones (a row broadcast, sliding windows) would have what lies
 // behind the last k row within their memory, so they are copied or go to the general kernel, which tests k.
 // (Testing k in each copy instead: dense 8192^3 weight gradient 851 -> 864 us, rows' gradient 878 -> 889 us.)
@@ -1081,7 +1086,8 @@ Plan plan_rows(ExpertArgs& g, bool kn, bool may) {
   Plan p{};
   const bool fast_a = chunks_ok(g.a, g.lda, g.k);
   const bool fast_w = kn ? k_rows_ok(g.b, g.ldb, g.n, g.sb) : chunks_ok(g.b, g.ldb, g.k, g.sb);
-  p.fast = (fast_a && fast_w) || (may && rows_worth_copying(g, kn));
+  p.fast = (fast_a && fast_w) || (may && rows_worth_copying(g, kn) && (fast_a || copy_ok(g.k)) &&
+                                  (fast_w || copy_ok(kn ? g.n : g.k)));
   if (!p.fast) {
     p.cut = cut_any(g, may);
     p.bytes = p.cut.splits > 1 ? p.cut.splits * g.rows * g.n * 4 : 0;
@@ -1097,7 +1103,8 @@ Plan plan_rows(ExpertArgs& g, bool kn, bool may) {
 Plan plan_weight(ExpertArgs& g, bool may) {
   Plan p{};
   const bool fast_y = k_rows_ok(g.a, g.lda, g.n), fast_x = k_rows_ok(g.b, g.ldb, g.k);
-  p.fast = (fast_y && fast_x) || (may && weight_worth_copying(g));
+  p.fast = (fast_y && fast_x) ||
+           (may && weight_worth_copying(g) && (fast_y || copy_ok(g.n)) && (fast_x || copy_ok(g.k)));
   if (!p.fast) return p;
   p.pad_a = !fast_y, p.pad_b = !fast_x;
   p.pads = (p.pad_a ? padded(g.rows, g.n) : 0) + (p.pad_b ? padded(g.rows, g.k) : 0);

@@ -25,3 +25,18 @@ def test_overlapping_k_rows_are_copied():
     assert rows_bytes(k, n, KN, rows, k, n) == 0
     assert rows_bytes(k, n - 8, KN, rows, k, n) == 2 * k * n
     assert rows_bytes(0, k, NK, rows, k, n) == 0 and rows_bytes(k, 0, NK, rows, k, n) == 0
+
+
+def test_copies_keep_to_32_bit_offsets():
+    """Rows wider than 2^22 elements are not copied, whatever would be gained: a copy's rows are as far apart."""
+    most = 1 << 22
+    assert weight_bytes(8 * most, 16, 64, most, 16) == 2 * 64 * most        # far apart, not wide: copied
+    assert weight_bytes(most - 1, 16, 64, most - 1, 16) == 2 * 64 * most
+    for n in (most + 1, most + 8, 36_000_001, 40_000_000):
+        assert weight_bytes(n, 16, 64, n, 16) == 0 and weight_bytes(16, n, 64, 16, n) == 0
+    # rows products: what is left is a general product in parts, or whole
+    wide, parts = most + 1, 64 * 4096 * 16 * 4
+    assert rows_bytes(most - 1, most - 1, NK, 4096, most - 1, 16) >= 2 * 4096 * most
+    assert rows_bytes(wide, wide, NK, 4096, wide, 16) <= parts < 2 * 4096 * most
+    assert rows_bytes(16, most - 1, KN, 4096, 16, most - 1) >= 2 * 16 * most
+    assert rows_bytes(16, wide, KN, 4096, 16, wide) == 0
