@@ -15,8 +15,10 @@
 
 #include <Python.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <cstring>
+#include <vector>
 
 #include <ATen/ATen.h>
 #include <torch/csrc/Exceptions.h>
@@ -378,9 +380,68 @@ PyObject* expert_weight_grad(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   END_HANDLE_TH_ERRORS
 }
 
+// Bytes [begin, end) of a clip's tensor
+struct Span {
+  uintptr_t begin, end;
+};
+Span span(const void* p, int64_t n, uint32_t code) {
+  const auto at = reinterpret_cast<uintptr_t>(p);
+  return {at, at + static_cast<uintptr_t>(n) * (code == 0 ? 4 : 2)};
+}
+
+// Every tensor that a clip writes has to lie apart from all others: the workgroups scale them at the same time.
+// Gradients that are only read may share memory.  Lists in the order of their addresses are known to be apart
+// in one pass; others are sorted (2000 tensors in another order 25 us).
+bool apart(const ClipTensor* table, Py_ssize_t n, const char* name) {
+  const auto in_place = [](const ClipTensor& t) { return t.out == t.g && t.out_dtype == t.g_dtype; };
+  Span written{UINTPTR_MAX, 0}, read{UINTPTR_MAX, 0};   // from the lowest to the highest byte
+  bool ordered = true;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    const ClipTensor& t = table[i];
+    if (t.n == 0) continue;
+    const Span o = span(t.out, t.n, t.out_dtype);
+    ordered = ordered && o.begin >= written.end;
+    written = {std::min(written.begin, o.begin), std::max(written.end, o.end)};
+    if (in_place(t)) continue;
+    const Span g = span(t.g, t.n, t.g_dtype);
+    read = {std::min(read.begin, g.begin), std::max(read.end, g.end)};
+  }
+  const bool mixed = read.begin < written.end && written.begin < read.end;
+  if (ordered && !mixed) return true;
+
+  struct Entry {
+    Span at;
+    Py_ssize_t tensor;
+  };
+  std::vector<Entry> outs, grads;
+  outs.reserve(n);
+  if (mixed) grads.reserve(n);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    const ClipTensor& t = table[i];
+    if (t.n == 0) continue;
+    outs.push_back({span(t.out, t.n, t.out_dtype), i});
+    if (mixed && !in_place(t)) grads.push_back({span(t.g, t.n, t.g_dtype), i});
+  }
+  for (auto* list : {&outs, &grads})
+    std::sort(list->begin(), list->end(), [](const Entry& a, const Entry& b) { return a.at.begin < b.at.begin; });
+  const auto shared = [name](const Entry& a, const Entry& b) {
+    PyErr_Format(PyExc_ValueError, "%s: tensors %zd and %zd share memory that the clip writes", name,
+                 std::min(a.tensor, b.tensor), std::max(a.tensor, b.tensor));
+    return false;
+  };
+  for (size_t i = 1; i < outs.size(); ++i)
+    if (outs[i].at.begin < outs[i - 1].at.end) return shared(outs[i - 1], outs[i]);
+  size_t w = 0;
+  for (const Entry& g : grads) {
+    while (w < outs.size() && outs[w].at.end <= g.at.begin) ++w;
+    if (w < outs.size() && outs[w].at.begin < g.at.end) return shared(outs[w], g);
+  }
+  return true;
+}
+
 // The entries of a clip's table (first_unit left 0).  Raises for tensors that the clip does not take:
-// another device, type or layout.
-bool fill_clip(PyObject* grads, PyObject* outs, ClipTensor* table, const char* name) {
+// another device, type or layout, and, where it writes them, memory that two of them share.
+bool fill_clip(PyObject* grads, PyObject* outs, ClipTensor* table, const char* name, bool writes) {
   const Py_ssize_t n = PyList_GET_SIZE(grads);
   if (PyList_GET_SIZE(outs) != n) {
     PyErr_SetString(PyExc_ValueError, "clip: lists of different lengths");
@@ -418,20 +479,20 @@ bool fill_clip(PyObject* grads, PyObject* outs, ClipTensor* table, const char* n
     t.n = g.numel();
     t.first_unit = 0;
   }
-  return true;
+  return !writes || apart(table, n, name);
 }
 
-// clip_table(grads, out, table_addr, name): fill_clip into the table at table_addr
+// clip_table(grads, out, table_addr, name, writes): fill_clip into the table at table_addr
 PyObject* clip_table(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (nargs != 4) {
-    PyErr_SetString(PyExc_TypeError, "clip_table(grads, out, table_addr, name)");
+  if (nargs != 5) {
+    PyErr_SetString(PyExc_TypeError, "clip_table(grads, out, table_addr, name, writes)");
     return nullptr;
   }
   uintptr_t ta;
   if (!unpack_list(args[0], "grads") || !unpack_list(args[1], "out") || !as_addr(args[2], &ta)) return nullptr;
   const char* name = PyUnicode_AsUTF8(args[3]);
-  if (!name || !fill_clip(args[0], args[1], reinterpret_cast<ClipTensor*>(ta), name)) return nullptr;
+  if (!name || !fill_clip(args[0], args[1], reinterpret_cast<ClipTensor*>(ta), name, args[4] == Py_True)) return nullptr;
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -456,7 +517,7 @@ PyObject* clip_grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     host = at::empty({static_cast<int64_t>(n * sizeof(ClipTensor))}, at::TensorOptions().dtype(at::kByte).pinned_memory(true));
     t = static_cast<ClipTensor*>(host.data_ptr());
   }
-  if (!fill_clip(args[0], args[1], t, "clip_grads")) return nullptr;
+  if (!fill_clip(args[0], args[1], t, "clip_grads", true)) return nullptr;
   const int64_t units = lib.clip_layout(t, static_cast<int32_t>(n));
   if (units < 0) return PyLong_FromLong(static_cast<long>(-units));
   const auto options = at::TensorOptions().device(first.device());

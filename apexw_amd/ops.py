@@ -355,14 +355,14 @@ def _clip_lists(grads, out, name):
     return grads, to, grads[0].device
 
 
-def _clip_table(grads, to, device, stream, name):
-    """The launch table on the device (made the current one): (table, entries, units).
+def _clip_table(grads, to, device, stream, name, writes=True):
+    """The launch table on the device (made the current one): (table, entries, units); writes: `to` is written.
 
     A captured call puts the entries into the graph: it may not allocate pinned memory, nor copy from a block
     that is given back when the call returns."""
     lib, capturing = _lib.load(), torch.cuda.is_current_stream_capturing()
     host = torch.empty(len(grads) * _lib.CLIP_TENSOR_DTYPE.itemsize, dtype=torch.uint8, pin_memory=not capturing)
-    _host().clip_table(grads, to, host.data_ptr(), name)
+    _host().clip_table(grads, to, host.data_ptr(), name, writes)
     units = lib.apexw_clip_layout(host.data_ptr(), len(grads))
     if units < 0:
         _lib.check(-units, "apexw_clip_layout")
@@ -387,7 +387,7 @@ def grad_norm(grads, norm_type=2.0):
     if device is None:
         return torch.tensor(0.0)
     with _Launch(device) as stream:
-        table, n, units = _clip_table(grads, to, device, stream, "grad_norm")
+        table, n, units = _clip_table(grads, to, device, stream, "grad_norm", False)
         ws = torch.empty(_lib.CLIP_PARTIALS, dtype=torch.float64, device=device)
         norm = torch.empty((), dtype=torch.float32, device=device)
         _lib.check(_lib.load().apexw_grad_norm(table.data_ptr(), n, units, order, ws.data_ptr(), norm.data_ptr(), stream),
@@ -419,7 +419,8 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None):
 
     out: tensors for the clipped copies, shaped and laid out like the gradients, of float32, bfloat16 or
     float16 each (fp32 accumulated gradients clipped into the parameters' type); None clips in place.  The
-    gradients may mix types; each is dense, of any layout."""
+    gradients may mix types; each is dense, of any layout.  What is written shares memory with no other tensor
+    of the lists (a tensor listed twice in place is refused)."""
     order = _order(norm_type, "clip_grads")
     if not max_norm >= 0:
         raise ValueError(f"clip_grads: expected max_norm >= 0, got {max_norm}")

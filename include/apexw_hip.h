@@ -889,7 +889,8 @@ int64_t apexw_expert_weight_grad_workspace(const void* dy, int64_t ld_dy, const 
  * for p = 1, 2 (order 1, 2) or infinity (order 0); a NaN makes norm and outputs NaN.  (The optimizer's own
  * clip, apexw_grad_clip_coef, leaves a coefficient for the step and sanitizes; this one writes the grads.)
  * Each entry of the table reads n elements at g and writes them at out (another buffer, also of another
- * dtype, or g itself, which is left alone where c is 1), element by element in memory order.
+ * dtype, or g itself, which is left alone where c is 1), element by element in memory order.  The memory of an
+ * out overlaps nothing else in the table, which the caller sees to: workgroups scale the entries concurrently.
  * apexw_clip_layout checks a HOST table, fills in first_unit and returns the number of work units (or minus
  * an apexw_status); the calls take its device copy.  apexw_clip_upload makes that copy by launches that carry the
  * entries in their arguments: a captured graph holds them, where a recorded copy from host memory would read what
