@@ -293,10 +293,16 @@ PyObject* layer_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs
       return none_or_error();
   if (!norm_param(w, where, width, code, &w_code) || !norm_param(b, where, width, code, &w_code)) return none_or_error();
   if (w_code == ~0u) w_code = code;
+  bool need[3];   // any truth values
+  for (int i = 0; i < 3; ++i) {
+    const int truth = PyObject_IsTrue(args[6 + i]);
+    if (truth < 0) return nullptr;
+    need[i] = truth != 0;
+  }
   at::Tensor dx, dw, db, ws;
-  if (args[6] == Py_True) dx = at::empty(x.sizes(), x.options());
-  if (args[7] == Py_True && w.defined()) dw = at::empty({width}, w.options());
-  if (args[8] == Py_True && b.defined()) db = at::empty({width}, b.options());
+  if (need[0]) dx = at::empty(x.sizes(), x.options());
+  if (need[1] && w.defined()) dw = at::empty({width}, w.options());
+  if (need[2] && b.defined()) db = at::empty({width}, b.options());
   if (dw.defined() || db.defined()) {
     const int64_t floats = lib.norm_workspace(rows, width);
     if (floats < 0) return PyLong_FromLong(static_cast<long>(-floats));
