@@ -95,10 +95,12 @@ template <class Table> APEXW_DEV int find_tensor(const Table& tab, int n, int64_
 }
 
 // the magnitudes of one thread's 32 elements of a unit joined into acc: sums of |x|^order (1, 2; a sum of
-// squares that leaves the fp32 range is formed again in 64 bits), or (order 0) the largest magnitude's bits,
+// squares that leaves the fp32 range is formed again in 64 bits, upwards by its infinity, downwards where it is
+// so small that squares below the normal numbers may be part of it), or (order 0) the largest magnitude's bits,
 // which order NaN above infinity above every number
 template <int GD, int order> APEXW_DEV void unit_norm(const apexw_clip_tensor& t, int64_t e0, double& acc, uint32_t& top) {
   float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  uint32_t bits = 0u;   // of any element but zero
 #pragma unroll
   for (int i = 0; i < kUnit / 2048; ++i) {
     const int64_t e = e0 + 2048 * i + 8 * threadIdx.x;
@@ -106,8 +108,10 @@ template <int GD, int order> APEXW_DEV void unit_norm(const apexw_clip_tensor& t
     load_some<GD>(t.g, e, t.n - e, x);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      if constexpr (order == 2) s[j & 3] = fmaf(x[j], x[j], s[j & 3]);
-      else if constexpr (order == 1) s[j & 3] += fabsf(x[j]);
+      if constexpr (order == 2) {
+        s[j & 3] = fmaf(x[j], x[j], s[j & 3]);
+        bits |= __float_as_uint(x[j]) << 1;
+      } else if constexpr (order == 1) s[j & 3] += fabsf(x[j]);
       else {
         const uint32_t b = __float_as_uint(x[j]) & 0x7FFFFFFFu;
         top = b > top ? b : top;
@@ -116,7 +120,8 @@ template <int GD, int order> APEXW_DEV void unit_norm(const apexw_clip_tensor& t
   }
   if (order == 0) return;
   const float sum = (s[0] + s[1]) + (s[2] + s[3]);
-  if (__builtin_isinf(sum)) {
+  // 32 squares lose at most 2^-145 in all by underflow: nothing next to 2^-96
+  if (__builtin_isinf(sum) || (order == 2 && sum < 0x1p-96f && bits != 0u)) {
     double d = 0.0;
     for (int i = 0; i < kUnit / 2048; ++i) {
       const int64_t e = e0 + 2048 * i + 8 * threadIdx.x;
