@@ -488,7 +488,17 @@ bool fill_clip(PyObject* grads, PyObject* outs, ClipTensor* table, const char* n
   return !writes || apart(table, n, name);
 }
 
-// clip_table(grads, out, table_addr, name, writes): fill_clip into the table at table_addr
+// New versions for what a clip writes, as every in-place operation gives: autograd refuses to go back through
+// what saved the old values.
+void bump_versions(PyObject* outs) {
+  for (Py_ssize_t i = 0; i < PyList_GET_SIZE(outs); ++i) {
+    const at::Tensor& o = THPVariable_Unpack(PyList_GET_ITEM(outs, i));
+    if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();
+  }
+}
+
+// clip_table(grads, out, table_addr, name, writes): fill_clip into the table at table_addr; a list that is about
+// to be written gets new versions
 PyObject* clip_table(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   if (nargs != 5) {
@@ -498,7 +508,9 @@ PyObject* clip_table(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   uintptr_t ta;
   if (!unpack_list(args[0], "grads") || !unpack_list(args[1], "out") || !as_addr(args[2], &ta)) return nullptr;
   const char* name = PyUnicode_AsUTF8(args[3]);
-  if (!name || !fill_clip(args[0], args[1], reinterpret_cast<ClipTensor*>(ta), name, args[4] == Py_True)) return nullptr;
+  const bool writes = args[4] == Py_True;
+  if (!name || !fill_clip(args[0], args[1], reinterpret_cast<ClipTensor*>(ta), name, writes)) return nullptr;
+  if (writes) bump_versions(args[1]);
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -533,7 +545,9 @@ PyObject* clip_grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const int status = call(n > kClipSmall ? static_cast<const ClipTensor*>(table.data_ptr()) : small, static_cast<int32_t>(n),
                           units, static_cast<int32_t>(order), static_cast<float>(max_norm),
                           static_cast<double*>(ws.data_ptr()), static_cast<float*>(norm.data_ptr()), where.stream);
-  return status ? PyLong_FromLong(status) : THPVariable_Wrap(norm);
+  if (status) return PyLong_FromLong(status);
+  bump_versions(args[1]);   // (while the GPU is at work)
+  return THPVariable_Wrap(norm);
   END_HANDLE_TH_ERRORS
 }
 
