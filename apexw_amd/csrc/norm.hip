@@ -257,7 +257,7 @@ __global__ __launch_bounds__(T < kWG ? kWG : T) void ln_backward_kernel(LnArgs a
       if (a.w) load_param<WD>(a.w, e, cnt, w[i]);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        // behind the row's end dy is 0, and so is every product
+        // behind the row's end dy is 0, and so is every product with a finite xh
         const float xh = (chunk_get<XD>(x[i], j) - mu) * rs, d = chunk_get<XD>(dy[i], j), g = d * w[i][j];
         dw[i][j] = fmaf(d, xh, dw[i][j]);
         db[i][j] += d;
@@ -266,6 +266,16 @@ __global__ __launch_bounds__(T < kWG ? kWG : T) void ln_backward_kernel(LnArgs a
       }
     }
     if (!a.y) continue;
+    // a mean so large over so small a deviation that xh behind the row's end is not: its own elements alone
+    if (__builtin_expect(s2 != s2, 0)) {
+      s2 = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if ((t + T * i) * V + j < a.width)
+            s2 = fmaf(chunk_get<XD>(dy[i], j) * w[i][j], (chunk_get<XD>(x[i], j) - mu) * rs, s2);
+    }
     s1 = lanes_sum<T>(s1);
     s2 = lanes_sum<T>(s2);
     if constexpr (T > 64) {
