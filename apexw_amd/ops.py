@@ -18,8 +18,8 @@ from ._plan import _host
 
 _CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 _ORDER = {1.0: 1, 2.0: 2, float("inf"): 0}
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else None
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # (None in a torch without GPU functions)
+_current = getattr(torch._C, "_cuda_getDevice", None)
 _NATIVE = None
 _ENTRIES = ("apexw_layer_norm_forward", "apexw_layer_norm_backward", "apexw_layer_norm_workspace", "apexw_expert_rows",
             "apexw_expert_rows_workspace", "apexw_expert_weight_grad", "apexw_expert_weight_grad_workspace",
