@@ -5,7 +5,8 @@
 //
 // Bound by memory: the norm reads every gradient, the scaling reads them again and writes the copies.
 // Measured: 872 M fp32 gradients clipped to bf16 591 + 1027 us, 5.9 and 5.1 TB/s; 204 M in 2000 ragged bf16
-// tensors 115 + 145 us, 3.6 and 5.6 TB/s; a 6-tensor MLP 4.5 + 3.9 us.  The norm has to be known before the
+// tensors 115 + 145 us (the norm 77, 5.3 TB/s, unless the copies of a call just before are still on their way out
+// of the cache; one tensor of that size 109 or 71 + 142); a 6-tensor MLP 4.5 + 3.9 us.  The norm has to be known before the
 // first element is written, so the gradients are read twice where they exceed the 256 MB cache; the scaling
 // starts with what the norm's pass read last.
 // Two launches.  The first leaves one partial sum per workgroup; every workgroup of the second adds the

@@ -3,13 +3,14 @@
 //   mu = mean(x), r = 1 / sqrt(mean((x - mu)^2) + eps), xh = (x - mu) r, y = xh w + b
 //   dx = r (g - mean(g) - xh mean(g xh)) with g = dy w;  dw = sum over rows of dy xh, db = of dy
 //
-// Both passes are bound by memory: the forward reads x and writes y, the backward reads x and dy and
-// writes dx.  A row is held in registers from its only read on, so its mean is taken before its squared
+// Both passes are bound by memory where rows are many: the forward reads x and writes y, the backward reads x
+// and dy and writes dx.  A row is held in registers from its only read on, so its mean is taken before its squared
 // deviations are summed (rows whose mean is far from zero lose nothing), all in fp32.
 // Measured: forward 16384 x 4096 bf16 54 us, 4.95 TB/s (a copy of 4 GiB reaches 4.75); backward 16384 x 768 bf16
-// with fp32 weights 18.8 us, 4.0 TB/s, and 3.9 for the columns; 4097 x 1021 fp32 13.9 and 4.6; 8192 x 4096 fp32
-// 88 us, 4.6 TB/s; one decode step's 8 x 768 3.7 us, most of it the launch.  Loading the next row before one is
-// worked on cost more in registers than it hid (20.4 to 23.8 us).
+// with fp32 weights 19.0 us, 4.0 TB/s, and 3.9 for the columns (65536 rows 56.9 us, 5.3 TB/s); 4097 x 1021 fp32
+// 13.6 and 4.6, 4096 x 1024 13.9 and 4.0; 8192 x 4096 fp32 88 us, 4.6 TB/s; one decode step's 8 x 768 3.7 us, most
+// of it the launch.  Loading the next row before one is worked on cost more in registers than it hid (20.4 to
+// 23.8 us).
 // A chunk is 16 bytes of x; T threads share a row, NC chunks each.  Chunks may lie at any element
 // address: a row of odd width starts anywhere, and global accesses need no alignment.
 #include <type_traits>
@@ -178,7 +179,8 @@ __global__ __launch_bounds__(T < kWG ? kWG : T) void ln_forward_kernel(LnArgs a)
   }
 }
 
-// Rows too long for registers: a workgroup per row, which it reads three times (the second and third from L2).
+// Rows too long for registers: a workgroup per row, which it reads three times (the second and third from L2);
+// 2048 x 32768 fp32 162 us.
 template <int XD, int WD>
 __global__ __launch_bounds__(1024) void ln_forward_long_kernel(LnArgs a) {
   constexpr int V = kVec<XD>, T = 1024;
@@ -337,7 +339,8 @@ __global__ __launch_bounds__(T < kWG ? kWG : T) void ln_backward_kernel(LnArgs a
   }
 }
 
-// dx of rows too long for registers: a workgroup per row, read twice.
+// dx of rows too long for registers: a workgroup per row, read twice.  An element a load: 4096 x 32768 bf16 338 us
+// (2.4 TB/s), and 158 for the columns below.
 template <int XD, int WD>
 __global__ __launch_bounds__(1024) void ln_backward_long_kernel(LnArgs a) {
   constexpr int T = 1024;
