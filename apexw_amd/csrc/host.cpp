@@ -398,7 +398,8 @@ Span span(const void* p, int64_t n, uint32_t code) {
 // Every tensor that a clip writes has to lie apart from all others: the workgroups scale them at the same time.
 // Gradients that are only read may share memory.  Lists in the order of their addresses are known to be apart
 // in one pass; others are sorted (2000 tensors in another order 25 us).
-bool apart(const ClipTensor* table, Py_ssize_t n, const char* name) {
+// total: the norm that the scaling reads, or null.
+bool apart(const ClipTensor* table, Py_ssize_t n, const char* name, const void* total) {
   const auto in_place = [](const ClipTensor& t) { return t.out == t.g && t.out_dtype == t.g_dtype; };
   Span written{UINTPTR_MAX, 0}, read{UINTPTR_MAX, 0};   // from the lowest to the highest byte
   bool ordered = true;
@@ -406,6 +407,10 @@ bool apart(const ClipTensor* table, Py_ssize_t n, const char* name) {
     const ClipTensor& t = table[i];
     if (t.n == 0) continue;
     const Span o = span(t.out, t.n, t.out_dtype);
+    if (o.begin < reinterpret_cast<uintptr_t>(total) + 4 && reinterpret_cast<uintptr_t>(total) < o.end) {
+      PyErr_Format(PyExc_ValueError, "%s: tensor %zd, which it writes, holds total_norm", name, i);
+      return false;
+    }
     ordered = ordered && o.begin >= written.end;
     written = {std::min(written.begin, o.begin), std::max(written.end, o.end)};
     if (in_place(t)) continue;
@@ -447,7 +452,8 @@ bool apart(const ClipTensor* table, Py_ssize_t n, const char* name) {
 
 // The entries of a clip's table (first_unit left 0).  Raises for tensors that the clip does not take:
 // another device, type or layout, and, where it writes them, memory that two of them share.
-bool fill_clip(PyObject* grads, PyObject* outs, ClipTensor* table, const char* name, bool writes) {
+bool fill_clip(PyObject* grads, PyObject* outs, ClipTensor* table, const char* name, bool writes,
+               const void* total = nullptr) {
   const Py_ssize_t n = PyList_GET_SIZE(grads);
   if (PyList_GET_SIZE(outs) != n) {
     PyErr_SetString(PyExc_ValueError, "clip: lists of different lengths");
@@ -485,7 +491,7 @@ bool fill_clip(PyObject* grads, PyObject* outs, ClipTensor* table, const char* n
     t.n = g.numel();
     t.first_unit = 0;
   }
-  return !writes || apart(table, n, name);
+  return !writes || apart(table, n, name, total);
 }
 
 // New versions for what a clip writes, as every in-place operation gives: autograd refuses to go back through
@@ -497,19 +503,23 @@ void bump_versions(PyObject* outs) {
   }
 }
 
-// clip_table(grads, out, table_addr, name, writes): fill_clip into the table at table_addr; a list that is about
-// to be written gets new versions
+// clip_table(grads, out, table_addr, name, writes, total_addr=0): fill_clip into the table at table_addr; a list
+// that is about to be written gets new versions.  total_addr: of the norm to scale by, or 0
 PyObject* clip_table(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (nargs != 5) {
-    PyErr_SetString(PyExc_TypeError, "clip_table(grads, out, table_addr, name, writes)");
+  if (nargs != 5 && nargs != 6) {
+    PyErr_SetString(PyExc_TypeError, "clip_table(grads, out, table_addr, name, writes, total_addr=0)");
     return nullptr;
   }
-  uintptr_t ta;
-  if (!unpack_list(args[0], "grads") || !unpack_list(args[1], "out") || !as_addr(args[2], &ta)) return nullptr;
+  uintptr_t ta, total = 0;
+  if (!unpack_list(args[0], "grads") || !unpack_list(args[1], "out") || !as_addr(args[2], &ta) ||
+      (nargs == 6 && !as_addr(args[5], &total)))
+    return nullptr;
   const char* name = PyUnicode_AsUTF8(args[3]);
   const bool writes = args[4] == Py_True;
-  if (!name || !fill_clip(args[0], args[1], reinterpret_cast<ClipTensor*>(ta), name, writes)) return nullptr;
+  if (!name || !fill_clip(args[0], args[1], reinterpret_cast<ClipTensor*>(ta), name, writes,
+                          reinterpret_cast<const void*>(total)))
+    return nullptr;
   if (writes) bump_versions(args[1]);
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS

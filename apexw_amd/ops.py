@@ -355,14 +355,15 @@ def _clip_lists(grads, out, name):
     return grads, to, grads[0].device
 
 
-def _clip_table(grads, to, device, stream, name, writes=True):
-    """The launch table on the device (made the current one): (table, entries, units); writes: `to` is written.
+def _clip_table(grads, to, device, stream, name, writes=True, total=0):
+    """The launch table on the device (made the current one): (table, entries, units); writes: `to` is written;
+    total: the address of the norm that it is scaled by.
 
     A captured call puts the entries into the graph: it may not allocate pinned memory, nor copy from a block
     that is given back when the call returns."""
     lib, capturing = _lib.load(), torch.cuda.is_current_stream_capturing()
     host = torch.empty(len(grads) * _lib.CLIP_TENSOR_DTYPE.itemsize, dtype=torch.uint8, pin_memory=not capturing)
-    _host().clip_table(grads, to, host.data_ptr(), name, writes)
+    _host().clip_table(grads, to, host.data_ptr(), name, writes, total)
     units = lib.apexw_clip_layout(host.data_ptr(), len(grads))
     if units < 0:
         _lib.check(-units, "apexw_clip_layout")
@@ -407,7 +408,7 @@ def scale_grads(grads, max_norm, total_norm, out=None):
         raise ValueError("scale_grads: expected total_norm as one float32")
     _on_device(total_norm, "scale_grads: total_norm", device)
     with _Launch(device) as stream:
-        table, n, units = _clip_table(grads, to, device, stream, "scale_grads")
+        table, n, units = _clip_table(grads, to, device, stream, "scale_grads", total=total_norm.data_ptr())
         _lib.check(_lib.load().apexw_grad_scale(table.data_ptr(), n, units, total_norm.data_ptr(), max_norm, stream),
                    "apexw_grad_scale")
 
