@@ -13,7 +13,7 @@ import numpy as np
 
 from ._build import LIB_PATH
 
-ABI_VERSION = 28
+ABI_VERSION = 29
 
 # dtype codes
 F32, BF16, F16, U8, I8 = 0, 1, 2, 3, 4
@@ -228,6 +228,21 @@ SIGNATURES = {
     "apexw_expert_weight_grad": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i32, _i64, _i64, _i64, _i32, _vp, _i32,
                                                 _vp, _vp]),
     "apexw_expert_weight_grad_workspace": (ctypes.c_int64, [_vp, _i64, _vp, _i64, _i32, _i64, _i64, _i64]),
+    "apexw_expert_order_workspace": (ctypes.c_int64, [_i64, _i32]),
+    "apexw_expert_order": (ctypes.c_int, [_vp, _i32, _i64, _i32, _vp, _vp, _vp, _vp, _vp]),
+    "apexw_expert_dispatch": (ctypes.c_int, [_vp, _i64, _i64, _i32, _i64, _i32, _vp, _vp, _vp, _vp]),
+    "apexw_expert_combine": (ctypes.c_int, [_vp, _i64, _i64, _i32, _i64, _i32, _vp, _vp, _i32, _vp, _vp]),
+    "apexw_expert_combine_backward": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i64, _i32, _i64, _i32, _vp, _vp, _vp, _i32,
+                                                     _vp, _vp, _vp]),
+    "apexw_embedding_forward": (ctypes.c_int, [_vp, _i32, _i64, _vp, _i64, _i64, _i64, _i32, _f32, _vp, _vp]),
+    "apexw_embedding_weight_grad_workspace": (ctypes.c_int64, [_i64, _i64, _i64]),
+    "apexw_embedding_weight_grad": (ctypes.c_int, [_vp, _i64, _vp, _i32, _i64, _i64, _i64, _i32, _f32, _vp, _i32, _vp,
+                                                   _vp]),
+    "apexw_linear_cross_entropy_workspace": (ctypes.c_int64, [_vp, _i64, _i64, _i64, _i64, _i32]),
+    "apexw_linear_cross_entropy_forward": (ctypes.c_int, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i32, _i64,
+                                                          _vp, _vp, _i32, _vp, _vp, _vp]),
+    "apexw_linear_cross_entropy_backward": (ctypes.c_int, [_vp, _i64, _i32, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i32,
+                                                           _vp, _i32, _i64, _vp, _vp, _vp, _vp, _vp]),
     "apexw_clip_layout": (ctypes.c_int64, [_vp, _i32]),
     "apexw_clip_upload": (ctypes.c_int, [_vp, _i32, _vp, _vp]),
     "apexw_grad_norm": (ctypes.c_int, [_vp, _i32, _i64, _i32, _vp, _vp, _vp]),

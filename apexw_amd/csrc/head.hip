@@ -1,0 +1,638 @@
+// Softmax cross entropy of a linear head over a large vocabulary, without its logits, and the gradient (gfx950).
+//
+//   l = x W^T (rows x vocabulary),  lse = log sum_v exp(l_v),  loss = lse - l_target
+//   G = (exp(l - lse) - onehot(target)) dloss,  dx = G W,  dW = G^T x
+// 16-bit operands, products on the matrix cores, logits and all statistics in fp32.
+//
+// Rows without a target (ignored, or outside the vocabulary) are left out before anything is multiplied: the rows that
+// count are packed together, whole chunks wide, so a masked batch costs what its other rows cost and what stands in
+// masked rows, NaN too, reaches nothing.  Their number is known on the device alone.
+//
+// Forward: the logits of a tile stay in registers, and each row leaves the maximum and the sum of exponentials over the
+// tile's columns; a second launch joins them.  Backward: a piece of the vocabulary at a time, G of the piece from the
+// logits computed again, rounded to 16 bits as an operand of the two products that take it; the piece is of a size that
+// the last-level cache holds.  dx adds up the pieces in fp32.
+#include "tiles.h"
+
+#include "chunks.h"
+
+namespace {
+
+constexpr float kLog2E = 1.44269504f;
+
+struct HeadState {          // device
+  int32_t count;            // rows that count
+  float factor;             // G's factor besides dloss
+  float scale;              // and what dx and dW are multiplied with in the end
+};
+struct HeadRow {            // a row that counts
+  float lse, d;
+  int32_t target, row;      // its place among all rows
+};
+struct HeadArgs {
+  const HeadState* state;
+  const HeadRow* rows;
+  float* target_logit;
+  float2* stats;            // [tile of columns][row]: maximum, sum of exp(l - maximum)
+  int64_t stats_ld;
+  int32_t first;            // the piece's first column
+};
+
+// ---------------------------------------------------------------------------
+// Rows that count, packed
+// ---------------------------------------------------------------------------
+
+struct PackArgs {
+  const uint16_t* x;
+  const void* target;
+  const float *lse, *dloss;   // backward
+  uint16_t* packed;
+  HeadState* state;
+  HeadRow* rows;
+  float *loss, *lse_out;      // forward: zeros for the rows that do not count
+  void* dx;                   // the same, backward
+  int64_t n, x_stride, dloss_stride, ignore;
+  int32_t width, wide, vocab, id64, per, mean, rescale;
+};
+
+APEXW_DEV int64_t target_of(const PackArgs& a, int64_t i) {
+  return a.id64 ? APEXW_GLOBAL(const int64_t, a.target)[i] : (int64_t)APEXW_GLOBAL(const int32_t, a.target)[i];
+}
+APEXW_DEV bool counts(const PackArgs& a, int64_t t) { return t != a.ignore && t >= 0 && t < a.vocab; }
+
+template <class T, class F> APEXW_DEV T over_workgroup(T x, T* lds, F&& f) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) x = f(x, __shfl_xor(x, off, 64));
+  if (lane_id() == 0) lds[threadIdx.x >> 6] = x;
+  __syncthreads();
+  x = f(f(lds[0], lds[1]), f(lds[2], lds[3]));
+  __syncthreads();
+  return x;
+}
+
+// A workgroup has `per` (up to 256) rows; how many rows before them count it finds by itself
+__global__ __launch_bounds__(256) void head_pack_kernel(PackArgs a) {
+  __shared__ int ints[4];
+  __shared__ float floats[4];
+  __shared__ int place[256];
+  const int64_t first = (int64_t)blockIdx.x * a.per, end = first + a.per < a.n ? first + a.per : a.n;
+  const bool last = blockIdx.x == gridDim.x - 1;
+  int before = 0;
+  float most = 0.0f;
+  const bool find_most = last && a.rescale;
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < first; i += 256) {
+    const bool c = counts(a, target_of(a, i));
+    before += c;
+    if (find_most && c) most = fmaxf(most, fabsf(a.dloss[i * a.dloss_stride]));
+  }
+  before = over_workgroup(before, ints, [](int p, int q) { return p + q; });
+
+  const int64_t mine = first + threadIdx.x;
+  const int64_t target = mine < end ? target_of(a, mine) : -1;
+  const bool has = mine < end && counts(a, target);
+  const uint64_t ballot = __ballot(has);
+  if (lane_id() == 0) ints[threadIdx.x >> 6] = __builtin_popcountll(ballot);
+  __syncthreads();
+  int at = before + __builtin_popcountll(ballot & ((1ull << lane_id()) - 1ull));
+  for (int w = 0; w < (int)(threadIdx.x >> 6); ++w) at += ints[w];
+  const int all = before + ints[0] + ints[1] + ints[2] + ints[3];
+  place[threadIdx.x] = has ? at : -1;
+  __syncthreads();
+  if (has) {
+    const float d = a.dloss ? a.dloss[mine * a.dloss_stride] : 0.0f;
+    a.rows[at] = HeadRow{a.lse ? a.lse[mine] : 0.0f, d, (int32_t)target, (int32_t)mine};
+    if (find_most) most = fmaxf(most, fabsf(d));
+  } else if (mine < end) {
+    if (a.loss) a.loss[mine] = 0.0f;
+    if (a.lse_out) a.lse_out[mine] = 0.0f;
+  }
+  if (last) {
+    if (a.rescale) most = over_workgroup(most, floats, [](float p, float q) { return fmaxf(p, q); });
+    if (threadIdx.x == 0) {
+      // the largest factor of a row, as a power of two: divided out of G, which fp16 would lose below 2^-24, and
+      // multiplied into the sums
+      const float mean = a.mean && all > 0 ? 1.0f / (float)all : 1.0f;
+      const uint32_t bits = __float_as_uint(most * mean) & 0x7F800000u;
+      const bool use = a.rescale && bits >= 0x01000000u && bits < 0x7E800000u;
+      const float scale = use ? __uint_as_float(bits) : 1.0f;
+      *a.state = HeadState{all, mean / scale, scale};
+    }
+  }
+  const int chunks = a.wide / 8, rows = (int)(end - first);
+  const bool whole = a.width % 8 == 0;
+  for (int i = threadIdx.x; i < rows * chunks; i += 256) {
+    const int r = i / chunks, c = i - r * chunks, p = place[r];
+    if (p >= 0) {
+      *(u32x4*)&a.packed[(int64_t)p * a.wide + c * 8] =
+          load_chunk(a.x + (first + r) * a.x_stride + c * 8, clamp8(a.width - c * 8));
+    } else if (a.dx) {
+      uint16_t* to = (uint16_t*)a.dx + (first + r) * a.width + c * 8;
+      if (whole) APEXW_GLOBAL(Chunk, to)->v = u32x4{0u, 0u, 0u, 0u};
+      else for (int j = 0; j < clamp8(a.width - c * 8); ++j) APEXW_GLOBAL(uint16_t, to)[j] = 0;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Tiles of logits
+// ---------------------------------------------------------------------------
+
+// A tile's first row and column, which `locate` packs into one number
+APEXW_DEV int64_t tile_at(int64_t row, int64_t col) { return row << 32 | col; }
+
+// -inf in the columns behind the last one
+template <int FA, int FB, class Acc> APEXW_DEV void mask_columns(Acc& acc, int wn, int cols, float to) {
+  const int c0 = 4 * (lane_id() >> 4);
+#pragma unroll
+  for (int j = 0; j < FB; ++j)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const bool out = wn + 16 * j + c0 + q >= cols;
+#pragma unroll
+      for (int i = 0; i < FA; ++i) acc[i][j][q] = out ? to : acc[i][j][q];
+    }
+}
+
+// Forward: each row's maximum and sum over the tile's columns, first over a wave's, then over the waves' through LDS
+struct Stats {
+  HeadArgs h;
+  template <class S> static constexpr int stores() { return 0; }
+  template <class S, int kWM, class Acc>
+  __device__ __forceinline__ void write(const ExpertArgs& g, Acc& acc, uint16_t* lds, int down, int across, int rows, int cols,
+                                        int64_t out0) const {
+    constexpr int FA = kWM / 16, FB = S::WN / 16, kAcross = S::BN / S::WN;
+    static_assert(kWM * 8 <= S::kOut * 2, "a wave's statistics in its part of LDS");
+    const int wm = down * kWM, wn = across * S::WN, lane = lane_id(), r0 = lane & 15;
+    const int64_t row0 = out0 >> 32;
+    const int col0 = (int)(uint32_t)out0;
+    float2* mine = (float2*)(lds + S::kStages * S::kStageElems + (down * kAcross + across) * S::kOut);
+    int target[FA];
+#pragma unroll
+    for (int i = 0; i < FA; ++i) {
+      const int r = wm + 16 * i + r0;
+      target[i] = r < rows ? h.rows[row0 + r].target - col0 - wn : -1;
+    }
+    if (cols < S::BN) mask_columns<FA, FB>(acc, wn, cols, -INFINITY);
+#pragma unroll
+    for (int i = 0; i < FA; ++i) {
+      float m = acc[i][0][0];
+#pragma unroll
+      for (int j = 0; j < FB; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) m = fmaxf(m, acc[i][j][q]);
+      m = fmaxf(m, __shfl_xor(m, 16, 64));
+      m = fmaxf(m, __shfl_xor(m, 32, 64));
+      const float from = m == -INFINITY ? 0.0f : m;
+      float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int j = 0; j < FB; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) s[q] += __builtin_amdgcn_exp2f((acc[i][j][q] - from) * kLog2E);
+      float sum = (s[0] + s[1]) + (s[2] + s[3]);
+      sum += __shfl_xor(sum, 16, 64);
+      sum += __shfl_xor(sum, 32, 64);
+      if (lane < 16) mine[16 * i + lane] = make_float2(m, sum);
+      const bool hit = target[i] >= 0 && target[i] < S::WN && (target[i] >> 2 & 3) == lane >> 4;
+      if (__ballot(hit)) {   // in a few of the vocabulary's tiles
+        float l = 0.0f;
+#pragma unroll
+        for (int j = 0; j < FB; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) l = target[i] == 16 * j + 4 * (lane >> 4) + q ? acc[i][j][q] : l;
+        if (hit) h.target_logit[row0 + wm + 16 * i + r0] = l;
+      }
+    }
+    barrier();
+    const int r = threadIdx.x;
+    if (r < kWM * (S::BM / S::WM) && r < rows) {
+      const float2* from = (const float2*)(lds + S::kStages * S::kStageElems + r / kWM * kAcross * S::kOut) + r % kWM;
+      float2 part[kAcross];
+      float m = -INFINITY, sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kAcross; ++w) part[w] = from[w * (S::kOut / 4)], m = fmaxf(m, part[w].x);
+      const float to = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (int w = 0; w < kAcross; ++w) sum += part[w].y * __builtin_amdgcn_exp2f((part[w].x - to) * kLog2E);
+      h.stats[col0 / S::BN * h.stats_ld + row0 + r] = make_float2(m, sum);
+    }
+  }
+};
+
+// Backward: the tile's part of G
+template <int DT> struct Prob {
+  HeadArgs h;
+  template <class S> static constexpr int stores() { return Store<DT>::template stores<S>(); }
+  template <class S, int kWM, class Acc>
+  __device__ __forceinline__ void write(const ExpertArgs& g, Acc& acc, uint16_t* lds, int down, int across, int rows, int cols,
+                                        int64_t out0) const {
+    constexpr int FA = kWM / 16, FB = S::WN / 16;
+    const int wm = down * kWM, wn = across * S::WN, lane = lane_id(), r0 = lane & 15;
+    const int64_t row0 = out0 >> 32;
+    const int col0 = (int)(uint32_t)out0;
+    const float factor = h.state->factor;
+    HeadRow info[FA];
+#pragma unroll
+    for (int i = 0; i < FA; ++i) {
+      const int r = wm + 16 * i + r0;
+      info[i] = h.rows[row0 + (r < rows ? r : rows - 1)];
+    }
+#pragma unroll
+    for (int i = 0; i < FA; ++i) {
+#pragma unroll
+      for (int j = 0; j < FB; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) acc[i][j][q] = __builtin_amdgcn_exp2f((acc[i][j][q] - info[i].lse) * kLog2E);
+      const int t = info[i].target - h.first - col0 - wn;
+      if (__ballot(t >= 0 && t < S::WN)) {
+#pragma unroll
+        for (int j = 0; j < FB; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) acc[i][j][q] -= t == 16 * j + 4 * (lane >> 4) + q ? 1.0f : 0.0f;
+      }
+      const float d = info[i].d * factor;
+#pragma unroll
+      for (int j = 0; j < FB; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) acc[i][j][q] *= d;
+    }
+    // whole chunks: zeros behind the last column
+    if (cols < S::BN) mask_columns<FA, FB>(acc, wn, cols, 0.0f);
+    Store<DT>::template put<S, kWM>(g, acc, lds, down, across, rows, (cols + 7) / 8 * 8, row0 * g.ldo + col0, Same{});
+  }
+};
+
+template <class S, int DT, class Out> __global__ __launch_bounds__(S::kThreads, 2) void head_logits_kernel(ExpertArgs g, Out out) {
+  __shared__ __attribute__((aligned(16))) uint16_t lds[S::kLds];
+  RowJobs<true> jobs(g, S::BM, S::BN);
+  stream<S, false, false, DT, true>(g, jobs, [&](const Job& j, Span& a, Span& b, int& rows, int& cols, int64_t& out0) {
+    const int64_t row = j.first + j.row, col = j.col * S::BN;
+    rows = j.last - (int)row, cols = g.n - (int)col, out0 = tile_at(row, col);
+    a.template set<false>(g.a + row * g.lda, g.lda, rows, g.wide, S::BM);
+    b.template set<false>(g.b + col * g.ldb, g.ldb, cols, g.wide, S::BN);
+  }, out, lds);
+}
+
+// ---------------------------------------------------------------------------
+// The rows' statistics joined, and their mean
+// ---------------------------------------------------------------------------
+
+// 16 rows a workgroup, a 16th of the tiles a thread
+__global__ __launch_bounds__(256) void head_join_kernel(HeadArgs h, int tiles, float* __restrict__ loss, float* __restrict__ lse) {
+  __shared__ float2 parts[16][16];
+  const int r = threadIdx.x & 15, q = threadIdx.x >> 4;
+  const int64_t row = (int64_t)blockIdx.x * 16 + r;
+  const int count = h.state->count;
+  if ((int64_t)blockIdx.x * 16 >= count) return;
+  float m = -INFINITY, s = 0.0f;
+  if (row < count)
+#pragma unroll 4
+    for (int t = q; t < tiles; t += 16) {
+      const float2 p = h.stats[t * h.stats_ld + row];
+      const float top = fmaxf(m, p.x), to = top == -INFINITY ? 0.0f : top;
+      s = s * __builtin_amdgcn_exp2f((m - to) * kLog2E) + p.y * __builtin_amdgcn_exp2f((p.x - to) * kLog2E);
+      m = top;
+    }
+  parts[q][r] = make_float2(m, s);
+  __syncthreads();
+  if (q != 0 || row >= count) return;
+  float top = -INFINITY, sum = 0.0f;
+  for (int i = 0; i < 16; ++i) top = fmaxf(top, parts[i][r].x);
+  const float to = top == -INFINITY ? 0.0f : top;
+  for (int i = 0; i < 16; ++i) sum += parts[i][r].y * __builtin_amdgcn_exp2f((parts[i][r].x - to) * kLog2E);
+  const float log_sum = logf(sum);
+  const int at = h.rows[row].row;
+  lse[at] = to + log_sum;
+  loss[at] = (to - h.target_logit[row]) + log_sum;
+}
+
+// The sum of the rows' losses, or their mean over the rows that count
+__global__ __launch_bounds__(1024) void head_total_kernel(const HeadState* state, const float* loss, int64_t n, int mean, float* total) {
+  __shared__ double parts[16];
+  double s = 0.0;
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < n; i += 1024) s += (double)loss[i];
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+  if (lane_id() == 0) parts[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x) return;
+  s = 0.0;
+  for (int i = 0; i < 16; ++i) s += parts[i];
+  *total = (float)(mean ? s / (double)state->count : s);
+}
+
+// ---------------------------------------------------------------------------
+// The two products with G
+// ---------------------------------------------------------------------------
+
+template <int OD> struct Scaled {
+  const HeadState* state;
+  template <class S> static constexpr int stores() { return Store<OD>::template stores<S>(); }
+  template <class S, int kWM, class Acc>
+  __device__ __forceinline__ void write(const ExpertArgs& g, Acc& acc, uint16_t* lds, int down, int across, int rows, int cols,
+                                        int64_t out0) const {
+    const float scale = state->scale;
+    Store<OD>::template put<S, kWM>(g, acc, lds, down, across, rows, cols, out0, [scale](f32x4 v, int, int) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[q] *= scale;
+      return v;
+    });
+  }
+};
+
+// dW of the piece: [columns of G] x [width of x], over the rows that count
+template <class S, int DT, int OD, class Out>
+__global__ __launch_bounds__(S::kThreads, 2) void head_weight_kernel(ExpertArgs g, Out out) {
+  __shared__ __attribute__((aligned(16))) uint16_t lds[S::kLds];
+  if (g.splits == 1) zero_weights<OD>(g);
+  WeightJobs jobs(g, S::BM, S::BN);
+  stream<S, true, true, DT, false>(g, jobs, [&](const Job& j, Span& a, Span& b, int& rows, int& cols, int64_t& out0) {
+    const int64_t row = j.row, col = j.col * S::BN, first = j.first;
+    rows = g.n - (int)row, cols = g.k - (int)col;
+    out0 = j.split * g.split_stride + row * g.k + col;
+    a.template set<true>(g.a + first * g.lda + row, g.lda, (rows + 7) / 8 * 8, j.last - j.first, S::BM);
+    b.template set<true>(g.b + first * g.ldb + col, g.ldb, (cols + 7) / 8 * 8, j.last - j.first, S::BN);
+  }, out, lds);
+}
+template <int OD>
+__global__ __launch_bounds__(256) void head_join_weight_kernel(ExpertArgs g, const HeadState* state, const float* __restrict__ partial) {
+  const int rows = state->count, len = rows ? split_rows(rows, g.splits) : 1, parts = (rows + len - 1) / len;
+  const int64_t n = (int64_t)g.n * g.k;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
+    store_elem<OD>(g.out, i, join(partial + i, g.split_stride, parts) * state->scale);
+}
+
+// The piece's part of dx: in fp32, added to the pieces before
+template <class S, int DT, bool kAdd> __global__ __launch_bounds__(S::kThreads, 2) void head_rows_kernel(ExpertArgs g) {
+  __shared__ __attribute__((aligned(16))) uint16_t lds[S::kLds];
+  RowJobs<true> jobs(g, S::BM, S::BN);
+  stream<S, false, true, DT, true>(g, jobs, [&](const Job& j, Span& a, Span& b, int& rows, int& cols, int64_t& out0) {
+    const int64_t row = j.first + j.row, col = j.col * S::BN;
+    const int k0 = j.split * g.part, wide = g.wide - k0 < g.part ? g.wide - k0 : g.part;
+    const int deep = g.k - k0 < g.part ? g.k - k0 : g.part;
+    rows = j.last - (int)row, cols = g.n - (int)col, out0 = j.split * g.split_stride + row * g.ldo + col;
+    a.template set<false>(g.a + row * g.lda + k0, g.lda, rows, wide, S::BM);
+    b.template set<true>(g.b + k0 * g.ldb + col, g.ldb, (cols + 7) / 8 * 8, deep, S::BN);
+  }, Store<APEXW_F32, kAdd>(), lds);
+}
+
+// dx: the parts' sums, scaled, each row at its place
+template <int DT> __global__ __launch_bounds__(256) void head_dx_kernel(HeadArgs h, const float* __restrict__ sums, int64_t stride,
+                                                                       int splits, int width, uint16_t* dx) {
+  const int count = h.state->count, per = (width + 3) / 4;
+  const float scale = h.state->scale;
+  const int64_t n = (int64_t)count * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / per;
+    const int c = (int)(i - r * per) * 4, has = width - c < 4 ? width - c : 4;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < splits; ++s) {
+      const float* p = sums + s * stride + r * width + c;
+      if (has == 4) {
+        const u32x4 w = APEXW_GLOBAL(const Chunk32, p)->v;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] += __uint_as_float(w[q]);
+      } else {
+        for (int q = 0; q < has; ++q) v[q] += p[q];
+      }
+    }
+    const int64_t at = (int64_t)h.rows[r].row * width + c;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (q < has) store_elem<DT>(dx, at + q, v[q] * scale);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
+
+int64_t whole(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+// bytes of G that a piece may have
+constexpr int64_t kPiece = 256ll << 20;
+
+struct HeadPlan {
+  int64_t n, width, wide, vocab, w_stride;
+  bool copy_w;
+  int64_t at_rows, at_x, at_w, at_logit, at_stats, at_g, at_sums, at_dw, bytes;
+  int64_t stats_ld, piece, piece_ld;
+  ExpertArgs logits, rows, weight;   // sizes of a whole piece's products
+  Cut cut_logits, cut_dx, cut_dw;
+  HeadPlan(const void* w, int64_t stride, int64_t n_, int64_t width_, int64_t vocab_, bool backward, bool need_dx, bool need_dw)
+      : n(n_), width(width_), wide((width_ + 7) / 8 * 8), vocab(vocab_), w_stride(stride), logits{}, rows{}, weight{} {
+    copy_w = !k_rows_ok(w, stride, width);
+    if (copy_w) w_stride = wide;
+    at_rows = 256;
+    at_x = at_rows + whole(n * (int64_t)sizeof(HeadRow));
+    at_w = at_x + whole(n * wide * 2);
+    int64_t at = at_w + (copy_w ? whole(vocab * wide * 2) : 0);
+    piece = vocab;
+    if (backward) {
+      piece = kPiece / (2 * (n > 0 ? n : 1)) / 256 * 256;
+      piece = piece < 1024 ? 1024 : piece;
+      piece = piece > vocab ? vocab : piece;
+    }
+    logits.rows = n, logits.experts = 1, logits.splits = 1, logits.part = INT32_MAX, logits.n = (int32_t)piece;
+    logits.k = (int32_t)width, logits.wide = (int32_t)wide, logits.lda = wide, logits.ldb = w_stride;
+    cut_logits = cut_rows(logits, false);
+    if (!backward) {
+      stats_ld = (n + 15) / 16 * 16;
+      at_logit = at, at += whole(n * 4);
+      at_stats = at, at += whole(stats_ld * ((vocab + 127) / 128) * 8);
+      bytes = at;
+      return;
+    }
+    piece_ld = (piece + 7) / 8 * 8;
+    at_g = at, at += whole(n * piece_ld * 2);
+    rows = logits, rows.n = (int32_t)width, rows.k = (int32_t)piece, rows.wide = (int32_t)piece_ld, rows.lda = piece_ld;
+    rows.ldo = width, rows.split_stride = n * width;
+    cut_dx = cut_rows(rows, true);
+    cut_up(rows, cut_dx.splits, kDepth);
+    at_sums = at, at += need_dx ? whole(rows.splits * n * width * 4) : 0;
+    weight = logits, weight.n = (int32_t)piece, weight.k = (int32_t)width, weight.lda = piece_ld, weight.ldb = wide;
+    weight.ldo = width, weight.split_stride = piece * width;
+    cut_dw = cut_weight(weight, true);
+    weight.splits = cut_dw.splits;
+    at_dw = at, at += need_dw && weight.splits > 1 ? whole(weight.splits * piece * width * 4) : 0;
+    bytes = at;
+  }
+};
+
+bool head_ok(int64_t n, int64_t width, int64_t vocab) {
+  return n >= 0 && n <= INT32_MAX - 65536 && width > 0 && width <= kMostLd && vocab > 0 && vocab <= INT32_MAX - 65536;
+}
+bool head_fits(const HeadPlan& p) { return rows_tiles<Small>(p.logits) <= INT32_MAX; }
+
+template <class S, int DT, class Out> void launch_logits_shape(const ExpertArgs& g, const Out& out, hipStream_t s) {
+  hipLaunchKernelGGL((head_logits_kernel<S, DT, Out>), dim3(stream_grid<S>(rows_tiles<S>(g))), dim3(S::kThreads), 0, s, g, out);
+}
+template <int DT, class Out> void launch_logits(ExpertArgs g, int shape, const Out& out, hipStream_t s) {
+  if (shape == 3) {
+    g.which = kMost;
+    launch_logits_shape<Large, DT>(g, out, s);
+    g.which = kRest;
+    launch_logits_shape<Wide, DT>(g, out, s);
+  } else if (shape == 2) {
+    launch_logits_shape<Wide, DT>(g, out, s);
+  } else if (shape == 1) {
+    launch_logits_shape<Mid, DT>(g, out, s);
+  } else {
+    launch_logits_shape<Small, DT>(g, out, s);
+  }
+}
+template <class S, int DT> void launch_dx_shape(const ExpertArgs& g, bool add, hipStream_t s) {
+  const dim3 grid(stream_grid<S>(rows_tiles<S>(g) * g.splits)), block(S::kThreads);
+  if (add) hipLaunchKernelGGL((head_rows_kernel<S, DT, true>), grid, block, 0, s, g);
+  else hipLaunchKernelGGL((head_rows_kernel<S, DT, false>), grid, block, 0, s, g);
+}
+template <int DT> void launch_dx(ExpertArgs g, int shape, bool add, hipStream_t s) {
+  if (shape == 3) {
+    g.which = kMost;
+    launch_dx_shape<Large, DT>(g, add, s);
+    g.which = kRest;
+    launch_dx_shape<Wide, DT>(g, add, s);
+  } else if (shape == 2) {
+    launch_dx_shape<Wide, DT>(g, add, s);
+  } else if (shape == 1) {
+    launch_dx_shape<Mid, DT>(g, add, s);
+  } else {
+    launch_dx_shape<Small, DT>(g, add, s);
+  }
+}
+template <int DT, int OD, class Out> void launch_dw_to(const ExpertArgs& g, int shape, const Out& out, hipStream_t s) {
+  if (shape == 3)
+    hipLaunchKernelGGL((head_weight_kernel<Large, DT, OD, Out>), dim3(stream_grid<Large>(weight_tiles<Large>(g) * g.splits)),
+                       dim3(Large::kThreads), 0, s, g, out);
+  else
+    hipLaunchKernelGGL((head_weight_kernel<Wide, DT, OD, Out>), dim3(stream_grid<Wide>(weight_tiles<Wide>(g) * g.splits)),
+                       dim3(Wide::kThreads), 0, s, g, out);
+}
+template <int DT> void launch_dw(const ExpertArgs& g, int shape, const HeadState* state, float* partial, hipStream_t s) {
+  if (g.splits == 1) return launch_dw_to<DT, DT>(g, shape, Scaled<DT>{state}, s);
+  ExpertArgs h = g;
+  h.out = partial;
+  launch_dw_to<DT, APEXW_F32>(h, shape, Store<APEXW_F32>(), s);
+  const int64_t grid = ((int64_t)g.n * g.k + 255) / 256;
+  hipLaunchKernelGGL(head_join_weight_kernel<DT>, dim3((unsigned)(grid < 4096 ? grid : 4096)), dim3(256), 0, s, g, state, partial);
+}
+
+// The weights, copied to whole chunks where they are not; rows packed
+const uint16_t* launch_pack(const HeadPlan& p, PackArgs& a, const void* w, int64_t stride, char* ws, hipStream_t s) {
+  a.state = (HeadState*)ws, a.rows = (HeadRow*)(ws + p.at_rows), a.packed = (uint16_t*)(ws + p.at_x);
+  a.n = p.n, a.width = (int32_t)p.width, a.wide = (int32_t)p.wide, a.vocab = (int32_t)p.vocab;
+  // about 1024 workgroups, of at least 4 rows
+  const int64_t per = (p.n + 1023) / 1024;
+  a.per = (int32_t)(per < 4 ? 4 : per > 256 ? 256 : per);
+  const int64_t grid = (p.n + a.per - 1) / a.per;
+  hipLaunchKernelGGL(head_pack_kernel, dim3((unsigned)(grid ? grid : 1)), dim3(256), 0, s, a);
+  if (!p.copy_w) return (const uint16_t*)w;
+  uint16_t* at = (uint16_t*)(ws + p.at_w);
+  const uint16_t* from = (const uint16_t*)w;
+  int64_t step = 0;
+  launch_pad(pad(from, stride, step, p.vocab, p.vocab, (int32_t)p.width, at), Pad{}, s);
+  return from;
+}
+
+template <class F> void by_half(int32_t dtype, F&& f) {
+  if (dtype == APEXW_BF16) f(std::integral_constant<int, APEXW_BF16>());
+  else f(std::integral_constant<int, APEXW_F16>());
+}
+
+}  // namespace
+
+extern "C" int64_t apexw_linear_cross_entropy_workspace(const void* weight, int64_t w_stride, int64_t n, int64_t width,
+                                                        int64_t vocab, int32_t backward) {
+  if (!head_ok(n, width, vocab)) return -APEXW_ERR_ARG;
+  return HeadPlan(weight, w_stride, n, width, vocab, backward != 0, backward & 1, backward & 2).bytes;
+}
+
+extern "C" int apexw_linear_cross_entropy_forward(const void* x, int64_t x_stride, int64_t n, int64_t width,
+                                                  const void* weight, int64_t w_stride, int64_t vocab, int32_t dtype,
+                                                  const void* target, int32_t id_bytes, int64_t ignore_index, float* loss,
+                                                  float* lse, int32_t reduction, float* total, void* workspace,
+                                                  void* stream) {
+  if (!head_ok(n, width, vocab) || x_stride < 0 || w_stride < 0 || (id_bytes != 4 && id_bytes != 8)) return APEXW_ERR_ARG;
+  if (!weight || !workspace || (n > 0 && (!x || !target || !loss || !lse))) return APEXW_ERR_ARG;
+  if (reduction < 0 || reduction > 2 || (reduction > 0 && !total)) return APEXW_ERR_ARG;
+  if (dtype != APEXW_BF16 && dtype != APEXW_F16) return APEXW_ERR_DTYPE;
+  if ((((uintptr_t)x | (uintptr_t)weight) & 1u) || ((uintptr_t)target & (id_bytes - 1)) || ((uintptr_t)workspace & 15u) ||
+      (((uintptr_t)loss | (uintptr_t)lse | (uintptr_t)total) & 3u))
+    return APEXW_ERR_ALIGN;
+  const HeadPlan p(weight, w_stride, n, width, vocab, false, false, false);
+  if (!head_fits(p)) return APEXW_ERR_SIZE;
+  hipStream_t s = (hipStream_t)stream;
+  char* ws = (char*)workspace;
+  PackArgs pack{};
+  pack.x = (const uint16_t*)x, pack.x_stride = x_stride, pack.target = target, pack.id64 = id_bytes == 8;
+  pack.ignore = ignore_index, pack.loss = loss, pack.lse_out = lse;
+  const uint16_t* w = launch_pack(p, pack, weight, w_stride, ws, s);
+  HeadArgs h{pack.state, pack.rows, (float*)(ws + p.at_logit), (float2*)(ws + p.at_stats), p.stats_ld, 0};
+  if (n > 0) {
+    ExpertArgs g = p.logits;
+    g.a = pack.packed, g.b = w, g.ends = &pack.state->count;
+    by_half(dtype, [&](auto d) { launch_logits<decltype(d)::value>(g, p.cut_logits.shape, Stats{h}, s); });
+    const int64_t tile = p.cut_logits.shape >= 2 ? 256 : 128;
+    hipLaunchKernelGGL(head_join_kernel, dim3((unsigned)((n + 15) / 16)), dim3(256), 0, s, h, (int)((vocab + tile - 1) / tile),
+                       loss, lse);
+  }
+  if (reduction) hipLaunchKernelGGL(head_total_kernel, dim3(1), dim3(1024), 0, s, pack.state, loss, n, (int)(reduction == 2), total);
+  return hipGetLastError() == hipSuccess ? APEXW_OK : APEXW_ERR_LAUNCH;
+}
+
+extern "C" int apexw_linear_cross_entropy_backward(const float* dloss, int64_t dloss_stride, int32_t mean, const void* x,
+                                                   int64_t x_stride, int64_t n, int64_t width, const void* weight,
+                                                   int64_t w_stride, int64_t vocab, int32_t dtype, const void* target,
+                                                   int32_t id_bytes, int64_t ignore_index, const float* lse, void* dx,
+                                                   void* dw, void* workspace, void* stream) {
+  if (!head_ok(n, width, vocab) || x_stride < 0 || w_stride < 0 || dloss_stride < 0 || (id_bytes != 4 && id_bytes != 8))
+    return APEXW_ERR_ARG;
+  if (!weight || !workspace || (n > 0 && (!x || !target || !dloss || !lse))) return APEXW_ERR_ARG;
+  if (dtype != APEXW_BF16 && dtype != APEXW_F16) return APEXW_ERR_DTYPE;
+  if ((((uintptr_t)x | (uintptr_t)weight | (uintptr_t)dx | (uintptr_t)dw) & 1u) || ((uintptr_t)target & (id_bytes - 1)) ||
+      ((uintptr_t)workspace & 15u) || (((uintptr_t)dloss | (uintptr_t)lse) & 3u))
+    return APEXW_ERR_ALIGN;
+  if (!dx && !dw) return APEXW_OK;
+  const HeadPlan p(weight, w_stride, n, width, vocab, true, dx != nullptr, dw != nullptr);
+  if (!head_fits(p)) return APEXW_ERR_SIZE;
+  hipStream_t s = (hipStream_t)stream;
+  char* ws = (char*)workspace;
+  PackArgs pack{};
+  pack.x = (const uint16_t*)x, pack.x_stride = x_stride, pack.target = target, pack.id64 = id_bytes == 8;
+  pack.ignore = ignore_index, pack.lse = lse, pack.dloss = dloss, pack.dloss_stride = dloss_stride, pack.dx = dx;
+  pack.mean = mean != 0, pack.rescale = dtype == APEXW_F16;
+  const uint16_t* w = launch_pack(p, pack, weight, w_stride, ws, s);
+  HeadArgs h{pack.state, pack.rows, nullptr, nullptr, 0, 0};
+  by_half(dtype, [&](auto d) {
+    constexpr int DT = decltype(d)::value;
+    for (int64_t v = 0; v < vocab; v += p.piece) {
+      const int32_t cols = (int32_t)(vocab - v < p.piece ? vocab - v : p.piece);
+      const uint16_t* wp = w + v * p.w_stride;
+      uint16_t* G = (uint16_t*)(ws + p.at_g);
+      if (n > 0) {
+        ExpertArgs g = p.logits;
+        g.a = pack.packed, g.b = wp, g.ends = &pack.state->count, g.n = cols, g.out = G, g.ldo = p.piece_ld;
+        h.first = (int32_t)v;
+        launch_logits<DT>(g, p.cut_logits.shape, Prob<DT>{h}, s);
+      }
+      if (dw) {
+        ExpertArgs g = p.weight;
+        g.a = G, g.b = pack.packed, g.ends = &pack.state->count, g.n = cols, g.out = (uint16_t*)dw + v * width;
+        launch_dw<DT>(g, p.cut_dw.shape, pack.state, (float*)(ws + p.at_dw), s);
+      }
+      if (dx && n > 0) {
+        ExpertArgs g = p.rows;
+        g.a = G, g.b = wp, g.ends = &pack.state->count, g.k = cols, g.wide = (cols + 7) / 8 * 8, g.out = ws + p.at_sums;
+        if (g.splits > 1) g.splits = (g.wide + g.part - 1) / g.part;
+        launch_dx<DT>(g, p.cut_dx.shape, v > 0, s);
+      }
+    }
+    if (dx && n > 0) {
+      const int64_t grid = (n * ((width + 3) / 4) + 255) / 256;
+      hipLaunchKernelGGL(head_dx_kernel<DT>, dim3((unsigned)(grid < 8192 ? grid : 8192)), dim3(256), 0, s, h,
+                         (const float*)(ws + p.at_sums), n * width, (int)p.rows.splits, (int)width, (uint16_t*)dx);
+    }
+  });
+  return hipGetLastError() == hipSuccess ? APEXW_OK : APEXW_ERR_LAUNCH;
+}

@@ -1,0 +1,203 @@
+// A stable sort of small integers by digits, for ids of experts and of words (gfx950).
+//
+// Items are given as ids; an id outside [0, limit) has the key `limit`, behind all others.  Each pass orders by one digit
+// of up to 9 bits: a launch that counts each workgroup's digits and one that places its items, where a workgroup adds up
+// the counts of those before it by itself (64 workgroups' counts are 128 KB, read from L2) so that no launch in between
+// scans them.  The rank of an item among its wave's is counted from ballots of the digit's bits, so equal keys keep
+// their order and equal calls give equal results.  Up to kSmall items go through all passes in one workgroup's LDS.
+#pragma once
+
+#include "common.h"
+
+namespace {
+
+constexpr int kDigits = 512, kSortThreads = 512, kSortWaves = kSortThreads / 64, kItems = 8;
+constexpr int kSmall = kSortThreads * kItems;   // items of a workgroup
+
+struct SortArgs {
+  const void* ids;        // int32 or int64
+  int32_t wide;           // int64
+  int32_t n;
+  uint32_t limit;
+  int32_t bits, passes;   // of a digit
+  u32x2* from;            // (key, item) of a pass after the first
+  u32x2* to;
+  uint32_t* counts;       // [workgroup][digit]
+  int32_t *source, *place, *ends;   // of the last pass for experts
+};
+
+APEXW_DEV u32x2 sort_item(const SortArgs& a, int i) {
+  uint32_t key;
+  if (a.wide) {
+    const int64_t id = APEXW_GLOBAL(const int64_t, a.ids)[i];
+    key = (uint64_t)id < a.limit ? (uint32_t)id : a.limit;
+  } else {
+    const uint32_t id = APEXW_GLOBAL(const uint32_t, a.ids)[i];
+    key = id < a.limit ? id : a.limit;
+  }
+  return u32x2{key, (uint32_t)i};
+}
+
+// lanes of the wave whose digit is this lane's, of those that `valid` names
+APEXW_DEV uint64_t same_digit(uint32_t d, int bits, uint64_t valid) {
+  uint64_t mask = valid;
+  for (int b = 0; b < bits; ++b) {
+    const uint64_t set = __ballot(d >> b & 1u);
+    mask &= d >> b & 1u ? set : ~set;
+  }
+  return mask;
+}
+
+// Exclusive prefix sum over the workgroup's threads; lds: one value a wave.  All threads call it.
+APEXW_DEV uint32_t sort_scan(uint32_t x, uint32_t* lds) {
+  uint32_t up = x;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint32_t y = __shfl_up(up, off, 64);
+    if (lane_id() >= off) up += y;
+  }
+  const int wave = threadIdx.x >> 6;
+  if (lane_id() == 63) lds[wave] = up;
+  __syncthreads();
+  uint32_t before = 0;
+  for (int w = 0; w < wave; ++w) before += lds[w];
+  __syncthreads();
+  return before + up - x;
+}
+
+struct SortLds {
+  uint32_t cnt[kSortWaves][kDigits];
+  uint32_t wave[kSortWaves];
+};
+
+// One pass over the items of this workgroup: rounds x 64 consecutive ones a wave from `first` on, get(i) the item i.
+// put(item, position, start of its digit's block) places each.  kAlone: the workgroup has all items.
+// digit_end(d, end): thread d gets the end of digit d's block.
+template <bool kAlone, class Get, class Put, class End>
+APEXW_DEV void sort_pass(const SortArgs& a, SortLds& l, int pass, int first, int rounds, Get&& get, Put&& put,
+                         End&& digit_end) {
+  const int digits = 1 << a.bits, wave = threadIdx.x >> 6, lane = lane_id(), shift = pass * a.bits;
+  const uint32_t low = (uint32_t)digits - 1u;
+  for (int i = threadIdx.x; i < kSortWaves * digits; i += kSortThreads) l.cnt[i >> a.bits][i & low] = 0u;
+  __syncthreads();
+  u32x2 item[kItems];
+  uint32_t rank[kItems];
+  const int base = first + wave * rounds * 64 + lane;
+#pragma unroll
+  for (int r = 0; r < kItems; ++r)
+    if (r < rounds && base + r * 64 < a.n) item[r] = get(base + r * 64);
+#pragma unroll
+  for (int r = 0; r < kItems; ++r) {
+    if (r >= rounds) break;
+    const bool valid = base + r * 64 < a.n;
+    const uint32_t d = valid ? item[r][0] >> shift & low : 0u;
+    const uint64_t mask = same_digit(d, a.bits, __ballot(valid));
+    const uint32_t ahead = __builtin_popcountll(mask & ((1ull << lane) - 1ull));
+    const uint32_t old = l.cnt[wave][d];
+    rank[r] = old + ahead;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (valid && ahead == 0u) l.cnt[wave][d] = old + (uint32_t)__builtin_popcountll(mask);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+  __syncthreads();
+  // thread d: the digit's items in the waves before, in the workgroups before, and in all
+  const int d = threadIdx.x;
+  uint32_t mine = 0u, before = 0u, all = 0u;
+  if (d < digits) {
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) {
+      const uint32_t c = l.cnt[w][d];
+      l.cnt[w][d] = mine;
+      mine += c;
+    }
+    if (kAlone) {
+      all = mine;
+    } else {
+      for (int b = 0; b < (int)gridDim.x; ++b) {
+        const uint32_t c = a.counts[(int64_t)b * digits + d];
+        all += c;
+        before += b < (int)blockIdx.x ? c : 0u;
+      }
+    }
+  }
+  const uint32_t start = sort_scan(all, l.wave);
+  if (d < digits) {
+    digit_end(d, start + all);
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) l.cnt[w][d] += start + before;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kItems; ++r)
+    if (r < rounds && base + r * 64 < a.n) put(item[r], l.cnt[wave][item[r][0] >> shift & low] + rank[r]);
+}
+
+// The counts of each workgroup's digits
+template <bool kFirst> __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortArgs a, int pass) {
+  __shared__ uint32_t cnt[kDigits];
+  const int digits = 1 << a.bits, shift = pass * a.bits, first = blockIdx.x * kSmall;
+  for (int i = threadIdx.x; i < digits; i += kSortThreads) cnt[i] = 0u;
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kItems; ++r) {
+    const int i = first + r * kSortThreads + threadIdx.x;
+    if (i >= a.n) continue;
+    const uint32_t key = kFirst ? sort_item(a, i)[0] : a.from[i][0];
+    atomicAdd(&cnt[key >> shift & (uint32_t)(digits - 1)], 1u);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < digits; i += kSortThreads) a.counts[(int64_t)blockIdx.x * digits + i] = cnt[i];
+}
+
+// where the last pass puts an item for experts
+APEXW_DEV void sort_order(const SortArgs& a, u32x2 item, uint32_t at) {
+  const bool none = item[0] == a.limit;
+  APEXW_GLOBAL(int32_t, a.source)[at] = none ? -1 : (int32_t)item[1];
+  APEXW_GLOBAL(int32_t, a.place)[item[1]] = none ? -1 : (int32_t)at;
+}
+
+// kOrder: the last pass of an experts' order, whose ends are the digits' where one pass sorts them
+template <bool kFirst, bool kOrder> __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(SortArgs a, int pass) {
+  __shared__ SortLds l;
+  sort_pass<false>(
+      a, l, pass, blockIdx.x * kSmall, kItems, [&](int i) { return kFirst ? sort_item(a, i) : a.from[i]; },
+      [&](u32x2 item, uint32_t at) {
+        if (kOrder) sort_order(a, item, at);
+        if (a.to) a.to[at] = item;
+      },
+      [&](int d, uint32_t end) {
+        if (kOrder && a.passes == 1 && blockIdx.x == 0 && (uint32_t)d < a.limit) a.ends[d] = (int32_t)end;
+      });
+}
+
+// All passes of up to kSmall items in one workgroup
+template <bool kOrder> APEXW_DEV void sort_small(const SortArgs& a) {
+  __shared__ SortLds l;
+  __shared__ u32x2 items[kSmall];
+  const int rounds = (a.n + kSortThreads - 1) / kSortThreads;
+  for (int pass = 0; pass < a.passes; ++pass) {
+    const bool last = pass == a.passes - 1;
+    sort_pass<true>(
+        a, l, pass, 0, rounds, [&](int i) { return pass == 0 ? sort_item(a, i) : items[i]; },
+        [&](u32x2 item, uint32_t at) {
+          if (!last) items[at] = item;
+          else if (kOrder) sort_order(a, item, at);
+          if (last && a.to) a.to[at] = item;
+        },
+        [&](int d, uint32_t end) {
+          if (kOrder && a.passes == 1 && (uint32_t)d < a.limit) a.ends[d] = (int32_t)end;
+        });
+    __syncthreads();
+  }
+}
+
+inline void sort_digits(SortArgs& a) {
+  int bits = 1;
+  while (bits < 32 && (uint64_t)a.limit >> bits) ++bits;   // of the keys 0 .. limit
+  a.passes = (bits + 8) / 9;
+  a.bits = (bits + a.passes - 1) / a.passes;
+}
+// workgroups of a pass
+inline int sort_groups(int64_t n) { return (int)((n + kSmall - 1) / kSmall); }
+
+}  // namespace

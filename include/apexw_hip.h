@@ -44,7 +44,7 @@
 extern "C" {
 #endif
 
-#define APEXW_ABI_VERSION 28
+#define APEXW_ABI_VERSION 29
 
 /* status codes */
 enum apexw_status {
@@ -882,6 +882,71 @@ int apexw_expert_weight_grad(const void* dy, int64_t ld_dy, const void* x, int64
                              int32_t dw_dtype, void* workspace, void* stream);
 int64_t apexw_expert_weight_grad_workspace(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, int32_t experts,
                                            int64_t rows, int64_t n, int64_t k);
+
+/*
+ * Tokens sorted by expert and back.  Choice c = t k + j (j < k) of token t names an expert; choices of an expert in
+ * [0, experts) get rows, sorted by expert and then by choice, the others none:
+ *   source[r] (choices int32): the choice of row r, -1 in rows behind the last expert's
+ *   place[c] (choices int32): the row of choice c, -1 without one;  ends[e] (experts int32): one past e's last row
+ * apexw_expert_order makes them from ids of 4 or 8 bytes (id_bytes); workspace: as many bytes as the _workspace call
+ * answers (16-byte aligned, in any state; NULL for 0).
+ * apexw_expert_dispatch: rows[r] = x[source[r] / k], zeros where source is negative (rows contiguous).
+ * apexw_expert_combine: out[t] = sum over j of weight[t k + j] y[place[t k + j]] over the choices that have a row; weight
+ *   (w_dtype: dtype or F32) may be NULL (ones; so this is also the gradient of dispatch).
+ * apexw_expert_combine_backward: dy[r] = weight[source[r]] dout[source[r] / k], zeros where source is negative;
+ *   dweight[c] = <dout[c / k], y[place[c]]>, 0 without a row.  dy, dweight may be NULL; y where dweight is.
+ * dtype F32 / BF16 / F16, any alignment beyond the element's; strides in elements; sums in fp32, in the order of j,
+ * rounded once.  source and place have to be each other's inverse; places that are no row count as -1.
+ * Up to 2^31 - 65536 choices, rows of up to APEXW_ROW_WIDTH elements.
+ */
+#define APEXW_ROW_WIDTH 16776960
+int64_t apexw_expert_order_workspace(int64_t choices, int32_t experts);   /* < 0: minus an apexw_status */
+int apexw_expert_order(const void* expert, int32_t id_bytes, int64_t choices, int32_t experts, int32_t* source,
+                       int32_t* place, int32_t* ends, void* workspace, void* stream);
+int apexw_expert_dispatch(const void* x, int64_t x_stride, int64_t tokens, int32_t k, int64_t width, int32_t dtype,
+                          const int32_t* source, const int32_t* place, void* rows, void* stream);
+int apexw_expert_combine(const void* y, int64_t y_stride, int64_t tokens, int32_t k, int64_t width, int32_t dtype,
+                         const int32_t* place, const void* weight, int32_t w_dtype, void* out, void* stream);
+int apexw_expert_combine_backward(const void* dout, int64_t dout_stride, const void* y, int64_t y_stride, int64_t tokens,
+                                  int32_t k, int64_t width, int32_t dtype, const int32_t* source, const int32_t* place,
+                                  const void* weight, int32_t w_dtype, void* dy, void* dweight, void* stream);
+
+/*
+ * Embedding: out[t] = scale weight[ids[t]] (contiguous rows of `width`), zeros for an id outside [0, vocab); its
+ * gradient dw[v] = scale (sum of dy[t] over ids[t] = v), [vocab x width] contiguous, dtype or F32, zeros for an id that
+ * no token has.  The sum is in fp32 in an order that the ids alone set.  workspace as above.
+ */
+int apexw_embedding_forward(const void* ids, int32_t id_bytes, int64_t n, const void* weight, int64_t w_stride,
+                            int64_t vocab, int64_t width, int32_t dtype, float scale, void* out, void* stream);
+int64_t apexw_embedding_weight_grad_workspace(int64_t n, int64_t vocab, int64_t width);
+int apexw_embedding_weight_grad(const void* dy, int64_t dy_stride, const void* ids, int32_t id_bytes, int64_t n,
+                                int64_t vocab, int64_t width, int32_t dtype, float scale, void* dw, int32_t dw_dtype,
+                                void* workspace, void* stream);
+
+/*
+ * Softmax cross entropy of a linear head, the logits l[i] = weight x[i] (vocab of them) never stored:
+ *   lse[i] = log(sum_v exp(l[i][v])),  loss[i] = lse[i] - l[i][target[i]]
+ *   G[i] = (exp(l[i] - lse[i]) - onehot(target[i])) dloss[i],  dx = G weight,  dw = G^T x
+ * x: n rows of `width` BF16 / F16 elements, x_stride apart; weight: vocab rows of the same type, w_stride apart.  Rows
+ * whose target is ignore_index or outside [0, vocab) count for nothing: loss, lse and dx are 0 there and dw has
+ * nothing of them, whatever they hold.  Products are summed in fp32; G is rounded to dtype.
+ * reduction: 0, or 1 (sum) or 2 (mean over the rows that count; NaN without any) of the losses into *total (fp32).
+ * backward: dloss_stride 0 is one number for all rows; mean != 0 divides it by the number of rows that count; dx
+ * ([n x width]) and dw ([vocab x width], both contiguous) may be NULL.
+ * workspace (16-byte aligned, in any state): as many bytes as the _workspace call answers; backward: 0, or bits 0 and 1
+ * for dx and dw.  Equal calls give equal bits.
+ */
+int64_t apexw_linear_cross_entropy_workspace(const void* weight, int64_t w_stride, int64_t n, int64_t width, int64_t vocab,
+                                             int32_t backward);
+int apexw_linear_cross_entropy_forward(const void* x, int64_t x_stride, int64_t n, int64_t width, const void* weight,
+                                       int64_t w_stride, int64_t vocab, int32_t dtype, const void* target,
+                                       int32_t id_bytes, int64_t ignore_index, float* loss, float* lse, int32_t reduction,
+                                       float* total, void* workspace, void* stream);
+int apexw_linear_cross_entropy_backward(const float* dloss, int64_t dloss_stride, int32_t mean, const void* x,
+                                        int64_t x_stride, int64_t n, int64_t width, const void* weight, int64_t w_stride,
+                                        int64_t vocab, int32_t dtype, const void* target, int32_t id_bytes,
+                                        int64_t ignore_index, const float* lse, void* dx, void* dw, void* workspace,
+                                        void* stream);
 
 /*
  * The clip of a list of gradients by their global norm, with torch.nn.utils.clip_grad_norm_'s arithmetic:
