@@ -458,10 +458,17 @@ template <int OD, bool kAdd = false> struct Store {
 //
 // A stage is two steps of 32 k by 16 x 16 x 32 MFMAs (at the power limit, which bounds large products of real
 // numbers, they reach 2160 TFLOP/s from registers where 32 x 32 x 16 ones reach 1950).  After an MFMA come at
-// most one fragment read of the next step and one copy, fenced in place: issued in bursts they stall the
-// wave's in-order issue.  The barrier stands between the steps, when the second one's fragments are in
-// registers: behind it the stage's buffer is free for the copies of the stage kStages on, and the next stage,
-// landed, gives its first fragments.  A's fragments are read into the registers of the ones just used.
+// most two fragment reads of the next step and one copy, fenced in place: issued in bursts they stall the
+// wave's in-order issue.  The second step's fragments are in registers when it begins, so the barrier stands
+// after its first two rows of products, where a wave has four of them and more (standing before them, the wait for
+// the last reads and for the other waves found the matrix cores idle).  Behind it the stage's buffer is free for the copies of the stage
+// kStages on, and the next stage, landed, gives its first fragments.  A's fragments are read into the registers of the
+// ones just used.  Behind the last tile's stages come copies of no memory, which leave zeros: a test around each copy
+// cost as much.
+//
+// Tried for 256 x 256 and not taken: a third stage of one operand, which leaves the copies two stages' time, with the
+// tile written from registers (1% slower: their latency does not bound a stage); four waves of 128 x 128, whose
+// fragments take two thirds of the LDS reads (the sums do not stay in place in 256 accumulation registers).
 template <class S, bool kAKN, bool kBKN, int DT, bool kHalves, class Jobs, class Place, class Out>
 APEXW_DEV void stream(const ExpertArgs& g, Jobs& jobs, Place&& locate, const Out& out, uint16_t* lds) {
   typedef Operand<kAKN, S::BM, S::kWaves> OpA;
@@ -490,8 +497,7 @@ APEXW_DEV void stream(const ExpertArgs& g, Jobs& jobs, Place&& locate, const Out
       return true;
     }
   };
-  bool more = take(copying, ia, ib, rows, cols, out0);
-  if (!more) return;
+  if (!take(copying, ia, ib, rows, cols, out0)) return;
   int here = copying, n = ia.stages, buf = 0;   // the tile being multiplied, its stages, the stage's buffer
 
   auto advance = [&]() {     // past the stage whose copies were issued
@@ -500,22 +506,21 @@ APEXW_DEV void stream(const ExpertArgs& g, Jobs& jobs, Place&& locate, const Out
     at = 0, ++copying;
     int r, c;
     int64_t o;
-    more = take(copying, ia, ib, r, c, o);
+    if (take(copying, ia, ib, r, c, o)) return;
+    ia.left = ib.left = 0, ia.stages = INT32_MAX;   // nothing from here on
   };
-  int ready = 0;             // stages in flight at the start
-  for (; ready < S::kStages && more; ++ready) {
+  auto tail_at = [&]() { return at == ia.stages - 1 ? ia.tail : kDepth; };
+#pragma unroll
+  for (int h = 0; h < S::kStages; ++h) {
     const u32x4 ba = A.buffer(ia, at), bb = B.buffer(ib, at);
-    const int tail = at == ia.stages - 1 ? ia.tail : kDepth;
+    const int tail = tail_at();
 #pragma unroll
-    for (int i = 0; i < OpA::kCopies; ++i) A.copy(ba, i, ready * kStageBytes, tail);
+    for (int i = 0; i < OpA::kCopies; ++i) A.copy(ba, i, h * kStageBytes, tail);
 #pragma unroll
-    for (int i = 0; i < OpB::kCopies; ++i) B.copy(bb, i, ready * kStageBytes, tail);
+    for (int i = 0; i < OpB::kCopies; ++i) B.copy(bb, i, h * kStageBytes, tail);
     advance();
   }
-
-  bool full = ready == S::kStages;   // the copies of the stage kStages - 1 on are under way
-  if (full) wait_copies<kCopies*(S::kStages - 1)>();
-  else wait_copies<0>();
+  wait_copies<kCopies*(S::kStages - 1)>();
   barrier();
 
   constexpr int kStores = Out::template stores<S>();   // of a wave and whole tile
@@ -537,51 +542,56 @@ APEXW_DEV void stream(const ExpertArgs& g, Jobs& jobs, Place&& locate, const Out
     for (int i = 0; i < FA; ++i) frag_a(lds + buf * S::kStageElems, 0, i);
 #pragma unroll
     for (int i = 0; i < FB; ++i) frag_b(lds + buf * S::kStageElems, 0, i);
-    // step s; blocks are computed transposed: a lane has four consecutive columns of a row.  Step s1 of the stage
-    // at st1 is next; side: what else is issued
-    auto step = [&](int s, const uint16_t* st1, int s1, auto&& side) {
-#pragma unroll
-      for (int j = 0; j < kMM; ++j) {
-        const int x = j / FB, y = j % FB;
-        acc[x][y] = mfma16<DT>(fb[s][y], fa[x], acc[x][y]);
-        __builtin_amdgcn_sched_barrier(0);
-        if (j < FB) frag_b(st1, s1, j);
-        if (y == FB - 1) frag_a(st1, s1, x);
-        side(j);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+    // Blocks are computed transposed: a lane has four consecutive columns of a row.  Step 0 reads the fragments of step 1,
+    // step 1 those of the next stage, from the barrier after kHold products on.
+    constexpr int kHold = FA >= 4 ? 2 * FB : 0;
+    static_assert(kMM - kHold >= FB + kHold / FB || kHold == 0, "a read after each product");
+    auto mm = [&](int s, int j) {
+      acc[j / FB][j % FB] = mfma16<DT>(fb[s][j % FB], fa[j / FB], acc[j / FB][j % FB]);
+      __builtin_amdgcn_sched_barrier(0);
     };
     for (int h = 0; h < n; ++h) {
-      const uint16_t* st = lds + buf * S::kStageElems;
       const int after = uniform(buf + 1 == S::kStages ? 0 : buf + 1);
-      step(0, st, 1, [](int) {});
-      // the next stage has landed; those after it may be on their way, and behind them the stores of the tile
-      // before (memory operations are counted off in their order)
-      if (fresh) {
-        if (full) wait_copies<kCopies*(S::kStages - 2) + kStores>();
-        else wait_copies<kStores>();
-        fresh = false;
-      } else {
-        if (full) wait_copies<kCopies*(S::kStages - 2)>();
-        else wait_copies<0>();
+      const uint16_t *st = lds + buf * S::kStageElems, *next = lds + after * S::kStageElems;
+#pragma unroll
+      for (int j = 0; j < kMM; ++j) {
+        mm(0, j);
+        if (j < FB) frag_b(st, 1, j);
+        if (j % FB == FB - 1) frag_a(st, 1, j / FB);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      barrier();
-      const bool refill = more;
-      const u32x4 ba = A.buffer(ia, at), bb = B.buffer(ib, at);   // (of no use without a stage to copy)
-      const int tail = at == ia.stages - 1 ? ia.tail : kDepth;
-      // (the last stage's reads of the next fragments are of no use)
-      step(1, lds + after * S::kStageElems, 0, [&](int j) {
-        if (refill) {
+      const u32x4 ba = A.buffer(ia, at), bb = B.buffer(ib, at);
+      const int tail = tail_at();
+      // the next stage has landed; those after it may be on their way, and behind them the stores of the tile before
+      // (memory operations are counted off in their order)
+      auto landed = [&]() {
+        if (fresh) wait_copies<kCopies*(S::kStages - 2) + kStores>();
+        else wait_copies<kCopies*(S::kStages - 2)>();
+        fresh = false;
+        barrier();
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      if (kHold == 0) landed();
+#pragma unroll
+      for (int j = 0; j < kMM; ++j) {
+        mm(1, j);
+        if (j == kHold - 1) landed();
+        // (the last stage's reads of the next fragments are of no use)
+        const int q = j - kHold;
+        if (q >= 0) {
+          if (q < FB) frag_b(next, 0, q);
+          if (q >= FB && q - FB < kHold / FB) frag_a(next, 0, q - FB);
+          if (j % FB == FB - 1) frag_a(next, 0, j / FB);
 #pragma unroll
           for (int i = 0; i < kCopies; ++i)
-            if ((kMM >= 2 * kCopies ? 2 * i + 1 : i * kMM / kCopies) == j) {
+            if ((kMM - kHold >= 2 * kCopies ? 2 * i + 1 : i * (kMM - kHold) / kCopies) == q) {
               if (i < OpA::kCopies) A.copy(ba, i, buf * kStageBytes, tail);
               else B.copy(bb, i - OpA::kCopies, buf * kStageBytes, tail);
             }
         }
-      });
-      if (refill) advance();
-      full = refill;
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      advance();
       buf = after;
     }
     out.template write<S, kWM>(g, acc, lds, down, across, rows, cols, out0);
@@ -598,9 +608,10 @@ APEXW_DEV void stream(const ExpertArgs& g, Jobs& jobs, Place&& locate, const Out
     }
     Span a, b;
     ++here;
-    if (!take(here, a, b, rows, cols, out0)) return;
+    if (!take(here, a, b, rows, cols, out0)) break;
     n = a.stages;
   }
+  wait_copies<0>();   // none lands in LDS that another workgroup has by then
 }
 
 // Zeros in the gradients of the experts without rows, in pieces of 16 K elements: piece p of them all goes to
