@@ -8,8 +8,8 @@
 // count are packed together, whole chunks wide, so a masked batch costs what its other rows cost and what stands in
 // masked rows, NaN too, reaches nothing.  Their number is known on the device alone.
 //
-// Forward: the logits of a tile stay in registers, and each row leaves the maximum and the sum of exponentials over the
-// tile's columns; a second launch joins them.  Backward: a piece of the vocabulary at a time, G of the piece from the
+// Forward: the logits of a tile stay in registers, and each row leaves the sum of exponentials over a wave's columns, relative
+// to its target's logit, which the packing forms; a second launch joins them.  Backward: a piece of the vocabulary at a time, G of the piece from the
 // logits computed again, rounded to 16 bits as an operand of the two products that take it; the piece is of a size that
 // the last-level cache holds.  dx adds up the pieces in fp32.
 #include "tiles.h"
@@ -18,24 +18,24 @@
 
 namespace {
 
-constexpr float kLog2E = 1.44269504f;
+constexpr float kLog2E = 1.44269504f, kLn2 = 0.693147181f;
 
 struct HeadState {          // device
   int32_t count;            // rows that count
-  float factor;             // G's factor besides dloss
-  float scale;              // and what dx and dW are multiplied with in the end
+  float factor, lift;       // G's factor besides dloss, and its logarithm to base 2
+  float scale;              // what dx and dW are multiplied with in the end
 };
-struct HeadRow {            // a row that counts
-  float lse, d;
+struct HeadRow {            // a row that counts; logarithms to base 2
+  float logit;              // its target's logit
+  float lse, d;             // backward
   int32_t target, row;      // its place among all rows
 };
 struct HeadArgs {
   const HeadState* state;
   const HeadRow* rows;
-  float* target_logit;
-  float2* stats;            // [tile of columns][row]: maximum, sum of exp(l - maximum)
-  int64_t stats_ld;
-  int32_t first;            // the piece's first column
+  const float* shift;       // one a row, of the exponents of its tiles
+  float* sums;              // [columns of a wave][row]: log2 of the sum of 2^(l log2 e - shift)
+  int64_t sums_ld;
 };
 
 // ---------------------------------------------------------------------------
@@ -43,15 +43,16 @@ struct HeadArgs {
 // ---------------------------------------------------------------------------
 
 struct PackArgs {
-  const uint16_t* x;
+  const uint16_t *x, *w;
   const void* target;
   const float *lse, *dloss;   // backward
   uint16_t* packed;
   HeadState* state;
   HeadRow* rows;
+  float* shift;
   float *loss, *lse_out;      // forward: zeros for the rows that do not count
   void* dx;                   // the same, backward
-  int64_t n, x_stride, dloss_stride, ignore;
+  int64_t n, x_stride, w_stride, dloss_stride, ignore;
   int32_t width, wide, vocab, id64, per, mean, rescale;
 };
 
@@ -70,8 +71,9 @@ template <class T, class F> APEXW_DEV T over_workgroup(T x, T* lds, F&& f) {
   return x;
 }
 
-// A workgroup has `per` (up to 256) rows; how many rows before them count it finds by itself
-__global__ __launch_bounds__(256) void head_pack_kernel(PackArgs a) {
+// A workgroup has `per` (up to 256) rows; how many rows before them count it finds by itself.  A wave takes a row at a
+// time: copies it, and forms its target's logit on the way.
+template <int DT> __global__ __launch_bounds__(256) void head_pack_kernel(PackArgs a) {
   __shared__ int ints[4];
   __shared__ float floats[4];
   __shared__ int place[256];
@@ -89,8 +91,7 @@ __global__ __launch_bounds__(256) void head_pack_kernel(PackArgs a) {
   before = over_workgroup(before, ints, [](int p, int q) { return p + q; });
 
   const int64_t mine = first + threadIdx.x;
-  const int64_t target = mine < end ? target_of(a, mine) : -1;
-  const bool has = mine < end && counts(a, target);
+  const bool has = mine < end && counts(a, target_of(a, mine));
   const uint64_t ballot = __ballot(has);
   if (lane_id() == 0) ints[threadIdx.x >> 6] = __builtin_popcountll(ballot);
   __syncthreads();
@@ -99,38 +100,63 @@ __global__ __launch_bounds__(256) void head_pack_kernel(PackArgs a) {
   const int all = before + ints[0] + ints[1] + ints[2] + ints[3];
   place[threadIdx.x] = has ? at : -1;
   __syncthreads();
-  if (has) {
-    const float d = a.dloss ? a.dloss[mine * a.dloss_stride] : 0.0f;
-    a.rows[at] = HeadRow{a.lse ? a.lse[mine] : 0.0f, d, (int32_t)target, (int32_t)mine};
-    if (find_most) most = fmaxf(most, fabsf(d));
-  } else if (mine < end) {
+  if (mine < end && !has) {
     if (a.loss) a.loss[mine] = 0.0f;
     if (a.lse_out) a.lse_out[mine] = 0.0f;
   }
   if (last) {
-    if (a.rescale) most = over_workgroup(most, floats, [](float p, float q) { return fmaxf(p, q); });
+    if (a.rescale) {
+      if (has) most = fmaxf(most, fabsf(a.dloss[mine * a.dloss_stride]));
+      most = over_workgroup(most, floats, [](float p, float q) { return fmaxf(p, q); });
+    }
     if (threadIdx.x == 0) {
       // the largest factor of a row, as a power of two: divided out of G, which fp16 would lose below 2^-24, and
       // multiplied into the sums
       const float mean = a.mean && all > 0 ? 1.0f / (float)all : 1.0f;
       const uint32_t bits = __float_as_uint(most * mean) & 0x7F800000u;
       const bool use = a.rescale && bits >= 0x01000000u && bits < 0x7E800000u;
-      const float scale = use ? __uint_as_float(bits) : 1.0f;
-      *a.state = HeadState{all, mean / scale, scale};
+      const float scale = use ? __uint_as_float(bits) : 1.0f, factor = mean / scale;
+      *a.state = HeadState{all, factor, log2f(factor), scale};
     }
   }
-  const int chunks = a.wide / 8, rows = (int)(end - first);
-  const bool whole = a.width % 8 == 0;
-  for (int i = threadIdx.x; i < rows * chunks; i += 256) {
-    const int r = i / chunks, c = i - r * chunks, p = place[r];
-    if (p >= 0) {
-      *(u32x4*)&a.packed[(int64_t)p * a.wide + c * 8] =
-          load_chunk(a.x + (first + r) * a.x_stride + c * 8, clamp8(a.width - c * 8));
-    } else if (a.dx) {
-      uint16_t* to = (uint16_t*)a.dx + (first + r) * a.width + c * 8;
-      if (whole) APEXW_GLOBAL(Chunk, to)->v = u32x4{0u, 0u, 0u, 0u};
-      else for (int j = 0; j < clamp8(a.width - c * 8); ++j) APEXW_GLOBAL(uint16_t, to)[j] = 0;
+
+  const int chunks = a.wide / 8, rows = (int)(end - first), lane = lane_id();
+  for (int r = threadIdx.x >> 6; r < rows; r += 4) {
+    const int64_t i = first + r;
+    const int p = uniform(place[r]);
+    if (p < 0) {
+      if (!a.dx) continue;
+      uint16_t* to = (uint16_t*)a.dx + i * a.width;
+      for (int c = lane; c < chunks; c += 64) {
+        const int n = clamp8(a.width - c * 8);
+        if (n == 8) APEXW_GLOBAL(Chunk, to + c * 8)->v = u32x4{0u, 0u, 0u, 0u};
+        else for (int j = 0; j < n; ++j) APEXW_GLOBAL(uint16_t, to)[c * 8 + j] = 0;
+      }
+      continue;
     }
+    const int target = (int)target_of(a, i);
+    const uint16_t *x = a.x + i * a.x_stride, *w = a.w + target * a.w_stride;
+    float dot = 0.0f;
+#pragma unroll 4
+    for (int c = lane; c < chunks; c += 64) {
+      const int n = clamp8(a.width - c * 8);
+      const u32x4 xv = load_chunk(x + c * 8, n), wv = load_chunk(w + c * 8, n);
+      *(u32x4*)&a.packed[(int64_t)p * a.wide + c * 8] = xv;
+      float xs[8], ws[8];
+      values<DT>(xv, xs), values<DT>(wv, ws);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dot = fmaf(xs[j], ws[j], dot);
+    }
+    dot = wave_sum(dot);
+    if (lane) continue;
+    HeadRow row{dot * kLog2E, 0.0f, 0.0f, target, (int32_t)i};
+    float shift = row.logit - row.logit == 0.0f ? row.logit : 0.0f;
+    if (a.lse) {
+      row.lse = a.lse[i] * kLog2E, row.d = a.dloss[i * a.dloss_stride];
+      const uint32_t bits = __float_as_uint(log2f(fabsf(row.d)) - row.lse);
+      shift = __uint_as_float((bits & ~1u) | (row.d < 0.0f));
+    }
+    a.rows[p] = row, a.shift[p] = shift;
   }
 }
 
@@ -141,7 +167,6 @@ __global__ __launch_bounds__(256) void head_pack_kernel(PackArgs a) {
 // A tile's first row and column, which `locate` packs into one number
 APEXW_DEV int64_t tile_at(int64_t row, int64_t col) { return row << 32 | col; }
 
-// -inf in the columns behind the last one
 template <int FA, int FB, class Acc> APEXW_DEV void mask_columns(Acc& acc, int wn, int cols, float to) {
   const int c0 = 4 * (lane_id() >> 4);
 #pragma unroll
@@ -154,113 +179,115 @@ template <int FA, int FB, class Acc> APEXW_DEV void mask_columns(Acc& acc, int w
     }
 }
 
-// Forward: each row's maximum and sum over the tile's columns, first over a wave's, then over the waves' through LDS
-struct Stats {
+// Each row's shift
+template <int FA> struct Shifts {
+  float v[FA];
+  __device__ __forceinline__ void load(const float* shift, int64_t row0, int row, int rows) {
+#pragma unroll
+    for (int i = 0; i < FA; ++i) v[i] = shift[row0 + (row + 16 * i < rows ? row + 16 * i : rows - 1)];
+  }
+  __device__ __forceinline__ void arrived() {
+#pragma unroll
+    for (int i = 0; i < FA; ++i) asm volatile("" : "+v"(v[i]));
+  }
+};
+
+// Forward: each row's sum of exponentials over a wave's columns, relative to its target's.  That is a maximum's part as
+// long as no logit is 83 above the target's (2^120); the rows of a block where one is are summed again from their maximum.
+struct Sums {
   HeadArgs h;
+  template <int FA> using Rows = Shifts<FA>;
+  template <class R> __device__ __forceinline__ void load(R& known, int64_t out0, int row, int rows) const {
+    known.load(h.shift, out0 >> 32, row, rows);
+  }
   template <class S> static constexpr int stores() { return 0; }
-  template <class S, int kWM, class Acc>
-  __device__ __forceinline__ void write(const ExpertArgs& g, Acc& acc, uint16_t* lds, int down, int across, int rows, int cols,
-                                        int64_t out0) const {
-    constexpr int FA = kWM / 16, FB = S::WN / 16, kAcross = S::BN / S::WN;
-    static_assert(kWM * 8 <= S::kOut * 2, "a wave's statistics in its part of LDS");
-    const int wm = down * kWM, wn = across * S::WN, lane = lane_id(), r0 = lane & 15;
+  template <class S, int kWM, class Acc, class R>
+  __device__ __forceinline__ void write(const ExpertArgs& g, Acc& acc, const R& known, uint16_t* lds, int down, int across,
+                                        int rows, int cols, int64_t out0) const {
+    constexpr int FA = kWM / 16, FB = S::WN / 16;
+    const int wm = down * kWM, wn = across * S::WN, lane = lane_id();
     const int64_t row0 = out0 >> 32;
     const int col0 = (int)(uint32_t)out0;
-    float2* mine = (float2*)(lds + S::kStages * S::kStageElems + (down * kAcross + across) * S::kOut);
-    int target[FA];
+    if (wn >= cols) return;
+    if (wn + S::WN > cols) mask_columns<FA, FB>(acc, wn, cols, -INFINITY);
+    float* to = h.sums + (col0 + wn) / S::WN * h.sums_ld + row0 + wm;
 #pragma unroll
     for (int i = 0; i < FA; ++i) {
-      const int r = wm + 16 * i + r0;
-      target[i] = r < rows ? h.rows[row0 + r].target - col0 - wn : -1;
-    }
-    if (cols < S::BN) mask_columns<FA, FB>(acc, wn, cols, -INFINITY);
-#pragma unroll
-    for (int i = 0; i < FA; ++i) {
-      float m = acc[i][0][0];
-#pragma unroll
-      for (int j = 0; j < FB; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) m = fmaxf(m, acc[i][j][q]);
-      m = fmaxf(m, __shfl_xor(m, 16, 64));
-      m = fmaxf(m, __shfl_xor(m, 32, 64));
-      const float from = m == -INFINITY ? 0.0f : m;
+      const float shift = known.v[i];
       float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int j = 0; j < FB; ++j)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) s[q] += __builtin_amdgcn_exp2f((acc[i][j][q] - from) * kLog2E);
+        for (int q = 0; q < 4; ++q) s[q] += __builtin_amdgcn_exp2f(fmaf(acc[i][j][q], kLog2E, -shift));
       float sum = (s[0] + s[1]) + (s[2] + s[3]);
       sum += __shfl_xor(sum, 16, 64);
       sum += __shfl_xor(sum, 32, 64);
-      if (lane < 16) mine[16 * i + lane] = make_float2(m, sum);
-      const bool hit = target[i] >= 0 && target[i] < S::WN && (target[i] >> 2 & 3) == lane >> 4;
-      if (__ballot(hit)) {   // in a few of the vocabulary's tiles
-        float l = 0.0f;
+      float part = __builtin_amdgcn_logf(sum);   // to base 2
+      if (__ballot(!(sum < 0x1p120f))) {
+        float m = acc[i][0][0];
 #pragma unroll
         for (int j = 0; j < FB; ++j)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) l = target[i] == 16 * j + 4 * (lane >> 4) + q ? acc[i][j][q] : l;
-        if (hit) h.target_logit[row0 + wm + 16 * i + r0] = l;
+          for (int q = 0; q < 4; ++q) m = fmaxf(m, acc[i][j][q]);
+        m = fmaxf(m, __shfl_xor(m, 16, 64));
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        const float top = m == -INFINITY ? 0.0f : m * kLog2E;
+        sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < FB; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][q], kLog2E, -top));
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        part = (top - shift) + __builtin_amdgcn_logf(sum);
       }
-    }
-    barrier();
-    const int r = threadIdx.x;
-    if (r < kWM * (S::BM / S::WM) && r < rows) {
-      const float2* from = (const float2*)(lds + S::kStages * S::kStageElems + r / kWM * kAcross * S::kOut) + r % kWM;
-      float2 part[kAcross];
-      float m = -INFINITY, sum = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kAcross; ++w) part[w] = from[w * (S::kOut / 4)], m = fmaxf(m, part[w].x);
-      const float to = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-      for (int w = 0; w < kAcross; ++w) sum += part[w].y * __builtin_amdgcn_exp2f((part[w].x - to) * kLog2E);
-      h.stats[col0 / S::BN * h.stats_ld + row0 + r] = make_float2(m, sum);
+      if (lane < 16 && wm + 16 * i + lane < rows) to[16 * i + lane] = part;
     }
   }
 };
 
-// Backward: the tile's part of G
+// Backward: the tile's part of G without the targets' ones, whole chunks of columns
 template <int DT> struct Prob {
   HeadArgs h;
+  template <int FA> using Rows = Shifts<FA>;
+  template <class R> __device__ __forceinline__ void load(R& known, int64_t out0, int row, int rows) const {
+    known.load(h.shift, out0 >> 32, row, rows);
+  }
   template <class S> static constexpr int stores() { return Store<DT>::template stores<S>(); }
-  template <class S, int kWM, class Acc>
-  __device__ __forceinline__ void write(const ExpertArgs& g, Acc& acc, uint16_t* lds, int down, int across, int rows, int cols,
-                                        int64_t out0) const {
+  template <class S, int kWM, class Acc, class R>
+  __device__ __forceinline__ void write(const ExpertArgs& g, Acc& acc, const R& known, uint16_t* lds, int down, int across,
+                                        int rows, int cols, int64_t out0) const {
     constexpr int FA = kWM / 16, FB = S::WN / 16;
-    const int wm = down * kWM, wn = across * S::WN, lane = lane_id(), r0 = lane & 15;
-    const int64_t row0 = out0 >> 32;
-    const int col0 = (int)(uint32_t)out0;
-    const float factor = h.state->factor;
-    HeadRow info[FA];
+    const float lift = h.state->lift;
 #pragma unroll
     for (int i = 0; i < FA; ++i) {
-      const int r = wm + 16 * i + r0;
-      info[i] = h.rows[row0 + (r < rows ? r : rows - 1)];
-    }
-#pragma unroll
-    for (int i = 0; i < FA; ++i) {
+      const uint32_t bits = __float_as_uint(known.v[i]);
+      const float shift = __uint_as_float(bits & ~1u) + lift;
 #pragma unroll
       for (int j = 0; j < FB; ++j)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) acc[i][j][q] = __builtin_amdgcn_exp2f((acc[i][j][q] - info[i].lse) * kLog2E);
-      const int t = info[i].target - h.first - col0 - wn;
-      if (__ballot(t >= 0 && t < S::WN)) {
+        for (int q = 0; q < 4; ++q) acc[i][j][q] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][q], kLog2E, shift));
+      if (__ballot(bits & 1u)) {
 #pragma unroll
         for (int j = 0; j < FB; ++j)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) acc[i][j][q] -= t == 16 * j + 4 * (lane >> 4) + q ? 1.0f : 0.0f;
+          for (int q = 0; q < 4; ++q) acc[i][j][q] = bits & 1u ? -acc[i][j][q] : acc[i][j][q];
       }
-      const float d = info[i].d * factor;
-#pragma unroll
-      for (int j = 0; j < FB; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) acc[i][j][q] *= d;
     }
-    // whole chunks: zeros behind the last column
-    if (cols < S::BN) mask_columns<FA, FB>(acc, wn, cols, 0.0f);
-    Store<DT>::template put<S, kWM>(g, acc, lds, down, across, rows, (cols + 7) / 8 * 8, row0 * g.ldo + col0, Same{});
+    if (cols < S::BN) mask_columns<FA, FB>(acc, across * S::WN, cols, 0.0f);
+    Store<DT>::template put<S, kWM>(g, acc, lds, down, across, rows, (cols + 7) / 8 * 8,
+                                    (out0 >> 32) * g.ldo + (int64_t)(uint32_t)out0, Same{});
   }
 };
+
+// The targets' elements of the piece's G
+template <int DT> __global__ __launch_bounds__(256) void head_targets_kernel(HeadArgs h, int first, int cols, void* g, int64_t ldg) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= h.state->count) return;
+  const HeadRow row = h.rows[i];
+  const int t = row.target - first;
+  if (t >= 0 && t < cols) store_elem<DT>(g, i * ldg + t, (exp2f(row.logit - row.lse) - 1.0f) * row.d * h.state->factor);
+}
 
 template <class S, int DT, class Out> __global__ __launch_bounds__(S::kThreads, 2) void head_logits_kernel(ExpertArgs g, Out out) {
   __shared__ __attribute__((aligned(16))) uint16_t lds[S::kLds];
@@ -277,33 +304,34 @@ template <class S, int DT, class Out> __global__ __launch_bounds__(S::kThreads, 
 // The rows' statistics joined, and their mean
 // ---------------------------------------------------------------------------
 
-// 16 rows a workgroup, a 16th of the tiles a thread
-__global__ __launch_bounds__(256) void head_join_kernel(HeadArgs h, int tiles, float* __restrict__ loss, float* __restrict__ lse) {
-  __shared__ float2 parts[16][16];
+// 16 rows a workgroup, a 64th of the sums a thread
+__global__ __launch_bounds__(1024) void head_join_kernel(HeadArgs h, int parts, float* __restrict__ loss, float* __restrict__ lse) {
+  __shared__ float2 lds[64][16];
   const int r = threadIdx.x & 15, q = threadIdx.x >> 4;
   const int64_t row = (int64_t)blockIdx.x * 16 + r;
   const int count = h.state->count;
   if ((int64_t)blockIdx.x * 16 >= count) return;
   float m = -INFINITY, s = 0.0f;
   if (row < count)
-#pragma unroll 4
-    for (int t = q; t < tiles; t += 16) {
-      const float2 p = h.stats[t * h.stats_ld + row];
-      const float top = fmaxf(m, p.x), to = top == -INFINITY ? 0.0f : top;
-      s = s * __builtin_amdgcn_exp2f((m - to) * kLog2E) + p.y * __builtin_amdgcn_exp2f((p.x - to) * kLog2E);
+#pragma unroll 8
+    for (int t = q; t < parts; t += 64) {
+      const float x = h.sums[t * h.sums_ld + row], top = fmaxf(m, x), to = top == -INFINITY ? 0.0f : top;
+      s = s * __builtin_amdgcn_exp2f(m - to) + __builtin_amdgcn_exp2f(x - to);
       m = top;
     }
-  parts[q][r] = make_float2(m, s);
+  lds[q][r] = make_float2(m, s);
   __syncthreads();
   if (q != 0 || row >= count) return;
-  float top = -INFINITY, sum = 0.0f;
-  for (int i = 0; i < 16; ++i) top = fmaxf(top, parts[i][r].x);
-  const float to = top == -INFINITY ? 0.0f : top;
-  for (int i = 0; i < 16; ++i) sum += parts[i][r].y * __builtin_amdgcn_exp2f((parts[i][r].x - to) * kLog2E);
-  const float log_sum = logf(sum);
-  const int at = h.rows[row].row;
-  lse[at] = to + log_sum;
-  loss[at] = (to - h.target_logit[row]) + log_sum;
+  for (int i = 1; i < 64; ++i) {
+    const float2 x = lds[i][r];
+    const float top = fmaxf(m, x.x), to = top == -INFINITY ? 0.0f : top;
+    s = s * __builtin_amdgcn_exp2f(m - to) + x.y * __builtin_amdgcn_exp2f(x.x - to);
+    m = top;
+  }
+  const HeadRow& info = h.rows[row];
+  const float sum = (m == -INFINITY ? 0.0f : m) + log2f(s), shift = h.shift[row];
+  lse[info.row] = (shift + sum) * kLn2;
+  loss[info.row] = ((shift - info.logit) + sum) * kLn2;
 }
 
 // The sum of the rows' losses, or their mean over the rows that count
@@ -328,10 +356,12 @@ __global__ __launch_bounds__(1024) void head_total_kernel(const HeadState* state
 
 template <int OD> struct Scaled {
   const HeadState* state;
+  template <int FA> using Rows = NoRows;
+  template <class R> __device__ __forceinline__ void load(R&, int64_t, int, int) const {}
   template <class S> static constexpr int stores() { return Store<OD>::template stores<S>(); }
   template <class S, int kWM, class Acc>
-  __device__ __forceinline__ void write(const ExpertArgs& g, Acc& acc, uint16_t* lds, int down, int across, int rows, int cols,
-                                        int64_t out0) const {
+  __device__ __forceinline__ void write(const ExpertArgs& g, Acc& acc, const NoRows&, uint16_t* lds, int down, int across,
+                                        int rows, int cols, int64_t out0) const {
     const float scale = state->scale;
     Store<OD>::template put<S, kWM>(g, acc, lds, down, across, rows, cols, out0, [scale](f32x4 v, int, int) {
 #pragma unroll
@@ -380,27 +410,31 @@ template <class S, int DT, bool kAdd> __global__ __launch_bounds__(S::kThreads, 
 // dx: the parts' sums, scaled, each row at its place
 template <int DT> __global__ __launch_bounds__(256) void head_dx_kernel(HeadArgs h, const float* __restrict__ sums, int64_t stride,
                                                                        int splits, int width, uint16_t* dx) {
-  const int count = h.state->count, per = (width + 3) / 4;
+  const int count = h.state->count, per = (width + 7) / 8;
   const float scale = h.state->scale;
   const int64_t n = (int64_t)count * per;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
     const int64_t r = i / per;
-    const int c = (int)(i - r * per) * 4, has = width - c < 4 ? width - c : 4;
-    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < splits; ++s) {
-      const float* p = sums + s * stride + r * width + c;
-      if (has == 4) {
-        const u32x4 w = APEXW_GLOBAL(const Chunk32, p)->v;
+    const int c = (int)(i - r * per) * 8, has = clamp8(width - c);
+    const float* p = sums + r * width + c;
+    uint16_t* to = dx + (int64_t)h.rows[r].row * width + c;
+    if (has == 8) {
+      float v[8] = {};
+      for (int s = 0; s < splits; ++s) {
+        const u32x4 lo = APEXW_GLOBAL(const Chunk32, p + s * stride)->v, hi = APEXW_GLOBAL(const Chunk32, p + s * stride + 4)->v;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] += __uint_as_float(w[q]);
-      } else {
-        for (int q = 0; q < has; ++q) v[q] += p[q];
+        for (int q = 0; q < 4; ++q) v[q] += __uint_as_float(lo[q]), v[4 + q] += __uint_as_float(hi[q]);
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] *= scale;
+      APEXW_GLOBAL(Chunk, to)->v = rounded<DT>(v);
+    } else {
+      for (int q = 0; q < has; ++q) {
+        float v = 0.0f;
+        for (int s = 0; s < splits; ++s) v += p[s * stride + q];
+        store_elem<DT>(to, q, v * scale);
       }
     }
-    const int64_t at = (int64_t)h.rows[r].row * width + c;
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (q < has) store_elem<DT>(dx, at + q, v[q] * scale);
   }
 }
 
@@ -416,8 +450,8 @@ constexpr int64_t kPiece = 256ll << 20;
 struct HeadPlan {
   int64_t n, width, wide, vocab, w_stride;
   bool copy_w;
-  int64_t at_rows, at_x, at_w, at_logit, at_stats, at_g, at_sums, at_dw, bytes;
-  int64_t stats_ld, piece, piece_ld;
+  int64_t at_rows, at_shift, at_x, at_w, at_parts, at_g, at_sums, at_dw, bytes;
+  int64_t parts_ld, piece, piece_ld;
   ExpertArgs logits, rows, weight;   // sizes of a whole piece's products
   Cut cut_logits, cut_dx, cut_dw;
   HeadPlan(const void* w, int64_t stride, int64_t n_, int64_t width_, int64_t vocab_, bool backward, bool need_dx, bool need_dw)
@@ -425,7 +459,8 @@ struct HeadPlan {
     copy_w = !k_rows_ok(w, stride, width);
     if (copy_w) w_stride = wide;
     at_rows = 256;
-    at_x = at_rows + whole(n * (int64_t)sizeof(HeadRow));
+    at_shift = at_rows + whole(n * (int64_t)sizeof(HeadRow));
+    at_x = at_shift + whole(n * 4);
     at_w = at_x + whole(n * wide * 2);
     int64_t at = at_w + (copy_w ? whole(vocab * wide * 2) : 0);
     piece = vocab;
@@ -438,9 +473,8 @@ struct HeadPlan {
     logits.k = (int32_t)width, logits.wide = (int32_t)wide, logits.lda = wide, logits.ldb = w_stride;
     cut_logits = cut_rows(logits, false);
     if (!backward) {
-      stats_ld = (n + 15) / 16 * 16;
-      at_logit = at, at += whole(n * 4);
-      at_stats = at, at += whole(stats_ld * ((vocab + 127) / 128) * 8);
+      parts_ld = (n + 15) / 16 * 16;
+      at_parts = at, at += whole(parts_ld * parts() * 4);
       bytes = at;
       return;
     }
@@ -458,7 +492,12 @@ struct HeadPlan {
     at_dw = at, at += need_dw && weight.splits > 1 ? whole(weight.splits * piece * width * 4) : 0;
     bytes = at;
   }
+  int64_t parts() const {   // waves across the vocabulary
+    const int64_t wave = cut_logits.shape == 0 ? Small::WN : Large::WN;
+    return (vocab + wave - 1) / wave;
+  }
 };
+static_assert(Large::WN == 64 && Wide::WN == 64 && Mid::WN == 64, "columns of a wave");
 
 bool head_ok(int64_t n, int64_t width, int64_t vocab) {
   return n >= 0 && n <= INT32_MAX - 65536 && width > 0 && width <= kMostLd && vocab > 0 && vocab <= INT32_MAX - 65536;
@@ -470,10 +509,7 @@ template <class S, int DT, class Out> void launch_logits_shape(const ExpertArgs&
 }
 template <int DT, class Out> void launch_logits(ExpertArgs g, int shape, const Out& out, hipStream_t s) {
   if (shape == 3) {
-    g.which = kMost;
     launch_logits_shape<Large, DT>(g, out, s);
-    g.which = kRest;
-    launch_logits_shape<Wide, DT>(g, out, s);
   } else if (shape == 2) {
     launch_logits_shape<Wide, DT>(g, out, s);
   } else if (shape == 1) {
@@ -489,10 +525,7 @@ template <class S, int DT> void launch_dx_shape(const ExpertArgs& g, bool add, h
 }
 template <int DT> void launch_dx(ExpertArgs g, int shape, bool add, hipStream_t s) {
   if (shape == 3) {
-    g.which = kMost;
     launch_dx_shape<Large, DT>(g, add, s);
-    g.which = kRest;
-    launch_dx_shape<Wide, DT>(g, add, s);
   } else if (shape == 2) {
     launch_dx_shape<Wide, DT>(g, add, s);
   } else if (shape == 1) {
@@ -519,14 +552,15 @@ template <int DT> void launch_dw(const ExpertArgs& g, int shape, const HeadState
 }
 
 // The weights, copied to whole chunks where they are not; rows packed
-const uint16_t* launch_pack(const HeadPlan& p, PackArgs& a, const void* w, int64_t stride, char* ws, hipStream_t s) {
-  a.state = (HeadState*)ws, a.rows = (HeadRow*)(ws + p.at_rows), a.packed = (uint16_t*)(ws + p.at_x);
+template <int DT> const uint16_t* launch_pack(const HeadPlan& p, PackArgs& a, const void* w, int64_t stride, char* ws, hipStream_t s) {
+  a.state = (HeadState*)ws, a.rows = (HeadRow*)(ws + p.at_rows), a.shift = (float*)(ws + p.at_shift);
+  a.packed = (uint16_t*)(ws + p.at_x), a.w = (const uint16_t*)w, a.w_stride = stride;
   a.n = p.n, a.width = (int32_t)p.width, a.wide = (int32_t)p.wide, a.vocab = (int32_t)p.vocab;
   // about 1024 workgroups, of at least 4 rows
   const int64_t per = (p.n + 1023) / 1024;
   a.per = (int32_t)(per < 4 ? 4 : per > 256 ? 256 : per);
   const int64_t grid = (p.n + a.per - 1) / a.per;
-  hipLaunchKernelGGL(head_pack_kernel, dim3((unsigned)(grid ? grid : 1)), dim3(256), 0, s, a);
+  hipLaunchKernelGGL(head_pack_kernel<DT>, dim3((unsigned)(grid ? grid : 1)), dim3(256), 0, s, a);
   if (!p.copy_w) return (const uint16_t*)w;
   uint16_t* at = (uint16_t*)(ws + p.at_w);
   const uint16_t* from = (const uint16_t*)w;
@@ -567,16 +601,16 @@ extern "C" int apexw_linear_cross_entropy_forward(const void* x, int64_t x_strid
   PackArgs pack{};
   pack.x = (const uint16_t*)x, pack.x_stride = x_stride, pack.target = target, pack.id64 = id_bytes == 8;
   pack.ignore = ignore_index, pack.loss = loss, pack.lse_out = lse;
-  const uint16_t* w = launch_pack(p, pack, weight, w_stride, ws, s);
-  HeadArgs h{pack.state, pack.rows, (float*)(ws + p.at_logit), (float2*)(ws + p.at_stats), p.stats_ld, 0};
-  if (n > 0) {
+  by_half(dtype, [&](auto d) {
+    constexpr int DT = decltype(d)::value;
+    const uint16_t* w = launch_pack<DT>(p, pack, weight, w_stride, ws, s);
+    if (n == 0) return;
+    const HeadArgs h{pack.state, pack.rows, pack.shift, (float*)(ws + p.at_parts), p.parts_ld};
     ExpertArgs g = p.logits;
     g.a = pack.packed, g.b = w, g.ends = &pack.state->count;
-    by_half(dtype, [&](auto d) { launch_logits<decltype(d)::value>(g, p.cut_logits.shape, Stats{h}, s); });
-    const int64_t tile = p.cut_logits.shape >= 2 ? 256 : 128;
-    hipLaunchKernelGGL(head_join_kernel, dim3((unsigned)((n + 15) / 16)), dim3(256), 0, s, h, (int)((vocab + tile - 1) / tile),
-                       loss, lse);
-  }
+    launch_logits<DT>(g, p.cut_logits.shape, Sums{h}, s);
+    hipLaunchKernelGGL(head_join_kernel, dim3((unsigned)((n + 15) / 16)), dim3(1024), 0, s, h, (int)p.parts(), loss, lse);
+  });
   if (reduction) hipLaunchKernelGGL(head_total_kernel, dim3(1), dim3(1024), 0, s, pack.state, loss, n, (int)(reduction == 2), total);
   return hipGetLastError() == hipSuccess ? APEXW_OK : APEXW_ERR_LAUNCH;
 }
@@ -602,10 +636,10 @@ extern "C" int apexw_linear_cross_entropy_backward(const float* dloss, int64_t d
   pack.x = (const uint16_t*)x, pack.x_stride = x_stride, pack.target = target, pack.id64 = id_bytes == 8;
   pack.ignore = ignore_index, pack.lse = lse, pack.dloss = dloss, pack.dloss_stride = dloss_stride, pack.dx = dx;
   pack.mean = mean != 0, pack.rescale = dtype == APEXW_F16;
-  const uint16_t* w = launch_pack(p, pack, weight, w_stride, ws, s);
-  HeadArgs h{pack.state, pack.rows, nullptr, nullptr, 0, 0};
   by_half(dtype, [&](auto d) {
     constexpr int DT = decltype(d)::value;
+    const uint16_t* w = launch_pack<DT>(p, pack, weight, w_stride, ws, s);
+    const HeadArgs h{pack.state, pack.rows, pack.shift, nullptr, 0};
     for (int64_t v = 0; v < vocab; v += p.piece) {
       const int32_t cols = (int32_t)(vocab - v < p.piece ? vocab - v : p.piece);
       const uint16_t* wp = w + v * p.w_stride;
@@ -613,8 +647,8 @@ extern "C" int apexw_linear_cross_entropy_backward(const float* dloss, int64_t d
       if (n > 0) {
         ExpertArgs g = p.logits;
         g.a = pack.packed, g.b = wp, g.ends = &pack.state->count, g.n = cols, g.out = G, g.ldo = p.piece_ld;
-        h.first = (int32_t)v;
         launch_logits<DT>(g, p.cut_logits.shape, Prob<DT>{h}, s);
+        hipLaunchKernelGGL(head_targets_kernel<DT>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, h, (int)v, cols, G, p.piece_ld);
       }
       if (dw) {
         ExpertArgs g = p.weight;

@@ -372,16 +372,22 @@ typedef Shape<128, 256, 64, 64, 3, 1> Wide;
 typedef Shape<64, 128, 32, 64, 3, 2> Mid;
 typedef Shape<32, 128, 32, 32, 3, 2> Small;
 
-// What becomes of a tile: as it is, or what `value` makes of the four sums of a lane, added to what is there (kAdd,
+// What becomes of a tile.  A policy's Rows are what it loads of the rows of its lane's blocks when the tile begins;
+// stores() says how many stores a wave makes of a whole tile.  Here: the tile as it is, or what `value` makes of the four sums of a lane, added to what is there (kAdd,
 // fp32), in whole lines.  value(v, r, c): columns c .. c + 3 of the tile's row r.
 struct Same {
   __device__ __forceinline__ f32x4 operator()(f32x4 v, int, int) const { return v; }
 };
+struct NoRows {   // nothing is known of a tile's rows beforehand
+  __device__ __forceinline__ void arrived() const {}
+};
 template <int OD, bool kAdd = false> struct Store {
+  template <int FA> using Rows = NoRows;
+  template <class R> __device__ __forceinline__ void load(R&, int64_t, int, int) const {}
   template <class S> static constexpr int stores() { return S::WM / 16 * (S::WN * (OD == APEXW_F32 ? 4 : 2) / 64); }
   template <class S, int kWM, class Acc>
-  __device__ __forceinline__ void write(const ExpertArgs& g, Acc& acc, uint16_t* lds, int down, int across, int rows,
-                                        int cols, int64_t out0) const {
+  __device__ __forceinline__ void write(const ExpertArgs& g, Acc& acc, const NoRows&, uint16_t* lds, int down, int across,
+                                        int rows, int cols, int64_t out0) const {
     put<S, kWM>(g, acc, lds, down, across, rows, cols, out0, Same{});
   }
 
@@ -535,6 +541,8 @@ APEXW_DEV void stream(const ExpertArgs& g, Jobs& jobs, Place&& locate, const Out
     for (int i = 0; i < FA; ++i)
 #pragma unroll
       for (int j = 0; j < FB; ++j) acc[i][j] = f32x4{};
+    typename Out::template Rows<FA> known;
+    out.load(known, out0, wm + (lane_id() & 15), rows);
     u32x4 fa[FA], fb[2][FB];
     auto frag_a = [&](const uint16_t* st, int s, int i) { fa[i] = OpA::frag(st, wm + 16 * i, s); };
     auto frag_b = [&](const uint16_t* st, int s, int i) { fb[s][i] = OpB::frag(st + OpA::kElems, wn + 16 * i, s); };
@@ -568,6 +576,7 @@ APEXW_DEV void stream(const ExpertArgs& g, Jobs& jobs, Place&& locate, const Out
         if (fresh) wait_copies<kCopies*(S::kStages - 2) + kStores>();
         else wait_copies<kCopies*(S::kStages - 2)>();
         fresh = false;
+        if (h == 0) known.arrived();   // waited for here, and not in the end behind the copies of then
         barrier();
         __builtin_amdgcn_sched_barrier(0);
       };
@@ -594,7 +603,7 @@ APEXW_DEV void stream(const ExpertArgs& g, Jobs& jobs, Place&& locate, const Out
       advance();
       buf = after;
     }
-    out.template write<S, kWM>(g, acc, lds, down, across, rows, cols, out0);
+    out.template write<S, kWM>(g, acc, known, lds, down, across, rows, cols, out0);
     fresh = kHigh == S::BM && rows >= S::BM && cols >= S::BN;
   };
 

@@ -5,8 +5,9 @@ up (the matrix cores may truncate): it is off by at most a = width 2^-23 of the 
 logit R below the largest rounds the difference and its product with log2 e and takes a constant of 25 bits, 3 R 2^-24,
 and 2^-22 for the instruction; fewer than 250 additions and products bring a row's sum together.  So
     lse is off by   b = a + (3 R + 250) 2^-24 + 2^-22 (|lse| + 20)      (logarithm and last additions)
-and the loss by 2 b.  With an lse that is given, a probability is off by the part e = a + (3 R + 8) 2^-24 + 2^-22 of
-itself, and G rounds by half a step of its type (in fp16 by 2^-25 of the largest |dloss| at least), so
+and the loss by 2 b.  With an lse that is given, a probability times dloss is formed as one power of 2, whose exponent's
+constant part is held in fp32 but for its lowest bit (2^-22 of it, with the roundings of its three terms), so it is off by
+the part e = a + (3 R + 8) 2^-24 + 2^-22 (1 + 1.5 |lse| + |log2 dloss| + 24) of itself, and G rounds by half a step of its type (in fp16 by 2^-25 of the largest |dloss| at least), so
     dx is off by    sum_v |W| (h |G| + e p |dloss| + t) + vocabulary 2^-23 sum_v |G W|
 before it rounds by half a step itself, and dW likewise over the rows.  Below 2^-126, the normal range of fp32 and
 bf16, the exponential's instruction and the matrix cores may give 0: t is 2^-126 times |dloss|'s largest or one at least,
@@ -57,7 +58,8 @@ class Exact:
     def check_backward(self, dloss, lse, dx, dw):
         d = torch.where(self.kept, dloss.reshape(-1).double(), 0)
         p = torch.exp(self.l - torch.where(self.kept, lse.reshape(-1).double(), self.lse)[:, None])
-        e = (self.a + (3 * self.R + 8) * 2.0 ** -24 + 2.0 ** -22)[:, None]
+        constant = 1.5 * self.lse.abs() + torch.where(d == 0, 1.0, d.abs()).log2().abs()
+        e = (self.a + (3 * self.R + 8) * 2.0 ** -24 + 2.0 ** -22 * (25 + constant))[:, None]
         err = e * p * d.abs()[:, None]
         p[torch.arange(len(p), device=p.device), self.at] -= 1
         G, half = p * d[:, None], HALF[self.w.dtype]
