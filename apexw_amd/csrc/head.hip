@@ -444,18 +444,73 @@ template <int DT> __global__ __launch_bounds__(256) void head_dx_kernel(HeadArgs
 
 int64_t whole(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
-// bytes of G that a piece may have
-constexpr int64_t kPiece = 256ll << 20;
+// The time of a product whose tiles the chip takes in rounds, in us: a stage's when every workgroup is at work and with
+// few (as for the experts' products), a tile's end, and the launch and bytes of parts that are joined.  kWhole: a last
+// round takes as long as the others; else its tiles are cut.
+struct Rate {
+  float most, least, end;
+  int slots, bm, bn;
+};
+template <class S> Rate rate(float most, float least, float end) {
+  return {most, least, end, apexw_cu_count() * S::kPerCU, S::BM, S::BN};
+}
+Rate rate_of(int shape) {
+  if (shape == 3) return rate<Large>(1.6f, 0.95f, 5.0f);
+  if (shape == 2) return rate<Wide>(0.95f, 0.65f, 4.0f);
+  if (shape == 1) return rate<Mid>(0.7f, 0.45f, 2.5f);
+  return rate<Small>(0.55f, 0.42f, 2.0f);
+}
+float time_of(int shape, int64_t down, int64_t across, int64_t depth, int splits, bool whole_rounds, float join_bytes) {
+  const Rate r = rate_of(shape);
+  const float tiles = (float)((down + r.bm - 1) / r.bm) * (float)((across + r.bn - 1) / r.bn);
+  const float rounds = tiles * (float)splits / (float)r.slots, full = floorf(rounds), rest = rounds - full;
+  const float stages = ceilf((float)((depth + kDepth - 1) / kDepth) / (float)splits);
+  const float join = splits > 1 ? 5.0f + (float)splits * join_bytes / 4e6f : 0.0f;
+  if (rounds <= 1.0f) return stages * (r.least + (r.most - r.least) * rounds) + r.end + join;
+  const float last = rest == 0.0f ? 0.0f : whole_rounds || splits > 1 || rest > 0.5f ? 1.0f : rest > 0.25f ? 0.6f : 0.4f;
+  return (full + last) * (stages * r.most + r.end) + join;
+}
+// the shape and parts of the least time; a part has to be worth a quarter more than it seems
+Cut best_cut(int least_shape, int64_t down, int64_t across, int64_t depth, bool may_split, bool whole_rounds, float join_bytes) {
+  Cut best{0, 0, 0.0f};
+  for (int shape = least_shape; shape < 4; ++shape)
+    for (int splits = 1; splits == 1 || (may_split && splits <= 64 && splits * 4 * kDepth <= depth); ++splits) {
+      if (splits > 4 && (splits & (splits - 1))) continue;
+      const float t = time_of(shape, down, across, depth, splits, whole_rounds, join_bytes), cost = splits > 1 ? 1.1f * t : t;
+      if (best.splits == 0 || cost < best.cost) best = {shape, splits, cost};
+    }
+  return best;
+}
+
+// Bytes of G that a piece may have.  (Between 128 MB and 4 GB the time changes by what the pieces' tiles leave of the
+// chip's rounds alone: 8192 x 4096 x 128256 19.9 to 20.6 ms.)
+constexpr int64_t kPiece = 1ll << 30;
+
+// The products of a piece of `cols` columns of the vocabulary
+struct Piece {
+  int64_t cols;
+  Cut logits, dw, dx;
+  float cost;
+  Piece() = default;
+  Piece(int64_t c, int64_t n, int64_t width, bool need_dx, bool need_dw) : cols(c) {
+    logits = best_cut(0, n, cols, width, false, false, 0.0f);
+    dw = best_cut(2, cols, width, n, true, true, 8.0f * (float)cols * (float)width);
+    dx = best_cut(0, n, width, cols, true, false, 12.0f * (float)n * (float)width);
+    // (adding to the pieces before reads and writes dx's sums)
+    cost = logits.cost + (need_dw ? dw.cost : 0.0f) + (need_dx ? dx.cost + 8.0f * (float)n * (float)width / 4e6f : 0.0f);
+  }
+};
 
 struct HeadPlan {
   int64_t n, width, wide, vocab, w_stride;
   bool copy_w;
   int64_t at_rows, at_shift, at_x, at_w, at_parts, at_g, at_sums, at_dw, bytes;
-  int64_t parts_ld, piece, piece_ld;
-  ExpertArgs logits, rows, weight;   // sizes of a whole piece's products
-  Cut cut_logits, cut_dx, cut_dw;
+  int64_t parts_ld, piece_ld;
+  Cut cut;                 // forward
+  Piece piece, last;       // backward
+  int dx_splits;
   HeadPlan(const void* w, int64_t stride, int64_t n_, int64_t width_, int64_t vocab_, bool backward, bool need_dx, bool need_dw)
-      : n(n_), width(width_), wide((width_ + 7) / 8 * 8), vocab(vocab_), w_stride(stride), logits{}, rows{}, weight{} {
+      : n(n_), width(width_), wide((width_ + 7) / 8 * 8), vocab(vocab_), w_stride(stride) {
     copy_w = !k_rows_ok(w, stride, width);
     if (copy_w) w_stride = wide;
     at_rows = 256;
@@ -463,37 +518,73 @@ struct HeadPlan {
     at_x = at_shift + whole(n * 4);
     at_w = at_x + whole(n * wide * 2);
     int64_t at = at_w + (copy_w ? whole(vocab * wide * 2) : 0);
-    piece = vocab;
-    if (backward) {
-      piece = kPiece / (2 * (n > 0 ? n : 1)) / 256 * 256;
-      piece = piece < 1024 ? 1024 : piece;
-      piece = piece > vocab ? vocab : piece;
-    }
-    logits.rows = n, logits.experts = 1, logits.splits = 1, logits.part = INT32_MAX, logits.n = (int32_t)piece;
-    logits.k = (int32_t)width, logits.wide = (int32_t)wide, logits.lda = wide, logits.ldb = w_stride;
-    cut_logits = cut_rows(logits, false);
     if (!backward) {
+      cut = best_cut(0, n, vocab, width, false, false, 0.0f);
       parts_ld = (n + 15) / 16 * 16;
       at_parts = at, at += whole(parts_ld * parts() * 4);
       bytes = at;
       return;
     }
-    piece_ld = (piece + 7) / 8 * 8;
+    cut_pieces(need_dx, need_dw);
+    piece_ld = (piece.cols + 7) / 8 * 8;
     at_g = at, at += whole(n * piece_ld * 2);
-    rows = logits, rows.n = (int32_t)width, rows.k = (int32_t)piece, rows.wide = (int32_t)piece_ld, rows.lda = piece_ld;
-    rows.ldo = width, rows.split_stride = n * width;
-    cut_dx = cut_rows(rows, true);
-    cut_up(rows, cut_dx.splits, kDepth);
-    at_sums = at, at += need_dx ? whole(rows.splits * n * width * 4) : 0;
-    weight = logits, weight.n = (int32_t)piece, weight.k = (int32_t)width, weight.lda = piece_ld, weight.ldb = wide;
-    weight.ldo = width, weight.split_stride = piece * width;
-    cut_dw = cut_weight(weight, true);
-    weight.splits = cut_dw.splits;
-    at_dw = at, at += need_dw && weight.splits > 1 ? whole(weight.splits * piece * width * 4) : 0;
+    dx_splits = dx(piece).splits;
+    at_sums = at, at += need_dx ? whole(dx_splits * n * width * 4) : 0;
+    int64_t parts = 0;
+    if (need_dw)
+      for (const Piece* q : {&piece, &last})
+        if (q->dw.splits > 1 && q->dw.splits * q->cols > parts) parts = q->dw.splits * q->cols;
+    at_dw = at, at += whole(parts * width * 4);
     bytes = at;
   }
+  // Pieces of as many columns as G's bytes allow, or fewer, so that the tiles of their weights' gradient fill whole
+  // rounds of the chip; the last piece has what is left
+  void cut_pieces(bool need_dx, bool need_dw) {
+    int64_t most = kPiece / (2 * (n > 0 ? n : 1)) / 256 * 256;
+    most = most < 1024 ? 1024 : most;
+    if (most >= vocab) {
+      piece = last = Piece(vocab, n, width, need_dx, need_dw);
+      return;
+    }
+    const int64_t across = (width + 255) / 256;
+    float least = 0.0f;
+    for (int i = 0; i < 5; ++i) {
+      const int64_t cols = i == 0 ? most : apexw_cu_count() * i / across * 256;
+      if (cols <= 0 || cols > most || 4 * cols < most) continue;
+      const Piece p(cols, n, width, need_dx, need_dw);
+      const int64_t count = (vocab - 1) / cols;
+      Piece q(vocab - count * cols, n, width, need_dx, need_dw);
+      const float cost = (float)count * p.cost + q.cost;
+      if (least == 0.0f || cost < least) least = cost, piece = p, last = q;
+    }
+    last.dx = piece.dx;   // (the first piece writes every part's sums)
+  }
+  const Piece& at_column(int64_t v) const { return v + piece.cols <= vocab ? piece : last; }
+
+  ExpertArgs args(int64_t columns) const {
+    ExpertArgs g{};
+    g.rows = n, g.experts = 1, g.splits = 1, g.part = INT32_MAX, g.n = (int32_t)columns, g.k = (int32_t)width;
+    g.wide = (int32_t)wide, g.lda = wide, g.ldb = w_stride;
+    return g;
+  }
+  ExpertArgs logits(const Piece& q) const {
+    ExpertArgs g = args(q.cols);
+    g.ldo = piece_ld;
+    return g;
+  }
+  ExpertArgs dw(const Piece& q) const {
+    ExpertArgs g = args(q.cols);
+    g.lda = piece_ld, g.ldb = wide, g.ldo = width, g.split_stride = q.cols * width, g.splits = q.dw.splits;
+    return g;
+  }
+  ExpertArgs dx(const Piece& q) const {
+    ExpertArgs g = args(width);
+    g.k = (int32_t)q.cols, g.wide = (int32_t)((q.cols + 7) / 8 * 8), g.lda = piece_ld, g.ldo = width, g.split_stride = n * width;
+    cut_up(g, q.dx.splits, kDepth);
+    return g;
+  }
   int64_t parts() const {   // waves across the vocabulary
-    const int64_t wave = cut_logits.shape == 0 ? Small::WN : Large::WN;
+    const int64_t wave = cut.shape == 0 ? Small::WN : Large::WN;
     return (vocab + wave - 1) / wave;
   }
 };
@@ -502,7 +593,7 @@ static_assert(Large::WN == 64 && Wide::WN == 64 && Mid::WN == 64, "columns of a 
 bool head_ok(int64_t n, int64_t width, int64_t vocab) {
   return n >= 0 && n <= INT32_MAX - 65536 && width > 0 && width <= kMostLd && vocab > 0 && vocab <= INT32_MAX - 65536;
 }
-bool head_fits(const HeadPlan& p) { return rows_tiles<Small>(p.logits) <= INT32_MAX; }
+bool head_fits(const HeadPlan& p) { return rows_tiles<Small>(p.args(p.vocab)) <= INT32_MAX; }
 
 template <class S, int DT, class Out> void launch_logits_shape(const ExpertArgs& g, const Out& out, hipStream_t s) {
   hipLaunchKernelGGL((head_logits_kernel<S, DT, Out>), dim3(stream_grid<S>(rows_tiles<S>(g))), dim3(S::kThreads), 0, s, g, out);
@@ -606,9 +697,9 @@ extern "C" int apexw_linear_cross_entropy_forward(const void* x, int64_t x_strid
     const uint16_t* w = launch_pack<DT>(p, pack, weight, w_stride, ws, s);
     if (n == 0) return;
     const HeadArgs h{pack.state, pack.rows, pack.shift, (float*)(ws + p.at_parts), p.parts_ld};
-    ExpertArgs g = p.logits;
+    ExpertArgs g = p.args(vocab);
     g.a = pack.packed, g.b = w, g.ends = &pack.state->count;
-    launch_logits<DT>(g, p.cut_logits.shape, Sums{h}, s);
+    launch_logits<DT>(g, p.cut.shape, Sums{h}, s);
     hipLaunchKernelGGL(head_join_kernel, dim3((unsigned)((n + 15) / 16)), dim3(1024), 0, s, h, (int)p.parts(), loss, lse);
   });
   if (reduction) hipLaunchKernelGGL(head_total_kernel, dim3(1), dim3(1024), 0, s, pack.state, loss, n, (int)(reduction == 2), total);
@@ -640,32 +731,32 @@ extern "C" int apexw_linear_cross_entropy_backward(const float* dloss, int64_t d
     constexpr int DT = decltype(d)::value;
     const uint16_t* w = launch_pack<DT>(p, pack, weight, w_stride, ws, s);
     const HeadArgs h{pack.state, pack.rows, pack.shift, nullptr, 0};
-    for (int64_t v = 0; v < vocab; v += p.piece) {
-      const int32_t cols = (int32_t)(vocab - v < p.piece ? vocab - v : p.piece);
+    uint16_t* G = (uint16_t*)(ws + p.at_g);
+    for (int64_t v = 0; v < vocab; v += p.piece.cols) {
+      const Piece& q = p.at_column(v);
       const uint16_t* wp = w + v * p.w_stride;
-      uint16_t* G = (uint16_t*)(ws + p.at_g);
       if (n > 0) {
-        ExpertArgs g = p.logits;
-        g.a = pack.packed, g.b = wp, g.ends = &pack.state->count, g.n = cols, g.out = G, g.ldo = p.piece_ld;
-        launch_logits<DT>(g, p.cut_logits.shape, Prob<DT>{h}, s);
-        hipLaunchKernelGGL(head_targets_kernel<DT>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, h, (int)v, cols, G, p.piece_ld);
+        ExpertArgs g = p.logits(q);
+        g.a = pack.packed, g.b = wp, g.ends = &pack.state->count, g.out = G;
+        launch_logits<DT>(g, q.logits.shape, Prob<DT>{h}, s);
+        hipLaunchKernelGGL(head_targets_kernel<DT>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, h, (int)v, (int)q.cols, G,
+                           p.piece_ld);
       }
       if (dw) {
-        ExpertArgs g = p.weight;
-        g.a = G, g.b = pack.packed, g.ends = &pack.state->count, g.n = cols, g.out = (uint16_t*)dw + v * width;
-        launch_dw<DT>(g, p.cut_dw.shape, pack.state, (float*)(ws + p.at_dw), s);
+        ExpertArgs g = p.dw(q);
+        g.a = G, g.b = pack.packed, g.ends = &pack.state->count, g.out = (uint16_t*)dw + v * width;
+        launch_dw<DT>(g, q.dw.shape, pack.state, (float*)(ws + p.at_dw), s);
       }
       if (dx && n > 0) {
-        ExpertArgs g = p.rows;
-        g.a = G, g.b = wp, g.ends = &pack.state->count, g.k = cols, g.wide = (cols + 7) / 8 * 8, g.out = ws + p.at_sums;
-        if (g.splits > 1) g.splits = (g.wide + g.part - 1) / g.part;
-        launch_dx<DT>(g, p.cut_dx.shape, v > 0, s);
+        ExpertArgs g = p.dx(q);
+        g.a = G, g.b = wp, g.ends = &pack.state->count, g.out = ws + p.at_sums;
+        launch_dx<DT>(g, q.dx.shape, v > 0, s);
       }
     }
     if (dx && n > 0) {
       const int64_t grid = (n * ((width + 3) / 4) + 255) / 256;
       hipLaunchKernelGGL(head_dx_kernel<DT>, dim3((unsigned)(grid < 8192 ? grid : 8192)), dim3(256), 0, s, h,
-                         (const float*)(ws + p.at_sums), n * width, (int)p.rows.splits, (int)width, (uint16_t*)dx);
+                         (const float*)(ws + p.at_sums), n * width, p.dx_splits, (int)width, (uint16_t*)dx);
     }
   });
   return hipGetLastError() == hipSuccess ? APEXW_OK : APEXW_ERR_LAUNCH;
