@@ -16,6 +16,7 @@
 #include <Python.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <cstring>
 #include <vector>
@@ -127,7 +128,7 @@ PyObject* scan(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 }
 
 // ---------------------------------------------------------------------------
-// The operators around the step (apexw_amd/ops.py): the usual call checked, its outputs allocated and the
+// The operators around the step (apexw_amd/ops.py, tokens.py, head.py): the usual call checked, its outputs allocated and the
 // library called in one go, which takes a third of the time that the same takes from Python.  Each function
 // returns None for what it does not take (another layout, device or type); the Python form then copies,
 // converts or raises.  A nonzero apexw_status comes back as an int.
@@ -157,6 +158,21 @@ struct Library {
   int64_t (*clip_layout)(ClipTensor*, int32_t);
   int (*clip_grads)(const ClipTensor*, int32_t, int64_t, int32_t, float, double*, float*, void*);
   int (*clip_grads_small)(const ClipTensor*, int32_t, int64_t, int32_t, float, double*, float*, void*);
+  int64_t (*order_workspace)(int64_t, int32_t);
+  int (*order)(const void*, int32_t, int64_t, int32_t, int32_t*, int32_t*, int32_t*, void*, void*);
+  int (*dispatch)(const void*, int64_t, int64_t, int32_t, int64_t, int32_t, const int32_t*, const int32_t*, void*, void*);
+  int (*combine)(const void*, int64_t, int64_t, int32_t, int64_t, int32_t, const int32_t*, const void*, int32_t, void*, void*);
+  int (*combine_backward)(const void*, int64_t, const void*, int64_t, int64_t, int32_t, int64_t, int32_t, const int32_t*,
+                          const int32_t*, const void*, int32_t, void*, void*, void*);
+  int (*embedding)(const void*, int32_t, int64_t, const void*, int64_t, int64_t, int64_t, int32_t, float, void*, void*);
+  int64_t (*embedding_grad_workspace)(int64_t, int64_t, int64_t);
+  int (*embedding_grad)(const void*, int64_t, const void*, int32_t, int64_t, int64_t, int64_t, int32_t, float, void*,
+                        int32_t, void*, void*);
+  int64_t (*head_workspace)(const void*, int64_t, int64_t, int64_t, int64_t, int32_t);
+  int (*head_forward)(const void*, int64_t, int64_t, int64_t, const void*, int64_t, int64_t, int32_t, const void*, int32_t,
+                      int64_t, float*, float*, int32_t, float*, void*, void*);
+  int (*head_backward)(const float*, int64_t, int32_t, const void*, int64_t, int64_t, int64_t, const void*, int64_t,
+                       int64_t, int32_t, const void*, int32_t, int64_t, const float*, void*, void*, void*, void*);
 } lib;
 constexpr int kEntries = sizeof(Library) / sizeof(void*);
 
@@ -561,6 +577,255 @@ PyObject* clip_grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// rows of any of the three types, whole in their last dimension
+bool matrix(const at::Tensor& t, const Where& w, uint32_t* code) {
+  return w.has(t) && dtype_code(t, code) && t.dim() == 2 && t.size(1) > 0 && t.stride(1) == 1;
+}
+// contiguous ids of 4 or 8 bytes
+bool ids_of(const at::Tensor& t, const Where& w, int32_t* bytes) {
+  if (!w.has(t) || !t.is_contiguous()) return false;
+  *bytes = t.scalar_type() == at::kLong ? 8 : t.scalar_type() == at::kInt ? 4 : 0;
+  return *bytes != 0;
+}
+// an order's source and place: the number of tokens and of choices of each
+bool order_of(const at::Tensor& source, const at::Tensor& place, const Where& w, int64_t* tokens, int32_t* k) {
+  if (!expert_ends(source, w) || !w.has(place) || place.scalar_type() != at::kInt || !place.is_contiguous() ||
+      (place.dim() != 1 && place.dim() != 2) || place.numel() != source.size(0))
+    return false;
+  *tokens = place.size(0);
+  *k = place.dim() == 2 ? static_cast<int32_t>(place.size(1)) : 1;
+  return true;
+}
+// a weight for each choice
+bool order_weight(const at::Tensor& t, const at::Tensor& place, const Where& w, uint32_t code, uint32_t* w_code) {
+  return w.has(t) && dtype_code(t, w_code) && (*w_code == code || *w_code == 0) && t.sizes() == place.sizes() && t.is_contiguous();
+}
+const int32_t* ints(const at::Tensor& t) { return static_cast<const int32_t*>(t.data_ptr()); }
+void* space(int64_t bytes, const at::Tensor& like, at::Tensor* ws) {
+  if (bytes > 0) *ws = at::empty({bytes}, like.options().dtype(at::kByte));
+  return const_cast<void*>(address(*ws));
+}
+bool all_tensors(PyObject* const* args, int n) {
+  for (int i = 0; i < n; ++i)
+    if (!THPVariable_Check(args[i])) return false;
+  return true;
+}
+
+// expert_order(expert, experts, stream, device) -> (source, place, ends)
+PyObject* expert_order(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Where where;
+  if (nargs != 4 || !THPVariable_Check(args[0]) || !PyLong_Check(args[1]) || !where.set(args[2], args[3])) return none_or_error();
+  const at::Tensor& expert = THPVariable_Unpack(args[0]);
+  const long experts = PyLong_AsLong(args[1]);
+  int32_t bytes;
+  if (PyErr_Occurred()) return nullptr;
+  if (!ids_of(expert, where, &bytes) || expert.numel() == 0 || expert.dim() < 1 || expert.dim() > 2 || experts < 1 ||
+      experts >= INT32_MAX)
+    return none_or_error();
+  const int64_t n = expert.numel(), need = lib.order_workspace(n, static_cast<int32_t>(experts));
+  if (need < 0) return PyLong_FromLong(static_cast<long>(-need));
+  const auto options = expert.options().dtype(at::kInt);
+  const at::Tensor source = at::empty({n}, options), place = at::empty(expert.sizes(), options), ends = at::empty({experts}, options);
+  at::Tensor ws;
+  const int status = lib.order(expert.data_ptr(), bytes, n, static_cast<int32_t>(experts), static_cast<int32_t*>(source.data_ptr()),
+                               static_cast<int32_t*>(place.data_ptr()), static_cast<int32_t*>(ends.data_ptr()),
+                               space(need, expert, &ws), where.stream);
+  if (status) return PyLong_FromLong(status);
+  const at::Tensor* out[] = {&source, &place, &ends};
+  return pack(out, 3);
+  END_HANDLE_TH_ERRORS
+}
+
+// expert_dispatch(x, source, place, stream, device) -> rows
+PyObject* expert_dispatch(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Where where;
+  if (nargs != 5 || !all_tensors(args, 3) || !where.set(args[3], args[4])) return none_or_error();
+  const at::Tensor &x = THPVariable_Unpack(args[0]), &source = THPVariable_Unpack(args[1]), &place = THPVariable_Unpack(args[2]);
+  uint32_t code;
+  int64_t tokens;
+  int32_t k;
+  if (!matrix(x, where, &code) || !order_of(source, place, where, &tokens, &k) || x.size(0) != tokens) return none_or_error();
+  const at::Tensor rows = at::empty({tokens * k, x.size(1)}, x.options());
+  const int status = lib.dispatch(x.data_ptr(), x.stride(0), tokens, k, x.size(1), code, ints(source), ints(place), rows.data_ptr(),
+                                  where.stream);
+  return status ? PyLong_FromLong(status) : THPVariable_Wrap(rows);
+  END_HANDLE_TH_ERRORS
+}
+
+// expert_combine(y, source, place, weight, stream, device) -> out
+PyObject* expert_combine(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Where where;
+  at::Tensor w;
+  if (nargs != 6 || !all_tensors(args, 3) || !optional_tensor(args[3], &w) || !where.set(args[4], args[5])) return none_or_error();
+  const at::Tensor &y = THPVariable_Unpack(args[0]), &source = THPVariable_Unpack(args[1]), &place = THPVariable_Unpack(args[2]);
+  uint32_t code, w_code;
+  int64_t tokens;
+  int32_t k;
+  if (!matrix(y, where, &code) || !order_of(source, place, where, &tokens, &k) || y.size(0) != source.size(0)) return none_or_error();
+  w_code = code;
+  if (w.defined() && !order_weight(w, place, where, code, &w_code)) return none_or_error();
+  const at::Tensor out = at::empty({tokens, y.size(1)}, y.options());
+  const int status = lib.combine(y.data_ptr(), y.stride(0), tokens, k, y.size(1), code, ints(place), address(w), w_code, out.data_ptr(),
+                                 where.stream);
+  return status ? PyLong_FromLong(status) : THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// expert_combine_backward(dout, y, source, place, weight, need_y, need_w, stream, device) -> (dy, dweight)
+PyObject* expert_combine_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Where where;
+  at::Tensor y;
+  if (nargs != 9 || !THPVariable_Check(args[0]) || !optional_tensor(args[1], &y) || !all_tensors(args + 2, 3) ||
+      !where.set(args[7], args[8]))
+    return none_or_error();
+  const at::Tensor &dout = THPVariable_Unpack(args[0]), &source = THPVariable_Unpack(args[2]), &place = THPVariable_Unpack(args[3]),
+                   &w = THPVariable_Unpack(args[4]);
+  const int need_y = PyObject_IsTrue(args[5]), need_w = PyObject_IsTrue(args[6]);
+  if (need_y < 0 || need_w < 0) return nullptr;
+  uint32_t code, y_code, w_code;
+  int64_t tokens;
+  int32_t k;
+  if (!matrix(dout, where, &code) || !order_of(source, place, where, &tokens, &k) || dout.size(0) != tokens ||
+      !order_weight(w, place, where, code, &w_code))
+    return none_or_error();
+  if (need_w && (!y.defined() || !matrix(y, where, &y_code) || y_code != code || y.size(0) != source.size(0) || y.size(1) != dout.size(1)))
+    return none_or_error();
+  at::Tensor dy, dw;
+  if (need_y) dy = at::empty({tokens * k, dout.size(1)}, dout.options());
+  if (need_w) dw = at::empty(w.sizes(), w.options());
+  const int status = lib.combine_backward(dout.data_ptr(), dout.stride(0), need_w ? y.data_ptr() : nullptr, need_w ? y.stride(0) : 0,
+                                          tokens, k, dout.size(1), code, ints(source), ints(place), w.data_ptr(), w_code,
+                                          const_cast<void*>(address(dy)), const_cast<void*>(address(dw)), where.stream);
+  if (status) return PyLong_FromLong(status);
+  const at::Tensor* out[] = {&dy, &dw};
+  return pack(out, 2);
+  END_HANDLE_TH_ERRORS
+}
+
+// embedding_forward(ids, weight, scale, stream, device) -> out
+PyObject* embedding_forward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Where where;
+  if (nargs != 5 || !all_tensors(args, 2) || !where.set(args[3], args[4])) return none_or_error();
+  const at::Tensor &ids = THPVariable_Unpack(args[0]), &w = THPVariable_Unpack(args[1]);
+  const double scale = PyFloat_AsDouble(args[2]);
+  if (PyErr_Occurred()) return nullptr;
+  uint32_t code;
+  int32_t bytes;
+  if (!ids_of(ids, where, &bytes) || !matrix(w, where, &code) || w.size(0) == 0 || !std::isfinite(scale)) return none_or_error();
+  std::vector<int64_t> shape(ids.sizes().begin(), ids.sizes().end());
+  shape.push_back(w.size(1));
+  const at::Tensor out = at::empty(shape, w.options());
+  const int status = lib.embedding(ids.data_ptr(), bytes, ids.numel(), w.data_ptr(), w.stride(0), w.size(0), w.size(1), code,
+                                   static_cast<float>(scale), out.data_ptr(), where.stream);
+  return status ? PyLong_FromLong(status) : THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// embedding_weight_grad(dy, ids, vocab, scale, fp32, stream, device) -> dW
+PyObject* embedding_weight_grad(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Where where;
+  if (nargs != 7 || !all_tensors(args, 2) || !PyLong_Check(args[2]) || !where.set(args[5], args[6])) return none_or_error();
+  const at::Tensor &dy = THPVariable_Unpack(args[0]), &ids = THPVariable_Unpack(args[1]);
+  const long vocab = PyLong_AsLong(args[2]);
+  const double scale = PyFloat_AsDouble(args[3]);
+  const bool fp32 = args[4] == Py_True;
+  if (PyErr_Occurred()) return nullptr;
+  uint32_t code;
+  int32_t bytes;
+  if (!ids_of(ids, where, &bytes) || !where.has(dy) || !dtype_code(dy, &code) || dy.dim() != ids.dim() + 1 || !dy.is_contiguous() ||
+      dy.numel() == 0 || dy.sizes().slice(0, ids.dim()) != ids.sizes() || vocab < 1 || vocab >= INT32_MAX || !std::isfinite(scale))
+    return none_or_error();
+  const int64_t n = ids.numel(), width = dy.size(-1), need = lib.embedding_grad_workspace(n, vocab, width);
+  if (need < 0) return PyLong_FromLong(static_cast<long>(-need));
+  const at::Tensor dw = at::empty({vocab, width}, fp32 ? dy.options().dtype(at::kFloat) : dy.options());
+  at::Tensor ws;
+  const int status = lib.embedding_grad(dy.data_ptr(), width, ids.data_ptr(), bytes, n, vocab, width, code, static_cast<float>(scale),
+                                        dw.data_ptr(), fp32 ? 0 : code, space(need, dy, &ws), where.stream);
+  return status ? PyLong_FromLong(status) : THPVariable_Wrap(dw);
+  END_HANDLE_TH_ERRORS
+}
+
+// rows, weights and targets of a linear head
+struct Head {
+  int64_t n, width, vocab;
+  uint32_t code;
+  int32_t bytes;
+  bool set(const at::Tensor& x, const at::Tensor& w, const at::Tensor& target, const Where& where) {
+    if (!where.has(x) || !dtype_code(x, &code) || code == 0 || x.dim() < 1 || x.numel() == 0 || !x.is_contiguous() ||
+        !where.has(w) || w.scalar_type() != x.scalar_type() || w.dim() != 2 || w.size(0) == 0 || w.stride(1) != 1 ||
+        w.size(1) != x.size(-1) || !ids_of(target, where, &bytes) || target.sizes() != x.sizes().slice(0, x.dim() - 1))
+      return false;
+    width = x.size(-1), n = x.numel() / width, vocab = w.size(0);
+    return true;
+  }
+};
+
+// head_forward(x, weight, target, ignore_index, reduction, stream, device) -> (loss, lse, total)
+PyObject* head_forward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Where where;
+  if (nargs != 7 || !all_tensors(args, 3) || !where.set(args[5], args[6])) return none_or_error();
+  const at::Tensor &x = THPVariable_Unpack(args[0]), &w = THPVariable_Unpack(args[1]), &target = THPVariable_Unpack(args[2]);
+  const long long ignore = PyLong_AsLongLong(args[3]);
+  const long reduction = PyLong_AsLong(args[4]);
+  if (PyErr_Occurred()) return nullptr;
+  Head h;
+  if (!h.set(x, w, target, where)) return none_or_error();
+  const int64_t need = lib.head_workspace(w.data_ptr(), w.stride(0), h.n, h.width, h.vocab, 0);
+  if (need < 0) return PyLong_FromLong(static_cast<long>(-need));
+  const auto options = x.options().dtype(at::kFloat);
+  const at::Tensor loss = at::empty(target.sizes(), options), lse = at::empty(target.sizes(), options);
+  at::Tensor total, ws;
+  if (reduction) total = at::empty({}, options);
+  const int status = lib.head_forward(x.data_ptr(), h.width, h.n, h.width, w.data_ptr(), w.stride(0), h.vocab, h.code,
+                                      target.data_ptr(), h.bytes, ignore, static_cast<float*>(loss.data_ptr()),
+                                      static_cast<float*>(lse.data_ptr()), static_cast<int32_t>(reduction),
+                                      static_cast<float*>(const_cast<void*>(address(total))), space(need, x, &ws), where.stream);
+  if (status) return PyLong_FromLong(status);
+  const at::Tensor* out[] = {&loss, &lse, &total};
+  return pack(out, 3);
+  END_HANDLE_TH_ERRORS
+}
+
+// head_backward(dloss, stride, mean, x, weight, target, lse, ignore_index, need_x, need_w, stream, device) -> (dx, dw)
+PyObject* head_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Where where;
+  if (nargs != 12 || !THPVariable_Check(args[0]) || !all_tensors(args + 3, 4) || !where.set(args[10], args[11]))
+    return none_or_error();
+  const at::Tensor &dloss = THPVariable_Unpack(args[0]), &x = THPVariable_Unpack(args[3]), &w = THPVariable_Unpack(args[4]),
+                   &target = THPVariable_Unpack(args[5]), &lse = THPVariable_Unpack(args[6]);
+  const long stride = PyLong_AsLong(args[1]), mean = PyLong_AsLong(args[2]);
+  const long long ignore = PyLong_AsLongLong(args[7]);
+  if (PyErr_Occurred()) return nullptr;
+  const int need_x = PyObject_IsTrue(args[8]), need_w = PyObject_IsTrue(args[9]);
+  if (need_x < 0 || need_w < 0) return nullptr;
+  Head h;
+  if ((!need_x && !need_w) || !h.set(x, w, target, where) || !where.has(dloss) || dloss.scalar_type() != at::kFloat ||
+      (stride ? dloss.numel() != h.n || !dloss.is_contiguous() : dloss.numel() < 1) || !where.has(lse) ||
+      lse.scalar_type() != at::kFloat || lse.numel() != h.n || !lse.is_contiguous())
+    return none_or_error();
+  const int64_t need = lib.head_workspace(w.data_ptr(), w.stride(0), h.n, h.width, h.vocab, (need_x ? 1 : 0) | (need_w ? 2 : 0));
+  if (need < 0) return PyLong_FromLong(static_cast<long>(-need));
+  at::Tensor dx, dw, ws;
+  if (need_x) dx = at::empty(x.sizes(), x.options());
+  if (need_w) dw = at::empty({h.vocab, h.width}, w.options());
+  const int status = lib.head_backward(static_cast<const float*>(dloss.data_ptr()), stride, static_cast<int32_t>(mean), x.data_ptr(),
+                                       h.width, h.n, h.width, w.data_ptr(), w.stride(0), h.vocab, h.code, target.data_ptr(),
+                                       h.bytes, ignore, static_cast<const float*>(lse.data_ptr()), const_cast<void*>(address(dx)),
+                                       const_cast<void*>(address(dw)), space(need, x, &ws), where.stream);
+  if (status) return PyLong_FromLong(status);
+  const at::Tensor* out[] = {&dx, &dw};
+  return pack(out, 2);
+  END_HANDLE_TH_ERRORS
+}
+
 template <class F> PyCFunction fast(F* f) { return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)); }
 
 PyMethodDef kMethods[] = {
@@ -570,6 +835,14 @@ PyMethodDef kMethods[] = {
     {"expert_rows", fast(expert_rows), METH_FASTCALL, "The usual call, or None."},
     {"expert_weight_grad", fast(expert_weight_grad), METH_FASTCALL, "The usual call, or None."},
     {"clip_grads", fast(clip_grads), METH_FASTCALL, "The usual call, or None."},
+    {"expert_order", fast(expert_order), METH_FASTCALL, "The usual call, or None."},
+    {"expert_dispatch", fast(expert_dispatch), METH_FASTCALL, "The usual call, or None."},
+    {"expert_combine", fast(expert_combine), METH_FASTCALL, "The usual call, or None."},
+    {"expert_combine_backward", fast(expert_combine_backward), METH_FASTCALL, "The usual call, or None."},
+    {"embedding_forward", fast(embedding_forward), METH_FASTCALL, "The usual call, or None."},
+    {"embedding_weight_grad", fast(embedding_weight_grad), METH_FASTCALL, "The usual call, or None."},
+    {"head_forward", fast(head_forward), METH_FASTCALL, "The usual call, or None."},
+    {"head_backward", fast(head_backward), METH_FASTCALL, "The usual call, or None."},
     {"clip_table", fast(clip_table), METH_FASTCALL,
      "Fill the table of a clip by the global norm from lists of tensors."},
     {"snapshot", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(snapshot)), METH_FASTCALL,

@@ -10,7 +10,7 @@ host, and equal calls give equal bits.  What is not supported raises before anyt
 import torch
 
 from . import _lib
-from .ops import _CODE, _Launch, _on_device, _ptr, _rows
+from .ops import _CODE, _current, _done, _Launch, _native, _on_device, _ptr, _raw_stream, _rows
 from .tokens import _ID_BYTES, _space
 
 _REDUCTION = {"none": 0, "sum": 1, "mean": 2}
@@ -37,6 +37,12 @@ def _check(x, weight, target):
 
 
 def _forward(x, weight, target, ignore_index, reduction):
+    native = _native(x)
+    if native is not None:
+        dev = _current()
+        out = native.head_forward(x, weight, target, ignore_index, reduction, _raw_stream(dev), dev)
+        if out is not None:
+            return _done(out, "apexw_linear_cross_entropy_forward")
     src, n, stride, weight, target = _check(x, weight, target)
     (vocab, width), lib = weight.shape, _lib.load()
     with _Launch(x.device) as stream:
@@ -53,6 +59,13 @@ def _forward(x, weight, target, ignore_index, reduction):
 
 
 def _backward(dloss, stride_d, mean, x, weight, target, lse, ignore_index, need):
+    native = _native(x)
+    if native is not None:
+        dev = _current()
+        out = native.head_backward(dloss, stride_d, mean, x, weight, target, lse, ignore_index, need[0], need[1],
+                                   _raw_stream(dev), dev)
+        if out is not None:
+            return _done(out, "apexw_linear_cross_entropy_backward")
     src, n, stride, weight, target = _check(x, weight, target)
     (vocab, width), lib = weight.shape, _lib.load()
     if not need[0] and not need[1]:

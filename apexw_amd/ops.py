@@ -23,7 +23,11 @@ _current = getattr(torch._C, "_cuda_getDevice", None)
 _NATIVE = None
 _ENTRIES = ("apexw_layer_norm_forward", "apexw_layer_norm_backward", "apexw_layer_norm_workspace", "apexw_expert_rows",
             "apexw_expert_rows_workspace", "apexw_expert_weight_grad", "apexw_expert_weight_grad_workspace",
-            "apexw_clip_layout", "apexw_clip_grads", "apexw_clip_grads_small")
+            "apexw_clip_layout", "apexw_clip_grads", "apexw_clip_grads_small", "apexw_expert_order_workspace",
+            "apexw_expert_order", "apexw_expert_dispatch", "apexw_expert_combine", "apexw_expert_combine_backward",
+            "apexw_embedding_forward", "apexw_embedding_weight_grad_workspace", "apexw_embedding_weight_grad",
+            "apexw_linear_cross_entropy_workspace", "apexw_linear_cross_entropy_forward",
+            "apexw_linear_cross_entropy_backward")
 
 
 def _native(t):

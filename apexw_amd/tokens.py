@@ -15,7 +15,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .ops import _CODE, _Launch, _on_device, _ptr, _rows
+from .ops import _CODE, _current, _done, _Launch, _native, _on_device, _ptr, _raw_stream, _rows
 
 _ID_BYTES = {torch.int32: 4, torch.int64: 8}
 
@@ -88,6 +88,12 @@ def expert_order(expert, experts):
     expert: the experts that each token chose, (tokens,) or (tokens, choices), int32 or int64.  An id outside
     [0, experts) belongs to no expert: such choices (padding, or what exceeds an expert's capacity) get no row.
     Rows of one expert keep the order of their choices.  ``order.ends`` is what ``expert_matmul`` takes."""
+    native = _native(expert)
+    if native is not None:
+        dev = _current()
+        out = native.expert_order(expert, experts, _raw_stream(dev), dev)
+        if out is not None:
+            return ExpertOrder._make(_done(out, "apexw_expert_order"))
     expert = _check_ids(expert, "expert_order: expert")
     if expert.dim() not in (1, 2) or 0 in expert.shape[1:]:
         raise ValueError(f"expert_order: expected (tokens,) or (tokens, choices), got {tuple(expert.shape)}")
@@ -108,6 +114,12 @@ def expert_dispatch_forward(x, order):
     """rows[r] = x[t] for the token t whose choice row r belongs to; zeros in rows that belong to none.
 
     x: (tokens, width) of float32, bfloat16 or float16; the result has a row for each choice."""
+    native = _native(x)
+    if native is not None:
+        dev = _current()
+        out = native.expert_dispatch(x, order[0], order[1], _raw_stream(dev), dev)
+        if out is not None:
+            return _done(out, "apexw_expert_dispatch")
     x, stride = _check_matrix(x, "expert_dispatch: x")
     tokens, k = _check_order(order, "expert_dispatch", x.device)
     if x.shape[0] != tokens:
@@ -125,6 +137,12 @@ def expert_combine_forward(y, order, weight=None):
 
     y: a row for each choice; weight: (tokens,) or (tokens, choices) as the order's, of y's type or float32, None
     for ones."""
+    native = _native(y)
+    if native is not None:
+        dev = _current()
+        out = native.expert_combine(y, order[0], order[1], weight, _raw_stream(dev), dev)
+        if out is not None:
+            return _done(out, "apexw_expert_combine")
     y, stride = _check_matrix(y, "expert_combine: y")
     tokens, k = _check_order(order, "expert_combine", y.device)
     if y.shape[0] != tokens * k:
@@ -150,6 +168,12 @@ def expert_combine_backward(dout, y, order, weight=None, need=(True, True)):
     ``need`` leaves out gradients nobody wants (None); y may be None where dweight is not wanted."""
     if weight is None:
         return expert_dispatch_forward(dout, order) if need[0] else None, None
+    native = _native(dout)
+    if native is not None:
+        dev = _current()
+        out = native.expert_combine_backward(dout, y, order[0], order[1], weight, need[0], need[1], _raw_stream(dev), dev)
+        if out is not None:
+            return _done(out, "apexw_expert_combine_backward")
     dout, dout_stride = _check_matrix(dout, "expert_combine: dout")
     tokens, k = _check_order(order, "expert_combine", dout.device)
     if dout.shape[0] != tokens:
@@ -217,6 +241,12 @@ def embedding_forward(ids, weight, scale=1.0):
     """out[...] = scale * weight[ids[...]], rounded once; zeros for an id outside the table.
 
     ids: int32 or int64 of any shape; weight: (vocabulary, width) of float32, bfloat16 or float16."""
+    native = _native(ids)
+    if native is not None:
+        dev = _current()
+        out = native.embedding_forward(ids, weight, scale, _raw_stream(dev), dev)
+        if out is not None:
+            return _done(out, "apexw_embedding_forward")
     ids = _check_ids(ids, "embedding: ids")
     weight, stride = _check_matrix(weight, "embedding: weight")
     _on_device(weight, "embedding: weight", ids.device)
@@ -236,6 +266,12 @@ def embedding_weight_grad(dy, ids, vocab, scale=1.0, dtype=None):
     weight, zero for an id that no token has; tokens whose id is outside the table count for nothing.
 
     dtype: dy's (the default) or float32.  Summed in fp32, in an order that the ids alone set."""
+    native = _native(dy)
+    if native is not None and dtype in (None, dy.dtype, torch.float32):
+        dev = _current()
+        out = native.embedding_weight_grad(dy, ids, vocab, scale, dtype is torch.float32, _raw_stream(dev), dev)
+        if out is not None:
+            return _done(out, "apexw_embedding_weight_grad")
     ids = _check_ids(ids, "embedding: ids")
     if dy.dtype not in _CODE:
         raise TypeError(f"embedding: expected float32, bfloat16 or float16 gradients, got {dy.dtype}")
