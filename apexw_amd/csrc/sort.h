@@ -3,7 +3,7 @@
 // Items are given as ids; an id outside [0, limit) has the key `limit`, behind all others.  Each pass orders by one digit
 // of up to 9 bits: a launch that counts each workgroup's digits and one that places its items, where a workgroup adds up
 // the counts of those before it by itself (64 workgroups' counts are 128 KB, read from L2) so that no launch in between
-// scans them.  The rank of an item among its wave's is counted from ballots of the digit's bits, so equal keys keep
+// scans them.  Up to 128 K items go in workgroups of 1024 (16384 ids in two passes 34 us by 4096, 21 by 1024).  The rank of an item among its wave's is counted from ballots of the digit's bits, so equal keys keep
 // their order and equal calls give equal results.  Up to kSmall items go through all passes in one workgroup's LDS.
 #pragma once
 
@@ -11,8 +11,9 @@
 
 namespace {
 
-constexpr int kDigits = 512, kSortThreads = 512, kSortWaves = kSortThreads / 64, kItems = 8;
-constexpr int kSmall = kSortThreads * kItems;   // items of a workgroup
+constexpr int kDigits = 512, kSortThreads = 512, kSortWaves = kSortThreads / 64;
+constexpr int kFew = 2, kMost = 8;               // items of a thread
+constexpr int kSmall = kSortThreads * kMost;     // items of one workgroup
 
 struct SortArgs {
   const void* ids;        // int32 or int64
@@ -23,6 +24,8 @@ struct SortArgs {
   u32x2* from;            // (key, item) of a pass after the first
   u32x2* to;
   uint32_t* counts;       // [workgroup][digit]
+  u32x4* clear;           // cleared on the way
+  int64_t clears;
   int32_t *source, *place, *ends;   // of the last pass for experts
 };
 
@@ -73,7 +76,7 @@ struct SortLds {
 // One pass over the items of this workgroup: rounds x 64 consecutive ones a wave from `first` on, get(i) the item i.
 // put(item, position, start of its digit's block) places each.  kAlone: the workgroup has all items.
 // digit_end(d, end): thread d gets the end of digit d's block.
-template <bool kAlone, class Get, class Put, class End>
+template <bool kAlone, int kItems, class Get, class Put, class End>
 APEXW_DEV void sort_pass(const SortArgs& a, SortLds& l, int pass, int first, int rounds, Get&& get, Put&& put,
                          End&& digit_end) {
   const int digits = 1 << a.bits, wave = threadIdx.x >> 6, lane = lane_id(), shift = pass * a.bits;
@@ -113,10 +116,13 @@ APEXW_DEV void sort_pass(const SortArgs& a, SortLds& l, int pass, int first, int
     if (kAlone) {
       all = mine;
     } else {
-      for (int b = 0; b < (int)gridDim.x; ++b) {
-        const uint32_t c = a.counts[(int64_t)b * digits + d];
-        all += c;
-        before += b < (int)blockIdx.x ? c : 0u;
+      constexpr int U = 16;   // loads in flight
+      for (int b0 = 0; b0 < (int)gridDim.x; b0 += U) {
+        uint32_t c[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) c[u] = b0 + u < (int)gridDim.x ? a.counts[(int64_t)(b0 + u) * digits + d] : 0u;
+#pragma unroll
+        for (int u = 0; u < U; ++u) all += c[u], before += b0 + u < (int)blockIdx.x ? c[u] : 0u;
       }
     }
   }
@@ -132,10 +138,15 @@ APEXW_DEV void sort_pass(const SortArgs& a, SortLds& l, int pass, int first, int
     if (r < rounds && base + r * 64 < a.n) put(item[r], l.cnt[wave][item[r][0] >> shift & low] + rank[r]);
 }
 
+APEXW_DEV void sort_clear(const SortArgs& a, int64_t group, int64_t groups) {
+  for (int64_t i = group * kSortThreads + threadIdx.x; i < a.clears; i += groups * kSortThreads) a.clear[i] = u32x4{0u, 0u, 0u, 0u};
+}
+
 // The counts of each workgroup's digits
-template <bool kFirst> __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortArgs a, int pass) {
+template <bool kFirst, int kItems> __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortArgs a, int pass) {
   __shared__ uint32_t cnt[kDigits];
-  const int digits = 1 << a.bits, shift = pass * a.bits, first = blockIdx.x * kSmall;
+  const int digits = 1 << a.bits, shift = pass * a.bits, first = blockIdx.x * kSortThreads * kItems;
+  if (kFirst) sort_clear(a, blockIdx.x, gridDim.x);
   for (int i = threadIdx.x; i < digits; i += kSortThreads) cnt[i] = 0u;
   __syncthreads();
 #pragma unroll
@@ -157,10 +168,10 @@ APEXW_DEV void sort_order(const SortArgs& a, u32x2 item, uint32_t at) {
 }
 
 // kOrder: the last pass of an experts' order, whose ends are the digits' where one pass sorts them
-template <bool kFirst, bool kOrder> __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(SortArgs a, int pass) {
+template <bool kFirst, bool kOrder, int kItems> __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(SortArgs a, int pass) {
   __shared__ SortLds l;
-  sort_pass<false>(
-      a, l, pass, blockIdx.x * kSmall, kItems, [&](int i) { return kFirst ? sort_item(a, i) : a.from[i]; },
+  sort_pass<false, kItems>(
+      a, l, pass, blockIdx.x * kSortThreads * kItems, kItems, [&](int i) { return kFirst ? sort_item(a, i) : a.from[i]; },
       [&](u32x2 item, uint32_t at) {
         if (kOrder) sort_order(a, item, at);
         if (a.to) a.to[at] = item;
@@ -177,7 +188,7 @@ template <bool kOrder> APEXW_DEV void sort_small(const SortArgs& a) {
   const int rounds = (a.n + kSortThreads - 1) / kSortThreads;
   for (int pass = 0; pass < a.passes; ++pass) {
     const bool last = pass == a.passes - 1;
-    sort_pass<true>(
+    sort_pass<true, kMost>(
         a, l, pass, 0, rounds, [&](int i) { return pass == 0 ? sort_item(a, i) : items[i]; },
         [&](u32x2 item, uint32_t at) {
           if (!last) items[at] = item;
@@ -197,7 +208,11 @@ inline void sort_digits(SortArgs& a) {
   a.passes = (bits + 8) / 9;
   a.bits = (bits + a.passes - 1) / a.passes;
 }
-// workgroups of a pass
-inline int sort_groups(int64_t n) { return (int)((n + kSmall - 1) / kSmall); }
+// items of a thread, workgroups of a pass
+inline int sort_items(int64_t n) { return n <= 128 * kSortThreads * kFew ? kFew : kMost; }
+inline int sort_groups(int64_t n) {
+  const int64_t per = kSortThreads * sort_items(n);
+  return (int)((n + per - 1) / per);
+}
 
 }  // namespace

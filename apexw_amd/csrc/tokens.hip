@@ -213,8 +213,9 @@ struct EmbeddingArgs {
   int32_t wide, width, log_t;
   float scale;
   const u32x2* sorted;      // (id, token)
+  int32_t* many;            // the number of ids of many tokens, and, behind 4 of them, which they are
   int32_t* ranges;          // [vocab][2]: where an id's tokens begin and end among the sorted, 0 0 for none
-  float* blocks;            // sums of whole blocks of kBlock sorted tokens of one id
+  float* blocks;            // sums of whole blocks of 2^log_block sorted tokens of one id
   int32_t log_block;
 };
 
@@ -249,36 +250,32 @@ template <int DT> __global__ __launch_bounds__(kWG) void embedding_kernel(Embedd
   }
 }
 
-__global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(SortArgs a) { sort_small<false>(a); }
-
-__global__ __launch_bounds__(256) void embedding_clear_kernel(u32x4* p, int64_t n) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = u32x4{0u, 0u, 0u, 0u};
+__global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(SortArgs a) {
+  if (blockIdx.x) return sort_clear(a, blockIdx.x - 1, gridDim.x - 1);
+  sort_small<false>(a);
 }
 
-// sum += the rows of sorted tokens [from, to), eight in flight, chunk c of each
-template <int DT> APEXW_DEV void add_rows(const EmbeddingArgs& a, const RowChunks<DT>& row, int c, int from, int to,
+// sum += the rows of sorted tokens [from, to), U in flight, chunk c of each
+template <int DT, int U> APEXW_DEV void add_rows(const EmbeddingArgs& a, const RowChunks<DT>& row, int c, int from, int to,
                                           float (&sum)[kVec<DT>]) {
-  constexpr int U = 8;
-  for (int p0 = from; p0 < to; p0 += 64) {
-    const int n = to - p0 < 64 ? to - p0 : 64;
-    const int token = lane_id() < n ? (int)a.sorted[p0 + lane_id()][1] : 0;
-    for (int q0 = 0; q0 < n; q0 += U) {
-      u32x4 v[U];
+  if (c >= row.count) return;
+  for (int p = from; p < to; p += U) {
+    uint32_t token[U];
+    u32x4 v[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (q0 + u < n) {
-          const int t = __builtin_amdgcn_readlane(token, q0 + u);
-          v[u] = c < row.count ? row.load(row_at<DT>(a.w, t * a.stride), c) : u32x4{0u, 0u, 0u, 0u};
-        }
+    for (int u = 0; u < U; ++u)
+      if (p + u < to) token[u] = a.sorted[p + u][1];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (q0 + u < n) {
-          float x[kVec<DT>];
-          values<DT>(v[u], x);
+    for (int u = 0; u < U; ++u)
+      if (p + u < to) v[u] = row.load(row_at<DT>(a.w, token[u] * a.stride), c);
 #pragma unroll
-          for (int i = 0; i < kVec<DT>; ++i) sum[i] += x[i];
-        }
-    }
+    for (int u = 0; u < U; ++u)
+      if (p + u < to) {
+        float x[kVec<DT>];
+        values<DT>(v[u], x);
+#pragma unroll
+        for (int i = 0; i < kVec<DT>; ++i) sum[i] += x[i];
+      }
   }
 }
 
@@ -305,7 +302,11 @@ struct Part {
   }
 };
 
-// Where each id's tokens lie, and the sums of the whole blocks of one id: 64 chunks of columns a workgroup
+// Ids of more tokens than this are summed by the four waves of a workgroup
+constexpr int kMany = 48, kManyGroups = 512;
+
+// Where each id's tokens lie, which ids have many, and the sums of the whole blocks of one id: 64 chunks of columns a
+// workgroup
 template <int DT> __global__ __launch_bounds__(kWG) void embedding_blocks_kernel(EmbeddingArgs a) {
   constexpr int V = kVec<DT>;
   __shared__ float lds[4][64][V];
@@ -314,7 +315,11 @@ template <int DT> __global__ __launch_bounds__(kWG) void embedding_blocks_kernel
     for (int i = first + threadIdx.x; i < n && i < first + size; i += kWG) {
       const uint32_t key = a.sorted[i][0];
       if (key >= a.vocab) continue;
-      if (i == 0 || a.sorted[i - 1][0] != key) a.ranges[2 * (int64_t)key] = i;
+      if (i == 0 || a.sorted[i - 1][0] != key) {
+        a.ranges[2 * (int64_t)key] = i;
+        // (the list's order is of no consequence)
+        if (i + kMany < n && a.sorted[i + kMany][0] == key) a.many[4 + atomicAdd(a.many, 1)] = (int32_t)key;
+      }
       if (i == n - 1 || a.sorted[i + 1][0] != key) a.ranges[2 * (int64_t)key + 1] = i + 1;
     }
   if (n - first < size) return;
@@ -324,7 +329,7 @@ template <int DT> __global__ __launch_bounds__(kWG) void embedding_blocks_kernel
   const int c = blockIdx.y * 64 + lane_id();
   float sum[V] = {};
   const Part p(first, first + size, threadIdx.x >> 6);
-  add_rows<DT>(a, row, c, p.from, p.to, sum);
+  add_rows<DT, 8>(a, row, c, p.from, p.to, sum);
   join_waves<V>(sum, lds);
   if (threadIdx.x < 64 && c < row.count) {
     float* to = a.blocks + (int64_t)blockIdx.x * row.count * V + c * V;
@@ -339,9 +344,9 @@ template <int DT> APEXW_DEV void add_range(const EmbeddingArgs& a, const RowChun
   constexpr int V = kVec<DT>;
   const int size = 1 << a.log_block, b0 = (lo + size - 1) >> a.log_block, b1 = hi >> a.log_block;
   const auto rows = [&](int from, int to) {
-    if (of == 1) return add_rows<DT>(a, row, c, from, to, sum);
+    if (of == 1) return add_rows<DT, 4>(a, row, c, from, to, sum);
     const Part p(from, to, q);
-    add_rows<DT>(a, row, c, p.from, p.to, sum);
+    add_rows<DT, 4>(a, row, c, p.from, p.to, sum);
   };
   if (b0 >= b1) return rows(lo, hi);
   rows(lo, b0 << a.log_block);
@@ -372,24 +377,12 @@ APEXW_DEV int keys_below(const u32x2* sorted, int n, uint32_t key) {
 }
 
 // The gradient's rows: up to 64 of them a workgroup, every (number of workgroups)th, so that frequent words, which have
-// neighbouring ids, go to different ones.  A wave takes 64 chunks of a row; rows of many tokens all four, a part each.
+// neighbouring ids, go to different ones.  A row is taken 64 chunks of columns a wave, narrow rows several a wave.  The
+// first kManyGroups workgroups take the ids of many tokens, 64 chunks each, a part of the tokens a wave: one that met
+// such an id among its rows would end long after the others (65536 tokens, a tenth of them one id, 128256 x 4096: 511 us).
 // kSearch: few tokens, whose ranges are searched for here
-constexpr int kMany = 48;
 template <int DT, int OD, bool kSearch> __global__ __launch_bounds__(kWG) void embedding_grad_kernel(EmbeddingArgs a, int rows) {
   constexpr int V = kVec<DT>;
-  __shared__ float lds[4][64][V];
-  __shared__ int range[64][2];
-  const int64_t groups = gridDim.x;
-  if ((int)threadIdx.x < rows) {
-    const int64_t v = blockIdx.x + threadIdx.x * groups;
-    int lo = 0, hi = 0;
-    if (v < a.vocab) {
-      if (kSearch) lo = keys_below(a.sorted, (int)a.n, (uint32_t)v), hi = keys_below(a.sorted, (int)a.n, (uint32_t)v + 1u);
-      else lo = a.ranges[2 * v], hi = a.ranges[2 * v + 1];
-    }
-    range[threadIdx.x][0] = lo, range[threadIdx.x][1] = hi;
-  }
-  __syncthreads();
   const RowChunks<DT> row(a.width);
   const int slabs = (row.count + 63) / 64, wave = uniform(threadIdx.x >> 6), lane = lane_id();
   const auto write = [&](int64_t v, int c, float (&sum)[V]) {
@@ -409,27 +402,45 @@ template <int DT, int OD, bool kSearch> __global__ __launch_bounds__(kWG) void e
       }
     }
   };
-  bool many = false;
-  for (int u = wave; u < rows * slabs; u += 4) {
-    const int r = u / slabs, c = (u - r * slabs) * 64 + lane, lo = uniform(range[r][0]), hi = uniform(range[r][1]);
-    const int64_t v = blockIdx.x + r * groups;
+  int first = 0;
+  if constexpr (!kSearch) {
+    first = kManyGroups;
+    if (blockIdx.x < kManyGroups) {
+      __shared__ float lds[4][64][V];
+      const int64_t units = (int64_t)a.many[0] * slabs;
+      for (int64_t u = blockIdx.x; u < units; u += kManyGroups) {
+        const int64_t v = a.many[4 + u / slabs];
+        const int c = (int)(u % slabs) * 64 + lane;
+        float sum[V] = {};
+        add_range<DT>(a, row, c, a.ranges[2 * v], a.ranges[2 * v + 1], wave, 4, sum);
+        join_waves<V>(sum, lds);
+        if (wave == 0) write(v, c, sum);
+      }
+      return;
+    }
+  }
+  __shared__ int range[64][2];
+  const int64_t groups = gridDim.x - first, group = blockIdx.x - first;
+  if ((int)threadIdx.x < rows) {
+    const int64_t v = group + threadIdx.x * groups;
+    int lo = 0, hi = 0;
+    if (v < a.vocab) {
+      if (kSearch) lo = keys_below(a.sorted, (int)a.n, (uint32_t)v), hi = keys_below(a.sorted, (int)a.n, (uint32_t)v + 1u);
+      else lo = a.ranges[2 * v], hi = a.ranges[2 * v + 1];
+    }
+    range[threadIdx.x][0] = lo, range[threadIdx.x][1] = hi;
+  }
+  __syncthreads();
+  // 2^log_t threads share 64 or fewer chunks
+  const int per = 64 >> a.log_t;
+  for (int u = wave * per + (lane >> a.log_t); u < rows * slabs; u += 4 * per) {
+    const int r = u / slabs, c = (u - r * slabs) * 64 + (lane & ((1 << a.log_t) - 1)), lo = range[r][0], hi = range[r][1];
+    const int64_t v = group + r * groups;
     if (v >= a.vocab) break;
-    if (hi - lo > kMany) continue;
+    if (!kSearch && hi - lo > kMany) continue;
     float sum[V] = {};
     if (hi > lo) add_range<DT>(a, row, c, lo, hi, 0, 1, sum);
     write(v, c, sum);
-  }
-  for (int r = 0; r < rows; ++r) many = many || range[r][1] - range[r][0] > kMany;
-  if (!many) return;
-  for (int r = 0; r < rows; ++r) {
-    const int lo = uniform(range[r][0]), hi = uniform(range[r][1]);
-    if (hi - lo <= kMany) continue;
-    for (int s = 0; s < slabs; ++s) {
-      float sum[V] = {};
-      add_range<DT>(a, row, s * 64 + lane, lo, hi, wave, 4, sum);
-      join_waves<V>(sum, lds);
-      if (wave == 0) write(blockIdx.x + r * groups, s * 64 + lane, sum);
-    }
   }
 }
 
@@ -446,7 +457,7 @@ struct SortSpace {
   int64_t counts, pairs, bytes;
   SortSpace(const SortArgs& a, bool wanted) {
     const bool small = a.n <= kSmall;
-    counts = small ? 0 : aligned((int64_t)sort_groups(a.n) << a.bits << 2);
+    counts = small ? 0 : aligned(((int64_t)sort_groups(a.n) << a.bits) * 4);
     pairs = aligned((int64_t)a.n * 8);
     const int lists = (wanted ? 1 : 0) + (small ? 0 : a.passes - 1 < 2 ? a.passes - 1 : 2);
     bytes = counts + pairs * (lists > 2 ? 2 : lists);
@@ -461,7 +472,7 @@ SortArgs sort_args(const void* ids, int32_t id_bytes, int64_t n, uint32_t limit)
 }
 
 // More than kSmall items: the passes, from one list to the other; the sorted pairs where they are wanted
-template <bool kOrder> const u32x2* launch_sort(SortArgs a, const SortSpace& space, bool wanted, char* ws, hipStream_t s) {
+template <bool kOrder, int kItems> const u32x2* launch_passes(SortArgs a, const SortSpace& space, bool wanted, char* ws, hipStream_t s) {
   a.counts = (uint32_t*)ws;
   u32x2* lists[2] = {(u32x2*)(ws + space.counts), (u32x2*)(ws + space.counts + space.pairs)};
   const dim3 grid((unsigned)sort_groups(a.n)), block(kSortThreads);
@@ -469,17 +480,21 @@ template <bool kOrder> const u32x2* launch_sort(SortArgs a, const SortSpace& spa
     const bool last = pass == a.passes - 1;
     a.from = pass ? lists[(pass - 1) & 1] : nullptr;
     a.to = last && !wanted ? nullptr : lists[pass & 1];
-    if (pass == 0) hipLaunchKernelGGL((sort_count_kernel<true>), grid, block, 0, s, a, pass);
-    else hipLaunchKernelGGL((sort_count_kernel<false>), grid, block, 0, s, a, pass);
+    if (pass == 0) hipLaunchKernelGGL((sort_count_kernel<true, kItems>), grid, block, 0, s, a, pass);
+    else hipLaunchKernelGGL((sort_count_kernel<false, kItems>), grid, block, 0, s, a, pass);
     if (kOrder && last) {
-      if (pass == 0) hipLaunchKernelGGL((sort_place_kernel<true, kOrder>), grid, block, 0, s, a, pass);
-      else hipLaunchKernelGGL((sort_place_kernel<false, kOrder>), grid, block, 0, s, a, pass);
+      if (pass == 0) hipLaunchKernelGGL((sort_place_kernel<true, kOrder, kItems>), grid, block, 0, s, a, pass);
+      else hipLaunchKernelGGL((sort_place_kernel<false, kOrder, kItems>), grid, block, 0, s, a, pass);
     } else {
-      if (pass == 0) hipLaunchKernelGGL((sort_place_kernel<true, false>), grid, block, 0, s, a, pass);
-      else hipLaunchKernelGGL((sort_place_kernel<false, false>), grid, block, 0, s, a, pass);
+      if (pass == 0) hipLaunchKernelGGL((sort_place_kernel<true, false, kItems>), grid, block, 0, s, a, pass);
+      else hipLaunchKernelGGL((sort_place_kernel<false, false, kItems>), grid, block, 0, s, a, pass);
     }
   }
   return a.to;
+}
+template <bool kOrder> const u32x2* launch_sort(const SortArgs& a, const SortSpace& space, bool wanted, char* ws, hipStream_t s) {
+  if (sort_items(a.n) == kFew) return launch_passes<kOrder, kFew>(a, space, wanted, ws, s);
+  return launch_passes<kOrder, kMost>(a, space, wanted, ws, s);
 }
 
 int log_threads(int64_t width, int32_t dtype, bool four_waves) {
@@ -513,19 +528,24 @@ template <class F> int by_types(int32_t dtype, int32_t w_dtype, F&& f) {
   return ok ? APEXW_OK : APEXW_ERR_DTYPE;
 }
 
+// Up to this many tokens no row of the gradient sums enough to be worth the launch that finds the ids of many
+constexpr int64_t kFewTokens = 256;
+
 struct GradPlan {
   SortArgs sort;
   SortSpace space;
   int log_block;
-  int64_t ranges, blocks, bytes;
+  int64_t many, ranges, blocks, bytes;
   GradPlan(const void* ids, int32_t id_bytes, int64_t n, uint32_t vocab, int64_t width)
       : sort(sort_args(ids, id_bytes, n, vocab)), space(sort, true) {
     // a row's sum is over up to twice a block's tokens and one sum for each block
-    log_block = n <= 32768 ? 6 : n <= 262144 ? 7 : 8;
-    ranges = n > kSmall ? aligned((int64_t)vocab * 8) : 0;
-    blocks = n > kSmall ? aligned((n >> log_block) * (width + 8) * 4) : 0;
-    bytes = space.bytes + ranges + blocks;
-    if (n <= kSmall) log_block = 30;   // no blocks
+    log_block = n <= 32768 ? 6 : n <= 131072 ? 7 : 8;
+    const bool few = n <= kFewTokens;
+    many = few ? 0 : aligned(16 + n / kMany * 4);
+    ranges = few ? 0 : aligned((int64_t)vocab * 8);
+    blocks = few ? 0 : aligned((n >> log_block) * (width + 8) * 4);
+    bytes = space.bytes + many + ranges + blocks;
+    if (few) log_block = 30;   // no blocks
   }
 };
 
@@ -656,27 +676,33 @@ extern "C" int apexw_embedding_weight_grad(const void* dy, int64_t dy_stride, co
   EmbeddingArgs a{};
   a.n = n, a.w = dy, a.stride = dy_stride, a.vocab = (uint32_t)vocab, a.width = (int32_t)width, a.scale = scale, a.out = dw;
   a.log_block = plan.log_block;
-  a.ranges = (int32_t*)(ws + plan.space.bytes), a.blocks = (float*)(ws + plan.space.bytes + plan.ranges);
-  const bool few = n <= kSmall;
+  a.log_t = log_threads(width, dtype, false);
+  a.many = (int32_t*)(ws + plan.space.bytes), a.ranges = (int32_t*)(ws + plan.space.bytes + plan.many);
+  a.blocks = (float*)(ws + plan.space.bytes + plan.many + plan.ranges);
+  const bool few = n <= kFewTokens;
+  SortArgs sort = plan.sort;
+  sort.clear = (u32x4*)a.many, sort.clears = (plan.many + plan.ranges) / 16;
   // rows a workgroup: 2048 workgroups and more, of up to 64 rows
   const int rows = (int)(vocab < 4096 ? 1 : vocab / 2048 < 64 ? vocab / 2048 : 64);
   const unsigned groups = (unsigned)((vocab + rows - 1) / rows);
   const int st = by_types(dtype, dw_dtype, [&](auto d, auto o) {
     constexpr int DT = decltype(d)::value, OD = decltype(o)::value;
-    if (few) {
-      SortArgs sort = plan.sort;
+    if (n <= kSmall) {
       a.sorted = sort.to = (u32x2*)ws;
-      if (n > 0) hipLaunchKernelGGL(embedding_sort_kernel, dim3(1), dim3(kSortThreads), 0, s, sort);
+      const int64_t clears = (sort.clears + kSortThreads * 4 - 1) / (kSortThreads * 4);
+      if (n > 0)
+        hipLaunchKernelGGL(embedding_sort_kernel, dim3((unsigned)(1 + (clears < 512 ? clears : 512))), dim3(kSortThreads), 0, s, sort);
+    } else {
+      a.sorted = launch_sort<false>(sort, plan.space, true, ws, s);
+    }
+    if (few) {
       hipLaunchKernelGGL((embedding_grad_kernel<DT, OD, true>), dim3(groups), dim3(kWG), 0, s, a, rows);
       return;
     }
-    const int64_t clear = plan.ranges / 16, grid = (clear + 255) / 256;
-    hipLaunchKernelGGL(embedding_clear_kernel, dim3((unsigned)(grid < 1024 ? grid : 1024)), dim3(256), 0, s, (u32x4*)a.ranges, clear);
-    a.sorted = launch_sort<false>(plan.sort, plan.space, true, ws, s);
     const int chunks = (int)((width + kVec<DT> - 1) / kVec<DT>);
     const unsigned blocks = (unsigned)((n + (1 << a.log_block) - 1) >> a.log_block);
     hipLaunchKernelGGL(embedding_blocks_kernel<DT>, dim3(blocks, (unsigned)((chunks + 63) / 64)), dim3(kWG), 0, s, a);
-    hipLaunchKernelGGL((embedding_grad_kernel<DT, OD, false>), dim3(groups), dim3(kWG), 0, s, a, rows);
+    hipLaunchKernelGGL((embedding_grad_kernel<DT, OD, false>), dim3(groups + kManyGroups), dim3(kWG), 0, s, a, rows);
   });
   return st ? st : launched();
 }
