@@ -420,6 +420,7 @@ template <int DT> __global__ __launch_bounds__(256) void head_dx_kernel(HeadArgs
     uint16_t* to = dx + (int64_t)h.rows[r].row * width + c;
     if (has == 8) {
       float v[8] = {};
+#pragma unroll 4
       for (int s = 0; s < splits; ++s) {
         const u32x4 lo = APEXW_GLOBAL(const Chunk32, p + s * stride)->v, hi = APEXW_GLOBAL(const Chunk32, p + s * stride + 4)->v;
 #pragma unroll
@@ -445,38 +446,42 @@ template <int DT> __global__ __launch_bounds__(256) void head_dx_kernel(HeadArgs
 int64_t whole(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
 // The time of a product whose tiles the chip takes in rounds, in us: a stage's when every workgroup is at work and with
-// few (as for the experts' products), a tile's end, and the launch and bytes of parts that are joined.  kWhole: a last
-// round takes as long as the others; else its tiles are cut.
+// few, the end of a tile that is written in 16 bits or in fp32 (a round's 64 MB at once), and the launch and bytes of
+// parts that are joined.  whole_rounds: a last round takes as long as the others; else its tiles are cut.  The rates
+// are those of dx of 16384, 13107 (156 tiles of 256 x 256: whole 579 us, in three parts 457, in four 518), 2048, 500 and
+// 64 rows with 768 x 21760, 1024 x 32000, 504 x 10007 and 768 x 50257, each shape in 1 to 16 parts.
 struct Rate {
-  float most, least, end;
+  float most, least, end16, end32;
   int slots, bm, bn;
 };
-template <class S> Rate rate(float most, float least, float end) {
-  return {most, least, end, apexw_cu_count() * S::kPerCU, S::BM, S::BN};
+template <class S> Rate rate(float most, float least, float end16, float end32) {
+  return {most, least, end16, end32, apexw_cu_count() * S::kPerCU, S::BM, S::BN};
 }
 Rate rate_of(int shape) {
-  if (shape == 3) return rate<Large>(1.6f, 0.95f, 5.0f);
-  if (shape == 2) return rate<Wide>(0.95f, 0.65f, 4.0f);
-  if (shape == 1) return rate<Mid>(0.7f, 0.45f, 2.5f);
-  return rate<Small>(0.55f, 0.42f, 2.0f);
+  if (shape == 3) return rate<Large>(1.65f, 1.35f, 9.0f, 30.0f);
+  if (shape == 2) return rate<Wide>(1.13f, 0.85f, 5.0f, 9.0f);
+  if (shape == 1) return rate<Mid>(0.72f, 0.48f, 4.0f, 7.0f);
+  return rate<Small>(0.6f, 0.42f, 3.0f, 4.0f);
 }
-float time_of(int shape, int64_t down, int64_t across, int64_t depth, int splits, bool whole_rounds, float join_bytes) {
+float time_of(int shape, int64_t down, int64_t across, int64_t depth, int splits, bool whole_rounds, bool fp32, float join_bytes) {
   const Rate r = rate_of(shape);
   const float tiles = (float)((down + r.bm - 1) / r.bm) * (float)((across + r.bn - 1) / r.bn);
   const float rounds = tiles * (float)splits / (float)r.slots, full = floorf(rounds), rest = rounds - full;
-  const float stages = ceilf((float)((depth + kDepth - 1) / kDepth) / (float)splits);
-  const float join = splits > 1 ? 5.0f + (float)splits * join_bytes / 4e6f : 0.0f;
-  if (rounds <= 1.0f) return stages * (r.least + (r.most - r.least) * rounds) + r.end + join;
+  const float stages = ceilf((float)((depth + kDepth - 1) / kDepth) / (float)splits), end = fp32 ? r.end32 : r.end16;
+  const float join = splits > 1 ? 5.0f + (float)(splits - 1) * join_bytes / 4e6f : 0.0f;
+  if (rounds <= 1.0f) return stages * (r.least + (r.most - r.least) * rounds) + 3.0f + (end - 3.0f) * rounds + join;
   const float last = rest == 0.0f ? 0.0f : whole_rounds || splits > 1 || rest > 0.5f ? 1.0f : rest > 0.25f ? 0.6f : 0.4f;
-  return (full + last) * (stages * r.most + r.end) + join;
+  return (full + last) * (stages * r.most + end) + join;
 }
-// the shape and parts of the least time; a part has to be worth a quarter more than it seems
-Cut best_cut(int least_shape, int64_t down, int64_t across, int64_t depth, bool may_split, bool whole_rounds, float join_bytes) {
+// the shape and parts of the least time; parts have to gain a tenth
+Cut best_cut(int least_shape, int64_t down, int64_t across, int64_t depth, bool may_split, bool whole_rounds, bool fp32,
+             float join_bytes) {
   Cut best{0, 0, 0.0f};
   for (int shape = least_shape; shape < 4; ++shape)
     for (int splits = 1; splits == 1 || (may_split && splits <= 64 && splits * 4 * kDepth <= depth); ++splits) {
       if (splits > 4 && (splits & (splits - 1))) continue;
-      const float t = time_of(shape, down, across, depth, splits, whole_rounds, join_bytes), cost = splits > 1 ? 1.1f * t : t;
+      const float t = time_of(shape, down, across, depth, splits, whole_rounds, fp32 || splits > 1, join_bytes);
+      const float cost = splits > 1 ? 1.1f * t : t;
       if (best.splits == 0 || cost < best.cost) best = {shape, splits, cost};
     }
   return best;
@@ -485,6 +490,9 @@ Cut best_cut(int least_shape, int64_t down, int64_t across, int64_t depth, bool 
 // Bytes of G that a piece may have.  (Between 128 MB and 4 GB the time changes by what the pieces' tiles leave of the
 // chip's rounds alone: 8192 x 4096 x 128256 19.9 to 20.6 ms.)
 constexpr int64_t kPiece = 1ll << 30;
+// Bytes of the pieces' sums of dx, which the last launch adds up; where there were more, each piece adds to the ones
+// before, at a third of the rate: a tile's values are loaded, added and stored one after the other
+constexpr int64_t kSums = 2ll << 30;
 
 // The products of a piece of `cols` columns of the vocabulary
 struct Piece {
@@ -493,10 +501,10 @@ struct Piece {
   float cost;
   Piece() = default;
   Piece(int64_t c, int64_t n, int64_t width, bool need_dx, bool need_dw) : cols(c) {
-    logits = best_cut(0, n, cols, width, false, false, 0.0f);
-    dw = best_cut(2, cols, width, n, true, true, 8.0f * (float)cols * (float)width);
-    dx = best_cut(0, n, width, cols, true, false, 12.0f * (float)n * (float)width);
-    // (adding to the pieces before reads and writes dx's sums)
+    logits = best_cut(0, n, cols, width, false, false, false, 0.0f);
+    dw = best_cut(2, cols, width, n, true, true, false, 8.0f * (float)cols * (float)width);
+    dx = best_cut(0, n, width, cols, true, false, true, 8.0f * (float)n * (float)width);
+    // (sums of dx that are written and read again)
     cost = logits.cost + (need_dw ? dw.cost : 0.0f) + (need_dx ? dx.cost + 8.0f * (float)n * (float)width / 4e6f : 0.0f);
   }
 };
@@ -508,7 +516,8 @@ struct HeadPlan {
   int64_t parts_ld, piece_ld;
   Cut cut;                 // forward
   Piece piece, last;       // backward
-  int dx_splits;
+  int dx_sums;             // parts of dx that are added up
+  bool add;                // each piece to the ones before
   HeadPlan(const void* w, int64_t stride, int64_t n_, int64_t width_, int64_t vocab_, bool backward, bool need_dx, bool need_dw)
       : n(n_), width(width_), wide((width_ + 7) / 8 * 8), vocab(vocab_), w_stride(stride) {
     copy_w = !k_rows_ok(w, stride, width);
@@ -519,7 +528,7 @@ struct HeadPlan {
     at_w = at_x + whole(n * wide * 2);
     int64_t at = at_w + (copy_w ? whole(vocab * wide * 2) : 0);
     if (!backward) {
-      cut = best_cut(0, n, vocab, width, false, false, 0.0f);
+      cut = best_cut(0, n, vocab, width, false, false, false, 0.0f);
       parts_ld = (n + 15) / 16 * 16;
       at_parts = at, at += whole(parts_ld * parts() * 4);
       bytes = at;
@@ -528,8 +537,11 @@ struct HeadPlan {
     cut_pieces(need_dx, need_dw);
     piece_ld = (piece.cols + 7) / 8 * 8;
     at_g = at, at += whole(n * piece_ld * 2);
-    dx_splits = dx(piece).splits;
-    at_sums = at, at += need_dx ? whole(dx_splits * n * width * 4) : 0;
+    dx_sums = dx(piece).splits;
+    const int64_t pieces = (vocab + piece.cols - 1) / piece.cols, rest = dx(last).splits;
+    add = ((pieces - 1) * dx_sums + rest) * n * width * 4 > kSums;
+    if (!add) dx_sums = (int)((pieces - 1) * dx_sums + rest);
+    at_sums = at, at += need_dx ? whole(dx_sums * n * width * 4) : 0;
     int64_t parts = 0;
     if (need_dw)
       for (const Piece* q : {&piece, &last})
@@ -557,7 +569,7 @@ struct HeadPlan {
       const float cost = (float)count * p.cost + q.cost;
       if (least == 0.0f || cost < least) least = cost, piece = p, last = q;
     }
-    last.dx = piece.dx;   // (the first piece writes every part's sums)
+    last.dx = piece.dx;   // (where pieces are added, the first one writes every part's sums)
   }
   const Piece& at_column(int64_t v) const { return v + piece.cols <= vocab ? piece : last; }
 
@@ -732,6 +744,7 @@ extern "C" int apexw_linear_cross_entropy_backward(const float* dloss, int64_t d
     const uint16_t* w = launch_pack<DT>(p, pack, weight, w_stride, ws, s);
     const HeadArgs h{pack.state, pack.rows, pack.shift, nullptr, 0};
     uint16_t* G = (uint16_t*)(ws + p.at_g);
+    float* sums = (float*)(ws + p.at_sums);
     for (int64_t v = 0; v < vocab; v += p.piece.cols) {
       const Piece& q = p.at_column(v);
       const uint16_t* wp = w + v * p.w_stride;
@@ -749,14 +762,15 @@ extern "C" int apexw_linear_cross_entropy_backward(const float* dloss, int64_t d
       }
       if (dx && n > 0) {
         ExpertArgs g = p.dx(q);
-        g.a = G, g.b = wp, g.ends = &pack.state->count, g.out = ws + p.at_sums;
-        launch_dx<DT>(g, q.dx.shape, v > 0, s);
+        g.a = G, g.b = wp, g.ends = &pack.state->count, g.out = sums;
+        launch_dx<DT>(g, q.dx.shape, p.add && v > 0, s);
+        if (!p.add) sums += g.splits * g.split_stride;
       }
     }
     if (dx && n > 0) {
       const int64_t grid = (n * ((width + 3) / 4) + 255) / 256;
       hipLaunchKernelGGL(head_dx_kernel<DT>, dim3((unsigned)(grid < 8192 ? grid : 8192)), dim3(256), 0, s, h,
-                         (const float*)(ws + p.at_sums), n * width, p.dx_splits, (int)width, (uint16_t*)dx);
+                         (const float*)(ws + p.at_sums), n * width, p.dx_sums, (int)width, (uint16_t*)dx);
     }
   });
   return hipGetLastError() == hipSuccess ? APEXW_OK : APEXW_ERR_LAUNCH;

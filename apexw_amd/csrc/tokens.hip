@@ -419,7 +419,7 @@ template <int DT, int OD, bool kSearch> __global__ __launch_bounds__(kWG) void e
       return;
     }
   }
-  __shared__ int range[64][2];
+  __shared__ int range[64][3];   // of a row: its tokens among the sorted, and the first one
   const int64_t groups = gridDim.x - first, group = blockIdx.x - first;
   if ((int)threadIdx.x < rows) {
     const int64_t v = group + threadIdx.x * groups;
@@ -429,18 +429,58 @@ template <int DT, int OD, bool kSearch> __global__ __launch_bounds__(kWG) void e
       else lo = a.ranges[2 * v], hi = a.ranges[2 * v + 1];
     }
     range[threadIdx.x][0] = lo, range[threadIdx.x][1] = hi;
+    range[threadIdx.x][2] = hi > lo ? (int)a.sorted[lo][1] : 0;
   }
   __syncthreads();
-  // 2^log_t threads share 64 or fewer chunks
-  const int per = 64 >> a.log_t;
-  for (int u = wave * per + (lane >> a.log_t); u < rows * slabs; u += 4 * per) {
-    const int r = u / slabs, c = (u - r * slabs) * 64 + (lane & ((1 << a.log_t) - 1)), lo = range[r][0], hi = range[r][1];
+  const auto light = [&](int64_t v, int lo, int hi, int token, int c) {
+    float sum[V] = {};
+    if (hi - lo == 1) {
+      if (c < row.count) values<DT>(row.load(row_at<DT>(a.w, token * a.stride), c), sum);
+    } else if (hi > lo) {
+      add_range<DT>(a, row, c, lo, hi, 0, 1, sum);
+    }
+    write(v, c, sum);
+  };
+  if (slabs == 1) {   // 2^log_t threads a row
+    const int per = 64 >> a.log_t, c = lane & ((1 << a.log_t) - 1);
+    for (int r = wave * per + (lane >> a.log_t); r < rows; r += 4 * per) {
+      const int64_t v = group + r * groups;
+      if (v >= a.vocab) break;
+      if (kSearch || range[r][1] - range[r][0] <= kMany) light(v, range[r][0], range[r][1], range[r][2], c);
+    }
+    return;
+  }
+  if (slabs < 4) {
+    for (int u = wave; u < rows * slabs; u += 4) {
+      const int r = u / slabs, c = (u - r * slabs) * 64 + lane;
+      const int64_t v = group + r * groups;
+      if (v >= a.vocab) break;
+      const int lo = range[r][0], hi = range[r][1];
+      if (!kSearch && hi - lo > kMany) continue;
+      float sum[V] = {};
+      if (hi > lo) add_range<DT>(a, row, c, lo, hi, 0, 1, sum);
+      write(v, c, sum);
+    }
+    return;
+  }
+  for (int r = 0; r < rows; ++r) {
     const int64_t v = group + r * groups;
     if (v >= a.vocab) break;
+    const int lo = range[r][0], hi = range[r][1], token = uniform(range[r][2]);   // (scalar loads of the sorted are slower)
     if (!kSearch && hi - lo > kMany) continue;
-    float sum[V] = {};
-    if (hi > lo) add_range<DT>(a, row, c, lo, hi, 0, 1, sum);
-    write(v, c, sum);
+    int s = wave;
+    for (; hi - lo <= 1 && s + 4 < slabs; s += 8) {   // two at once
+      const int c0 = s * 64 + lane, c1 = c0 + 256;
+      float x[V] = {}, y[V] = {};
+      if (hi > lo) {
+        const void* from = row_at<DT>(a.w, token * a.stride);
+        const u32x4 p = row.load(from, c0), q = row.load(from, c1 < row.count ? c1 : c0);
+        values<DT>(p, x), values<DT>(q, y);
+      }
+      write(v, c0, x);
+      write(v, c1, y);
+    }
+    for (; s < slabs; s += 4) light(v, lo, hi, token, s * 64 + lane);
   }
 }
 
