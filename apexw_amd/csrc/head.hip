@@ -34,7 +34,7 @@ struct HeadArgs {
   const HeadState* state;
   const HeadRow* rows;
   const float* shift;       // one a row, of the exponents of its tiles
-  float* sums;              // [columns of a wave][row]: log2 of the sum of 2^(l log2 e - shift)
+  float* sums;              // [columns of a wave or tile][row]: log2 of the sum of 2^(l log2 e - shift)
   int64_t sums_ld;
 };
 
@@ -73,20 +73,31 @@ template <class T, class F> APEXW_DEV T over_workgroup(T x, T* lds, F&& f) {
 
 // A workgroup has `per` (up to 256) rows; how many rows before them count it finds by itself.  A wave takes a row at a
 // time: copies it, and forms its target's logit on the way.
-template <int DT> __global__ __launch_bounds__(256) void head_pack_kernel(PackArgs a) {
+template <int DT> __global__ __launch_bounds__(256) void head_pack_kernel(PackArgs a, Pad weights, int groups) {
+  if ((int)blockIdx.x >= groups) {   // the weights, copied to whole chunks
+    if (weights.rows * ((weights.width + 7) / 8) < (1ll << 31)) pad_rows<uint32_t>(weights, blockIdx.x - groups, gridDim.x - groups);
+    else pad_rows<uint64_t>(weights, blockIdx.x - groups, gridDim.x - groups);
+    return;
+  }
   __shared__ int ints[4];
   __shared__ float floats[4];
   __shared__ int place[256];
   const int64_t first = (int64_t)blockIdx.x * a.per, end = first + a.per < a.n ? first + a.per : a.n;
-  const bool last = blockIdx.x == gridDim.x - 1;
+  const bool last = (int)blockIdx.x == groups - 1;
   int before = 0;
   float most = 0.0f;
   const bool find_most = last && a.rescale;
-#pragma unroll 4
-  for (int64_t i = threadIdx.x; i < first; i += 256) {
-    const bool c = counts(a, target_of(a, i));
-    before += c;
-    if (find_most && c) most = fmaxf(most, fabsf(a.dloss[i * a.dloss_stride]));
+  constexpr int U = 16;   // loads in flight
+  for (int64_t i0 = threadIdx.x; i0 < first; i0 += 256 * U) {
+    int64_t t[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) t[u] = i0 + 256 * u < first ? target_of(a, i0 + 256 * u) : -1;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool c = counts(a, t[u]);
+      before += c;
+      if (find_most && c) most = fmaxf(most, fabsf(a.dloss[(i0 + 256 * u) * a.dloss_stride]));
+    }
   }
   before = over_workgroup(before, ints, [](int p, int q) { return p + q; });
 
@@ -184,7 +195,7 @@ template <int FA> struct Shifts {
   float v[FA];
   __device__ __forceinline__ void load(const float* shift, int64_t row0, int row, int rows) {
 #pragma unroll
-    for (int i = 0; i < FA; ++i) v[i] = shift[row0 + (row + 16 * i < rows ? row + 16 * i : rows - 1)];
+    for (int i = 0; i < FA; ++i) v[i] = shift[row0 + min(row + 16 * i, rows - 1)];
   }
   __device__ __forceinline__ void arrived() {
 #pragma unroll
@@ -208,9 +219,13 @@ struct Sums {
     const int wm = down * kWM, wn = across * S::WN, lane = lane_id();
     const int64_t row0 = out0 >> 32;
     const int col0 = (int)(uint32_t)out0;
-    if (wn >= cols) return;
+    // tiles of one wave's rows: the waves' sums are joined here, since what few rows take is the last launch's time
+    constexpr bool kJoin = S::BM == S::WM;
+    constexpr int kAcross = S::BN / S::WN;
+    if (!kJoin && wn >= cols) return;
     if (wn + S::WN > cols) mask_columns<FA, FB>(acc, wn, cols, -INFINITY);
-    float* to = h.sums + (col0 + wn) / S::WN * h.sums_ld + row0 + wm;
+    float* parts = (float*)(lds + S::kStages * S::kStageElems);
+    float* to = kJoin ? parts + across * S::WM : h.sums + (col0 + wn) / S::WN * h.sums_ld + row0 + wm;
 #pragma unroll
     for (int i = 0; i < FA; ++i) {
       const float shift = known.v[i];
@@ -243,12 +258,28 @@ struct Sums {
       }
       if (lane < 16 && wm + 16 * i + lane < rows) to[16 * i + lane] = part;
     }
+    if constexpr (kJoin) {
+      barrier();
+      const int r = threadIdx.x;
+      if (r < rows && r < kWM) {
+        float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kAcross; ++w) top = fmaxf(top, parts[w * S::WM + r]);
+        const float from = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int w = 0; w < kAcross; ++w) sum += __builtin_amdgcn_exp2f(parts[w * S::WM + r] - from);
+        h.sums[col0 / S::BN * h.sums_ld + row0 + r] = from + __builtin_amdgcn_logf(sum);
+      }
+    }
   }
 };
 
-// Backward: the tile's part of G without the targets' ones, whole chunks of columns
+// Backward: the tile's part of G, whole chunks of columns; a tile of 256 x 256, whose registers are all in use, leaves
+// the targets' elements to a launch behind it
+constexpr bool targets_apart(int shape) { return shape == 3; }
 template <int DT> struct Prob {
   HeadArgs h;
+  int32_t first;   // the piece's first column
   template <int FA> using Rows = Shifts<FA>;
   template <class R> __device__ __forceinline__ void load(R& known, int64_t out0, int row, int rows) const {
     known.load(h.shift, out0 >> 32, row, rows);
@@ -273,6 +304,18 @@ template <int DT> struct Prob {
 #pragma unroll
           for (int q = 0; q < 4; ++q) acc[i][j][q] = bits & 1u ? -acc[i][j][q] : acc[i][j][q];
       }
+      if constexpr (!std::is_same_v<S, Large>) {
+        const int r = down * kWM + 16 * i + (lane_id() & 15);
+        const HeadRow& row = h.rows[(out0 >> 32) + min(r, rows - 1)];
+        const int t = row.target - first - (int)(uint32_t)out0 - across * S::WN;
+        if (__ballot(t >= 0 && t < S::WN)) {
+          const float d = row.d * h.state->factor;
+#pragma unroll
+          for (int j = 0; j < FB; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) acc[i][j][q] -= t == 16 * j + 4 * (lane_id() >> 4) + q ? d : 0.0f;
+        }
+      }
     }
     if (cols < S::BN) mask_columns<FA, FB>(acc, across * S::WN, cols, 0.0f);
     Store<DT>::template put<S, kWM>(g, acc, lds, down, across, rows, (cols + 7) / 8 * 8,
@@ -280,7 +323,7 @@ template <int DT> struct Prob {
   }
 };
 
-// The targets' elements of the piece's G
+// The targets' elements of the piece's G, from the logits that the packing formed
 template <int DT> __global__ __launch_bounds__(256) void head_targets_kernel(HeadArgs h, int first, int cols, void* g, int64_t ldg) {
   const int i = blockIdx.x * 256 + threadIdx.x;
   if (i >= h.state->count) return;
@@ -502,6 +545,11 @@ struct Piece {
   Piece() = default;
   Piece(int64_t c, int64_t n, int64_t width, bool need_dx, bool need_dw) : cols(c) {
     logits = best_cut(0, n, cols, width, false, false, false, 0.0f);
+    if (targets_apart(logits.shape)) {   // a launch more
+      const float other = time_of(2, n, cols, width, 1, false, false, 0.0f);
+      if (other < logits.cost + 4.0f) logits = {2, 1, other};
+      else logits.cost += 4.0f;
+    }
     dw = best_cut(2, cols, width, n, true, true, false, 8.0f * (float)cols * (float)width);
     dx = best_cut(0, n, width, cols, true, false, true, 8.0f * (float)n * (float)width);
     // (sums of dx that are written and read again)
@@ -595,12 +643,12 @@ struct HeadPlan {
     cut_up(g, q.dx.splits, kDepth);
     return g;
   }
-  int64_t parts() const {   // waves across the vocabulary
-    const int64_t wave = cut.shape == 0 ? Small::WN : Large::WN;
+  int64_t parts() const {   // sums of a row
+    const int64_t wave = cut.shape == 0 ? Small::BN : Large::WN;
     return (vocab + wave - 1) / wave;
   }
 };
-static_assert(Large::WN == 64 && Wide::WN == 64 && Mid::WN == 64, "columns of a wave");
+static_assert(Large::WN == 64 && Wide::WN == 64 && Mid::WN == 64 && Small::BM == Small::WM, "columns of a sum");
 
 bool head_ok(int64_t n, int64_t width, int64_t vocab) {
   return n >= 0 && n <= INT32_MAX - 65536 && width > 0 && width <= kMostLd && vocab > 0 && vocab <= INT32_MAX - 65536;
@@ -662,13 +710,18 @@ template <int DT> const uint16_t* launch_pack(const HeadPlan& p, PackArgs& a, co
   // about 1024 workgroups, of at least 4 rows
   const int64_t per = (p.n + 1023) / 1024;
   a.per = (int32_t)(per < 4 ? 4 : per > 256 ? 256 : per);
-  const int64_t grid = (p.n + a.per - 1) / a.per;
-  hipLaunchKernelGGL(head_pack_kernel<DT>, dim3((unsigned)(grid ? grid : 1)), dim3(256), 0, s, a);
-  if (!p.copy_w) return (const uint16_t*)w;
-  uint16_t* at = (uint16_t*)(ws + p.at_w);
+  const int groups = p.n ? (int)((p.n + a.per - 1) / a.per) : 1;
   const uint16_t* from = (const uint16_t*)w;
-  int64_t step = 0;
-  launch_pad(pad(from, stride, step, p.vocab, p.vocab, (int32_t)p.width, at), Pad{}, s);
+  Pad weights{};
+  int64_t copies = 0;
+  if (p.copy_w) {
+    uint16_t* at = (uint16_t*)(ws + p.at_w);
+    int64_t step = 0;
+    weights = pad(from, stride, step, p.vocab, p.vocab, (int32_t)p.width, at);
+    copies = p.vocab * p.width / 2048 + 1;
+  }
+  hipLaunchKernelGGL(head_pack_kernel<DT>, dim3((unsigned)(groups + (copies < 8192 ? copies : 8192))), dim3(256), 0, s, a, weights,
+                     groups);
   return from;
 }
 
@@ -751,9 +804,10 @@ extern "C" int apexw_linear_cross_entropy_backward(const float* dloss, int64_t d
       if (n > 0) {
         ExpertArgs g = p.logits(q);
         g.a = pack.packed, g.b = wp, g.ends = &pack.state->count, g.out = G;
-        launch_logits<DT>(g, q.logits.shape, Prob<DT>{h}, s);
-        hipLaunchKernelGGL(head_targets_kernel<DT>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, h, (int)v, (int)q.cols, G,
-                           p.piece_ld);
+        launch_logits<DT>(g, q.logits.shape, Prob<DT>{h, (int32_t)v}, s);
+        if (targets_apart(q.logits.shape))
+          hipLaunchKernelGGL(head_targets_kernel<DT>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, h, (int)v, (int)q.cols, G,
+                             p.piece_ld);
       }
       if (dw) {
         ExpertArgs g = p.dw(q);

@@ -675,9 +675,9 @@ struct Pad {
 };
 
 // I: the index type; 32-bit quotients where all chunks are counted in 32 bits
-template <class I> APEXW_DEV void pad_rows(const Pad& p) {
-  const I per = (I)((p.width + 7) / 8), high = (I)p.high, n = (I)p.rows * per, stride = (I)gridDim.x * 256;
-  for (I i = (I)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
+template <class I> APEXW_DEV void pad_rows(const Pad& p, unsigned group, unsigned groups) {
+  const I per = (I)((p.width + 7) / 8), high = (I)p.high, n = (I)p.rows * per, stride = (I)groups * 256;
+  for (I i = (I)group * 256 + threadIdx.x; i < n; i += stride) {
     const I row = i / per, c = i - row * per, group = row / high;
     p.dst[i] = load_chunk(p.src + (int64_t)group * p.step + (int64_t)(row - group * high) * p.ld + (int64_t)c * 8,
                           clamp8(p.width - (int64_t)c * 8));
@@ -685,8 +685,8 @@ template <class I> APEXW_DEV void pad_rows(const Pad& p) {
 }
 __global__ __launch_bounds__(256) void pad_kernel(Pad a, Pad b) {
   const Pad& p = blockIdx.y ? b : a;
-  if (p.rows * ((p.width + 7) / 8) < (1ll << 31)) pad_rows<uint32_t>(p);
-  else pad_rows<uint64_t>(p);
+  if (p.rows * ((p.width + 7) / 8) < (1ll << 31)) pad_rows<uint32_t>(p, blockIdx.x, gridDim.x);
+  else pad_rows<uint64_t>(p, blockIdx.x, gridDim.x);
 }
 
 // the most elements from row to row: a stage's copies reach 256 rows by 32-bit byte offsets
