@@ -53,7 +53,7 @@ struct PackArgs {
   float *loss, *lse_out;      // forward: zeros for the rows that do not count
   void* dx;                   // the same, backward
   int64_t n, x_stride, w_stride, dloss_stride, ignore;
-  int32_t width, wide, vocab, id64, per, mean, rescale;
+  int32_t width, wide, vocab, id64, per, mean;
 };
 
 APEXW_DEV int64_t target_of(const PackArgs& a, int64_t i) {
@@ -86,7 +86,7 @@ template <int DT> __global__ __launch_bounds__(256) void head_pack_kernel(PackAr
   const bool last = (int)blockIdx.x == groups - 1;
   int before = 0;
   float most = 0.0f;
-  const bool find_most = last && a.rescale;
+  const bool find_most = last && a.dloss;
   constexpr int U = 16;   // loads in flight
   for (int64_t i0 = threadIdx.x; i0 < first; i0 += 256 * U) {
     int64_t t[U];
@@ -116,17 +116,17 @@ template <int DT> __global__ __launch_bounds__(256) void head_pack_kernel(PackAr
     if (a.lse_out) a.lse_out[mine] = 0.0f;
   }
   if (last) {
-    if (a.rescale) {
+    if (a.dloss) {
       if (has) most = fmaxf(most, fabsf(a.dloss[mine * a.dloss_stride]));
       most = over_workgroup(most, floats, [](float p, float q) { return fmaxf(p, q); });
     }
     if (threadIdx.x == 0) {
-      // the largest factor of a row, as a power of two: divided out of G, which fp16 would lose below 2^-24, and
-      // multiplied into the sums
+      // The largest dloss is divided out of G and multiplied into the sums: a row that is far from its target then has
+      // -1 there, which no rounding changes (where all rows have one dloss, its own rounding would be every row's), and
+      // fp16 loses nothing below 2^-24.
       const float mean = a.mean && all > 0 ? 1.0f / (float)all : 1.0f;
-      const uint32_t bits = __float_as_uint(most * mean) & 0x7F800000u;
-      const bool use = a.rescale && bits >= 0x01000000u && bits < 0x7E800000u;
-      const float scale = use ? __uint_as_float(bits) : 1.0f, factor = mean / scale;
+      const bool use = most >= 0x1p-120f && most < 0x1p120f;
+      const float factor = use ? 1.0f / most : 1.0f, scale = use ? most * mean : mean;
       *a.state = HeadState{all, factor, log2f(factor), scale};
     }
   }
@@ -791,7 +791,7 @@ extern "C" int apexw_linear_cross_entropy_backward(const float* dloss, int64_t d
   PackArgs pack{};
   pack.x = (const uint16_t*)x, pack.x_stride = x_stride, pack.target = target, pack.id64 = id_bytes == 8;
   pack.ignore = ignore_index, pack.lse = lse, pack.dloss = dloss, pack.dloss_stride = dloss_stride, pack.dx = dx;
-  pack.mean = mean != 0, pack.rescale = dtype == APEXW_F16;
+  pack.mean = mean != 0;
   by_half(dtype, [&](auto d) {
     constexpr int DT = decltype(d)::value;
     const uint16_t* w = launch_pack<DT>(p, pack, weight, w_stride, ws, s);
