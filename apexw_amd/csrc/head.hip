@@ -71,8 +71,8 @@ template <class T, class F> APEXW_DEV T over_workgroup(T x, T* lds, F&& f) {
   return x;
 }
 
-// A workgroup has `per` (up to 256) rows; how many rows before them count it finds by itself.  A wave takes a row at a
-// time: copies it, and forms its target's logit on the way.
+// A workgroup has `per` rows, 256 at a time; how many rows before them count it finds by itself.  A wave takes a row at
+// a time: copies it, and forms its target's logit on the way.
 template <int DT> __global__ __launch_bounds__(256) void head_pack_kernel(PackArgs a, Pad weights, int groups) {
   if ((int)blockIdx.x >= groups) {   // the weights, copied to whole chunks
     if (weights.rows * ((weights.width + 7) / 8) < (1ll << 31)) pad_rows<uint32_t>(weights, blockIdx.x - groups, gridDim.x - groups);
@@ -101,73 +101,75 @@ template <int DT> __global__ __launch_bounds__(256) void head_pack_kernel(PackAr
   }
   before = over_workgroup(before, ints, [](int p, int q) { return p + q; });
 
-  const int64_t mine = first + threadIdx.x;
-  const bool has = mine < end && counts(a, target_of(a, mine));
-  const uint64_t ballot = __ballot(has);
-  if (lane_id() == 0) ints[threadIdx.x >> 6] = __builtin_popcountll(ballot);
-  __syncthreads();
-  int at = before + __builtin_popcountll(ballot & ((1ull << lane_id()) - 1ull));
-  for (int w = 0; w < (int)(threadIdx.x >> 6); ++w) at += ints[w];
-  const int all = before + ints[0] + ints[1] + ints[2] + ints[3];
-  place[threadIdx.x] = has ? at : -1;
-  __syncthreads();
-  if (mine < end && !has) {
-    if (a.loss) a.loss[mine] = 0.0f;
-    if (a.lse_out) a.lse_out[mine] = 0.0f;
-  }
-  if (last) {
-    if (a.dloss) {
-      if (has) most = fmaxf(most, fabsf(a.dloss[mine * a.dloss_stride]));
-      most = over_workgroup(most, floats, [](float p, float q) { return fmaxf(p, q); });
+  for (int64_t from = first; from == first || from < end; from += 256) {
+    const int64_t to = from + 256 < end ? from + 256 : end;
+    const int64_t mine = from + threadIdx.x;
+    const bool has = mine < to && counts(a, target_of(a, mine));
+    const uint64_t ballot = __ballot(has);
+    if (lane_id() == 0) ints[threadIdx.x >> 6] = __builtin_popcountll(ballot);
+    __syncthreads();
+    int at = before + __builtin_popcountll(ballot & ((1ull << lane_id()) - 1ull));
+    for (int w = 0; w < (int)(threadIdx.x >> 6); ++w) at += ints[w];
+    const int all = before + ints[0] + ints[1] + ints[2] + ints[3];
+    place[threadIdx.x] = has ? at : -1;
+    __syncthreads();
+    if (mine < to && !has) {
+      if (a.loss) a.loss[mine] = 0.0f;
+      if (a.lse_out) a.lse_out[mine] = 0.0f;
     }
-    if (threadIdx.x == 0) {
-      // The largest dloss is divided out of G and multiplied into the sums: a row that is far from its target then has
-      // -1 there, which no rounding changes (where all rows have one dloss, its own rounding would be every row's), and
-      // fp16 loses nothing below 2^-24.
-      const float mean = a.mean && all > 0 ? 1.0f / (float)all : 1.0f;
-      const bool use = most >= 0x1p-120f && most < 0x1p120f;
-      const float factor = use ? 1.0f / most : 1.0f, scale = use ? most * mean : mean;
-      *a.state = HeadState{all, factor, log2f(factor), scale};
+    if (last && a.dloss && has) most = fmaxf(most, fabsf(a.dloss[mine * a.dloss_stride]));
+    if (last && to == end) {
+      if (a.dloss) most = over_workgroup(most, floats, [](float p, float q) { return fmaxf(p, q); });
+      if (threadIdx.x == 0) {
+        // The largest dloss is divided out of G and multiplied into the sums: a row that is far from its target then has
+        // -1 there, which no rounding changes (where all rows have one dloss, its own rounding would be every row's), and
+        // fp16 loses nothing below 2^-24.
+        const float mean = a.mean && all > 0 ? 1.0f / (float)all : 1.0f;
+        const bool use = most >= 0x1p-120f && most < 0x1p120f;
+        const float factor = use ? 1.0f / most : 1.0f, scale = use ? most * mean : mean;
+        *a.state = HeadState{all, factor, log2f(factor), scale};
+      }
     }
-  }
 
-  const int chunks = a.wide / 8, rows = (int)(end - first), lane = lane_id();
-  for (int r = threadIdx.x >> 6; r < rows; r += 4) {
-    const int64_t i = first + r;
-    const int p = uniform(place[r]);
-    if (p < 0) {
-      if (!a.dx) continue;
-      uint16_t* to = (uint16_t*)a.dx + i * a.width;
+    const int chunks = a.wide / 8, rows = (int)(to - from), lane = lane_id();
+    for (int r = threadIdx.x >> 6; r < rows; r += 4) {
+      const int64_t i = from + r;
+      const int p = uniform(place[r]);
+      if (p < 0) {
+        if (!a.dx) continue;
+        uint16_t* dx = (uint16_t*)a.dx + i * a.width;
+        for (int c = lane; c < chunks; c += 64) {
+          const int n = clamp8(a.width - c * 8);
+          if (n == 8) APEXW_GLOBAL(Chunk, dx + c * 8)->v = u32x4{0u, 0u, 0u, 0u};
+          else for (int j = 0; j < n; ++j) APEXW_GLOBAL(uint16_t, dx)[c * 8 + j] = 0;
+        }
+        continue;
+      }
+      const int target = (int)target_of(a, i);
+      const uint16_t *x = a.x + i * a.x_stride, *w = a.w + target * a.w_stride;
+      float dot = 0.0f;
+#pragma unroll 4
       for (int c = lane; c < chunks; c += 64) {
         const int n = clamp8(a.width - c * 8);
-        if (n == 8) APEXW_GLOBAL(Chunk, to + c * 8)->v = u32x4{0u, 0u, 0u, 0u};
-        else for (int j = 0; j < n; ++j) APEXW_GLOBAL(uint16_t, to)[c * 8 + j] = 0;
-      }
-      continue;
-    }
-    const int target = (int)target_of(a, i);
-    const uint16_t *x = a.x + i * a.x_stride, *w = a.w + target * a.w_stride;
-    float dot = 0.0f;
-#pragma unroll 4
-    for (int c = lane; c < chunks; c += 64) {
-      const int n = clamp8(a.width - c * 8);
-      const u32x4 xv = load_chunk(x + c * 8, n), wv = load_chunk(w + c * 8, n);
-      *(u32x4*)&a.packed[(int64_t)p * a.wide + c * 8] = xv;
-      float xs[8], ws[8];
-      values<DT>(xv, xs), values<DT>(wv, ws);
+        const u32x4 xv = load_chunk(x + c * 8, n), wv = load_chunk(w + c * 8, n);
+        *(u32x4*)&a.packed[(int64_t)p * a.wide + c * 8] = xv;
+        float xs[8], ws[8];
+        values<DT>(xv, xs), values<DT>(wv, ws);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) dot = fmaf(xs[j], ws[j], dot);
+        for (int j = 0; j < 8; ++j) dot = fmaf(xs[j], ws[j], dot);
+      }
+      dot = wave_sum(dot);
+      if (lane) continue;
+      HeadRow row{dot * kLog2E, 0.0f, 0.0f, target, (int32_t)i};
+      float shift = row.logit - row.logit == 0.0f ? row.logit : 0.0f;
+      if (a.lse) {
+        row.lse = a.lse[i] * kLog2E, row.d = a.dloss[i * a.dloss_stride];
+        const uint32_t bits = __float_as_uint(log2f(fabsf(row.d)) - row.lse);
+        shift = __uint_as_float((bits & ~1u) | (row.d < 0.0f));
+      }
+      a.rows[p] = row, a.shift[p] = shift;
     }
-    dot = wave_sum(dot);
-    if (lane) continue;
-    HeadRow row{dot * kLog2E, 0.0f, 0.0f, target, (int32_t)i};
-    float shift = row.logit - row.logit == 0.0f ? row.logit : 0.0f;
-    if (a.lse) {
-      row.lse = a.lse[i] * kLog2E, row.d = a.dloss[i * a.dloss_stride];
-      const uint32_t bits = __float_as_uint(log2f(fabsf(row.d)) - row.lse);
-      shift = __uint_as_float((bits & ~1u) | (row.d < 0.0f));
-    }
-    a.rows[p] = row, a.shift[p] = shift;
+    before = all;
   }
 }
 
@@ -653,7 +655,8 @@ static_assert(Large::WN == 64 && Wide::WN == 64 && Mid::WN == 64 && Small::BM ==
 bool head_ok(int64_t n, int64_t width, int64_t vocab) {
   return n >= 0 && n <= INT32_MAX - 65536 && width > 0 && width <= kMostLd && vocab > 0 && vocab <= INT32_MAX - 65536;
 }
-bool head_fits(const HeadPlan& p) { return rows_tiles<Small>(p.args(p.vocab)) <= INT32_MAX; }
+// (the join's 1024 threads for 16 rows are fewer than 2^32)
+bool head_fits(const HeadPlan& p) { return p.n < 1ll << 26 && rows_tiles<Small>(p.args(p.vocab)) <= INT32_MAX; }
 
 template <class S, int DT, class Out> void launch_logits_shape(const ExpertArgs& g, const Out& out, hipStream_t s) {
   hipLaunchKernelGGL((head_logits_kernel<S, DT, Out>), dim3(stream_grid<S>(rows_tiles<S>(g))), dim3(S::kThreads), 0, s, g, out);
@@ -709,7 +712,7 @@ template <int DT> const uint16_t* launch_pack(const HeadPlan& p, PackArgs& a, co
   a.n = p.n, a.width = (int32_t)p.width, a.wide = (int32_t)p.wide, a.vocab = (int32_t)p.vocab;
   // about 1024 workgroups, of at least 4 rows
   const int64_t per = (p.n + 1023) / 1024;
-  a.per = (int32_t)(per < 4 ? 4 : per > 256 ? 256 : per);
+  a.per = (int32_t)(per < 4 ? 4 : per);
   const int groups = p.n ? (int)((p.n + a.per - 1) / a.per) : 1;
   const uint16_t* from = (const uint16_t*)w;
   Pad weights{};
@@ -735,7 +738,8 @@ template <class F> void by_half(int32_t dtype, F&& f) {
 extern "C" int64_t apexw_linear_cross_entropy_workspace(const void* weight, int64_t w_stride, int64_t n, int64_t width,
                                                         int64_t vocab, int32_t backward) {
   if (!head_ok(n, width, vocab)) return -APEXW_ERR_ARG;
-  return HeadPlan(weight, w_stride, n, width, vocab, backward != 0, backward & 1, backward & 2).bytes;
+  const HeadPlan p(weight, w_stride, n, width, vocab, backward != 0, backward & 1, backward & 2);
+  return head_fits(p) ? p.bytes : -APEXW_ERR_SIZE;
 }
 
 extern "C" int apexw_linear_cross_entropy_forward(const void* x, int64_t x_stride, int64_t n, int64_t width,

@@ -16,6 +16,7 @@
 #include <Python.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <cstdint>
 #include <cstring>
@@ -716,7 +717,7 @@ PyObject* embedding_forward(PyObject*, PyObject* const* args, Py_ssize_t nargs) 
   if (PyErr_Occurred()) return nullptr;
   uint32_t code;
   int32_t bytes;
-  if (!ids_of(ids, where, &bytes) || !matrix(w, where, &code) || w.size(0) == 0 || !std::isfinite(scale)) return none_or_error();
+  if (!ids_of(ids, where, &bytes) || !matrix(w, where, &code) || w.size(0) == 0 || !(std::fabs(scale) <= FLT_MAX)) return none_or_error();
   std::vector<int64_t> shape(ids.sizes().begin(), ids.sizes().end());
   shape.push_back(w.size(1));
   const at::Tensor out = at::empty(shape, w.options());
@@ -739,7 +740,7 @@ PyObject* embedding_weight_grad(PyObject*, PyObject* const* args, Py_ssize_t nar
   uint32_t code;
   int32_t bytes;
   if (!ids_of(ids, where, &bytes) || !where.has(dy) || !dtype_code(dy, &code) || dy.dim() != ids.dim() + 1 || !dy.is_contiguous() ||
-      dy.numel() == 0 || dy.sizes().slice(0, ids.dim()) != ids.sizes() || vocab < 1 || vocab >= INT32_MAX || !std::isfinite(scale))
+      dy.numel() == 0 || dy.sizes().slice(0, ids.dim()) != ids.sizes() || vocab < 1 || vocab >= INT32_MAX || !(std::fabs(scale) <= FLT_MAX))
     return none_or_error();
   const int64_t n = ids.numel(), width = dy.size(-1), need = lib.embedding_grad_workspace(n, vocab, width);
   if (need < 0) return PyLong_FromLong(static_cast<long>(-need));

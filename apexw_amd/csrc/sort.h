@@ -1,10 +1,16 @@
 // A stable sort of small integers by digits, for ids of experts and of words (gfx950).
 //
 // Items are given as ids; an id outside [0, limit) has the key `limit`, behind all others.  Each pass orders by one digit
-// of up to 9 bits: a launch that counts each workgroup's digits and one that places its items, where a workgroup adds up
-// the counts of those before it by itself (64 workgroups' counts are 128 KB, read from L2) so that no launch in between
-// scans them.  Up to 128 K items go in workgroups of 1024 (16384 ids in two passes 34 us by 4096, 21 by 1024).  The rank of an item among its wave's is counted from ballots of the digit's bits, so equal keys keep
-// their order and equal calls give equal results.  Up to kSmall items go through all passes in one workgroup's LDS.
+// of up to 9 bits: a launch that counts each workgroup's digits and one that places its items.  There a workgroup adds up
+// the counts of those before it by itself (64 workgroups' counts are 128 KB, read from L2), or, where more than kScan
+// workgroups would each read that many, a launch in between does (8 M items of 64 experts 318 us without it, 82 with; at
+// 800000 23 and 18, at 65536 the launch costs as much as it saves).  Up to 512 K items go in workgroups of 1024, more in
+// workgroups of 4096 (262144 ids of 50000, two passes, 36 us by 1024, 47 by 4096; 800000 67 and 64).  The rank of an item
+// among its wave's is counted from ballots of the digit's bits, so equal keys keep their order and equal calls give equal
+// results.  Up to kSmall items go through all passes in one workgroup's LDS.
+//
+// What bounds it is the chain of launches and, in each, of dependent accesses: 16384 ids in two passes take 18 us, the
+// counts' launches 3 to 4 and the places' 5.5 each, for 0.5 MB that they move.
 #pragma once
 
 #include "common.h"
@@ -14,6 +20,7 @@ namespace {
 constexpr int kDigits = 512, kSortThreads = 512, kSortWaves = kSortThreads / 64;
 constexpr int kFew = 2, kMost = 8;               // items of a thread
 constexpr int kSmall = kSortThreads * kMost;     // items of one workgroup
+constexpr int kScan = 64;
 
 struct SortArgs {
   const void* ids;        // int32 or int64
@@ -23,7 +30,7 @@ struct SortArgs {
   int32_t bits, passes;   // of a digit
   u32x2* from;            // (key, item) of a pass after the first
   u32x2* to;
-  uint32_t* counts;       // [workgroup][digit]
+  uint32_t* counts;       // [workgroup][digit]; where there are more than kScan: of those before, and of all behind them
   u32x4* clear;           // cleared on the way
   int64_t clears;
   int32_t *source, *place, *ends;   // of the last pass for experts
@@ -115,6 +122,8 @@ APEXW_DEV void sort_pass(const SortArgs& a, SortLds& l, int pass, int first, int
     }
     if (kAlone) {
       all = mine;
+    } else if (gridDim.x > kScan) {
+      before = a.counts[(int64_t)blockIdx.x * digits + d], all = a.counts[(int64_t)gridDim.x * digits + d];
     } else {
       constexpr int U = 16;   // loads in flight
       for (int b0 = 0; b0 < (int)gridDim.x; b0 += U) {
@@ -158,6 +167,38 @@ template <bool kFirst, int kItems> __global__ __launch_bounds__(kSortThreads) vo
   }
   __syncthreads();
   for (int i = threadIdx.x; i < digits; i += kSortThreads) a.counts[(int64_t)blockIdx.x * digits + i] = cnt[i];
+}
+
+// The counts of many workgroups added up: a lane has a digit, a wave a 16th of the workgroups
+__global__ __launch_bounds__(1024) void sort_scan_kernel(uint32_t* counts, int groups, int digits) {
+  __shared__ uint32_t sums[16][64];
+  const int wave = threadIdx.x >> 6, lane = lane_id(), d = blockIdx.x * 64 + lane;
+  const int len = (groups + 15) / 16, g0 = wave * len, g1 = g0 + len < groups ? g0 + len : groups;
+  constexpr int U = 16;   // loads in flight
+  uint32_t* at = counts + d;
+  uint32_t sum = 0u;
+  if (d < digits)
+    for (int g = g0; g < g1; g += U) {
+      uint32_t c[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) c[u] = g + u < g1 ? at[(int64_t)(g + u) * digits] : 0u;
+#pragma unroll
+      for (int u = 0; u < U; ++u) sum += c[u];
+    }
+  sums[wave][lane] = sum;
+  __syncthreads();
+  if (d >= digits) return;
+  uint32_t before = 0u;
+  for (int w = 0; w < wave; ++w) before += sums[w][lane];
+  if (wave == 15) at[(int64_t)groups * digits] = before + sum;
+  for (int g = g0; g < g1; g += U) {
+    uint32_t c[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) c[u] = g + u < g1 ? at[(int64_t)(g + u) * digits] : 0u;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (g + u < g1) at[(int64_t)(g + u) * digits] = before, before += c[u];
+  }
 }
 
 // where the last pass puts an item for experts
@@ -209,7 +250,7 @@ inline void sort_digits(SortArgs& a) {
   a.bits = (bits + a.passes - 1) / a.passes;
 }
 // items of a thread, workgroups of a pass
-inline int sort_items(int64_t n) { return n <= 128 * kSortThreads * kFew ? kFew : kMost; }
+inline int sort_items(int64_t n) { return n <= 512 * kSortThreads * kFew ? kFew : kMost; }
 inline int sort_groups(int64_t n) {
   const int64_t per = kSortThreads * sort_items(n);
   return (int)((n + per - 1) / per);

@@ -41,6 +41,13 @@ __global__ __launch_bounds__(256) void order_ends_kernel(const u32x2* __restrict
 // Dispatch and combine
 // ---------------------------------------------------------------------------
 
+// A grid's first dimension times 256 threads has to stay below 2^32, so many workgroups go along two
+constexpr int64_t kAcross = 1 << 20;
+APEXW_DEV int64_t group_of() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+dim3 groups_grid(int64_t groups) {
+  return dim3((unsigned)(groups < kAcross ? groups : kAcross), (unsigned)((groups + kAcross - 1) / kAcross));
+}
+
 // T threads (a power of two, up to 256) share a token
 struct TokenArgs {
   const void *x, *y;           // rows by token, rows by expert
@@ -58,7 +65,7 @@ struct Token {
   int lane, step;
   bool here;
   __device__ __forceinline__ explicit Token(const TokenArgs& a)
-      : t((int64_t)blockIdx.x * (kWG >> a.log_t) + (threadIdx.x >> a.log_t)), lane(threadIdx.x & ((1 << a.log_t) - 1)),
+      : t(group_of() * (kWG >> a.log_t) + (threadIdx.x >> a.log_t)), lane(threadIdx.x & ((1 << a.log_t) - 1)),
         step(1 << a.log_t), here(t < a.tokens) {}
 };
 APEXW_DEV int64_t row_of(const TokenArgs& a, int64_t choice) {   // -1 for any place that is no row
@@ -228,7 +235,7 @@ template <int DT> APEXW_DEV u32x4 scaled(u32x4 w, float scale) {
 }
 
 template <int DT> __global__ __launch_bounds__(kWG) void embedding_kernel(EmbeddingArgs a) {
-  const int64_t t = (int64_t)blockIdx.x * (kWG >> a.log_t) + (threadIdx.x >> a.log_t);
+  const int64_t t = group_of() * (kWG >> a.log_t) + (threadIdx.x >> a.log_t);
   if (t >= a.n) return;
   const RowChunks<DT> row(a.width);
   const int step = 1 << a.log_t, lane = threadIdx.x & (step - 1);
@@ -497,7 +504,7 @@ struct SortSpace {
   int64_t counts, pairs, bytes;
   SortSpace(const SortArgs& a, bool wanted) {
     const bool small = a.n <= kSmall;
-    counts = small ? 0 : aligned(((int64_t)sort_groups(a.n) << a.bits) * 4);
+    counts = small ? 0 : aligned(((int64_t)(sort_groups(a.n) + 1) << a.bits) * 4);
     pairs = aligned((int64_t)a.n * 8);
     const int lists = (wanted ? 1 : 0) + (small ? 0 : a.passes - 1 < 2 ? a.passes - 1 : 2);
     bytes = counts + pairs * (lists > 2 ? 2 : lists);
@@ -522,6 +529,8 @@ template <bool kOrder, int kItems> const u32x2* launch_passes(SortArgs a, const 
     a.to = last && !wanted ? nullptr : lists[pass & 1];
     if (pass == 0) hipLaunchKernelGGL((sort_count_kernel<true, kItems>), grid, block, 0, s, a, pass);
     else hipLaunchKernelGGL((sort_count_kernel<false, kItems>), grid, block, 0, s, a, pass);
+    if (grid.x > kScan)
+      hipLaunchKernelGGL(sort_scan_kernel, dim3((unsigned)((1 << a.bits) + 63) / 64), dim3(1024), 0, s, a.counts, (int)grid.x, 1 << a.bits);
     if (kOrder && last) {
       if (pass == 0) hipLaunchKernelGGL((sort_place_kernel<true, kOrder, kItems>), grid, block, 0, s, a, pass);
       else hipLaunchKernelGGL((sort_place_kernel<false, kOrder, kItems>), grid, block, 0, s, a, pass);
@@ -551,7 +560,7 @@ TokenArgs token_args(int64_t tokens, int32_t k, int64_t width, int32_t dtype, co
 }
 dim3 token_grid(const TokenArgs& a) {
   const int64_t per = kWG >> a.log_t;
-  return dim3((unsigned)((a.tokens + per - 1) / per));
+  return groups_grid((a.tokens + per - 1) / per);
 }
 bool tokens_ok(int64_t tokens, int32_t k, int64_t width) {
   return tokens >= 0 && k > 0 && rows_ok(tokens, width) && tokens <= (INT32_MAX - 65536) / k;
@@ -570,6 +579,9 @@ template <class F> int by_types(int32_t dtype, int32_t w_dtype, F&& f) {
 
 // Up to this many tokens no row of the gradient sums enough to be worth the launch that finds the ids of many
 constexpr int64_t kFewTokens = 256;
+
+// Rows of a gradient: 64 to a workgroup of 256 threads, fewer than 2^32 in all
+constexpr int64_t kMostWords = 1 << 29;
 
 struct GradPlan {
   SortArgs sort;
@@ -690,14 +702,14 @@ extern "C" int apexw_embedding_forward(const void* ids, int32_t id_bytes, int64_
   const int64_t per = kWG >> a.log_t;
   const bool ok = by_row_type(dtype, [&](auto d) {
     if (n > 0)
-      hipLaunchKernelGGL(embedding_kernel<decltype(d)::value>, dim3((unsigned)((n + per - 1) / per)), dim3(kWG), 0,
-                         (hipStream_t)stream, a);
+      hipLaunchKernelGGL(embedding_kernel<decltype(d)::value>, groups_grid((n + per - 1) / per), dim3(kWG), 0, (hipStream_t)stream, a);
   });
   return ok ? launched() : APEXW_ERR_DTYPE;
 }
 
 extern "C" int64_t apexw_embedding_weight_grad_workspace(int64_t n, int64_t vocab, int64_t width) {
   if (!rows_ok(n, width) || vocab <= 0 || vocab > INT32_MAX - 1) return -APEXW_ERR_ARG;
+  if (vocab > kMostWords) return -APEXW_ERR_SIZE;
   return GradPlan(nullptr, 4, n, (uint32_t)vocab, width).bytes;
 }
 
@@ -710,6 +722,7 @@ extern "C" int apexw_embedding_weight_grad(const void* dy, int64_t dy_stride, co
   if (row_misaligned(dy, dtype) || row_misaligned(dw, dw_dtype) || ((uintptr_t)ids & (id_bytes - 1)) ||
       ((uintptr_t)workspace & 15u))
     return APEXW_ERR_ALIGN;
+  if (vocab > kMostWords) return APEXW_ERR_SIZE;
   const GradPlan plan(ids, id_bytes, n, (uint32_t)vocab, width);
   hipStream_t s = (hipStream_t)stream;
   char* ws = (char*)workspace;

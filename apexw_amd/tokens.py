@@ -9,7 +9,6 @@ there; nothing is read back on the host.  Sums are taken in fp32 in a fixed orde
 What they do not support raises before anything is launched.
 """
 
-import math
 from typing import NamedTuple
 
 import torch
@@ -233,8 +232,8 @@ def expert_combine(y, order, weight=None):
 
 # ---------------------------------------------------------------------------- embedding
 def _check_scale(scale):
-    if not math.isfinite(scale):
-        raise ValueError(f"embedding: expected a finite scale, got {scale}")
+    if not abs(scale) <= torch.finfo(torch.float32).max:
+        raise ValueError(f"embedding: expected a scale that float32 holds, got {scale}")
 
 
 def embedding_forward(ids, weight, scale=1.0):

@@ -914,7 +914,8 @@ int apexw_expert_combine_backward(const void* dout, int64_t dout_stride, const v
 /*
  * Embedding: out[t] = scale weight[ids[t]] (contiguous rows of `width`), zeros for an id outside [0, vocab); its
  * gradient dw[v] = scale (sum of dy[t] over ids[t] = v), [vocab x width] contiguous, dtype or F32, zeros for an id that
- * no token has.  The sum is in fp32 in an order that the ids alone set.  workspace as above.
+ * no token has.  The sum is in fp32 in an order that the ids alone set.  workspace as above.  APEXW_ERR_SIZE: a
+ * gradient of more than 2^29 rows.
  */
 int apexw_embedding_forward(const void* ids, int32_t id_bytes, int64_t n, const void* weight, int64_t w_stride,
                             int64_t vocab, int64_t width, int32_t dtype, float scale, void* out, void* stream);
@@ -934,7 +935,7 @@ int apexw_embedding_weight_grad(const void* dy, int64_t dy_stride, const void* i
  * backward: dloss_stride 0 is one number for all rows; mean != 0 divides it by the number of rows that count; dx
  * ([n x width]) and dw ([vocab x width], both contiguous) may be NULL.
  * workspace (16-byte aligned, in any state): as many bytes as the _workspace call answers; backward: 0, or bits 0 and 1
- * for dx and dw.  Equal calls give equal bits.
+ * for dx and dw.  Equal calls give equal bits.  APEXW_ERR_SIZE: 2^26 rows or more, or more tiles than a launch holds.
  */
 int64_t apexw_linear_cross_entropy_workspace(const void* weight, int64_t w_stride, int64_t n, int64_t width, int64_t vocab,
                                              int32_t backward);

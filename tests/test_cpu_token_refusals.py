@@ -136,3 +136,14 @@ def test_entry_points_refuse_without_launching():
                            ({"d": ok + 2}, 4), ({"dx": None, "dw": None}, 0)):
         assert back(*{**call, **change}.values()) == status, change
     assert space(ok, 8, 4, 0, 10, 0) == -1 and space(ok, 8, 400, 8, 1000, 3) > space(ok, 8, 400, 8, 1000, 0) > 0
+
+
+def test_sizes_that_no_launch_holds():
+    lib = _lib.load()
+    assert lib.apexw_embedding_weight_grad_workspace(5, 2 ** 29, 1) > 0
+    assert lib.apexw_embedding_weight_grad_workspace(5, 2 ** 29 + 1, 1) == -_lib.ERR_SIZE
+    ok = 2 ** 40
+    assert lib.apexw_embedding_weight_grad(ok, 8, ok, 8, 4, 2 ** 30, 8, 1, 1.0, ok, 1, ok, None) == _lib.ERR_SIZE
+    space = lib.apexw_linear_cross_entropy_workspace
+    assert space(ok, 8, 2 ** 26 - 1, 8, 1000, 0) > 0 and space(ok, 8, 2 ** 26, 8, 1000, 0) == -_lib.ERR_SIZE
+    assert space(ok, 8, 2 ** 25, 8, 2 ** 30, 3) == -_lib.ERR_SIZE
