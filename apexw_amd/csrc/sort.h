@@ -31,7 +31,7 @@ struct SortArgs {
   u32x2* from;            // (key, item) of a pass after the first
   u32x2* to;
   uint32_t* counts;       // [workgroup][digit]; where there are more than kScan: of those before, and of all behind them
-  u32x4* clear;           // cleared on the way
+  char* clear;            // cleared on the way, an even number of bytes
   int64_t clears;
   int32_t *source, *place, *ends;   // of the last pass for experts
 };
@@ -147,8 +147,19 @@ APEXW_DEV void sort_pass(const SortArgs& a, SortLds& l, int pass, int first, int
     if (r < rounds && base + r * 64 < a.n) put(item[r], l.cnt[wave][item[r][0] >> shift & low] + rank[r]);
 }
 
+// kClear bytes in a row at a time (the last chunk overlaps the one before)
+constexpr int64_t kClear = 4 * kSortThreads * 16;
 APEXW_DEV void sort_clear(const SortArgs& a, int64_t group, int64_t groups) {
-  for (int64_t i = group * kSortThreads + threadIdx.x; i < a.clears; i += groups * kSortThreads) a.clear[i] = u32x4{0u, 0u, 0u, 0u};
+  struct __attribute__((packed, aligned(2))) Chunk2 { u32x4 v; };
+  const int64_t last = a.clears - 16;
+  for (int64_t from = group * kClear; from < a.clears; from += groups * kClear)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t at = from + (i * kSortThreads + threadIdx.x) * 16;
+      if (at >= a.clears) break;
+      if (last >= 0) APEXW_GLOBAL(Chunk2, a.clear + (at < last ? at : last))->v = u32x4{0u, 0u, 0u, 0u};
+      else for (int64_t j = 0; j < a.clears; j += 2) *APEXW_GLOBAL(uint16_t, a.clear + j) = 0;
+    }
 }
 
 // The counts of each workgroup's digits

@@ -372,69 +372,79 @@ template <int DT> APEXW_DEV void add_range(const EmbeddingArgs& a, const RowChun
   rows(b1 << a.log_block, hi);
 }
 
-// The number of sorted keys below `key`
-APEXW_DEV int keys_below(const u32x2* sorted, int n, uint32_t key) {
-  int lo = 0, hi = n;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (sorted[mid][0] < key) lo = mid + 1;
-    else hi = mid;
+// A row of the gradient, chunk c
+template <int DT, int OD> APEXW_DEV void write_sum(const EmbeddingArgs& a, const RowChunks<DT>& row, int64_t v, int c, float (&sum)[kVec<DT>]) {
+  constexpr int V = kVec<DT>;
+  if (c >= row.count) return;
+#pragma unroll
+  for (int i = 0; i < V; ++i) sum[i] *= a.scale;
+  if constexpr (OD == DT) {
+    row.store(row_at<OD>(a.out, v * a.width), c, rounded<DT>(sum));
+  } else {
+    const int at = row.begin(c);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const u32x4 w = {__float_as_uint(sum[4 * q]), __float_as_uint(sum[4 * q + 1]), __float_as_uint(sum[4 * q + 2]),
+                       __float_as_uint(sum[4 * q + 3])};
+      if (a.width >= V) chunk_to<OD>(a.out, v * a.width + at + 4 * q, w);
+      else part_to<OD>(a.out, v * a.width + 4 * q, a.width - 4 * q, w);
+    }
   }
-  return lo;
+}
+
+// Few tokens, whose sort clears the gradient beside it: a workgroup has 64 chunks of columns of the id that a token is
+// the first one of, a part of its tokens a wave.  (50257 x 768 bf16, 1 to 1024 tokens 16 to 18 us, by the other kernels
+// 25 to 32; 2048 tokens 25 and 33, but 87 and 35 where all are of one id.)
+constexpr int kFewTokens = 1024;
+template <int DT, int OD> __global__ __launch_bounds__(kWG) void embedding_few_kernel(EmbeddingArgs a) {
+  constexpr int V = kVec<DT>;
+  __shared__ float lds[4][64][V];
+  const int lo = blockIdx.x, n = (int)a.n;
+  const uint32_t key = a.sorted[lo][0];
+  if (key >= a.vocab || (lo > 0 && a.sorted[lo - 1][0] == key)) return;
+  int hi = lo;
+  for (int i = lo; i < n; i += kWG) {
+    const int more = __syncthreads_count(i + (int)threadIdx.x < n && a.sorted[i + threadIdx.x][0] == key);
+    hi += more;
+    if (more < kWG) break;
+  }
+  const RowChunks<DT> row(a.width);
+  const int c = blockIdx.y * 64 + lane_id();
+  float sum[V] = {};
+  const Part p(lo, hi, threadIdx.x >> 6);
+  add_rows<DT, 16>(a, row, c, p.from, p.to, sum);
+  join_waves<V>(sum, lds);
+  if (threadIdx.x < 64) write_sum<DT, OD>(a, row, key, c, sum);
 }
 
 // The gradient's rows: up to 64 of them a workgroup, every (number of workgroups)th, so that frequent words, which have
 // neighbouring ids, go to different ones.  A row is taken 64 chunks of columns a wave, narrow rows several a wave.  The
 // first kManyGroups workgroups take the ids of many tokens, 64 chunks each, a part of the tokens a wave: one that met
 // such an id among its rows would end long after the others (65536 tokens, a tenth of them one id, 128256 x 4096: 511 us).
-// kSearch: few tokens, whose ranges are searched for here
-template <int DT, int OD, bool kSearch> __global__ __launch_bounds__(kWG) void embedding_grad_kernel(EmbeddingArgs a, int rows) {
+template <int DT, int OD> __global__ __launch_bounds__(kWG) void embedding_grad_kernel(EmbeddingArgs a, int rows) {
   constexpr int V = kVec<DT>;
   const RowChunks<DT> row(a.width);
   const int slabs = (row.count + 63) / 64, wave = uniform(threadIdx.x >> 6), lane = lane_id();
-  const auto write = [&](int64_t v, int c, float (&sum)[V]) {
-    if (c >= row.count) return;
-#pragma unroll
-    for (int i = 0; i < V; ++i) sum[i] *= a.scale;
-    if constexpr (OD == DT) {
-      row.store(row_at<OD>(a.out, v * a.width), c, rounded<DT>(sum));
-    } else {
-      const int at = row.begin(c);
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const u32x4 w = {__float_as_uint(sum[4 * q]), __float_as_uint(sum[4 * q + 1]), __float_as_uint(sum[4 * q + 2]),
-                         __float_as_uint(sum[4 * q + 3])};
-        if (a.width >= V) chunk_to<OD>(a.out, v * a.width + at + 4 * q, w);
-        else part_to<OD>(a.out, v * a.width + 4 * q, a.width - 4 * q, w);
-      }
+  const auto write = [&](int64_t v, int c, float (&sum)[V]) { write_sum<DT, OD>(a, row, v, c, sum); };
+  if (blockIdx.x < kManyGroups) {
+    __shared__ float lds[4][64][V];
+    const int64_t units = (int64_t)a.many[0] * slabs;
+    for (int64_t u = blockIdx.x; u < units; u += kManyGroups) {
+      const int64_t v = a.many[4 + u / slabs];
+      const int c = (int)(u % slabs) * 64 + lane;
+      float sum[V] = {};
+      add_range<DT>(a, row, c, a.ranges[2 * v], a.ranges[2 * v + 1], wave, 4, sum);
+      join_waves<V>(sum, lds);
+      if (wave == 0) write(v, c, sum);
     }
-  };
-  int first = 0;
-  if constexpr (!kSearch) {
-    first = kManyGroups;
-    if (blockIdx.x < kManyGroups) {
-      __shared__ float lds[4][64][V];
-      const int64_t units = (int64_t)a.many[0] * slabs;
-      for (int64_t u = blockIdx.x; u < units; u += kManyGroups) {
-        const int64_t v = a.many[4 + u / slabs];
-        const int c = (int)(u % slabs) * 64 + lane;
-        float sum[V] = {};
-        add_range<DT>(a, row, c, a.ranges[2 * v], a.ranges[2 * v + 1], wave, 4, sum);
-        join_waves<V>(sum, lds);
-        if (wave == 0) write(v, c, sum);
-      }
-      return;
-    }
+    return;
   }
   __shared__ int range[64][3];   // of a row: its tokens among the sorted, and the first one
-  const int64_t groups = gridDim.x - first, group = blockIdx.x - first;
+  const int64_t groups = gridDim.x - kManyGroups, group = blockIdx.x - kManyGroups;
   if ((int)threadIdx.x < rows) {
     const int64_t v = group + threadIdx.x * groups;
     int lo = 0, hi = 0;
-    if (v < a.vocab) {
-      if (kSearch) lo = keys_below(a.sorted, (int)a.n, (uint32_t)v), hi = keys_below(a.sorted, (int)a.n, (uint32_t)v + 1u);
-      else lo = a.ranges[2 * v], hi = a.ranges[2 * v + 1];
-    }
+    if (v < a.vocab) lo = a.ranges[2 * v], hi = a.ranges[2 * v + 1];
     range[threadIdx.x][0] = lo, range[threadIdx.x][1] = hi;
     range[threadIdx.x][2] = hi > lo ? (int)a.sorted[lo][1] : 0;
   }
@@ -453,7 +463,7 @@ template <int DT, int OD, bool kSearch> __global__ __launch_bounds__(kWG) void e
     for (int r = wave * per + (lane >> a.log_t); r < rows; r += 4 * per) {
       const int64_t v = group + r * groups;
       if (v >= a.vocab) break;
-      if (kSearch || range[r][1] - range[r][0] <= kMany) light(v, range[r][0], range[r][1], range[r][2], c);
+      if (range[r][1] - range[r][0] <= kMany) light(v, range[r][0], range[r][1], range[r][2], c);
     }
     return;
   }
@@ -463,7 +473,7 @@ template <int DT, int OD, bool kSearch> __global__ __launch_bounds__(kWG) void e
       const int64_t v = group + r * groups;
       if (v >= a.vocab) break;
       const int lo = range[r][0], hi = range[r][1];
-      if (!kSearch && hi - lo > kMany) continue;
+      if (hi - lo > kMany) continue;
       float sum[V] = {};
       if (hi > lo) add_range<DT>(a, row, c, lo, hi, 0, 1, sum);
       write(v, c, sum);
@@ -474,7 +484,7 @@ template <int DT, int OD, bool kSearch> __global__ __launch_bounds__(kWG) void e
     const int64_t v = group + r * groups;
     if (v >= a.vocab) break;
     const int lo = range[r][0], hi = range[r][1], token = uniform(range[r][2]);   // (scalar loads of the sorted are slower)
-    if (!kSearch && hi - lo > kMany) continue;
+    if (hi - lo > kMany) continue;
     int s = wave;
     for (; hi - lo <= 1 && s + 4 < slabs; s += 8) {   // two at once
       const int c0 = s * 64 + lane, c1 = c0 + 256;
@@ -577,11 +587,10 @@ template <class F> int by_types(int32_t dtype, int32_t w_dtype, F&& f) {
   return ok ? APEXW_OK : APEXW_ERR_DTYPE;
 }
 
-// Up to this many tokens no row of the gradient sums enough to be worth the launch that finds the ids of many
-constexpr int64_t kFewTokens = 256;
-
 // Rows of a gradient: 64 to a workgroup of 256 threads, fewer than 2^32 in all
 constexpr int64_t kMostWords = 1 << 29;
+
+constexpr int64_t kClears = 1 << 20;   // workgroups that clear, at most; 2048 take 226 us for 1 GB, one for each 32 KB 187
 
 struct GradPlan {
   SortArgs sort;
@@ -597,7 +606,6 @@ struct GradPlan {
     ranges = few ? 0 : aligned((int64_t)vocab * 8);
     blocks = few ? 0 : aligned((n >> log_block) * (width + 8) * 4);
     bytes = space.bytes + many + ranges + blocks;
-    if (few) log_block = 30;   // no blocks
   }
 };
 
@@ -734,7 +742,8 @@ extern "C" int apexw_embedding_weight_grad(const void* dy, int64_t dy_stride, co
   a.blocks = (float*)(ws + plan.space.bytes + plan.many + plan.ranges);
   const bool few = n <= kFewTokens;
   SortArgs sort = plan.sort;
-  sort.clear = (u32x4*)a.many, sort.clears = (plan.many + plan.ranges) / 16;
+  sort.clear = (char*)a.many, sort.clears = plan.many + plan.ranges;
+  if (few) sort.clear = (char*)dw, sort.clears = vocab * width * (dw_dtype == APEXW_F32 ? 4 : 2);
   // rows a workgroup: 2048 workgroups and more, of up to 64 rows
   const int rows = (int)(vocab < 4096 ? 1 : vocab / 2048 < 64 ? vocab / 2048 : 64);
   const unsigned groups = (unsigned)((vocab + rows - 1) / rows);
@@ -742,20 +751,20 @@ extern "C" int apexw_embedding_weight_grad(const void* dy, int64_t dy_stride, co
     constexpr int DT = decltype(d)::value, OD = decltype(o)::value;
     if (n <= kSmall) {
       a.sorted = sort.to = (u32x2*)ws;
-      const int64_t clears = (sort.clears + kSortThreads * 4 - 1) / (kSortThreads * 4);
-      if (n > 0)
-        hipLaunchKernelGGL(embedding_sort_kernel, dim3((unsigned)(1 + (clears < 512 ? clears : 512))), dim3(kSortThreads), 0, s, sort);
+      const int64_t clears = (sort.clears + kClear - 1) / kClear;
+      hipLaunchKernelGGL(embedding_sort_kernel, dim3((unsigned)(1 + (clears < kClears ? clears : kClears))), dim3(kSortThreads), 0, s, sort);
     } else {
       a.sorted = launch_sort<false>(sort, plan.space, true, ws, s);
     }
     if (few) {
-      hipLaunchKernelGGL((embedding_grad_kernel<DT, OD, true>), dim3(groups), dim3(kWG), 0, s, a, rows);
+      const dim3 grid((unsigned)n, (unsigned)((width + 64 * kVec<DT> - 1) / (64 * kVec<DT>)));
+      if (n > 0) hipLaunchKernelGGL((embedding_few_kernel<DT, OD>), grid, dim3(kWG), 0, s, a);
       return;
     }
     const int chunks = (int)((width + kVec<DT> - 1) / kVec<DT>);
     const unsigned blocks = (unsigned)((n + (1 << a.log_block) - 1) >> a.log_block);
     hipLaunchKernelGGL(embedding_blocks_kernel<DT>, dim3(blocks, (unsigned)((chunks + 63) / 64)), dim3(kWG), 0, s, a);
-    hipLaunchKernelGGL((embedding_grad_kernel<DT, OD, false>), dim3(groups + kManyGroups), dim3(kWG), 0, s, a, rows);
+    hipLaunchKernelGGL((embedding_grad_kernel<DT, OD>), dim3(groups + kManyGroups), dim3(kWG), 0, s, a, rows);
   });
   return st ? st : launched();
 }
