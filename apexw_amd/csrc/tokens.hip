@@ -138,11 +138,12 @@ template <int DT, int WD> __global__ __launch_bounds__(kWG) void combine_kernel(
   }
 }
 
-// x: the gradient of the combined rows
+// x: the gradient of the combined rows.  Two choices at a time: 4 take 102 registers, half of the waves (4097 x 1021 fp32, 3
+// choices, 34 us, by two 26)
 template <int DT, int WD> __global__ __launch_bounds__(kWG) void combine_backward_kernel(TokenArgs a) {
   const Token me(a);
   const RowChunks<DT> row(a.width);
-  constexpr int KU = 4, V = kVec<DT>;
+  constexpr int KU = 2, V = kVec<DT>;
   __shared__ float parts[kWG / 64][KU];
   const void* x = row_at<DT>(a.x, me.here ? me.t * a.x_stride : 0);
   for (int j0 = 0; j0 < a.k; j0 += KU) {
@@ -556,11 +557,14 @@ template <bool kOrder> const u32x2* launch_sort(const SortArgs& a, const SortSpa
   return launch_passes<kOrder, kMost>(a, space, wanted, ws, s);
 }
 
+// Threads of a row: a wave or less, or four where a row has a chunk for each of their threads.  (us with one and with
+// four, k choices, bf16: combine's gradient of 16384 x 768, k = 1, 16.1 and 31.5, 8192 x 1536, k = 2, 22 and 25, 8192 x 2048,
+// k = 8, 126 and 119; dispatch of 16384 x 768 10.2 and 15.6; combine of 8192 x 2048, k = 8, 76 and 59.)
 int log_threads(int64_t width, int32_t dtype, bool four_waves) {
   const int64_t chunks = (width + (dtype == APEXW_F32 ? 3 : 7)) / (dtype == APEXW_F32 ? 4 : 8);
   int log_t = 4;
-  while (log_t < (four_waves ? 8 : 6) && (1 << log_t) < chunks) ++log_t;
-  return log_t == 7 ? 8 : log_t;
+  while (log_t < 6 && (1 << log_t) < chunks) ++log_t;
+  return four_waves && chunks >= kWG ? 8 : log_t;
 }
 TokenArgs token_args(int64_t tokens, int32_t k, int64_t width, int32_t dtype, const int32_t* source, const int32_t* place) {
   TokenArgs a{};
