@@ -1,6 +1,6 @@
 """Each way that the cross entropy of a linear head may take -- the four tile shapes of the logits, forward and
-backward, the shapes and parts of the two products with the probabilities, one piece of the vocabulary and more, sums
-of pieces joined in the end or added as they come, weights copied to whole chunks -- at a size that takes it, against
+backward, the shapes and parts of the two products with the probabilities, one piece of the vocabulary and more,
+weights copied to whole chunks -- at a size that takes it, against
 float64 with the bars of test_gpu_linear_cross_entropy.  The kernels that ran are read from a profile, so a size that a
 changed rule sends elsewhere fails here."""
 
@@ -76,14 +76,14 @@ def test_way(what, rows, width, vocab, dtype, ignored):
     check(set(what.split()), rows, width, vocab, dtype, ignored)
 
 
-@pytest.mark.parametrize("rows,width,vocab,added", [(60000, 64, 20011, False), (100000, 1024, 30010, True)])
-def test_pieces(rows, width, vocab, added):
-    """Several pieces, their sums of dx joined in the end, or, where those would be many bytes, added."""
+@pytest.mark.parametrize("rows,width,vocab", [(60000, 64, 20011), (100000, 1024, 30010)])
+def test_pieces(rows, width, vocab):
+    """Several pieces, each of whose sums of dx is added to the ones before."""
     x, w, target = make(rows, width, vocab, BF16, 0.3)
     dloss = torch.full((rows,), 1.0 / rows, device="cuda")
     _, lse = apexw_amd.linear_cross_entropy_forward(x, w, target)
     (dx, dw), ways = taken(lambda: apexw_amd.linear_cross_entropy_backward(dloss, x, w, target, lse))
-    assert ("added" in ways) == added
+    assert "added" in ways
     # against the formula over some of the rows and of the vocabulary, with the bars of `check_backward`
     some = torch.randperm(rows, generator=torch.Generator().manual_seed(1))[:500].cuda()
     words = torch.cat([torch.arange(0, 300), torch.arange(vocab - 300, vocab)]).cuda()
