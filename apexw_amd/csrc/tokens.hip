@@ -9,6 +9,16 @@
 //
 // All of it is bound by memory.  Dispatch, combine and its gradient go token by token: a token's row is read (written)
 // once and its k rows by expert, whole, wherever they lie.
+//
+// Measured, kernels alone (a large copy: 4.7 TB/s):
+//   order and dispatch, 16384 tokens x 2 of 8 experts, 4096 bf16     4.7 + 5.1 and 66 us   6.1 TB/s
+//   the same, 16 x 2 of 64, 2048 bf16                                3.7 and 3.6 us
+//   combine, 8192 tokens x 8, 2048 bf16                              59 us   5.1 TB/s
+//   combine's gradient, 4097 tokens x 3, 1021 fp32                   26 us   4.4 TB/s
+//   embedding, 16384 of 128256 x 4096 bf16                           34 us   (ids that recur are read from the cache)
+//   its gradient, 16384 tokens, 50257 x 768 bf16                     sort 19, blocks 6.6, rows 21 us
+//   the same, 65536 tokens, 128256 x 4096 bf16                       sort 27, blocks 71, rows 285 us   4.1 TB/s in all
+// (The blocks' launch of the last one moves 130 MB, but the memory is still writing the last call's 1 GB.)
 #include <type_traits>
 
 #include "chunks.h"
