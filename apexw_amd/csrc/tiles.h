@@ -373,8 +373,9 @@ typedef Shape<64, 128, 32, 64, 3, 2> Mid;
 typedef Shape<32, 128, 32, 32, 3, 2> Small;
 
 // What becomes of a tile.  A policy's Rows are what it loads of the rows of its lane's blocks when the tile begins;
-// stores() says how many stores a wave makes of a whole tile.  Here: the tile as it is, or what `value` makes of the four sums of a lane, added to what is there (kAdd,
-// fp32), in whole lines.  value(v, r, c): columns c .. c + 3 of the tile's row r.
+// stores() says how many stores a wave makes of a whole tile.  Here: the tile as it is, or what `value` makes of the four
+// sums of a lane, added to what is there (kAdd, fp32), in whole lines.  value(v, r, c): columns c .. c + 3 of the tile's
+// row r.
 struct Same {
   __device__ __forceinline__ f32x4 operator()(f32x4 v, int, int) const { return v; }
 };
@@ -467,9 +468,9 @@ template <int OD, bool kAdd = false> struct Store {
 // most two fragment reads of the next step and one copy, fenced in place: issued in bursts they stall the
 // wave's in-order issue.  The second step's fragments are in registers when it begins, so the barrier stands
 // after its first two rows of products, where a wave has four of them and more (standing before them, the wait for
-// the last reads and for the other waves found the matrix cores idle).  Behind it the stage's buffer is free for the copies of the stage
-// kStages on, and the next stage, landed, gives its first fragments.  A's fragments are read into the registers of the
-// ones just used.  Behind the last tile's stages come copies of no memory, which leave zeros: a test around each copy
+// the last reads and for the other waves found the matrix cores idle).  Behind it the stage's buffer is free for the
+// copies of the stage kStages on, and the next stage, landed, gives its first fragments.  A's fragments are read into the
+// registers of the ones just used.  Behind the last tile's stages come copies of no memory, which leave zeros: a test around each copy
 // cost as much.
 //
 // Tried for 256 x 256 and not taken: a third stage of one operand, which leaves the copies two stages' time, with the

@@ -344,3 +344,15 @@ def test_equal_calls_give_equal_bits():
     for _ in range(4):
         assert torch.equal(first, apexw_amd.embedding_weight_grad(dy, ids, 3000, dtype=torch.float32))
         assert all(torch.equal(a, b) for a, b in zip(order, apexw_amd.expert_order(e, 16)))
+
+
+# up to 1024 tokens each id that occurs is summed by itself, beside a cleared gradient of any number of bytes
+@pytest.mark.parametrize("dtype,grad", [(torch.bfloat16, None), (torch.float16, torch.float32), (torch.float32, None)])
+@pytest.mark.parametrize("tokens", [1, 255, 257, 1024, 1025])
+def test_embedding_gradient_of_few(tokens, dtype, grad):
+    for vocab, width in ((1, 1), (3, 1), (7, 1), (2, 3), (5, 9), (1000, 8), (300, 513), (50257, 24)):
+        ids = words((tokens,), vocab) - int(tokens % 2)
+        check_embedding(ids, vocab, width, dtype, 1.5, (grad,))
+        check_embedding(torch.full((tokens,), vocab - 1, device="cuda"), vocab, width, dtype, 1.0, (grad,))
+    dy = torch.full((tokens, 8), float("nan"), device="cuda", dtype=dtype)
+    assert (apexw_amd.embedding_weight_grad(dy, torch.full((tokens,), -1, device="cuda"), 9, dtype=grad) == 0).all()
