@@ -14,9 +14,9 @@
 // operand of the two products that take it.  dx adds up the pieces in fp32.
 //
 // Measured, kernels alone, bf16:
-//   forward, 8192 rows, 4096 x 128256       pack 36, logits 6200 to 6350, join 26 us   1360 to 1390 TFLOP/s
+//   forward, 8192 rows, 4096 x 128256       pack 36, logits 6200 to 6350, join 24 us   1360 to 1390 TFLOP/s
 //   (a library's product alone 5990 us; the chip's power bounds both)
-//   forward, 8 rows, 768 x 50257            pack 5.6, logits 16, join 5.5 us           4.8 TB/s of weights
+//   forward, 8 rows, 768 x 50257            logits 15, join 4.4 us                     5.2 TB/s of weights
 //   backward, 13107 rows, 768 x 50257       pack 42, G 968, dW 890, dx 1290, dx's end 12 us
 //   (products alone by a library 910, 1097 and 970 us)
 //   backward, 501 rows, 500 x 10007 fp16    pack 10, G 19, dW 20, dx 19, dx's end 8 us
@@ -284,6 +284,110 @@ struct Sums {
   }
 };
 
+// Forward of few rows, up to one tile's, as they stand: without a packing launch before it a tile's sum is from its own
+// maximum, and the tile that has a row's target leaves its logit.  (8 rows, 768 x 50257: 20.2 us a call, 26.7 with the
+// packing, 5.6 of it its launch.)
+struct FewTargets {
+  const uint32_t* id;
+  int64_t ignore;
+  int32_t id64, vocab;
+  // (loaded in words, so that nothing waits for them before the end)
+  __device__ __forceinline__ uint32_t low(int row) const { return APEXW_GLOBAL(const uint32_t, id)[id64 ? 2 * row : row]; }
+  __device__ __forceinline__ uint32_t high(int row) const { return APEXW_GLOBAL(const uint32_t, id)[id64 ? 2 * row + 1 : row]; }
+  __device__ __forceinline__ int target(uint32_t lo, uint32_t hi) const {   // -1 for a row that does not count
+    const int64_t t = id64 ? (int64_t)((uint64_t)hi << 32 | lo) : (int64_t)(int32_t)lo;
+    return t != ignore && t >= 0 && t < vocab ? (int)t : -1;
+  }
+};
+struct FewSums {
+  HeadArgs h;
+  FewTargets targets;
+  float* logits;   // of each row's target, to base 2
+  template <int FA> struct Rows {
+    uint32_t lo[FA], hi[FA];
+    __device__ __forceinline__ void arrived() {
+#pragma unroll
+      for (int i = 0; i < FA; ++i) asm volatile("" : "+v"(lo[i]), "+v"(hi[i]));
+    }
+  };
+  template <int FA> __device__ __forceinline__ void load(Rows<FA>& known, int64_t, int row, int rows) const {
+#pragma unroll
+    for (int i = 0; i < FA; ++i) {
+      const int r = min(row + 16 * i, rows - 1);
+      known.lo[i] = targets.low(r), known.hi[i] = targets.high(r);
+    }
+  }
+  template <class S> static constexpr int stores() { return 0; }
+  template <class S, int kWM, class Acc, class R>
+  __device__ __forceinline__ void write(const ExpertArgs& g, Acc& acc, const R& known, uint16_t* lds, int down, int across,
+                                        int rows, int cols, int64_t out0) const {
+    constexpr int FA = kWM / 16, FB = S::WN / 16, kAcross = S::BN / S::WN;
+    static_assert(S::BM == S::WM, "a wave has a tile's rows");
+    const int wn = across * S::WN, lane = lane_id(), col0 = (int)(uint32_t)out0;
+    float* parts = (float*)(lds + S::kStages * S::kStageElems);
+    if (wn + S::WN > cols) mask_columns<FA, FB>(acc, wn, cols, -INFINITY);
+#pragma unroll
+    for (int i = 0; i < FA; ++i) {
+      const int r = 16 * i + (lane & 15), t = r < rows ? targets.target(known.lo[i], known.hi[i]) - col0 - wn : -1;
+      if (__ballot(t >= 0 && t < S::WN)) {
+#pragma unroll
+        for (int j = 0; j < FB; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (t == 16 * j + 4 * (lane >> 4) + q) logits[r] = acc[i][j][q] * kLog2E;
+      }
+      float m = acc[i][0][0];
+#pragma unroll
+      for (int j = 0; j < FB; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) m = fmaxf(m, acc[i][j][q]);
+      m = fmaxf(m, __shfl_xor(m, 16, 64));
+      m = fmaxf(m, __shfl_xor(m, 32, 64));
+      const float top = m == -INFINITY ? 0.0f : m * kLog2E;
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < FB; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][q], kLog2E, -top));
+      sum += __shfl_xor(sum, 16, 64);
+      sum += __shfl_xor(sum, 32, 64);
+      if (lane < 16) parts[across * S::WM + 16 * i + lane] = top + __builtin_amdgcn_logf(sum);
+    }
+    barrier();
+    const int r = threadIdx.x;
+    if (r >= rows || r >= kWM) return;
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kAcross; ++w) top = fmaxf(top, parts[w * S::WM + r]);
+    const float from = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int w = 0; w < kAcross; ++w) sum += __builtin_amdgcn_exp2f(parts[w * S::WM + r] - from);
+    h.sums[col0 / S::BN * h.sums_ld + r] = from + __builtin_amdgcn_logf(sum);
+  }
+};
+// One tile's rows against all columns
+struct FewJobs {
+  int rows, tiles;
+  __device__ __forceinline__ Job get(int i) const {
+    const int64_t t = (int64_t)i * gridDim.x + blockIdx.x;
+    return t < tiles ? Job{0, 0, rows, 0, (int)t, 0} : Job{-1, 0, 0, 0, 0, 0};
+  }
+};
+template <int DT> __global__ __launch_bounds__(Small::kThreads, 2) void head_few_kernel(ExpertArgs g, FewSums out, HeadState* state) {
+  __shared__ __attribute__((aligned(16))) uint16_t lds[Small::kLds];
+  FewJobs jobs{(int)g.rows, (g.n + Small::BN - 1) / Small::BN};
+  stream<Small, false, false, DT, true>(g, jobs, [&](const Job& j, Span& a, Span& b, int& rows, int& cols, int64_t& out0) {
+    const int64_t col = j.col * Small::BN;
+    rows = j.last, cols = g.n - (int)col, out0 = tile_at(0, col);
+    a.template set<false>(g.a, g.lda, rows, g.wide, Small::BM);
+    b.template set<false>(g.b + col * g.ldb, g.ldb, cols, g.wide, Small::BN);
+  }, out, lds);
+  if (blockIdx.x || threadIdx.x >= 64) return;
+  const int r = (int)threadIdx.x < g.rows ? threadIdx.x : 0;
+  const uint64_t count = __ballot((int)threadIdx.x < g.rows && out.targets.target(out.targets.low(r), out.targets.high(r)) >= 0);
+  if (threadIdx.x == 0) state->count = __builtin_popcountll(count);
+}
+
 // Backward: the tile's part of G, whole chunks of columns; a tile of 256 x 256, whose registers are all in use, leaves
 // the targets' elements to a launch behind it
 constexpr bool targets_apart(int shape) { return shape == 3; }
@@ -357,32 +461,40 @@ template <class S, int DT, class Out> __global__ __launch_bounds__(S::kThreads, 
 // The rows' statistics joined, and their mean
 // ---------------------------------------------------------------------------
 
-// 16 rows a workgroup, a 64th of the sums a thread
-__global__ __launch_bounds__(1024) void head_join_kernel(HeadArgs h, int parts, float* __restrict__ loss, float* __restrict__ lse) {
-  __shared__ float2 lds[64][16];
+// 16 rows a workgroup, a 64th of the sums a thread; `few` rows as they stand, or 0
+__global__ __launch_bounds__(1024) void head_join_kernel(HeadArgs h, int parts, int few, FewTargets targets, float* __restrict__ loss,
+                                                         float* __restrict__ lse) {
+  __shared__ float2 lds[16][16];
   const int r = threadIdx.x & 15, q = threadIdx.x >> 4;
   const int64_t row = (int64_t)blockIdx.x * 16 + r;
-  const int count = h.state->count;
+  const int count = few ? few : h.state->count;
   if ((int64_t)blockIdx.x * 16 >= count) return;
   float m = -INFINITY, s = 0.0f;
+  const auto add = [&](float x, float y) {   // y 2^x
+    const float top = fmaxf(m, x), to = top == -INFINITY ? 0.0f : top;
+    s = s * __builtin_amdgcn_exp2f(m - to) + y * __builtin_amdgcn_exp2f(x - to);
+    m = top;
+  };
   if (row < count)
 #pragma unroll 8
-    for (int t = q; t < parts; t += 64) {
-      const float x = h.sums[t * h.sums_ld + row], top = fmaxf(m, x), to = top == -INFINITY ? 0.0f : top;
-      s = s * __builtin_amdgcn_exp2f(m - to) + __builtin_amdgcn_exp2f(x - to);
-      m = top;
-    }
-  lds[q][r] = make_float2(m, s);
+    for (int t = q; t < parts; t += 64) add(h.sums[t * h.sums_ld + row], 1.0f);
+  for (int off = 16; off < 64; off <<= 1) {
+    const float x = __shfl_xor(m, off, 64), y = __shfl_xor(s, off, 64);
+    add(x, y);
+  }
+  if ((q & 3) == 0) lds[q >> 2][r] = make_float2(m, s);
   __syncthreads();
   if (q != 0 || row >= count) return;
-  for (int i = 1; i < 64; ++i) {
-    const float2 x = lds[i][r];
-    const float top = fmaxf(m, x.x), to = top == -INFINITY ? 0.0f : top;
-    s = s * __builtin_amdgcn_exp2f(m - to) + x.y * __builtin_amdgcn_exp2f(x.x - to);
-    m = top;
+#pragma unroll
+  for (int i = 1; i < 16; ++i) add(lds[i][r].x, lds[i][r].y);
+  const float sum = (m == -INFINITY ? 0.0f : m) + log2f(s), shift = h.shift[row];
+  if (few) {
+    const bool has = targets.target(targets.low((int)row), targets.high((int)row)) >= 0;
+    lse[row] = has ? sum * kLn2 : 0.0f;
+    loss[row] = has ? (sum - shift) * kLn2 : 0.0f;
+    return;
   }
   const HeadRow& info = h.rows[row];
-  const float sum = (m == -INFINITY ? 0.0f : m) + log2f(s), shift = h.shift[row];
   lse[info.row] = (shift + sum) * kLn2;
   loss[info.row] = ((shift - info.logit) + sum) * kLn2;
 }
@@ -704,9 +816,12 @@ template <int DT> void launch_dw(const ExpertArgs& g, int shape, const HeadState
   hipLaunchKernelGGL(head_join_weight_kernel<DT>, dim3((unsigned)(grid < 4096 ? grid : 4096)), dim3(256), 0, s, g, state, partial);
 }
 
+void set_state(const HeadPlan& p, PackArgs& a, char* ws) {
+  a.state = (HeadState*)ws, a.rows = (HeadRow*)(ws + p.at_rows), a.shift = (float*)(ws + p.at_shift);
+}
 // The weights, copied to whole chunks where they are not; rows packed
 template <int DT> const uint16_t* launch_pack(const HeadPlan& p, PackArgs& a, const void* w, int64_t stride, char* ws, hipStream_t s) {
-  a.state = (HeadState*)ws, a.rows = (HeadRow*)(ws + p.at_rows), a.shift = (float*)(ws + p.at_shift);
+  set_state(p, a, ws);
   a.packed = (uint16_t*)(ws + p.at_x), a.w = (const uint16_t*)w, a.w_stride = stride;
   a.n = p.n, a.width = (int32_t)p.width, a.wide = (int32_t)p.wide, a.vocab = (int32_t)p.vocab;
   // about 1024 workgroups, of at least 4 rows
@@ -762,13 +877,24 @@ extern "C" int apexw_linear_cross_entropy_forward(const void* x, int64_t x_strid
   pack.ignore = ignore_index, pack.loss = loss, pack.lse_out = lse;
   by_half(dtype, [&](auto d) {
     constexpr int DT = decltype(d)::value;
-    const uint16_t* w = launch_pack<DT>(p, pack, weight, w_stride, ws, s);
+    ExpertArgs g = p.args(vocab);
+    const FewTargets targets{(const uint32_t*)target, ignore_index, pack.id64, (int32_t)vocab};
+    const bool few = n > 0 && n <= Small::BM && p.cut.shape == 0 && !p.copy_w && k_rows_ok(x, x_stride, width);
+    const uint16_t* w = (const uint16_t*)weight;
+    if (few) set_state(p, pack, ws);
+    else w = launch_pack<DT>(p, pack, weight, w_stride, ws, s);
     if (n == 0) return;
     const HeadArgs h{pack.state, pack.rows, pack.shift, (float*)(ws + p.at_parts), p.parts_ld};
-    ExpertArgs g = p.args(vocab);
-    g.a = pack.packed, g.b = w, g.ends = &pack.state->count;
-    launch_logits<DT>(g, p.cut.shape, Sums{h}, s);
-    hipLaunchKernelGGL(head_join_kernel, dim3((unsigned)((n + 15) / 16)), dim3(1024), 0, s, h, (int)p.parts(), loss, lse);
+    if (few) {
+      g.a = (const uint16_t*)x, g.lda = x_stride, g.b = w;
+      hipLaunchKernelGGL(head_few_kernel<DT>, dim3(stream_grid<Small>((vocab + Small::BN - 1) / Small::BN)), dim3(Small::kThreads), 0, s,
+                         g, FewSums{h, targets, pack.shift}, pack.state);
+    } else {
+      g.a = pack.packed, g.b = w, g.ends = &pack.state->count;
+      launch_logits<DT>(g, p.cut.shape, Sums{h}, s);
+    }
+    hipLaunchKernelGGL(head_join_kernel, dim3((unsigned)((n + 15) / 16)), dim3(1024), 0, s, h, (int)p.parts(), few ? (int)n : 0, targets,
+                       loss, lse);
   });
   if (reduction) hipLaunchKernelGGL(head_total_kernel, dim3(1), dim3(1024), 0, s, pack.state, loss, n, (int)(reduction == 2), total);
   return hipGetLastError() == hipSuccess ? APEXW_OK : APEXW_ERR_LAUNCH;

@@ -1,4 +1,4 @@
-"""Each way that the cross entropy of a linear head may take -- the four tile shapes of the logits, forward and
+"""Each way that the cross entropy of a linear head may take -- few rows as they stand, the four tile shapes of the logits, forward and
 backward, the shapes and parts of the two products with the probabilities, one piece of the vocabulary and more,
 weights copied to whole chunks -- at a size that takes it, against
 float64 with the bars of test_gpu_linear_cross_entropy.  The kernels that ran are read from a profile, so a size that a
@@ -33,6 +33,8 @@ def taken(call):
             ways.add("added")
         if "join_weight" in name:
             ways.add("dw:parts")
+        if "head_few" in name:
+            ways.add("few")
         if "head_targets" in name:
             ways.add("targets")
     return out, ways
@@ -58,7 +60,9 @@ CASES = [
     ("forward logits:Large", 2049, 520, 16500, BF16, 0.1), ("forward logits:Large", 2176, 264, 20011, FP16, 0.0),
     ("forward logits:Wide", 582, 701, 7374, BF16, 0.2), ("forward logits:Wide", 641, 264, 9003, FP16, 0.0),
     ("forward logits:Mid", 1500, 101, 2003, BF16, 0.1), ("forward logits:Mid", 4605, 1569, 416, FP16, 0.3),
-    ("forward logits:Small", 31, 768, 5003, BF16, 0.1), ("forward logits:Small", 640, 1021, 1500, FP16, 0.0),
+    ("forward logits:Small", 31, 765, 5003, BF16, 0.1), ("forward few", 31, 768, 5003, BF16, 0.1),
+    ("forward few", 1, 64, 129, FP16, 0.0), ("forward few", 32, 1024, 70001, BF16, 0.3), ("forward few", 16, 4096, 300, FP16, 0.0),
+    ("forward logits:Small", 640, 1021, 1500, FP16, 0.0),
     ("logits:Large targets dx:Large dw:Large", 4800, 768, 16500, BF16, 0.1),
     ("logits:Large targets dx:Large dw:Wide", 5798, 325, 14144, FP16, 0.0),
     ("logits:Large targets dx:Mid dw:Large dw:parts", 6677, 24, 18997, BF16, 0.1),
@@ -97,3 +101,40 @@ def test_pieces(rows, width, vocab):
     # a probability is off by its part e and G by half a step: 2^-8 and the logits' error, below 2^-14 here
     bar = (2.0 ** -8 + 2.0 ** -12 + rows * 2.0 ** -23) * mag + 2.0 ** -8 * want.abs()
     assert float(((dw[words].double() - want).abs() - bar).max()) <= 0
+
+
+@pytest.mark.parametrize("rows", [1, 15, 17, 32])
+def test_few_rows(rows):
+    """Rows as they stand: other targets that do not count, distances between rows, logits far apart, what stands in rows
+    that do not count, the mean."""
+    x, w, target = make(rows, 136, 1000, BF16, lean=40.0)
+    wide = torch.randn(rows, 144, device="cuda").bfloat16()
+    wide[:, 8:] = x
+    target[::3], ignored = 7, 7
+    if rows > 3:
+        target[1], target[2] = 1000, -1
+    exact = Exact(x, w, target, ignored)
+    for t in (target, target.int()):
+        for rows_of in (x, wide[:, 8:]):
+            loss, lse = apexw_amd.linear_cross_entropy_forward(rows_of, w, t, ignored)
+            exact.check_forward(loss, lse)
+    bad = x.clone()
+    bad[~exact.kept] = float("nan")
+    loss, lse = apexw_amd.linear_cross_entropy_forward(bad, w, target, ignored)
+    exact.check_forward(loss, lse)
+    mean = apexw_amd.linear_cross_entropy(bad, w, target, ignored)
+    kept = int(exact.kept.sum())
+    assert mean.isnan() if kept == 0 else float(mean) == pytest.approx(float(loss.double().sum()) / kept, rel=1e-6)
+    assert float(apexw_amd.linear_cross_entropy(bad, w, target, ignored, "sum")) == pytest.approx(float(loss.double().sum()), rel=1e-6)
+
+
+def test_few_rows_of_infinite_logits():
+    """A row whose logits overflow to infinity or are not numbers makes its own results alone so."""
+    x, w, target = make(9, 64, 500, BF16)
+    x[2], x[5] = 1e38, float("nan")
+    w[3] = w[3].abs() * 100
+    loss, lse = apexw_amd.linear_cross_entropy_forward(x, w, target)
+    others = torch.tensor([0, 1, 3, 4, 6, 7, 8], device="cuda")
+    assert not loss[2].isfinite() and loss[5].isnan() and lse[5].isnan()
+    part = Exact(x[others], w, target[others])
+    part.check_forward(loss[others], lse[others])
