@@ -32,7 +32,7 @@ namespace {
 // Order
 // ---------------------------------------------------------------------------
 
-__global__ __launch_bounds__(kSortThreads) void order_small_kernel(SortArgs a) { sort_small<true>(a); }
+template <int kItems> __global__ __launch_bounds__(kSortThreads) void order_small_kernel(SortArgs a) { sort_small<true, kItems>(a); }
 
 // ends[e] = items of keys up to e, for orders that took more than one pass
 __global__ __launch_bounds__(256) void order_ends_kernel(const u32x2* __restrict__ sorted, int n, uint32_t experts, int32_t* ends) {
@@ -268,9 +268,9 @@ template <int DT> __global__ __launch_bounds__(kWG) void embedding_kernel(Embedd
   }
 }
 
-__global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(SortArgs a) {
+template <int kItems> __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(SortArgs a) {
   if (blockIdx.x) return sort_clear(a, blockIdx.x - 1, gridDim.x - 1);
-  sort_small<false>(a);
+  sort_small<false, kItems>(a);
 }
 
 // sum += the rows of sorted tokens [from, to), U in flight, chunk c of each
@@ -404,7 +404,7 @@ template <int DT, int OD> APEXW_DEV void write_sum(const EmbeddingArgs& a, const
 }
 
 // Few tokens, whose sort clears the gradient beside it: a workgroup has 64 chunks of columns of the id that a token is
-// the first one of, a part of its tokens a wave.  (50257 x 768 bf16, 1 to 1024 tokens 16 to 18 us, by the other kernels
+// the first one of, a part of its tokens a wave.  (50257 x 768 bf16, 1 to 1024 tokens 15 to 18 us, by the other kernels
 // 25 to 32; 2048 tokens 25 and 33, but 87 and 35 where all are of one id.)
 constexpr int kFewTokens = 1024;
 template <int DT, int OD> __global__ __launch_bounds__(kWG) void embedding_few_kernel(EmbeddingArgs a) {
@@ -604,7 +604,8 @@ template <class F> int by_types(int32_t dtype, int32_t w_dtype, F&& f) {
 // Rows of a gradient: 64 to a workgroup of 256 threads, fewer than 2^32 in all
 constexpr int64_t kMostWords = 1 << 29;
 
-constexpr int64_t kClears = 1 << 20;   // workgroups that clear, at most; 2048 take 226 us for 1 GB, one for each 32 KB 187
+// Workgroups that clear, at most (with 2048 in a loop 1 GB takes 226 us, with one for each 32 KB 187)
+constexpr int64_t kClears = 1 << 20;
 
 struct GradPlan {
   SortArgs sort;
@@ -648,7 +649,8 @@ extern "C" int apexw_expert_order(const void* expert, int32_t id_bytes, int64_t 
   const u32x2* sorted = nullptr;
   if (a.n <= kSmall) {
     sorted = a.to = wanted ? (u32x2*)workspace : nullptr;
-    hipLaunchKernelGGL(order_small_kernel, dim3(1), dim3(kSortThreads), 0, s, a);
+    if (a.n <= kFew * kSortThreads) hipLaunchKernelGGL(order_small_kernel<kFew>, dim3(1), dim3(kSortThreads), 0, s, a);
+    else hipLaunchKernelGGL(order_small_kernel<kMost>, dim3(1), dim3(kSortThreads), 0, s, a);
   } else {
     sorted = launch_sort<true>(a, space, wanted, (char*)workspace, s);
   }
@@ -766,7 +768,9 @@ extern "C" int apexw_embedding_weight_grad(const void* dy, int64_t dy_stride, co
     if (n <= kSmall) {
       a.sorted = sort.to = (u32x2*)ws;
       const int64_t clears = (sort.clears + kClear - 1) / kClear;
-      hipLaunchKernelGGL(embedding_sort_kernel, dim3((unsigned)(1 + (clears < kClears ? clears : kClears))), dim3(kSortThreads), 0, s, sort);
+      const dim3 grid((unsigned)(1 + (clears < kClears ? clears : kClears)));
+      if (n <= kFew * kSortThreads) hipLaunchKernelGGL(embedding_sort_kernel<kFew>, grid, dim3(kSortThreads), 0, s, sort);
+      else hipLaunchKernelGGL(embedding_sort_kernel<kMost>, grid, dim3(kSortThreads), 0, s, sort);
     } else {
       a.sorted = launch_sort<false>(sort, plan.space, true, ws, s);
     }
