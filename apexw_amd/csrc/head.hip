@@ -130,11 +130,13 @@ template <int DT> __global__ __launch_bounds__(256) void head_pack_kernel(PackAr
       if (a.dloss) most = over_workgroup(most, floats, [](float p, float q) { return fmaxf(p, q); });
       if (threadIdx.x == 0) {
         // The largest dloss is divided out of G and multiplied into the sums: a row that is far from its target then has
-        // -1 there, which no rounding changes (where all rows have one dloss, its own rounding would be every row's), and
-        // fp16 loses nothing below 2^-24.
+        // -2^14 there, which no rounding changes (where all rows have one dloss, its own rounding would be every row's).
+        // The 2^14 leave fp16 its range below: a G of 2^-28 of the largest keeps its bits, one of 2^-39 is the least that is
+        // not 0 (largest 1: 2^-14 and 2^-25, and a quarter of G was 0 where logits spread by 3 over 50257 words); 2^2 are
+        // left above.
         const float mean = a.mean && all > 0 ? 1.0f / (float)all : 1.0f;
-        const bool use = most >= 0x1p-120f && most < 0x1p120f;
-        const float factor = use ? 1.0f / most : 1.0f, scale = use ? most * mean : mean;
+        const bool use = most >= 0x1p-100f && most < INFINITY;
+        const float factor = use ? 0x1p14f / most : 1.0f, scale = use ? most * 0x1p-14f * mean : mean;
         *a.state = HeadState{all, factor, log2f(factor), scale};
       }
     }

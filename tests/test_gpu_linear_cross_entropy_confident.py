@@ -1,0 +1,47 @@
+"""Losses of rows that are nearly certain of their target, whose logits are large.
+
+Bars.  The loss is log(1 + sum of exp(l_v - l_t) over the other words).  Where the target's term in the sum and its logit
+are one number, what is off in the logits (at most a = width 2^-23 of the sum of the magnitudes each, and 3 R 2^-24 for
+the difference's rounding, R their range) reaches the loss by the other words alone, whose part is 1 - p.  To that come
+250 additions and products of 2^-24 of a sum that is about 1, the instructions' 2^-20, and roundings of the loss itself,
+2^-21 of it."""
+
+import pytest
+import torch
+
+import apexw_amd
+
+pytestmark = pytest.mark.gpu
+
+
+def make(rows, width, vocab, dtype, scale):
+    """Every second row certain of its target by thousands of units of the logits' last place, the others less so."""
+    g = torch.Generator().manual_seed(rows + width + vocab)
+    w = torch.randn(vocab, width, generator=g) * width ** -0.5
+    target = torch.randint(0, vocab, (rows,), generator=g)
+    lean = torch.where(torch.arange(rows) % 2 == 0, 1.0, torch.rand(rows, generator=g))[:, None]
+    x = torch.randn(rows, width, generator=g) + scale * lean * w[target]
+    return x.to(dtype).cuda(), w.to(dtype).cuda(), target.cuda()
+
+
+def check(rows, width, vocab, dtype, scale=400.0):
+    x, w, target = make(rows, width, vocab, dtype, scale)
+    loss, lse = apexw_amd.linear_cross_entropy_forward(x, w, target)
+    x64, w64 = x.double(), w.double()
+    l = x64 @ w64.t()
+    want = torch.logsumexp(l, 1) - l.gather(1, target[:, None])[:, 0]
+    others = -torch.expm1(-want)
+    a = width * 2.0 ** -23 * (x64.abs() @ w64.abs().t()).max(1)[0]
+    R = l.max(1)[0] - l.min(1)[0]
+    bar = others * (2 * a + 3 * R * 2.0 ** -24) + 250 * 2.0 ** -24 + 2.0 ** -20 + 2.0 ** -21 * want
+    assert float(l.max()) > 100 and float(want.min()) < 1e-12
+    assert (loss >= 0).all(), f"a loss of {float(loss.min())}"
+    over = (loss.double() - want).abs() - bar
+    assert float(over.max()) <= 0, f"over the bar by {float(over.max())}"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,width,vocab", [(33, 4096, 300), (40, 1021, 5003), (200, 4096, 2000), (582, 701, 7374),
+                                              (1500, 1029, 2003), (2049, 520, 16500)])
+def test_packed_rows(rows, width, vocab, dtype):
+    check(rows, width, vocab, dtype)
