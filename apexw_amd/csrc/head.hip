@@ -34,13 +34,20 @@ struct HeadState {          // device
   float scale;              // what dx and dW are multiplied with in the end
 };
 struct HeadRow {            // a row that counts; logarithms to base 2
-  float logit;              // its target's logit
+  float logit;              // its target's logit; forward: what its tile has of it above the shift
   float lse, d;             // backward
   int32_t target, row;      // its place among all rows
 };
+// A row's shift, forward: 3 to 10% below its target's logit, its low bits the target, so that the wave that has it knows.
+// (All targets loaded in the end of every tile of 256 x 256: 16384 x 768 x 51200 1088 -> 1160 us.)
+constexpr uint32_t kPlace = 0x3FFFF;
+APEXW_DEV float with_place(float logit, int target) {
+  const float below = logit - fabsf(logit) * 0x1p-4f;
+  return __uint_as_float((__float_as_uint(below) & ~kPlace) | ((uint32_t)target & kPlace));
+}
 struct HeadArgs {
   const HeadState* state;
-  const HeadRow* rows;
+  HeadRow* rows;
   const float* shift;       // one a row, of the exponents of its tiles
   float* sums;              // [columns of a wave or tile][row]: log2 of the sum of 2^(l log2 e - shift)
   int64_t sums_ld;
@@ -176,6 +183,8 @@ template <int DT> __global__ __launch_bounds__(256) void head_pack_kernel(PackAr
         row.lse = a.lse[i] * kLog2E, row.d = a.dloss[i * a.dloss_stride];
         const uint32_t bits = __float_as_uint(log2f(fabsf(row.d)) - row.lse);
         shift = __uint_as_float((bits & ~1u) | (row.d < 0.0f));
+      } else {
+        shift = with_place(shift, target);
       }
       a.rows[p] = row, a.shift[p] = shift;
     }
@@ -215,8 +224,11 @@ template <int FA> struct Shifts {
   }
 };
 
-// Forward: each row's sum of exponentials over a wave's columns, relative to its target's.  That is a maximum's part as
-// long as no logit is 83 above the target's (2^120); the rows of a block where one is are summed again from their maximum.
+// Forward: each row's sum of exponentials over a wave's columns, relative to its shift.  That is a maximum's part as long as no
+// logit is 83 above it (2^120) and one is 83 below or more; the rows of a block where this is not so are summed again from
+// their maximum.  The packing's target's logit is off from the tile's by their orders of summing (3e-4 at logits of
+// 1000), so the wave that has the target leaves its exponent as it is in the sum: a row certain of its target has a loss of 0.
+// (16384 x 768 x 51200 1094 -> 1107 us, 8192 x 4096 x 128256 6266 -> 6313.)
 struct Sums {
   HeadArgs h;
   template <int FA> using Rows = Shifts<FA>;
@@ -238,6 +250,7 @@ struct Sums {
     if (wn + S::WN > cols) mask_columns<FA, FB>(acc, wn, cols, -INFINITY);
     float* parts = (float*)(lds + S::kStages * S::kStageElems);
     float* to = kJoin ? parts + across * S::WM : h.sums + (col0 + wn) / S::WN * h.sums_ld + row0 + wm;
+    const uint32_t place = (uint32_t)(col0 + wn) & kPlace;
 #pragma unroll
     for (int i = 0; i < FA; ++i) {
       const float shift = known.v[i];
@@ -250,7 +263,7 @@ struct Sums {
       sum += __shfl_xor(sum, 16, 64);
       sum += __shfl_xor(sum, 32, 64);
       float part = __builtin_amdgcn_logf(sum);   // to base 2
-      if (__ballot(!(sum < 0x1p120f))) {
+      if (__builtin_expect(__ballot(!(fabsf(part) < 120.0f)) != 0, 0)) {
         float m = acc[i][0][0];
 #pragma unroll
         for (int j = 0; j < FB; ++j)
@@ -258,17 +271,28 @@ struct Sums {
           for (int q = 0; q < 4; ++q) m = fmaxf(m, acc[i][j][q]);
         m = fmaxf(m, __shfl_xor(m, 16, 64));
         m = fmaxf(m, __shfl_xor(m, 32, 64));
-        const float top = m == -INFINITY ? 0.0f : m * kLog2E;
+        const float top = m == -INFINITY ? 0.0f : m;
         sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < FB; ++j)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][q], kLog2E, -top));
+          for (int q = 0; q < 4; ++q) sum += __builtin_amdgcn_exp2f((acc[i][j][q] - top) * kLog2E);
         sum += __shfl_xor(sum, 16, 64);
         sum += __shfl_xor(sum, 32, 64);
-        part = (top - shift) + __builtin_amdgcn_logf(sum);
+        part = fmaf(top, kLog2E, -shift) + __builtin_amdgcn_logf(sum);
       }
       if (lane < 16 && wm + 16 * i + lane < rows) to[16 * i + lane] = part;
+      uint32_t t = (__float_as_uint(shift) & kPlace) - place;
+      if (__builtin_expect(__ballot(t < S::WN) != 0, 0)) {
+        const int r = wm + 16 * i + (lane & 15);
+        if (g.n > (int)kPlace) t = (uint32_t)(h.rows[row0 + min(r, rows - 1)].target - col0 - wn);
+        float logit = 0.0f;
+#pragma unroll
+        for (int j = 0; j < FB; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) logit = (t & ~12u) == 16u * j + q ? acc[i][j][q] : logit;
+        if (t < S::WN && r < rows && (int)(t >> 2 & 3u) == lane >> 4) h.rows[row0 + r].logit = fmaf(logit, kLog2E, -shift);
+      }
     }
     if constexpr (kJoin) {
       barrier();
@@ -498,7 +522,8 @@ __global__ __launch_bounds__(1024) void head_join_kernel(HeadArgs h, int parts, 
   }
   const HeadRow& info = h.rows[row];
   lse[info.row] = (shift + sum) * kLn2;
-  loss[info.row] = ((shift - info.logit) + sum) * kLn2;
+  const float above = (sum - info.logit) * kLn2;   // (not below 0 but for roundings; NaN stays)
+  loss[info.row] = above < 0.0f ? 0.0f : above;
 }
 
 // The sum of the rows' losses, or their mean over the rows that count

@@ -45,3 +45,36 @@ def check(rows, width, vocab, dtype, scale=400.0):
                                               (1500, 1029, 2003), (2049, 520, 16500)])
 def test_packed_rows(rows, width, vocab, dtype):
     check(rows, width, vocab, dtype)
+
+
+@pytest.mark.parametrize("rows,width,vocab", [(300, 264, 2003), (70, 4096, 300), (2049, 520, 16500)])
+def test_logits_of_any_size(rows, width, vocab):
+    """Logits up to some 10^9, of both signs: the exponents' range is left wherever a target is not the largest."""
+    for scale in (1e-30, 1e-3, 1e5, 1e9):
+        x, w, target = make(rows, width, vocab, torch.bfloat16, 40.0)
+        for y in (x * scale, x * -scale):
+            loss, lse = apexw_amd.linear_cross_entropy_forward(y, w, target)
+            l = y.double() @ w.double().t()
+            at = l.gather(1, target[:, None])[:, 0]
+            want = torch.logsumexp(l, 1)
+            # b and 2 b of test_gpu_linear_cross_entropy
+            a = width * 2.0 ** -23 * (y.double().abs() @ w.double().abs().t()).max(1)[0]
+            bar = a + (3 * (l.max(1)[0] - l.min(1)[0]) + 250) * 2.0 ** -24 + 2.0 ** -22 * (want.abs() + 20)
+            assert (loss >= 0).all() and loss.isfinite().all() and lse.isfinite().all()
+            assert float(((lse.double() - want).abs() - bar).max()) <= 0
+            assert float(((loss.double() - (want - at)).abs() - 2 * bar).max()) <= 0
+
+
+def test_vocabulary_beyond_the_places():
+    """More than 2^18 words: several words share a place in a row's shift."""
+    x, w, target = make(70, 64, 300001, torch.bfloat16, 100.0)
+    target[:8] = torch.tensor([0, 131072, 131071, 262144, 300000, 31, 131103, 262175])
+    x[:8] = (60.0 * w[target[:8]].float()).bfloat16()
+    loss, lse = apexw_amd.linear_cross_entropy_forward(x, w, target)
+    l = x.double() @ w.double().t()
+    want = torch.logsumexp(l, 1)
+    # b and 2 b of test_gpu_linear_cross_entropy; its 250 additions are 64 in a wave, 4700 waves' sums over 64 threads and 20
+    a = 64 * 2.0 ** -23 * (x.double().abs() @ w.double().abs().t()).max(1)[0]
+    bar = a + (3 * (l.max(1)[0] - l.min(1)[0]) + 250) * 2.0 ** -24 + 2.0 ** -22 * (want.abs() + 20)
+    assert float(((lse.double() - want).abs() - bar).max()) <= 0
+    assert float(((loss.double() - (want - l.gather(1, target[:, None])[:, 0])).abs() - 2 * bar).max()) <= 0
