@@ -34,22 +34,21 @@ struct HeadState {          // device
   float scale;              // what dx and dW are multiplied with in the end
 };
 struct HeadRow {            // a row that counts; logarithms to base 2
-  float logit;              // its target's logit; forward: what its tile has of it above the shift
+  float logit;              // its target's logit; forward, from its tile: less the shift
   float lse, d;             // backward
   int32_t target, row;      // its place among all rows
 };
-// A row's shift, forward: 3 to 10% below its target's logit, its low bits the target, so that the wave that has it knows.
-// (All targets loaded in the end of every tile of 256 x 256: 16384 x 768 x 51200 1088 -> 1160 us.)
+// A row's shift, forward: its target's logit but for the low bits (a 32nd of it at most), which say the target, so that the
+// wave that has it knows.  (All targets loaded in the end of every tile of 256 x 256: 16384 x 768 x 51200 1088 -> 1160 us.)
 constexpr uint32_t kPlace = 0x3FFFF;
 APEXW_DEV float with_place(float logit, int target) {
-  const float below = logit - fabsf(logit) * 0x1p-4f;
-  return __uint_as_float((__float_as_uint(below) & ~kPlace) | ((uint32_t)target & kPlace));
+  return __uint_as_float((__float_as_uint(logit) & ~kPlace) | ((uint32_t)target & kPlace));
 }
 struct HeadArgs {
   const HeadState* state;
   HeadRow* rows;
   const float* shift;       // one a row, of the exponents of its tiles
-  float* sums;              // [columns of a wave or tile][row]: log2 of the sum of 2^(l log2 e - shift)
+  float* sums;              // [columns of a wave or tile][row]: log2 of the sum of 2^(l log2 e - shift), or few rows' pairs
   int64_t sums_ld;
 };
 
@@ -310,8 +309,15 @@ struct Sums {
   }
 };
 
-// Forward of few rows, up to one tile's, as they stand: without a packing launch before it a tile's sum is from its own
-// maximum, and the tile that has a row's target leaves its logit.  (8 rows, 768 x 50257: 20.2 us a call, 26.7 with the
+// y 2^(x unit) more, as a sum from the larger x
+APEXW_DEV void add_sum(float2& a, float2 b, float unit) {
+  const float top = fmaxf(a.x, b.x), to = top == -INFINITY ? 0.0f : top;
+  a = make_float2(top, a.y * __builtin_amdgcn_exp2f((a.x - to) * unit) + b.y * __builtin_amdgcn_exp2f((b.x - to) * unit));
+}
+
+// Forward of few rows, up to one tile's, as they stand: without a packing launch before it a tile leaves its maximum and
+// the sum from it (one logarithm of both would round at the logits' size), and the tile that has a row's target leaves its
+// logit.  (8 rows, 768 x 50257: 20.2 us a call, 26.7 with the
 // packing, 5.6 of it its launch.)
 struct FewTargets {
   const uint32_t* id;
@@ -328,7 +334,7 @@ struct FewTargets {
 struct FewSums {
   HeadArgs h;
   FewTargets targets;
-  float* logits;   // of each row's target, to base 2
+  float* logits;   // of each row's target
   template <int FA> struct Rows {
     uint32_t lo[FA], hi[FA];
     __device__ __forceinline__ void arrived() {
@@ -350,7 +356,7 @@ struct FewSums {
     constexpr int FA = kWM / 16, FB = S::WN / 16, kAcross = S::BN / S::WN;
     static_assert(S::BM == S::WM, "a wave has a tile's rows");
     const int wn = across * S::WN, lane = lane_id(), col0 = (int)(uint32_t)out0;
-    float* parts = (float*)(lds + S::kStages * S::kStageElems);
+    float2* parts = (float2*)(lds + S::kStages * S::kStageElems);
     if (wn + S::WN > cols) mask_columns<FA, FB>(acc, wn, cols, -INFINITY);
 #pragma unroll
     for (int i = 0; i < FA; ++i) {
@@ -360,7 +366,7 @@ struct FewSums {
         for (int j = 0; j < FB; ++j)
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            if (t == 16 * j + 4 * (lane >> 4) + q) logits[r] = acc[i][j][q] * kLog2E;
+            if (t == 16 * j + 4 * (lane >> 4) + q) logits[r] = acc[i][j][q];
       }
       float m = acc[i][0][0];
 #pragma unroll
@@ -369,26 +375,23 @@ struct FewSums {
         for (int q = 0; q < 4; ++q) m = fmaxf(m, acc[i][j][q]);
       m = fmaxf(m, __shfl_xor(m, 16, 64));
       m = fmaxf(m, __shfl_xor(m, 32, 64));
-      const float top = m == -INFINITY ? 0.0f : m * kLog2E;
+      const float top = m == -INFINITY ? 0.0f : m;
       float sum = 0.0f;
 #pragma unroll
       for (int j = 0; j < FB; ++j)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][q], kLog2E, -top));
+        for (int q = 0; q < 4; ++q) sum += __builtin_amdgcn_exp2f((acc[i][j][q] - top) * kLog2E);
       sum += __shfl_xor(sum, 16, 64);
       sum += __shfl_xor(sum, 32, 64);
-      if (lane < 16) parts[across * S::WM + 16 * i + lane] = top + __builtin_amdgcn_logf(sum);
+      if (lane < 16) parts[across * S::WM + 16 * i + lane] = make_float2(m, sum);
     }
     barrier();
     const int r = threadIdx.x;
     if (r >= rows || r >= kWM) return;
-    float top = -INFINITY, sum = 0.0f;
+    float2 all = parts[r];
 #pragma unroll
-    for (int w = 0; w < kAcross; ++w) top = fmaxf(top, parts[w * S::WM + r]);
-    const float from = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-    for (int w = 0; w < kAcross; ++w) sum += __builtin_amdgcn_exp2f(parts[w * S::WM + r] - from);
-    h.sums[col0 / S::BN * h.sums_ld + r] = from + __builtin_amdgcn_logf(sum);
+    for (int w = 1; w < kAcross; ++w) add_sum(all, parts[w * S::WM + r], kLog2E);
+    ((float2*)h.sums)[col0 / S::BN * h.sums_ld + r] = all;
   }
 };
 // One tile's rows against all columns
@@ -495,31 +498,32 @@ __global__ __launch_bounds__(1024) void head_join_kernel(HeadArgs h, int parts, 
   const int64_t row = (int64_t)blockIdx.x * 16 + r;
   const int count = few ? few : h.state->count;
   if ((int64_t)blockIdx.x * 16 >= count) return;
-  float m = -INFINITY, s = 0.0f;
-  const auto add = [&](float x, float y) {   // y 2^x
-    const float top = fmaxf(m, x), to = top == -INFINITY ? 0.0f : top;
-    s = s * __builtin_amdgcn_exp2f(m - to) + y * __builtin_amdgcn_exp2f(x - to);
-    m = top;
-  };
-  if (row < count)
+  float2 all = {-INFINITY, 0.0f};
+  const float unit = few ? kLog2E : 1.0f;
+  if (row < count) {
+    if (few) {
 #pragma unroll 8
-    for (int t = q; t < parts; t += 64) add(h.sums[t * h.sums_ld + row], 1.0f);
-  for (int off = 16; off < 64; off <<= 1) {
-    const float x = __shfl_xor(m, off, 64), y = __shfl_xor(s, off, 64);
-    add(x, y);
+      for (int t = q; t < parts; t += 64) add_sum(all, ((const float2*)h.sums)[t * h.sums_ld + row], unit);
+    } else {
+#pragma unroll 8
+      for (int t = q; t < parts; t += 64) add_sum(all, make_float2(h.sums[t * h.sums_ld + row], 1.0f), unit);
+    }
   }
-  if ((q & 3) == 0) lds[q >> 2][r] = make_float2(m, s);
+  for (int off = 16; off < 64; off <<= 1) add_sum(all, make_float2(__shfl_xor(all.x, off, 64), __shfl_xor(all.y, off, 64)), unit);
+  if ((q & 3) == 0) lds[q >> 2][r] = all;
   __syncthreads();
   if (q != 0 || row >= count) return;
 #pragma unroll
-  for (int i = 1; i < 16; ++i) add(lds[i][r].x, lds[i][r].y);
-  const float sum = (m == -INFINITY ? 0.0f : m) + log2f(s), shift = h.shift[row];
+  for (int i = 1; i < 16; ++i) add_sum(all, lds[i][r], unit);
+  const float top = all.x == -INFINITY ? 0.0f : all.x, shift = h.shift[row];
   if (few) {
     const bool has = targets.target(targets.low((int)row), targets.high((int)row)) >= 0;
-    lse[row] = has ? sum * kLn2 : 0.0f;
-    loss[row] = has ? (sum - shift) * kLn2 : 0.0f;
+    const float sum = log2f(all.y) * kLn2;
+    lse[row] = has ? top + sum : 0.0f;
+    loss[row] = has ? (top - shift) + sum : 0.0f;
     return;
   }
+  const float sum = top + log2f(all.y);
   const HeadRow& info = h.rows[row];
   lse[info.row] = (shift + sum) * kLn2;
   const float above = (sum - info.logit) * kLn2;   // (not below 0 but for roundings; NaN stays)
@@ -722,7 +726,7 @@ struct HeadPlan {
     if (!backward) {
       cut = best_cut(0, n, vocab, width, false, false, false, 0.0f);
       parts_ld = (n + 15) / 16 * 16;
-      at_parts = at, at += whole(parts_ld * parts() * 4);
+      at_parts = at, at += whole(parts_ld * parts() * (n <= Small::BM ? 8 : 4));   // (few rows: maximum and sum)
       bytes = at;
       return;
     }

@@ -34,7 +34,7 @@ def check(rows, width, vocab, dtype, scale=400.0):
     a = width * 2.0 ** -23 * (x64.abs() @ w64.abs().t()).max(1)[0]
     R = l.max(1)[0] - l.min(1)[0]
     bar = others * (2 * a + 3 * R * 2.0 ** -24) + 250 * 2.0 ** -24 + 2.0 ** -20 + 2.0 ** -21 * want
-    assert float(l.max()) > 100 and float(want.min()) < 1e-12
+    assert float(l.max()) > scale / 2 and float(want.min()) < 1e-12
     assert (loss >= 0).all(), f"a loss of {float(loss.min())}"
     over = (loss.double() - want).abs() - bar
     assert float(over.max()) <= 0, f"over the bar by {float(over.max())}"
@@ -78,3 +78,38 @@ def test_vocabulary_beyond_the_places():
     bar = a + (3 * (l.max(1)[0] - l.min(1)[0]) + 250) * 2.0 ** -24 + 2.0 ** -22 * (want.abs() + 20)
     assert float(((lse.double() - want).abs() - bar).max()) <= 0
     assert float(((loss.double() - (want - l.gather(1, target[:, None])[:, 0])).abs() - 2 * bar).max()) <= 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,width,vocab", [(1, 64, 129), (8, 768, 5003), (16, 4096, 300), (32, 1024, 40001)])
+def test_few_rows(rows, width, vocab, dtype):
+    """Rows as they stand, without a packing."""
+    for scale in (400.0, 100.0):
+        check(rows, width, vocab, dtype, scale)
+
+
+@pytest.mark.parametrize("rows,width,vocab", [(5, 264, 2003), (32, 4096, 300)])
+def test_few_rows_of_any_size(rows, width, vocab):
+    test_logits_of_any_size(rows, width, vocab)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("offset", [0.0, 30.0, 1000.0, -1000.0])
+@pytest.mark.parametrize("rows", [1, 20, 32, 33, 300, 2049])
+def test_offset(rows, offset, dtype):
+    """A number that all logits of a row share changes nothing.  Logits are sums that fp32 holds exactly here, so a is 0."""
+    g = torch.Generator().manual_seed(rows)
+    w = torch.zeros(5003, 8)
+    w[:, 0], w[:, 1:4] = 1.0, torch.randint(-32, 33, (5003, 3), generator=g) / 32.0
+    x = torch.zeros(rows, 8)
+    x[:, 0], x[:, 1:4] = offset, torch.randint(-8, 9, (rows, 3), generator=g) / 2.0
+    target = torch.randint(0, 5003, (rows,), generator=g).cuda()
+    x, w = x.to(dtype).cuda(), w.to(dtype).cuda()
+    loss, lse = apexw_amd.linear_cross_entropy_forward(x, w, target)
+    l = x.double() @ w.double().t()
+    full = torch.logsumexp(l, 1)
+    want = full - l.gather(1, target[:, None])[:, 0]
+    bar = (3 * (l.max(1)[0] - l.min(1)[0]) + 250) * 2.0 ** -24 + 2.0 ** -20 + 2.0 ** -21 * want
+    over = (loss.double() - want).abs() - bar
+    assert float(over.max()) <= 0, f"over the bar by {float(over.max())}"
+    assert float(((lse.double() - full).abs() - bar - 2.0 ** -22 * full.abs()).max()) <= 0
