@@ -495,9 +495,9 @@ __global__ __launch_bounds__(1024) void head_join_kernel(HeadArgs h, int parts, 
                                                          float* __restrict__ lse) {
   __shared__ float2 lds[16][16];
   const int r = threadIdx.x & 15, q = threadIdx.x >> 4;
-  const int64_t row = (int64_t)blockIdx.x * 16 + r;
+  const int64_t first = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 16, row = first + r;
   const int count = few ? few : h.state->count;
-  if ((int64_t)blockIdx.x * 16 >= count) return;
+  if (first >= count) return;
   float2 all = {-INFINITY, 0.0f};
   const float unit = few ? kLog2E : 1.0f;
   if (row < count) {
@@ -797,7 +797,8 @@ static_assert(Large::WN == 64 && Wide::WN == 64 && Mid::WN == 64 && Small::BM ==
 bool head_ok(int64_t n, int64_t width, int64_t vocab) {
   return n >= 0 && n <= INT32_MAX - 65536 && width > 0 && width <= kMostLd && vocab > 0 && vocab <= INT32_MAX - 65536;
 }
-// (the join's 1024 threads for 16 rows are fewer than 2^32)
+// The join's workgroups along a grid's first dimension, which times 1024 threads has to stay below 2^32
+constexpr int64_t kJoins = 1 << 21;
 bool head_fits(const HeadPlan& p) { return p.n < 1ll << 26 && rows_tiles<Small>(p.args(p.vocab)) <= INT32_MAX; }
 
 template <class S, int DT, class Out> void launch_logits_shape(const ExpertArgs& g, const Out& out, hipStream_t s) {
@@ -924,8 +925,9 @@ extern "C" int apexw_linear_cross_entropy_forward(const void* x, int64_t x_strid
       g.a = pack.packed, g.b = w, g.ends = &pack.state->count;
       launch_logits<DT>(g, p.cut.shape, Sums{h}, s);
     }
-    hipLaunchKernelGGL(head_join_kernel, dim3((unsigned)((n + 15) / 16)), dim3(1024), 0, s, h, (int)p.parts(), few ? (int)n : 0, targets,
-                       loss, lse);
+    const int64_t joins = (n + 15) / 16;
+    const dim3 grid((unsigned)(joins < kJoins ? joins : kJoins), (unsigned)((joins + kJoins - 1) / kJoins));
+    hipLaunchKernelGGL(head_join_kernel, grid, dim3(1024), 0, s, h, (int)p.parts(), few ? (int)n : 0, targets, loss, lse);
   });
   if (reduction) hipLaunchKernelGGL(head_total_kernel, dim3(1), dim3(1024), 0, s, pack.state, loss, n, (int)(reduction == 2), total);
   return hipGetLastError() == hipSuccess ? APEXW_OK : APEXW_ERR_LAUNCH;
