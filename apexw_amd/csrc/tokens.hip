@@ -655,7 +655,7 @@ extern "C" int apexw_expert_order(const void* expert, int32_t id_bytes, int64_t 
     sorted = launch_sort<true>(a, space, wanted, (char*)workspace, s);
   }
   if (wanted) {
-    const int grid = (experts + 255) / 256;
+    const int64_t grid = ((int64_t)experts + 255) / 256;
     hipLaunchKernelGGL(order_ends_kernel, dim3((unsigned)(grid < 1024 ? grid : 1024)), dim3(256), 0, s, sorted, a.n,
                        (uint32_t)experts, ends);
   }
