@@ -180,6 +180,8 @@ def expert_combine_backward(dout, y, order, weight=None, need=(True, True)):
     weight, w_dtype = _check_weight(weight, order, dout.dtype, "expert_combine", dout.device)
     y_stride = 0
     if need[1]:
+        if y is None:
+            raise ValueError("expert_combine: the weights' gradient takes y, got None")
         if y.dtype != dout.dtype:
             raise TypeError(f"expert_combine: rows of {y.dtype} and gradients of {dout.dtype}")
         y, y_stride = _check_matrix(y, "expert_combine: y", tokens * k, dout.shape[1])
