@@ -34,8 +34,8 @@ struct HeadState {          // device
   float scale;              // what dx and dW are multiplied with in the end
 };
 struct HeadRow {            // a row that counts; logarithms to base 2
-  float logit;              // its target's logit; forward, from its tile: less the shift
-  float lse, d;             // backward
+  float logit;              // its target's logit; forward: less the shift
+  float lse, d;             // backward; forward, lse: the target's logit less the shift as its tile has it
   int32_t target, row;      // its place among all rows
 };
 // A row's shift, forward: its target's logit but for the low bits (a 32nd of it at most), which say the target, so that the
@@ -184,6 +184,7 @@ template <int DT> __global__ __launch_bounds__(256) void head_pack_kernel(PackAr
         shift = __uint_as_float((bits & ~1u) | (row.d < 0.0f));
       } else {
         shift = with_place(shift, target);
+        row.logit = fmaf(dot, kLog2E, -shift);
       }
       a.rows[p] = row, a.shift[p] = shift;
     }
@@ -226,7 +227,8 @@ template <int FA> struct Shifts {
 // Forward: each row's sum of exponentials over a wave's columns, relative to its shift.  That is a maximum's part as long as no
 // logit is 83 above it (2^120) and one is 83 below or more; the rows of a block where this is not so are summed again from
 // their maximum.  The packing's target's logit is off from the tile's by their orders of summing (3e-4 at logits of
-// 1000), so the wave that has the target leaves its exponent as it is in the sum: a row certain of its target has a loss of 0.
+// 1000), so the wave that has the target leaves its exponent as it is in the sum, where the join puts the packing's for it
+// (which is the nearer one): a row certain of its target has a loss of 0, not of that difference.
 // (16384 x 768 x 51200 1094 -> 1107 us, 8192 x 4096 x 128256 6266 -> 6313.)
 struct Sums {
   HeadArgs h;
@@ -290,7 +292,7 @@ struct Sums {
         for (int j = 0; j < FB; ++j)
 #pragma unroll
           for (int q = 0; q < 4; ++q) logit = (t & ~12u) == 16u * j + q ? acc[i][j][q] : logit;
-        if (t < S::WN && r < rows && (int)(t >> 2 & 3u) == lane >> 4) h.rows[row0 + r].logit = fmaf(logit, kLog2E, -shift);
+        if (t < S::WN && r < rows && (int)(t >> 2 & 3u) == lane >> 4) h.rows[row0 + r].lse = fmaf(logit, kLog2E, -shift);
       }
     }
     if constexpr (kJoin) {
@@ -523,8 +525,11 @@ __global__ __launch_bounds__(1024) void head_join_kernel(HeadArgs h, int parts, 
     loss[row] = has ? (top - shift) + sum : 0.0f;
     return;
   }
-  const float sum = top + log2f(all.y);
   const HeadRow& info = h.rows[row];
+  const float others = all.y - __builtin_amdgcn_exp2f(info.lse - top);
+  all = others <= 0.0f ? make_float2(-INFINITY, 0.0f) : make_float2(top, others);
+  add_sum(all, make_float2(info.logit, 1.0f), 1.0f);
+  const float sum = all.x + log2f(all.y);
   lse[info.row] = (shift + sum) * kLn2;
   const float above = (sum - info.logit) * kLn2;   // (not below 0 but for roundings; NaN stays)
   loss[info.row] = above < 0.0f ? 0.0f : above;
