@@ -9,14 +9,16 @@
 // masked rows, NaN too, reaches nothing.  Their number is known on the device alone.
 //
 // Forward: the logits of a tile stay in registers, and each row leaves the sum of exponentials over a wave's columns,
-// relative to its target's logit, which the packing forms; a second launch joins them.  Backward: a piece of the
-// vocabulary at a time, which bounds G's memory; G of the piece from the logits computed again, rounded to 16 bits as an
-// operand of the two products that take it.  dx adds up the pieces in fp32.
+// relative to a number near its target's logit, which the packing forms; a second launch joins them.  Backward: a piece
+// of the vocabulary at a time, which bounds G's memory; G of the piece from the logits computed again, rounded to 16 bits as
+// an operand of the two products that take it: the matrix cores take no other beside 16-bit rows and weights, and a second
+// half of G would double the two products.  It is most of what the gradients are off by besides their own rounding (against 64
+// bits 0.0019 of the result in bf16 and 0.00025 in fp16, 0.0017 and 0.00021 with G in fp32).  dx adds up the pieces in fp32.
 //
 // Measured, kernels alone, bf16:
-//   forward, 8192 rows, 4096 x 128256       pack 36, logits 6200 to 6350, join 24 us   1360 to 1390 TFLOP/s
+//   forward, 8192 rows, 4096 x 128256       pack 36, logits 6200 to 6370, join 24 us   1350 to 1390 TFLOP/s
 //   (a library's product alone 5990 us; the chip's power bounds both)
-//   forward, 8 rows, 768 x 50257            logits 15, join 4.4 us                     5.2 TB/s of weights
+//   forward, 8 rows, 768 x 50257            logits 15, join 4.8 us                     5.2 TB/s of weights
 //   backward, 13107 rows, 768 x 50257       pack 42, G 968, dW 890, dx 1290, dx's end 12 us
 //   (products alone by a library 910, 1097 and 970 us)
 //   backward, 501 rows, 500 x 10007 fp16    pack 10, G 19, dW 20, dx 19, dx's end 8 us
@@ -712,6 +714,8 @@ struct Piece {
   }
 };
 
+// (Shapes, parts and pieces are those of all n rows: how many count is known on the device alone.  Rows that do not count
+// make no tiles, but a batch that is mostly masked runs in tiles chosen for the whole of it.)
 struct HeadPlan {
   int64_t n, width, wide, vocab, w_stride;
   bool copy_w;
