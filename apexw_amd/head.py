@@ -96,8 +96,8 @@ def linear_cross_entropy_backward(dloss, x, weight, target, lse, ignore_index=-1
     """(dx, dweight) from the gradient dloss (float32) of each row's loss and the lse that the forward half gave.
 
     Rows that count for nothing get zeros in dx and give nothing to dweight, whatever they hold; ``need`` leaves out
-    gradients nobody wants (None).  The softmax minus the target's one, times dloss, is rounded to x's type before
-    the two products, which are summed in fp32 and rounded once."""
+    gradients nobody wants (None).  The softmax minus the target's one, times dloss, is rounded to x's type (scaled
+    so that the largest |dloss| is 2^14) before the two products, which are summed in fp32 and rounded once."""
     for t, name in ((dloss, "dloss"), (lse, "lse")):
         if t.dtype != torch.float32 or t.shape != target.shape:
             raise ValueError(f"linear_cross_entropy: expected {name} as one float32 for each row {tuple(target.shape)}, got "

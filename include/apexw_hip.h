@@ -930,7 +930,8 @@ int apexw_embedding_weight_grad(const void* dy, int64_t dy_stride, const void* i
  *   G[i] = (exp(l[i] - lse[i]) - onehot(target[i])) dloss[i],  dx = G weight,  dw = G^T x
  * x: n rows of `width` BF16 / F16 elements, x_stride apart; weight: vocab rows of the same type, w_stride apart.  Rows
  * whose target is ignore_index or outside [0, vocab) count for nothing: loss, lse and dx are 0 there and dw has
- * nothing of them, whatever they hold.  Products are summed in fp32; G is rounded to dtype.
+ * nothing of them, whatever they hold.  Products are summed in fp32; G is rounded to dtype, scaled so that the largest
+ * |dloss| is 2^14.
  * reduction: 0, or 1 (sum) or 2 (mean over the rows that count; NaN without any) of the losses into *total (fp32).
  * backward: dloss_stride 0 is one number for all rows; mean != 0 divides it by the number of rows that count; dx
  * ([n x width]) and dw ([vocab x width], both contiguous) may be NULL.
